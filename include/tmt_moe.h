@@ -377,6 +377,88 @@ int tmt_moe_adamw_chunks(tmt_moe_adamw* opt, int32_t* chunks);
  * model.cu:219, checkpoint.h:149). */
 int tmt_moe_f32_to_bf16(void* stream, const float* in, uint16_t* out, int64_t n);
 
+/*
+ * A linear layer on microscaled (MX) numbers, next to the block's MXFP4
+ * experts: TMT's dense layers (the cell's and MLA's projections, the head),
+ * whose reference is one cuBLAS product each (linalg.cu:9-41, bf16 only). No
+ * handle; the reference has no microscaled path.
+ *
+ * Blocks of 32 values along a row share one e8m0 scale byte s, 2^(s - 127);
+ * s = 255 makes the block NaN. Rows [rows][K] are held as
+ *   codes   [rows][K/2] bytes (MX_FP4: e2m1, low nibble = even column) or
+ *           [rows][K] bytes (MX_FP8: e4m3);
+ *   scales  [K/32][lds] bytes, block-major, lds >= rows: (K/32) * lds bytes,
+ *           of which columns rows .. lds-1 are never written and never count.
+ * An MXFP4 matrix with lds == rows is a W_up[e] / W_down[e] of
+ * tmt_moe_forward_mxfp4.
+ *
+ * Every product sums exact terms in fp32 (a code times its scale is exact in
+ * bf16) and rounds once. Y = beta * Y + ...; with beta == 0 the output is
+ * not read. Outputs must not overlap inputs. T any number >= 0, N a multiple
+ * of 16, K a multiple of 64. Strides are in elements; bf16 and fp32 rows start
+ * at 16-byte boundaries (base and stride), codes and scales of a product too
+ * (scale strides are multiples of 16). Elements between a row's width and its
+ * stride are neither read into a result nor written.
+ *
+ * All calls enqueue on `stream` on the current device, allocate nothing and
+ * do not synchronise. The products take a workspace of
+ * tmt_moe_linear_workspace_size bytes (device memory, 256-byte aligned, NULL
+ * where that is 0), used only inside the call: calls that share one must be
+ * ordered by the caller. A workspace for T serves every call of fewer tokens
+ * with the same N and K. Results are the same, bit for bit, from run to run.
+ */
+enum { TMT_MOE_MX_FP4 = 0, TMT_MOE_MX_FP8 = 1 };
+enum { TMT_MOE_BF16 = 0, TMT_MOE_F32 = 1 };
+
+/*
+ * X [rows][ldx] (bf16 or fp32) to codes and scales. Per block, with amax its
+ * largest magnitude:
+ *   MX_FP4  scale exponent floor(log2 amax) - 2, nearest e2m1 value (ties to
+ *           the even code), saturating at 6: the format of the expert weights;
+ *   MX_FP8  the smallest exponent with amax <= 448 * 2^e, nearest e4m3 value
+ *           (ties to even): nothing saturates, so a value is off by at most
+ *           2^-4 of itself or half a step of e4m3's subnormals.
+ * Exponents are clamped to [-127, 127]; a block of zeros takes exponent 0; a
+ * block with an infinity or a NaN takes s = 255. K a multiple of 32; lds any
+ * number >= rows.
+ */
+int tmt_moe_mx_quantize(void* stream, int32_t format, int32_t dtype, const void* X, int64_t ldx, int32_t rows,
+                        int32_t K, uint8_t* codes, uint8_t* scales, int64_t lds);
+/* The values that codes and scales stand for, exact in fp32 (and in bf16 down
+ * to its subnormals, where they are rounded once). */
+int tmt_moe_mx_dequantize(void* stream, int32_t format, const uint8_t* codes, const uint8_t* scales, int64_t lds,
+                          int32_t rows, int32_t K, int32_t dtype, void* X, int64_t ldx);
+
+enum {
+    TMT_MOE_LINEAR_FORWARD = 0,  /* tmt_moe_mxfp4_linear */
+    TMT_MOE_LINEAR_MATMUL = 1,   /* tmt_moe_mxfp4_matmul */
+    TMT_MOE_LINEAR_DX = 2,       /* tmt_moe_mxfp4_linear_dx */
+    TMT_MOE_LINEAR_DW = 3        /* tmt_moe_mxfp8_linear_dw */
+};
+int tmt_moe_linear_workspace_size(int32_t op, int32_t T, int32_t N, int32_t K, size_t* bytes);
+
+/* Y [T][ldy] = beta * Y + X W^T: X [T][ldx] bf16, W [N][K] MXFP4, Y bf16. */
+int tmt_moe_mxfp4_linear(void* stream, int32_t T, int32_t N, int32_t K, const uint16_t* X, int64_t ldx,
+                         const uint8_t* W, const uint8_t* W_scale, int64_t ldws, uint16_t* Y, int64_t ldy,
+                         float beta, void* workspace, size_t workspace_bytes);
+/* The same with X [T][K] in MXFP4 too (tmt_moe_mx_quantize), on the scaled
+ * matrix instructions. */
+int tmt_moe_mxfp4_matmul(void* stream, int32_t T, int32_t N, int32_t K, const uint8_t* X, const uint8_t* X_scale,
+                         int64_t ldxs, const uint8_t* W, const uint8_t* W_scale, int64_t ldws, uint16_t* Y,
+                         int64_t ldy, float beta, void* workspace, size_t workspace_bytes);
+/* The gradient at the layer's input, dX [T][lddx] = beta * dX + dY W:
+ * dY [T][lddy] bf16, W [N][K] MXFP4, dX bf16. */
+int tmt_moe_mxfp4_linear_dx(void* stream, int32_t T, int32_t N, int32_t K, const uint16_t* dY, int64_t lddy,
+                            const uint8_t* W, const uint8_t* W_scale, int64_t ldws, uint16_t* dX, int64_t lddx,
+                            float beta, void* workspace, size_t workspace_bytes);
+/* The gradient at the layer's fp32 master weights, dW [N][lddw] = beta * dW +
+ * dY^T X, from the input kept as an MXFP8 checkpoint: dY [T][lddy] bf16,
+ * X [T][K] MXFP8, dW fp32 (as tmt_moe_adamw_step takes it). T == 0 gives
+ * beta * dW. */
+int tmt_moe_mxfp8_linear_dw(void* stream, int32_t T, int32_t N, int32_t K, const uint16_t* dY, int64_t lddy,
+                            const uint8_t* X, const uint8_t* X_scale, int64_t ldxs, float* dW, int64_t lddw,
+                            float beta, void* workspace, size_t workspace_bytes);
+
 /* Thread-local message of the last failing call on this thread. */
 const char* tmt_moe_last_error(void);
 

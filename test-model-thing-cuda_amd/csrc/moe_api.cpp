@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/tmt_moe.h"
+#include "api_util.hpp"
 #include "moe_internal.hpp"
 
 using namespace tmt;
@@ -31,9 +32,9 @@ using namespace tmt;
 constexpr size_t kNoAllocScratchBytes = size_t(4) << 20;
 static __device__ __align__(256) float scratch[kNoAllocScratchBytes / sizeof(float)];
 
-namespace {
+namespace tmt {
 
-thread_local std::string g_last_error;
+static thread_local std::string g_last_error;
 
 int fail(int code, const char* fmt, ...) {
     char buf[512];
@@ -45,15 +46,9 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-#define HIP_TRY(call)                                                              \
-    do {                                                                           \
-        hipError_t err__ = (call);                                                 \
-        if (err__ != hipSuccess)                                                   \
-            return fail(TMT_MOE_EDEVICE, "%s failed: %s", #call, hipGetErrorString(err__)); \
-    } while (0)
+}  // namespace tmt
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool aligned_to(const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1u)) == 0; }
+namespace {
 
 // Device address of `scratch` on the current device, looked up on the first
 // call made with that device current and kept per device.

@@ -53,11 +53,25 @@ EXPORTED = (
     "tmt_moe_adamw_chunks",
     "tmt_moe_f32_to_bf16",
     "tmt_moe_mxfp4_planes",
+    "tmt_moe_mx_quantize",
+    "tmt_moe_mx_dequantize",
+    "tmt_moe_linear_workspace_size",
+    "tmt_moe_mxfp4_linear",
+    "tmt_moe_mxfp4_matmul",
+    "tmt_moe_mxfp4_linear_dx",
+    "tmt_moe_mxfp8_linear_dw",
     "tmt_moe_set_profiling",
     "tmt_moe_read_profile",
     "tmt_moe_phase_name",
     "tmt_moe_last_error",
 )
+
+MX_FP4 = 0
+MX_FP8 = 1
+LINEAR_FORWARD = 0
+LINEAR_MATMUL = 1
+LINEAR_DX = 2
+LINEAR_DW = 3
 
 NPHASES = 15
 
@@ -114,6 +128,13 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.tmt_moe_adamw_chunks.argtypes = [vp, ctypes.POINTER(i32)]
     lib.tmt_moe_f32_to_bf16.argtypes = [vp, vp, vp, ctypes.c_int64]
     lib.tmt_moe_mxfp4_planes.argtypes = [vp, vp, i32, i32, vp]
+    i64, size = ctypes.c_int64, ctypes.c_size_t
+    lib.tmt_moe_mx_quantize.argtypes = [vp, i32, i32, vp, i64, i32, i32, vp, vp, i64]
+    lib.tmt_moe_mx_dequantize.argtypes = [vp, i32, vp, vp, i64, i32, i32, i32, vp, i64]
+    lib.tmt_moe_linear_workspace_size.argtypes = [i32, i32, i32, i32, ctypes.POINTER(size)]
+    for name in ("tmt_moe_mxfp4_linear", "tmt_moe_mxfp4_linear_dx", "tmt_moe_mxfp8_linear_dw"):
+        getattr(lib, name).argtypes = [vp, i32, i32, i32, vp, i64, vp, vp, i64, vp, i64, f32, vp, size]
+    lib.tmt_moe_mxfp4_matmul.argtypes = [vp, i32, i32, i32, vp, vp, i64, vp, vp, i64, vp, i64, f32, vp, size]
     lib.tmt_moe_read_stats.argtypes = [vp, vp, vp, vp, vp]
     lib.tmt_moe_stats_device_ptr.argtypes = [vp, pp]
     lib.tmt_moe_read_routing.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp]
@@ -231,6 +252,131 @@ def mxfp4_planes(codes, planes, stream=None) -> None:
     take: one expert matrix, device tensors, enqueued on `stream`."""
     N, half = int(codes.shape[0]), int(codes.shape[1])
     _check(load_library().tmt_moe_mxfp4_planes(_stream(stream), _ptr(codes), N, 2 * half, _ptr(planes)))
+
+
+def _rows(what: str, t, dtype) -> tuple:
+    """(pointer, row stride) of a matrix whose rows are contiguous."""
+    if t.dim() != 2 or t.dtype != dtype:
+        raise ValueError(f"{what} must be a matrix of {dtype}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"the rows of {what} must be contiguous")
+    _same_device(what, t)
+    return int(t.data_ptr()), int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
+
+
+def _same_device(what: str, t) -> None:
+    import torch
+    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{what} is on {t.device}, not on the current GPU")
+
+
+def _mx(what: str, codes, scales, rows: int, K: int, fmt: int) -> tuple:
+    """(codes, scales, scale stride) of a microscaled matrix [rows, K]."""
+    import torch
+    c, ldc = _rows(f"codes of {what}", codes, torch.uint8)
+    width = K // 2 if fmt == MX_FP4 else K
+    if tuple(codes.shape) != (rows, width) or (rows > 1 and ldc != width):
+        raise ValueError(f"codes of {what} must be a contiguous [{rows}, {width}], not {list(codes.shape)}")
+    s, lds = _rows(f"scales of {what}", scales, torch.uint8)
+    if scales.shape[0] != K // 32 or scales.shape[1] < rows:
+        raise ValueError(f"scales of {what} must be [{K // 32}, {rows} or more], not {list(scales.shape)}")
+    return c, s, lds
+
+
+def _mx_dtype(what: str, t) -> int:
+    import torch
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{what} must be bfloat16 or float32, not {t.dtype}")
+    return 0 if t.dtype == torch.bfloat16 else 1
+
+
+def mx_quantize(X, codes, scales, fmt: int = MX_FP4, stream=None) -> None:
+    """X [rows, K] (bf16 or fp32) to microscaled codes ([rows, K/2] for MX_FP4,
+    [rows, K] for MX_FP8) and block-major scales [K/32, rows or more], uint8."""
+    dtype = _mx_dtype("X", X)
+    x, ldx = _rows("X", X, X.dtype)
+    rows, K = int(X.shape[0]), int(X.shape[1])
+    c, s, lds = _mx("X", codes, scales, rows, K, fmt)
+    _check(load_library().tmt_moe_mx_quantize(_stream(stream), fmt, dtype, x, ldx, rows, K, c, s, lds))
+
+
+def mx_dequantize(codes, scales, X, fmt: int = MX_FP4, stream=None) -> None:
+    """The values of codes and scales (as mx_quantize writes them) into
+    X [rows, K], bf16 or fp32."""
+    dtype = _mx_dtype("X", X)
+    x, ldx = _rows("X", X, X.dtype)
+    rows, K = int(X.shape[0]), int(X.shape[1])
+    c, s, lds = _mx("X", codes, scales, rows, K, fmt)
+    _check(load_library().tmt_moe_mx_dequantize(_stream(stream), fmt, c, s, lds, rows, K, dtype, x, ldx))
+
+
+def linear_workspace_size(op: int, T: int, N: int, K: int) -> int:
+    """Bytes of device workspace that the product `op` (LINEAR_FORWARD,
+    LINEAR_MATMUL, LINEAR_DX, LINEAR_DW) needs for up to T tokens."""
+    out = ctypes.c_size_t(0)
+    _check(load_library().tmt_moe_linear_workspace_size(op, T, N, K, ctypes.byref(out)))
+    return int(out.value)
+
+
+def _ws(workspace) -> tuple:
+    if workspace is None:
+        return 0, ctypes.c_size_t(0)
+    _same_device("workspace", workspace)
+    return _ptr(workspace), ctypes.c_size_t(workspace.numel() * workspace.element_size())
+
+
+def _shaped(what: str, t, rows: int, cols: int) -> None:
+    if tuple(t.shape) != (rows, cols):
+        raise ValueError(f"{what} must be [{rows}, {cols}], not {list(t.shape)}")
+
+
+def mxfp4_linear(X, codes, scales, Y, beta: float = 0.0, workspace=None, stream=None) -> None:
+    """Y <- beta*Y + X W^T. X [T, K], Y [T, N] bf16; W [N, K] as MXFP4 codes
+    [N, K/2] and scales [K/32, N or more] (a multiple of 16)."""
+    import torch
+    x, ldx = _rows("X", X, torch.bfloat16)
+    y, ldy = _rows("Y", Y, torch.bfloat16)
+    T, K, N = int(X.shape[0]), int(X.shape[1]), int(Y.shape[1])
+    _shaped("Y", Y, T, N)
+    c, s, lds = _mx("W", codes, scales, N, K, MX_FP4)
+    _check(load_library().tmt_moe_mxfp4_linear(_stream(stream), T, N, K, x, ldx, c, s, lds, y, ldy,
+                                               ctypes.c_float(beta), *_ws(workspace)))
+
+
+def mxfp4_matmul(X_codes, X_scales, codes, scales, Y, beta: float = 0.0, workspace=None, stream=None) -> None:
+    """Y <- beta*Y + X W^T with X [T, K] and W [N, K] both in MXFP4; Y [T, N] bf16."""
+    import torch
+    y, ldy = _rows("Y", Y, torch.bfloat16)
+    T, N, K = int(Y.shape[0]), int(Y.shape[1]), 2 * int(codes.shape[1])
+    xc, xs, xlds = _mx("X", X_codes, X_scales, T, K, MX_FP4)
+    c, s, lds = _mx("W", codes, scales, N, K, MX_FP4)
+    _check(load_library().tmt_moe_mxfp4_matmul(_stream(stream), T, N, K, xc, xs, xlds, c, s, lds, y, ldy,
+                                               ctypes.c_float(beta), *_ws(workspace)))
+
+
+def mxfp4_linear_dx(dY, codes, scales, dX, beta: float = 0.0, workspace=None, stream=None) -> None:
+    """dX <- beta*dX + dY W. dY [T, N], dX [T, K] bf16; W as in mxfp4_linear."""
+    import torch
+    x, ldx = _rows("dY", dY, torch.bfloat16)
+    y, ldy = _rows("dX", dX, torch.bfloat16)
+    T, N, K = int(dY.shape[0]), int(dY.shape[1]), int(dX.shape[1])
+    _shaped("dX", dX, T, K)
+    c, s, lds = _mx("W", codes, scales, N, K, MX_FP4)
+    _check(load_library().tmt_moe_mxfp4_linear_dx(_stream(stream), T, N, K, x, ldx, c, s, lds, y, ldy,
+                                                  ctypes.c_float(beta), *_ws(workspace)))
+
+
+def mxfp8_linear_dw(dY, codes, scales, dW, beta: float = 0.0, workspace=None, stream=None) -> None:
+    """dW <- beta*dW + dY^T X from the MXFP8 checkpoint of X [T, K] (codes [T, K],
+    scales [K/32, T or more], a multiple of 16). dY [T, N] bf16, dW [N, K] fp32."""
+    import torch
+    x, ldx = _rows("dY", dY, torch.bfloat16)
+    y, ldy = _rows("dW", dW, torch.float32)
+    T, N, K = int(dY.shape[0]), int(dY.shape[1]), int(dW.shape[1])
+    _shaped("dW", dW, N, K)
+    c, s, lds = _mx("X", codes, scales, T, K, MX_FP8)
+    _check(load_library().tmt_moe_mxfp8_linear_dw(_stream(stream), T, N, K, x, ldx, c, s, lds, y, ldy,
+                                                  ctypes.c_float(beta), *_ws(workspace)))
 
 
 class MoE:
