@@ -1,8 +1,32 @@
 // linear.hip -- products of the linear layer on microscaled numbers.
 //
 // Every operand value is exact in bf16 (an e2m1 code has two significant
-// bits, an e4m3 code four, and scales are powers of two), so each product is
-// one bf16 matrix product with fp32 sums of exact terms.
+// bits, an e4m3 code four, and scales are powers of two), so a product with
+// bf16 rows is one bf16 matrix product with fp32 sums of exact terms.
+//
+//   FORWARD  Y[t][n] = sum_k X[t][k] W[n][k]     X and the codes along k
+//   MATMUL   the same with X in MXFP4, on the scaled matrix instructions
+//   DX       dX[t][k] = sum_n dY[t][n] W[n][k]   codes across the reduction
+//   DW       dW[n][k] = sum_t dY[t][n] X[t][k]   both operands across it
+//
+// Tiles of 256 x 256 outputs (one workgroup of 4 waves per CU, a wave 128 x
+// 128 = 4 x 4 v_mfma_f32_32x32x16_bf16 tiles) or 128 x 128 (two workgroups
+// per CU, a wave 64 x 64); linear_plan chooses. Workgroups are persistent and
+// walk units (a tile, or a part of one along the reduction). All operands
+// stream from global memory into LDS rings by direct loads, and the stream
+// does not stop between units: a unit's last steps already load the next
+// one's first, and its epilogue stages outputs in LDS of its own, so the
+// matrix cores wait for neither a first load nor a drained ring.
+//
+// FORWARD expands the codes where a fragment is read (8 codes, 4 bytes of
+// LDS, a lane: four conversion instructions under the MFMAs). In DX and DW
+// the reduction runs across the codes' rows, every element of a fragment
+// with a scale of its own, so each code is expanded once per workgroup: raw
+// codes land in LDS, 32 reduction rows a sub-step, are converted one sub-step
+// ahead into a row-contiguous bf16 tile, and fragments are read from that with
+// the transposing ds_read_b64_tr_b16.
+#include <algorithm>
+
 #include "linear.hpp"
 #include "moe_internal.hpp"
 #include "mx_format.hpp"
@@ -11,103 +35,935 @@ namespace tmt {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-__device__ __forceinline__ uint16_t fp4_at(const uint8_t* codes, const uint8_t* scales, int64_t lds, int K, int64_t row, int k) {
-    const uint32_t q = (codes[row * (K / 2) + k / 2] >> (4 * (k & 1))) & 15;
-    float v[8];
-    from_e2m1(q, v);
-    return f2bf(v[0] * e8m0_value(scales[(k / 32) * lds + row]));
+// What is read for reduction rows past the end: the products of a step's tail
+// are zero times zero, whatever lies behind the operands.
+__device__ __align__(16) const uint32_t zero_piece[4] = {0, 0, 0, 0};
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 16 bytes per lane from a wave-uniform base and a 32-bit lane offset into
+// LDS at lds_base + 16 * lane (lds_base wave-uniform); M0 is written.
+__device__ __forceinline__ void dma16s(const void* sbase, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "m0");
+}
+// The same from a 64-bit lane address, and 4 bytes per lane.
+__device__ __forceinline__ void dma16v(const void* g, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base) : "m0");
+}
+__device__ __forceinline__ void dma4v(const void* g, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_base) : "m0");
+}
+#pragma clang diagnostic pop
+// A wave-uniform pointer in scalar registers.
+__device__ __forceinline__ const uint8_t* uniform(const void* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return reinterpret_cast<const uint8_t*>(((uint64_t)hi << 32) | lo);
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Workgroup barrier behind the LDS accesses only: a compiler's barrier would
+// also wait for the last unit's output stores.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// 8 e2m1 codes with the scale 2^(s - 127) (or NaN) as 8 bf16.
+__device__ __forceinline__ uint4 expand_fp4(uint32_t w, float sc) {
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3)));
+}
+// 8 e4m3 codes.
+__device__ __forceinline__ uint4 expand_fp8(uint2 w, float sc) {
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, sc, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, sc, true)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, true)));
 }
 
-constexpr int BT = 64, BK = 32, LD = BK + 8;
+// ---- units -----------------------------------------------------------------
+// tiles_m x tiles_c output tiles. The first `whole` are units of their own;
+// the `tail` others, the last round's, are cut into `parts` along the
+// reduction, `chunk` (a multiple of 256) each: a launch of its own writes
+// their fp32 partial tiles, which linear_fixup_kernel adds in part order.
+struct LinearPlan {
+    int tile = 256, tiles_m = 0, tiles_c = 0, whole = 0, tail = 0, parts = 1, chunk = 0;
+};
+struct Unit {
+    int m0, c0, kbeg, kend, part;
+};
+// Consecutive tiles go down 4 rows of tiles (or what 32 tiles leave where
+// there are few columns), then to the next column, so that the 32 tiles that
+// an XCD works on share operand slices in its L2.
+__device__ __forceinline__ void tile_at(const LinearPlan& pl, int j, int& mt, int& ct) {
+    const int rows = pl.tiles_c >= 8 ? 4 : 32 / pl.tiles_c;
+    const int blk = j / (rows * pl.tiles_c), rem = j - blk * (rows * pl.tiles_c);
+    const int in = min(rows, pl.tiles_m - blk * rows);
+    ct = rem / in;
+    mt = blk * rows + (rem - ct * in);
+}
+// Unit of the workgroup's slot vb (blockIdx.x, + gridDim.x, ...). The hardware
+// hands workgroup b to XCD b % 8 and the grid is a multiple of 8 where a
+// workgroup takes several slots; each XCD takes runs of consecutive units.
+template <int TILE, bool SPLIT>
+__device__ __forceinline__ bool unit_at(const LinearPlan& pl, int R, int vb, Unit& u) {
+    const int n = SPLIT ? pl.tail * pl.parts : pl.whole, whole = n & ~255, per = (n - whole + 7) / 8;
+    int j;
+    if (vb < whole) {
+        j = (((vb >> 8) << 3) + (vb & 7)) * 32 + ((vb >> 3) & 31);
+    } else {
+        const int i = (vb - whole) >> 3;
+        j = whole + (vb & 7) * per + i;
+        if (i >= per || j >= n) return false;
+    }
+    int mt, ct;
+    u.kbeg = 0;
+    u.kend = R;
+    u.part = j;
+    if constexpr (SPLIT) {
+        const int q = j / pl.parts;
+        u.kbeg = (j - q * pl.parts) * pl.chunk;
+        u.kend = min(R, u.kbeg + pl.chunk);
+        j = pl.whole + q;
+    }
+    tile_at(pl, j, mt, ct);
+    u.m0 = mt * TILE;
+    u.c0 = ct * TILE;
+    return true;
+}
 
-// 64 x 64 outputs per workgroup, a wave each 32 x 32; both operands staged
-// K-contiguous in LDS, element by element.
-template <int OP>
-__global__ __launch_bounds__(256) void linear_simple_kernel(LinearParams p, int M, int C, int R, int tiles_c) {
-    __shared__ __align__(16) uint16_t as[BT * LD], bs[BT * LD];
-    const int m0 = (int)(blockIdx.x / tiles_c) * BT, c0 = (int)(blockIdx.x % tiles_c) * BT;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = (wave >> 1) * 32, wc = (wave & 1) * 32;
-    f32x16 acc;
+// ---- epilogue ----------------------------------------------------------------
+// acc[i][j][r] = C[m][c] with m = 32 i + lane % 32 and c = 32 j + 8 (r / 4) +
+// 4 (lane / 32) + r % 4 in the wave's WT x WT outputs. 32 rows by 32 JS columns
+// at a time go through the wave's own LDS, so that a row's columns leave as one
+// run of 16-byte stores; no barrier.
+template <bool F32, int JS>
+struct Stage {
+    static constexpr int ROWB = 32 * JS * (F32 ? 4 : 2);  // bytes per staged row
+    static constexpr int BYTES = 32 * ROWB;
+};
+
+template <int N>
+__device__ __forceinline__ void clear(f32x16 (&acc)[N][N]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-    for (int k0 = 0; k0 < R; k0 += BK) {
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int i = 0; i < BT * BK / 256; ++i) {
-            const int q = tid + 256 * i;
-            // neighbouring lanes along the operand's contiguous direction
-            const bool kc = OP != LINEAR_DW;
-            const int r = kc ? q / BK : q % BT, k = kc ? q % BK : q / BT;
-            const int m = m0 + r, kk = k0 + k;
-            uint16_t v = 0;
-            if (m < M && kk < R) {
-                if constexpr (OP == LINEAR_MATMUL) v = fp4_at(p.xq, p.xs, p.xlds, p.K, m, kk);
-                else if constexpr (OP == LINEAR_DW) v = p.x[(int64_t)kk * p.ldx + m];
-                else v = p.x[(int64_t)m * p.ldx + kk];
-            }
-            as[r * LD + k] = v;
-            const bool bkc = OP == LINEAR_FORWARD || OP == LINEAR_MATMUL;
-            const int br = bkc ? q / BK : q % BT, bk = bkc ? q % BK : q / BT;
-            const int c = c0 + br, kb = k0 + bk;
-            v = 0;
-            if (c < C && kb < R) {
-                if constexpr (OP == LINEAR_DW) {
-                    float f[4];
-                    from_e4m3(p.w[(int64_t)kb * p.K + c], f);
-                    v = f2bf(f[0] * e8m0_value(p.ws[(c / 32) * p.wlds + kb]));
-                } else if constexpr (OP == LINEAR_DX) {
-                    v = fp4_at(p.w, p.ws, p.wlds, p.K, kb, c);
-                } else {
-                    v = fp4_at(p.w, p.ws, p.wlds, p.K, c, kb);
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+}
+
+__device__ __forceinline__ void wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// out: the wave's first output element, ld its row stride; rows, cols: valid
+// ones. beta times what is there is added in fp32.
+template <int WT, bool F32, int JS>
+__device__ __forceinline__ void store_wave(f32x16 (&acc)[WT / 32][WT / 32], uint8_t* st, void* out, int64_t ld, int rows,
+                                           int cols, float beta) {
+    using S = Stage<F32, JS>;
+    constexpr int N = WT / 32;
+    constexpr int CH = S::ROWB / 16, RPI = 64 / CH;  // 16-byte chunks per staged row, rows per store
+    const int lane = threadIdx.x & 63, lr = lane & 31;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int jg = 0; jg < N; jg += JS) {
+            // the outputs not yet staged stay in the accumulator registers
+#pragma unroll
+            for (int i2 = i; i2 < N; ++i2)
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (i2 > i || j >= jg) asm volatile("" : "+a"(acc[i2][j]));
+#pragma unroll
+            for (int j = 0; j < JS; ++j) {
+                const f32x16& a = acc[i][jg + j];
+                uint2 old[4] = {};  // bf16 outputs that are added to
+                if (!F32 && beta != 0.0f) {
+                    const uint16_t* y = static_cast<const uint16_t*>(out) + (int64_t)min(32 * i + lr, rows - 1) * ld;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        old[q] = *reinterpret_cast<const uint2*>(y + min(32 * (jg + j) + 8 * q + 4 * (lane >> 5), cols - 4));
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if constexpr (F32) {
+                        const int ch = j * 8 + 2 * q + (lane >> 5);
+                        *reinterpret_cast<f32x4*>(st + lr * S::ROWB + ((ch ^ (lr & (CH - 1))) * 16)) =
+                            f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+                    } else {
+                        const int ch = j * 4 + q;
+                        *reinterpret_cast<uint2*>(st + lr * S::ROWB + ((ch ^ (lr & (CH - 1))) * 16) + (lane >> 5) * 8) =
+                            make_uint2(pack_bf2(a[4 * q] + beta * bf_lo(old[q].x), a[4 * q + 1] + beta * bf_hi(old[q].x)),
+                                       pack_bf2(a[4 * q + 2] + beta * bf_lo(old[q].y), a[4 * q + 3] + beta * bf_hi(old[q].y)));
+                    }
                 }
             }
-            bs[br * LD + bk] = v;
-        }
-        __syncthreads();
+            wave_lds_fence();
+            const int cl = lane % CH, c = 32 * jg + cl * (F32 ? 4 : 8);
 #pragma unroll
-        for (int s = 0; s < BK / 16; ++s) {
-            const int k = 16 * s + 8 * (lane >> 5);
-            const uint4 a = *reinterpret_cast<const uint4*>(as + (wm + (lane & 31)) * LD + k);
-            const uint4 b = *reinterpret_cast<const uint4*>(bs + (wc + (lane & 31)) * LD + k);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), acc, 0, 0, 0);
+            for (int k = 0; k < 32 / RPI; ++k) {
+                const int rr = lane / CH + RPI * k, m = 32 * i + rr;
+                const uint4 v = *reinterpret_cast<const uint4*>(st + rr * S::ROWB + ((cl ^ (rr & (CH - 1))) * 16));
+                if (m >= rows || c >= cols) continue;
+                if constexpr (F32) {
+                    float* o = static_cast<float*>(out) + (int64_t)m * ld + c;
+                    f32x4 f = __builtin_bit_cast(f32x4, v);
+                    if (beta != 0.0f) f = f + beta * *reinterpret_cast<const f32x4*>(o);
+                    st16_nt(o, __builtin_bit_cast(uint4, f));
+                } else {
+                    st16_nt(static_cast<uint16_t*>(out) + (int64_t)m * ld + c, v);
+                }
+            }
+            wave_lds_fence();
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads();
-    }
-    const int m = m0 + wm + (lane & 31);
-    if (m >= M) return;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int c = c0 + wc + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-        if (c >= C) continue;
-        const int64_t at = (int64_t)m * p.ldy + c;
-        if constexpr (OP == LINEAR_DW) {
-            float* y = static_cast<float*>(p.y) + at;
-            *y = p.beta != 0.0f ? p.beta * *y + acc[r] : acc[r];
+}
+
+// Writes a unit's wave outputs: to the result or, SPLIT, as a partial tile
+// (fp32; bf16 results' partial tiles leave from the registers, whose LDS holds
+// no fp32 rows).
+template <int TILE, bool F32, int JS, bool SPLIT>
+__device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64], uint8_t* st, const LinearParams& p,
+                                            const Unit& u, int M, int C, int wrow, int wcol) {
+    constexpr int WT = TILE / 2;
+    const int rows = M - u.m0 - wrow, cols = C - u.c0 - wcol;
+    if (rows <= 0 || cols <= 0) return;
+    if constexpr (SPLIT) {
+        float* o = p.part + (int64_t)u.part * TILE * TILE + wrow * TILE + wcol;
+        if constexpr (F32) {
+            store_wave<WT, true, JS>(acc, st, o, TILE, rows, cols, 0.0f);
         } else {
-            uint16_t* y = static_cast<uint16_t*>(p.y) + at;
-            *y = f2bf(p.beta != 0.0f ? p.beta * bf1(*y) + acc[r] : acc[r]);
+            const int lane = threadIdx.x & 63;
+#pragma unroll
+            for (int i = 0; i < WT / 32; ++i) {
+                const int m = 32 * i + (lane & 31);
+#pragma unroll
+                for (int j = 0; j < WT / 32; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int c = 32 * j + 8 * q + 4 * (lane >> 5);
+                        if (m < rows && c < cols)
+                            *reinterpret_cast<f32x4*>(o + m * TILE + c) = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1],
+                                                                               acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    }
+            }
         }
+    } else {
+        const int64_t at = (int64_t)(u.m0 + wrow) * p.ldy + u.c0 + wcol;
+        if constexpr (F32) store_wave<WT, true, JS>(acc, st, static_cast<float*>(p.y) + at, p.ldy, rows, cols, p.beta);
+        else store_wave<WT, false, JS>(acc, st, static_cast<uint16_t*>(p.y) + at, p.ldy, rows, cols, p.beta);
+    }
+}
+
+// ---- forward -------------------------------------------------------------------
+// Per K = 64 step: activations [TILE rows][64] bf16 in a ring of 3 (rows of
+// 128 bytes, 16-byte chunks XOR-swizzled by row / 2), codes [TILE rows][32
+// bytes] and scales [2 blocks][TILE] in a ring of 2. Step s loads the codes of
+// step s + 1 and the activations of step s + 2, spread over its MFMAs.
+template <int TILE>
+struct Fwd {
+    static constexpr int WT = TILE / 2, MI = WT / 32;
+    static constexpr int A_BYTES = TILE * 128, A_LOADS = A_BYTES / 4096;  // 1 KiB loads per wave
+    static constexpr int Q_BYTES = TILE * 32, Q_LOADS = Q_BYTES / 4096;
+    static constexpr int B_BYTES = Q_BYTES + 1024;  // codes, then scales (2 * TILE bytes of a 1 KiB load)
+    static constexpr int A0 = 0, B0 = 3 * A_BYTES, ST0 = B0 + 2 * B_BYTES;
+    static constexpr int LDS = ST0 + 4 * Stage<false, MI>::BYTES;
+    static constexpr int WGS = TILE == 256 ? 1 : 2;
+    static_assert(LDS * WGS <= 160 * 1024, "LDS");
+};
+
+template <int TILE, bool SPLIT>
+__global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(LinearParams p, LinearPlan pl) {
+    using G = Fwd<TILE>;
+    constexpr int MI = G::MI, WT = G::WT;
+    __shared__ uint4 lds_raw[G::LDS / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const uint32_t lds0 = lds_u32(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT;
+    const int K = p.K;
+
+    Unit u;
+    int vb = blockIdx.x;
+    if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) return;
+
+    // ---- load cursors: the unit and step that the next loads belong to. Past
+    // the last unit they stay on its last step (loaded again, never used).
+    uint32_t a_off[G::A_LOADS], q_off[G::Q_LOADS];
+    const uint8_t *a_base = nullptr, *q_base = nullptr, *sc_ptr = nullptr;
+    Unit ua = u, ub = u;
+    int vba = vb, vbb = vb, ka = u.kbeg, kb = u.kbeg;
+    auto set_a = [&]() {
+        a_base = reinterpret_cast<const uint8_t*>(p.x + (int64_t)ua.m0 * p.ldx);
+#pragma unroll
+        for (int i = 0; i < G::A_LOADS; ++i) {
+            const int r = 8 * (wave * G::A_LOADS + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+            a_off[i] = (uint32_t)min(r, p.T - 1 - ua.m0) * (uint32_t)(p.ldx * 2) + c * 16;
+        }
+    };
+    auto set_b = [&]() {
+        q_base = p.w + (int64_t)ub.c0 * (K / 2);
+#pragma unroll
+        for (int i = 0; i < G::Q_LOADS; ++i) {
+            const int s = (wave * G::Q_LOADS + i) * 64 + lane, m = s >> 1, half = (s & 1) ^ ((m >> 3) & 1);
+            q_off[i] = (uint32_t)min(m, p.N - 1 - ub.c0) * (uint32_t)(K / 2) + half * 16;
+        }
+        constexpr int G16 = TILE / 16;
+        sc_ptr = p.ws + (int64_t)((lane / G16) & 1) * p.wlds + min(ub.c0 + 16 * (lane % G16), p.N - 16);
+    };
+    set_a();
+    set_b();
+    int sla = 0, slb = 0;  // ring slots of the next loads
+    auto load_a = [&](int i) {
+        dma16s(uniform(a_base + (int64_t)ka * 2), a_off[i], lds0 + G::A0 + sla * G::A_BYTES + (wave * G::A_LOADS + i) * 1024);
+    };
+    auto load_b = [&](int i) {
+        const uint32_t at = lds0 + G::B0 + slb * G::B_BYTES;
+        if (i < G::Q_LOADS) dma16s(uniform(q_base + kb / 2), q_off[i], at + (wave * G::Q_LOADS + i) * 1024);
+        else dma16v(sc_ptr + (int64_t)(kb / 32) * p.wlds, at + G::Q_BYTES);
+    };
+    auto next_a = [&]() {
+        sla = sla == 2 ? 0 : sla + 1;
+        if (ka + 64 < ua.kend) {
+            ka += 64;
+        } else {
+            Unit n;
+            if (unit_at<TILE, SPLIT>(pl, K, vba + gridDim.x, n)) {
+                vba += gridDim.x;
+                ua = n;
+                ka = n.kbeg;
+                set_a();
+            }
+        }
+    };
+    auto next_b = [&]() {
+        slb ^= 1;
+        if (kb + 64 < ub.kend) {
+            kb += 64;
+        } else {
+            Unit n;
+            if (unit_at<TILE, SPLIT>(pl, K, vbb + gridDim.x, n)) {
+                vbb += gridDim.x;
+                ub = n;
+                kb = n.kbeg;
+                set_b();
+            }
+        }
+    };
+
+    // ---- fragments -----------------------------------------------------------
+    struct Frag {
+        uint4 a[MI], b[MI];
+    };
+    auto load_frag = [&](Frag& f, int sa, int sb, int s) {
+        const uint8_t* ta = lds + G::A0 + sa * G::A_BYTES;
+        const uint8_t* tb = lds + G::B0 + sb * G::B_BYTES;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int r = wrow + 32 * i + (lane & 31), c = (2 * s + (lane >> 5)) ^ ((r >> 1) & 7);
+            f.a[i] = *reinterpret_cast<const uint4*>(ta + r * 128 + c * 16);
+        }
+        // lane: 8 codes k = 16 s + 8 (lane / 32) .. + 7 of row lane % 32
+        const int blk = s >> 1, within = (8 * s + 4 * (lane >> 5)) & 15;
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+            const int r = wcol + 32 * j + (lane & 31);
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(tb + r * 32 + ((blk ^ ((r >> 3) & 1)) * 16) + within);
+            f.b[j] = expand_fp4(w, e8m0_value(tb[G::Q_BYTES + blk * TILE + r]));
+        }
+    };
+    f32x16 acc[MI][MI];
+    constexpr int ND = G::A_LOADS + G::Q_LOADS + 1;
+    // MFMAs of one k16 step with loads [d0, d0 + dn) spread over them
+    auto mma = [&](const Frag& f, int d0, int dn) {
+        constexpr int NM = MI * MI;
+        int dq = 0;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < MI; ++j) {
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.b[j]),
+                                                                    __builtin_bit_cast(bf16x8, f.a[i]), acc[i][j], 0, 0, 0);
+                const int q = i * MI + j;
+#pragma unroll
+                for (int rep = 0; rep < 4; ++rep)
+                    if (dq < dn && (q + 1) * dn >= (dq + 1) * NM) {
+                        const int d = d0 + dq;
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (d <= G::Q_LOADS) load_b(d);
+                        else load_a(d - G::Q_LOADS - 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                        ++dq;
+                    }
+            }
+    };
+
+    // ---- stream ----------------------------------------------------------------
+#pragma unroll
+    for (int i = 0; i < G::A_LOADS; ++i) load_a(i);
+    next_a();
+#pragma unroll
+    for (int i = 0; i <= G::Q_LOADS; ++i) load_b(i);
+    next_b();
+#pragma unroll
+    for (int i = 0; i < G::A_LOADS; ++i) load_a(i);
+    next_a();
+    wait_vm<G::A_LOADS>();
+    lds_barrier();
+    int sa = 0, sb = 0;  // ring slots being multiplied
+    Frag f[2];
+    load_frag(f[0], 0, 0, 0);
+    uint8_t* st = lds + G::ST0 + wave * Stage<false, MI>::BYTES;
+    for (;;) {
+        clear(acc);
+        for (int k = u.kbeg; k < u.kend; k += 64) {
+            load_frag(f[1], sa, sb, 1);
+            mma(f[0], 0, ND / 3);
+            load_frag(f[0], sa, sb, 2);
+            mma(f[1], ND / 3, 2 * ND / 3 - ND / 3);
+            load_frag(f[1], sa, sb, 3);
+            mma(f[0], 2 * ND / 3, ND - 2 * ND / 3);
+            next_b();
+            next_a();
+            // all but the last activation loads: the next step is whole in LDS
+            wait_vm<G::A_LOADS>();
+            lds_barrier();
+            sa = sa == 2 ? 0 : sa + 1;
+            sb ^= 1;
+            load_frag(f[0], sa, sb, 0);
+            mma(f[1], 0, 0);
+#pragma unroll
+            for (int q = 0; q < MI * MI / 2; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);  // MFMA
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);  // DS read
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, MI * MI / 2, 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        finish_unit<TILE, false, MI, SPLIT>(acc, st, p, u, p.T, p.N, wrow, wcol);
+        vb += gridDim.x;
+        if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) break;
+        load_frag(f[0], sa, sb, 0);  // again: the fragments' registers served the epilogue
+    }
+    wait_vm<0>();  // no load may land in LDS that the next workgroup owns
+}
+
+// ---- gradients -----------------------------------------------------------------
+// Sub-steps of 32 reduction rows. DX: dY [TILE rows][64] in a ring of 3 as the
+// forward's activations, half of a K = 64 tile loaded per sub-step. DW: dY
+// [32 t][TILE n] in a ring of 4, 16-byte chunks XOR-swizzled by 4 (t % 4).
+// Raw codes [32][TILE] and scales [TILE / 32][32] in a ring of 3, bf16 tiles
+// [32][TILE] (swizzled as DW's dY) in a ring of 2. Sub-step i multiplies tile
+// i, expands raw i + 1, and loads raw i + 3 and the activations of sub-steps
+// 4 (DX) or 3 (DW) ahead.
+template <int OP, int TILE>
+struct Grad {
+    static constexpr bool DW = OP == LINEAR_DW;
+    static constexpr int WT = TILE / 2, MI = WT / 32;
+    static constexpr int A_BYTES = DW ? TILE * 64 : TILE * 128, A_SLOTS = DW ? 4 : 3;
+    static constexpr int A_LOADS = TILE * 64 / 4096;  // 1 KiB loads per wave and sub-step
+    static constexpr int CB = DW ? 8 : 4;             // code bytes of 8 columns
+    static constexpr int ROWQ = TILE / 8 * CB;        // code bytes per raw row
+    static constexpr int Q_BYTES = 32 * ROWQ;
+    static constexpr int Q_LOADS = (Q_BYTES + 4095) / 4096;
+    static constexpr int R_BYTES = Q_BYTES + 256;     // codes, then scales
+    static constexpr int B_BYTES = TILE * 64;
+    static constexpr int A0 = 0, B0 = A_SLOTS * A_BYTES, R0 = B0 + 2 * B_BYTES, ST0 = R0 + 3 * R_BYTES;
+    static constexpr int STB = Stage<DW, MI / 2>::BYTES;
+    static constexpr int LDS = ST0 + 4 * STB;
+    static constexpr int WGS = TILE == 256 ? 1 : 2;
+    static_assert(LDS * WGS <= 160 * 1024, "LDS");
+};
+
+
+template <int OP, int TILE, bool SPLIT>
+__global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel(LinearParams p, LinearPlan pl) {
+    using G = Grad<OP, TILE>;
+    constexpr bool DW = G::DW;
+    constexpr int MI = G::MI, WT = G::WT;
+    __shared__ uint4 lds_raw[G::LDS / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const uint32_t lds0 = lds_u32(lds);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT;
+    const int M = DW ? p.N : p.T, C = p.K, R = DW ? p.T : p.N;
+    const int64_t rowq = DW ? p.K : p.K / 2;  // code bytes per row of the weights / checkpoint
+
+    Unit u;
+    int vb = blockIdx.x;
+    if (!unit_at<TILE, SPLIT>(pl, R, vb, u)) return;
+
+    // ---- cursors: unit and reduction row of the activations and raw codes
+    // loaded next, and of the raw codes expanded next
+    struct Cursor {
+        Unit u;
+        int vb, k;
+    };
+    Cursor ca{u, vb, u.kbeg}, cq{u, vb, u.kbeg}, ce{u, vb, u.kbeg};
+    // 32 rows on (a unit's sub-steps fill its K = 64 steps); true: a new unit.
+    // Past the last unit the cursor stays on its last sub-step.
+    auto advance = [&](Cursor& c) {
+        if (c.k + 32 < c.u.kbeg + ((c.u.kend - c.u.kbeg + 63) & ~63)) {
+            c.k += 32;
+            return false;
+        }
+        Unit n;
+        if (!unit_at<TILE, SPLIT>(pl, R, c.vb + gridDim.x, n)) return false;
+        c.vb += gridDim.x;
+        c.u = n;
+        c.k = n.kbeg;
+        return true;
+    };
+    constexpr int NA = DW ? G::A_LOADS : 2 * G::A_LOADS;
+    uint32_t a_off[NA], q_off[G::Q_LOADS];
+    const uint8_t* sc_ptr = nullptr;
+    // DW: reduction row and chunk of the lane in load i of a 32-row tile
+    constexpr int AC = TILE / 8;  // chunks per row
+    auto set_a = [&]() {
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            if constexpr (DW) {
+                const int k = (64 / AC) * (wave * G::A_LOADS + i) + lane / AC, c = (lane % AC) ^ (4 * (k & 3));
+                a_off[i] = (uint32_t)k * (uint32_t)(p.ldx * 2) + (uint32_t)min(c * 8, p.N - 8 - ca.u.m0) * 2;
+            } else {
+                const int r = 8 * (wave * NA + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+                a_off[i] = (uint32_t)min(r, p.T - 1 - ca.u.m0) * (uint32_t)(p.ldx * 2) + c * 16;
+            }
+        }
+    };
+    constexpr int PPR = G::ROWQ / 16;             // 16-byte pieces per raw row
+    constexpr int QL = G::Q_BYTES / 1024;         // wave loads of a raw tile (fewer than the waves: loaded twice)
+    auto set_q = [&]() {
+#pragma unroll
+        for (int i = 0; i < G::Q_LOADS; ++i) {
+            const int s = ((wave * G::Q_LOADS + i) % QL) * 64 + lane;
+            const int64_t col = (int64_t)cq.u.c0 * G::CB / 8 + (s % PPR) * 16;
+            q_off[i] = (uint32_t)((s / PPR) * rowq + (col < rowq - 16 ? col : rowq - 16));
+        }
+        sc_ptr = p.ws + (int64_t)min(cq.u.c0 / 32 + (lane >> 3), p.K / 32 - 1) * p.wlds;
+    };
+    set_a();
+    set_q();
+    int sla = 0, slq = 0;  // ring slots of the next loads
+    const int last_sc = (int)(p.wlds < 0x7fffffff ? p.wlds : 0x7fffffff) - 4;
+    auto load_q = [&]() {
+        const uint32_t at = lds0 + G::R0 + slq * G::R_BYTES;
+        const uint8_t* base = uniform(p.w + cq.k * rowq);
+        if (cq.k + 32 <= cq.u.kend) {
+#pragma unroll
+            for (int i = 0; i < G::Q_LOADS; ++i) dma16s(base, q_off[i], at + ((wave * G::Q_LOADS + i) % QL) * 1024);
+        } else {  // rows past the end are zeros
+#pragma unroll
+            for (int i = 0; i < G::Q_LOADS; ++i) {
+                const int row = (((wave * G::Q_LOADS + i) % QL) * 64 + lane) / PPR;
+                const void* g = cq.k + row < cq.u.kend ? (const void*)(base + q_off[i]) : (const void*)zero_piece;
+                dma16v(g, at + ((wave * G::Q_LOADS + i) % QL) * 1024);
+            }
+        }
+        dma4v(sc_ptr + min(cq.k + 4 * (lane & 7), last_sc), at + G::Q_BYTES);
+        slq = slq == 2 ? 0 : slq + 1;
+        if (advance(cq)) set_q();
+    };
+    auto load_a = [&](int half) {  // half: DX, which half of the K = 64 tile
+        const uint32_t at = lds0 + G::A0 + sla * G::A_BYTES;
+        if constexpr (DW) {
+            const uint8_t* base = uniform(p.x + (int64_t)ca.k * p.ldx + ca.u.m0);
+            if (ca.k + 32 <= ca.u.kend) {
+#pragma unroll
+                for (int i = 0; i < G::A_LOADS; ++i) dma16s(base, a_off[i], at + (wave * G::A_LOADS + i) * 1024);
+            } else {
+#pragma unroll
+                for (int i = 0; i < G::A_LOADS; ++i) {
+                    const int k = (64 / AC) * (wave * G::A_LOADS + i) + lane / AC;
+                    const void* g = ca.k + k < ca.u.kend ? (const void*)(base + a_off[i]) : (const void*)zero_piece;
+                    dma16v(g, at + (wave * G::A_LOADS + i) * 1024);
+                }
+            }
+            sla = (sla + 1) & 3;
+        } else {
+            const int k64 = ca.k - 32 * half;  // first reduction row of the tile
+            const uint8_t* base = uniform(p.x + (int64_t)ca.u.m0 * p.ldx + k64);
+            if (k64 + 64 <= ca.u.kend) {
+#pragma unroll
+                for (int i = 0; i < G::A_LOADS; ++i) {
+                    const int ii = half * G::A_LOADS + i;
+                    dma16s(base, a_off[ii], at + (wave * NA + ii) * 1024);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < G::A_LOADS; ++i) {
+                    const int ii = half * G::A_LOADS + i;
+                    const int r = 8 * (wave * NA + ii) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+                    const void* g = k64 + 8 * c < ca.u.kend ? (const void*)(base + a_off[ii]) : (const void*)zero_piece;
+                    dma16v(g, at + (wave * NA + ii) * 1024);
+                }
+            }
+            if (half == 1) sla = sla == 2 ? 0 : sla + 1;
+        }
+        if (advance(ca)) set_a();
+    };
+    // Raw slot sr of the expand cursor's rows into bf16 slot sb.
+    auto expand = [&](int sr, int sb) {
+        const uint8_t* raw = lds + G::R0 + sr * G::R_BYTES;
+        uint8_t* out = lds + G::B0 + sb * G::B_BYTES;
+        const int c = tid % AC, r0 = tid / AC;
+        const int valid = ce.u.kend - ce.k;
+#pragma unroll
+        for (int q = 0; q < 32 * AC / 256; ++q) {
+            const int row = r0 + q * (256 / AC);
+            const float sc = row < valid ? e8m0_value(raw[G::Q_BYTES + (c >> 2) * 32 + row]) : 1.0f;
+            uint4 v;
+            if constexpr (DW) v = expand_fp8(*reinterpret_cast<const uint2*>(raw + row * G::ROWQ + c * 8), sc);
+            else v = expand_fp4(*reinterpret_cast<const uint32_t*>(raw + row * G::ROWQ + c * 4), sc);
+            *reinterpret_cast<uint4*>(out + row * (TILE * 2) + ((c ^ (4 * (row & 3))) * 16)) = v;
+        }
+        advance(ce);
+    };
+
+    // ---- fragments -----------------------------------------------------------
+    struct Frag {
+        uint4 a[MI], b[MI];
+    };
+    // 8 reduction rows 16 s + 8 (lane / 32) .. of column cbase + lane % 32, from
+    // a row-contiguous tile: inside each 16-lane group, lane r points at row
+    // k0 + r / 4, columns c0 + 4 (r % 4) .. + 3, and lane i receives column
+    // c0 + i of rows k0 .. k0 + 3
+    auto read_across = [&](const uint8_t* t, int cbase, int s) {
+        const int g = lane >> 4, r = lane & 15;
+        const int col = cbase + 16 * (g & 1) + 4 * (r & 3);
+        uint32_t w[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = 16 * s + 8 * (g >> 1) + (r >> 2) + 4 * h;
+            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(t + k * (TILE * 2) + (((col >> 3) ^ (4 * (k & 3))) * 16) + (col & 7) * 2));
+            w[2 * h] = (uint32_t)(uint16_t)v[0] | ((uint32_t)(uint16_t)v[1] << 16);
+            w[2 * h + 1] = (uint32_t)(uint16_t)v[2] | ((uint32_t)(uint16_t)v[3] << 16);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    // k16 step s of the sub-step in activation slot sa (DX: half `half` of it)
+    // and bf16 slot sb
+    auto load_frag = [&](Frag& f, int sa, int half, int sb, int s) {
+        const uint8_t* ta = lds + G::A0 + sa * G::A_BYTES;
+        const uint8_t* tb = lds + G::B0 + sb * G::B_BYTES;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            if constexpr (DW) {
+                f.a[i] = read_across(ta, wrow + 32 * i, s);
+            } else {
+                const int r = wrow + 32 * i + (lane & 31), c = (2 * (2 * half + s) + (lane >> 5)) ^ ((r >> 1) & 7);
+                f.a[i] = *reinterpret_cast<const uint4*>(ta + r * 128 + c * 16);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < MI; ++j) f.b[j] = read_across(tb, wcol + 32 * j, s);
+    };
+    f32x16 acc[MI][MI];
+    auto mma = [&](const Frag& f) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < MI; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.b[j]),
+                                                                    __builtin_bit_cast(bf16x8, f.a[i]), acc[i][j], 0, 0, 0);
+    };
+
+    // ---- stream ----------------------------------------------------------------
+    load_q();
+    load_q();
+    load_q();
+    load_a(0);
+    load_a(1);
+    load_a(0);
+    if constexpr (!DW) load_a(1);
+    wait_vm<0>();
+    lds_barrier();
+    expand(0, 0);
+    lds_barrier();
+    int sa = 0, sr = 1;  // activation slot multiplied, raw slot expanded next
+    Frag f[2];
+    load_frag(f[0], 0, 0, 0, 0);
+    uint8_t* st = lds + G::ST0 + wave * G::STB;
+    for (;;) {
+        clear(acc);
+        for (int k = u.kbeg; k < u.kend; k += 64) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                load_frag(f[1], sa, h, h, 1);
+                load_q();
+                load_a(h);
+                __builtin_amdgcn_sched_barrier(0);
+                expand(sr, h ^ 1);
+                sr = sr == 2 ? 0 : sr + 1;
+                __builtin_amdgcn_sched_barrier(0);
+                mma(f[0]);
+                // Outstanding at most: the activations of the last sub-step
+                // and all loads of this one. The next sub-step's activations
+                // and the raw codes it expands are in LDS.
+                wait_vm<2 * G::A_LOADS + G::Q_LOADS + 1>();
+                lds_barrier();
+                if (DW || h == 1) sa = sa == G::A_SLOTS - 1 ? 0 : sa + 1;
+                load_frag(f[0], sa, h ^ 1, h ^ 1, 0);
+                mma(f[1]);
+            }
+        }
+        finish_unit<TILE, DW, MI / 2, SPLIT>(acc, st, p, u, M, C, wrow, wcol);
+        vb += gridDim.x;
+        if (!unit_at<TILE, SPLIT>(pl, R, vb, u)) break;
+        load_frag(f[0], sa, 0, 0, 0);  // again: the fragments' registers served the epilogue
+    }
+    wait_vm<0>();  // no load may land in LDS that the next workgroup owns
+}
+
+// ---- both operands in MXFP4 ------------------------------------------------------
+// 128 x 128 outputs on the scaled matrix instruction, which takes 32 codes of
+// a row and their scale byte from each lane: 32 x 32 outputs over K = 64. Steps
+// of K = 256 make 128-byte row segments (a CU takes a 1 KiB load of those in
+// half the time of 64-byte ones). Ring of 2: codes of both operands [128
+// rows][128 bytes], chunks XOR-swizzled by row / 2, and scales [8 blocks][128]
+// each. A unit's first step is loaded before the previous unit's epilogue,
+// which stages through the other slot; two workgroups per CU, so that one's
+// output stores (what bounds a large product: at K = 1024 an output byte for
+// every byte of codes) drain while the other multiplies.
+struct Mx {
+    static constexpr int TILE = 128, WT = 64, MI = 2;
+    static constexpr int CODES = TILE * 128, LOADS = CODES / 4096;  // per operand; 1 KiB loads per wave
+    static constexpr int SLOT = 2 * CODES + 2048;
+    static constexpr int LDS = 2 * SLOT;
+};
+
+template <bool SPLIT>
+__global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, LinearPlan pl) {
+    using G = Mx;
+    constexpr int MI = G::MI, WT = G::WT, TILE = G::TILE;
+    __shared__ uint4 lds_raw[G::LDS / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const uint32_t lds0 = lds_u32(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT;
+    const int K = p.K;
+    Unit u;
+    int vb = blockIdx.x;
+    if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) return;
+
+    // Step k of unit n into slot `slot`. Pieces past the row's end are clamped
+    // into it (they are not multiplied), rows past the operand's too.
+    auto load_step = [&](const Unit& n, int k, int slot) {
+        const uint32_t at = lds0 + slot * G::SLOT;
+        const uint8_t* ba = uniform(p.xq + (int64_t)n.m0 * (K / 2));
+        const uint8_t* bw = uniform(p.w + (int64_t)n.c0 * (K / 2));
+#pragma unroll
+        for (int i = 0; i < G::LOADS; ++i) {
+            const int q = wave * G::LOADS + i, r = 8 * q + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+            const uint32_t col = (uint32_t)min(k / 2 + c * 16, K / 2 - 16);
+            dma16s(ba, (uint32_t)min(r, p.T - 1 - n.m0) * (uint32_t)(K / 2) + col, at + q * 1024);
+            dma16s(bw, (uint32_t)min(r, p.N - 1 - n.c0) * (uint32_t)(K / 2) + col, at + G::CODES + q * 1024);
+        }
+        // waves 0 and 1: the scales of X and W; 2 and 3 the same again
+        const int64_t blk = min(k / 32 + (lane >> 3), K / 32 - 1);
+        const int row = 16 * (lane & 7);
+        const uint8_t* sx = p.xs + blk * p.xlds + min((int64_t)n.m0 + row, p.xlds - 16);
+        const uint8_t* sw = p.ws + blk * p.wlds + min((int64_t)n.c0 + row, p.wlds - 16);
+        dma16v((wave & 1) ? sw : sx, at + 2 * G::CODES + (wave & 1) * 1024);
+    };
+    f32x16 acc[MI][MI];
+    clear(acc);
+    int slot = 0;
+    load_step(u, u.kbeg, 0);
+    for (;;) {
+        Unit n = u;
+        const bool more = unit_at<TILE, SPLIT>(pl, K, vb + gridDim.x, n);
+        for (int k = u.kbeg; k < u.kend; k += 256) {
+            wait_vm<0>();
+            lds_barrier();  // step k is whole in LDS, and the other slot is read
+            if (k + 256 < u.kend) load_step(u, k + 256, slot ^ 1);
+            else if (more) load_step(n, n.kbeg, slot ^ 1);
+            const uint8_t* st = lds + slot * G::SLOT;
+            const int groups = min(4, (u.kend - k) / 64);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (g >= groups) break;
+                i32x8 a[MI], b[MI];
+                int as[MI], bs[MI];
+                const int blk = 2 * g + (lane >> 5);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const int ra = wrow + 32 * i + (lane & 31), rb = wcol + 32 * i + (lane & 31);
+                    const i32x4 va = *reinterpret_cast<const i32x4*>(st + ra * 128 + ((blk ^ ((ra >> 1) & 7)) * 16));
+                    const i32x4 vw = *reinterpret_cast<const i32x4*>(st + G::CODES + rb * 128 + ((blk ^ ((rb >> 1) & 7)) * 16));
+                    a[i] = __builtin_shufflevector(va, va, 0, 1, 2, 3, -1, -1, -1, -1);
+                    b[i] = __builtin_shufflevector(vw, vw, 0, 1, 2, 3, -1, -1, -1, -1);
+                    as[i] = st[2 * G::CODES + blk * 128 + ra];
+                    bs[i] = st[2 * G::CODES + 1024 + blk * 128 + rb];
+                }
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < MI; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 4, 4, 0, bs[j], 0, as[i]);
+            }
+            slot ^= 1;
+        }
+        lds_barrier();  // the last step's slot is read: the epilogue stages there
+        finish_unit<TILE, false, MI, SPLIT>(acc, lds + (slot ^ 1) * G::SLOT + wave * Stage<false, MI>::BYTES, p, u, p.T, p.N,
+                                            wrow, wcol);
+        if (!more) break;
+        u = n;
+        vb += gridDim.x;
+        clear(acc);
+    }
+}
+
+// ---- the last round's sums ------------------------------------------------------
+// Tail tile j is the sum of its partial tiles in part order, plus beta times
+// what is there, rounded once. A thread takes 4 columns of a row.
+template <int TILE, bool F32>
+__global__ __launch_bounds__(256) void linear_fixup_kernel(LinearParams p, LinearPlan pl, int M, int C) {
+    constexpr int TPR = TILE / 4, RPW = 256 / TPR, SLABS = TILE / RPW;
+    const int j = blockIdx.x / SLABS, slab = blockIdx.x % SLABS;
+    int mt, ct;
+    tile_at(pl, pl.whole + j, mt, ct);
+    const int r = slab * RPW + threadIdx.x / TPR, c = (threadIdx.x % TPR) * 4;
+    const int m = mt * TILE + r, col = ct * TILE + c;
+    if (m >= M || col >= C) return;
+    const float* src = p.part + (int64_t)j * pl.parts * TILE * TILE + r * TILE + c;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q0 = 0; q0 < pl.parts; q0 += 8) {  // up to 8 loads in flight
+        f32x4 v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const f32x4*>(src + (int64_t)min(q0 + q, pl.parts - 1) * TILE * TILE);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q0 + q < pl.parts) sum = sum + v[q];
+    }
+    const int64_t at = (int64_t)m * p.ldy + col;
+    if constexpr (F32) {
+        f32x4* y = reinterpret_cast<f32x4*>(static_cast<float*>(p.y) + at);
+        if (p.beta != 0.0f) sum = sum + p.beta * *y;
+        *y = sum;
+    } else {
+        uint2* y = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at);
+        if (p.beta != 0.0f) {
+            const uint2 old = *y;
+            sum = sum + p.beta * f32x4{bf_lo(old.x), bf_hi(old.x), bf_lo(old.y), bf_hi(old.y)};
+        }
+        *y = make_uint2(pack_bf2(sum[0], sum[1]), pack_bf2(sum[2], sum[3]));
+    }
+}
+
+// dW = beta dW: the weight gradient over no tokens.
+__global__ __launch_bounds__(256) void linear_scale_kernel(float* y, int64_t ldy, int rows, int cols, float beta) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int r = (int)(i / cols), c = (int)(i % cols);
+    if (r >= rows) return;
+    float* o = y + (int64_t)r * ldy + c;
+    *o = beta != 0.0f ? beta * *o : 0.0f;
+}
+
+struct Sizes {
+    int M, C, R;  // output rows and columns, reduction length
+};
+Sizes sizes(LinearOp op, int T, int N, int K) {
+    if (op == LINEAR_DX) return {T, K, N};
+    if (op == LINEAR_DW) return {N, K, T};
+    return {T, N, K};
+}
+
+// Workgroups that run at a time.
+int64_t tile_slots(int tile) { return (int64_t)cu_count() * (tile == 256 ? 1 : 2); }
+
+constexpr int kMinSteps = 8;  // K = 64 steps that a part of a split reduction has at least
+
+LinearPlan plan_tiles(const Sizes& z, int tile) {
+    LinearPlan pl;
+    pl.tile = tile;
+    pl.tiles_m = (z.M + tile - 1) / tile;
+    pl.tiles_c = (z.C + tile - 1) / tile;
+    const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_c;
+    const int64_t slots = tile_slots(tile);
+    const int64_t whole = tiles / slots * slots, rest = tiles - whole;
+    const int nk = (z.R + 63) / 64;
+    const int64_t parts = rest > 0 ? std::min<int64_t>(slots / rest, nk / kMinSteps) : 1;
+    pl.whole = (int)tiles;
+    if (parts >= 2) {
+        pl.whole = (int)whole;
+        pl.tail = (int)rest;
+        pl.chunk = (int)((nk + 4 * parts - 1) / (4 * parts)) * 256;  // whole steps of every kernel
+        pl.parts = (nk * 64 + pl.chunk - 1) / pl.chunk;
+    }
+    return pl;
+}
+
+LinearPlan linear_plan(LinearOp op, int T, int N, int K) {
+    const Sizes z = sizes(op, T, N, K);
+    const int64_t t256 = (int64_t)((z.M + 255) / 256) * ((z.C + 255) / 256);
+    if (op == LINEAR_MATMUL) return plan_tiles(z, 128);
+    return plan_tiles(z, t256 >= cu_count() / 2 ? 256 : 128);
+}
+
+template <int OP, int TILE, bool SPLIT>
+void launch_units(const LinearParams& p, const LinearPlan& pl, int units, hipStream_t s) {
+    const int grid = std::min((units + 7) & ~7, (int)tile_slots(TILE) & ~7);
+    if constexpr (OP == LINEAR_MATMUL) linear_mx_kernel<SPLIT><<<grid, 256, 0, s>>>(p, pl);
+    else if constexpr (OP == LINEAR_FORWARD) linear_fwd_kernel<TILE, SPLIT><<<grid, 256, 0, s>>>(p, pl);
+    else linear_grad_kernel<OP, TILE, SPLIT><<<grid, 256, 0, s>>>(p, pl);
+}
+template <int OP, int TILE>
+void launch_tiles(const LinearParams& p, const LinearPlan& pl, hipStream_t s) {
+    if (pl.whole > 0) launch_units<OP, TILE, false>(p, pl, pl.whole, s);
+    if (pl.tail > 0) {
+        launch_units<OP, TILE, true>(p, pl, pl.tail * pl.parts, s);
+        constexpr int SLABS = TILE / (256 / (TILE / 4));
+        const Sizes z = sizes((LinearOp)OP, p.T, p.N, p.K);
+        linear_fixup_kernel<TILE, OP == LINEAR_DW><<<pl.tail * SLABS, 256, 0, s>>>(p, pl, z.M, z.C);
     }
 }
 
 }  // namespace
 
-size_t linear_workspace(LinearOp, int, int, int) { return 0; }
+// An upper bound over all token counts up to T, so that a workspace for T
+// serves fewer: tail tiles times parts fill at most the workgroup slots, and
+// neither tiles nor parts fall with T.
+size_t linear_workspace(LinearOp op, int T, int N, int K) {
+    const Sizes z = sizes(op, T, N, K);
+    size_t most = 0;
+    for (int tile = 128; tile <= 256; tile *= 2) {
+        const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
+        const int64_t parts = (z.R + 63) / 64 / kMinSteps;
+        if (parts < 2) continue;
+        const int64_t units = std::min(tiles * parts, tile_slots(tile));
+        most = std::max(most, (size_t)units * tile * tile * 4);
+    }
+    return most;
+}
 
 hipError_t launch_linear(LinearOp op, const LinearParams& p, hipStream_t s) {
-    const int M = op == LINEAR_DW ? p.N : p.T, C = op == LINEAR_FORWARD || op == LINEAR_MATMUL ? p.N : p.K;
-    const int R = op == LINEAR_DW ? p.T : op == LINEAR_DX ? p.N : p.K;
-    if (M <= 0 || C <= 0) return hipSuccess;
-    const int tc = (C + BT - 1) / BT;
-    const int64_t grid = (int64_t)((M + BT - 1) / BT) * tc;
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    const unsigned g = (unsigned)grid;
+    if (op != LINEAR_DW && p.T <= 0) return hipSuccess;
+    if (op == LINEAR_DW && p.T == 0) {
+        if (p.beta == 1.0f) return hipSuccess;
+        const int64_t n = (int64_t)p.N * p.K;
+        linear_scale_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(static_cast<float*>(p.y), p.ldy, p.N, p.K, p.beta);
+        return hipGetLastError();
+    }
+    const LinearPlan pl = linear_plan(op, p.T, p.N, p.K);
+    const bool big = pl.tile == 256;
     switch (op) {
-        case LINEAR_FORWARD: linear_simple_kernel<LINEAR_FORWARD><<<g, 256, 0, s>>>(p, M, C, R, tc); break;
-        case LINEAR_MATMUL: linear_simple_kernel<LINEAR_MATMUL><<<g, 256, 0, s>>>(p, M, C, R, tc); break;
-        case LINEAR_DX: linear_simple_kernel<LINEAR_DX><<<g, 256, 0, s>>>(p, M, C, R, tc); break;
-        case LINEAR_DW: linear_simple_kernel<LINEAR_DW><<<g, 256, 0, s>>>(p, M, C, R, tc); break;
+        case LINEAR_FORWARD: big ? launch_tiles<LINEAR_FORWARD, 256>(p, pl, s) : launch_tiles<LINEAR_FORWARD, 128>(p, pl, s); break;
+        case LINEAR_MATMUL: launch_tiles<LINEAR_MATMUL, 128>(p, pl, s); break;
+        case LINEAR_DX: big ? launch_tiles<LINEAR_DX, 256>(p, pl, s) : launch_tiles<LINEAR_DX, 128>(p, pl, s); break;
+        case LINEAR_DW: big ? launch_tiles<LINEAR_DW, 256>(p, pl, s) : launch_tiles<LINEAR_DW, 128>(p, pl, s); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
