@@ -254,60 +254,84 @@ def mxfp4_planes(codes, planes, stream=None) -> None:
     _check(load_library().tmt_moe_mxfp4_planes(_stream(stream), _ptr(codes), N, 2 * half, _ptr(planes)))
 
 
-def _rows(what: str, t, dtype) -> tuple:
-    """(pointer, row stride) of a matrix whose rows are contiguous."""
-    if t.dim() != 2 or t.dtype != dtype:
-        raise ValueError(f"{what} must be a matrix of {dtype}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"the rows of {what} must be contiguous")
-    _same_device(what, t)
-    return int(t.data_ptr()), int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
-
-
-def _same_device(what: str, t) -> None:
+def _here(stream) -> tuple:
+    """(index of the current GPU, raw handle of `stream` or of its current stream)."""
     import torch
-    if t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+    dev = torch.cuda.current_device()
+    if stream is None:
+        return dev, torch._C._cuda_getCurrentRawStream(dev)
+    return dev, stream.cuda_stream
+
+
+def _matrix(what: str, t, dtype, dev: int, rows: int, cols: int) -> tuple:
+    """(pointer, row stride) of a [rows, cols] matrix on GPU `dev` whose rows
+    are contiguous."""
+    if t.dtype is not dtype or t.dim() != 2:
+        raise ValueError(f"{what} must be a matrix of {dtype}, not {list(t.shape)} of {t.dtype}")
+    if t.get_device() != dev:
         raise ValueError(f"{what} is on {t.device}, not on the current GPU")
+    if t.shape != (rows, cols):
+        raise ValueError(f"{what} must be [{rows}, {cols}], not {list(t.shape)}")
+    ld, one = t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError(f"the rows of {what} must be contiguous")
+    return t.data_ptr(), ld if rows > 1 else cols
 
 
-def _mx(what: str, codes, scales, rows: int, K: int, fmt: int) -> tuple:
+def _mx(what: str, codes, scales, dev: int, rows: int, K: int, fmt: int) -> tuple:
     """(codes, scales, scale stride) of a microscaled matrix [rows, K]."""
     import torch
-    c, ldc = _rows(f"codes of {what}", codes, torch.uint8)
-    width = K // 2 if fmt == MX_FP4 else K
-    if tuple(codes.shape) != (rows, width) or (rows > 1 and ldc != width):
-        raise ValueError(f"codes of {what} must be a contiguous [{rows}, {width}], not {list(codes.shape)}")
-    s, lds = _rows(f"scales of {what}", scales, torch.uint8)
-    if scales.shape[0] != K // 32 or scales.shape[1] < rows:
+    width = K if fmt == MX_FP8 else K // 2
+    c, ld = _matrix("codes of " + what, codes, torch.uint8, dev, rows, width)
+    if ld != width:
+        raise ValueError(f"the codes of {what} must be contiguous")
+    n = scales.shape[-1]
+    if n < rows:
         raise ValueError(f"scales of {what} must be [{K // 32}, {rows} or more], not {list(scales.shape)}")
+    s, lds = _matrix("scales of " + what, scales, torch.uint8, dev, K // 32, n)
     return c, s, lds
 
 
-def _mx_dtype(what: str, t) -> int:
+def _ws(workspace, dev: int) -> tuple:
+    if workspace is None:
+        return 0, 0
+    if workspace.get_device() != dev:
+        raise ValueError(f"workspace is on {workspace.device}, not on the current GPU")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _mx_rows(X, codes, scales, fmt, stream):
     import torch
-    if t.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{what} must be bfloat16 or float32, not {t.dtype}")
-    return 0 if t.dtype == torch.bfloat16 else 1
+    if X.dtype is torch.bfloat16:
+        dtype = 0
+    elif X.dtype is torch.float32:
+        dtype = 1
+    else:
+        raise ValueError(f"X must be bfloat16 or float32, not {X.dtype}")
+    dev, raw = _here(stream)
+    rows, K = X.shape
+    x, ldx = _matrix("X", X, X.dtype, dev, rows, K)
+    return (raw, dtype, x, ldx, rows, K) + _mx("X", codes, scales, dev, rows, K, fmt)
 
 
 def mx_quantize(X, codes, scales, fmt: int = MX_FP4, stream=None) -> None:
     """X [rows, K] (bf16 or fp32) to microscaled codes ([rows, K/2] for MX_FP4,
     [rows, K] for MX_FP8) and block-major scales [K/32, rows or more], uint8."""
-    dtype = _mx_dtype("X", X)
-    x, ldx = _rows("X", X, X.dtype)
-    rows, K = int(X.shape[0]), int(X.shape[1])
-    c, s, lds = _mx("X", codes, scales, rows, K, fmt)
-    _check(load_library().tmt_moe_mx_quantize(_stream(stream), fmt, dtype, x, ldx, rows, K, c, s, lds))
+    lib = load_library()
+    raw, dtype, x, ldx, rows, K, c, s, lds = _mx_rows(X, codes, scales, fmt, stream)
+    rc = lib.tmt_moe_mx_quantize(raw, fmt, dtype, x, ldx, rows, K, c, s, lds)
+    if rc:
+        _check(rc)
 
 
 def mx_dequantize(codes, scales, X, fmt: int = MX_FP4, stream=None) -> None:
     """The values of codes and scales (as mx_quantize writes them) into
     X [rows, K], bf16 or fp32."""
-    dtype = _mx_dtype("X", X)
-    x, ldx = _rows("X", X, X.dtype)
-    rows, K = int(X.shape[0]), int(X.shape[1])
-    c, s, lds = _mx("X", codes, scales, rows, K, fmt)
-    _check(load_library().tmt_moe_mx_dequantize(_stream(stream), fmt, c, s, lds, rows, K, dtype, x, ldx))
+    lib = load_library()
+    raw, dtype, x, ldx, rows, K, c, s, lds = _mx_rows(X, codes, scales, fmt, stream)
+    rc = lib.tmt_moe_mx_dequantize(raw, fmt, c, s, lds, rows, K, dtype, x, ldx)
+    if rc:
+        _check(rc)
 
 
 def linear_workspace_size(op: int, T: int, N: int, K: int) -> int:
@@ -318,65 +342,55 @@ def linear_workspace_size(op: int, T: int, N: int, K: int) -> int:
     return int(out.value)
 
 
-def _ws(workspace) -> tuple:
-    if workspace is None:
-        return 0, ctypes.c_size_t(0)
-    _same_device("workspace", workspace)
-    return _ptr(workspace), ctypes.c_size_t(workspace.numel() * workspace.element_size())
-
-
-def _shaped(what: str, t, rows: int, cols: int) -> None:
-    if tuple(t.shape) != (rows, cols):
-        raise ValueError(f"{what} must be [{rows}, {cols}], not {list(t.shape)}")
+def _product(fn, T, N, K, x, x_cols, mx, mx_rows, fmt, y, y_rows, y_cols, y_dtype, names, beta, workspace, stream):
+    """One product of a bf16 matrix x with a microscaled one."""
+    import torch
+    dev, raw = _here(stream)
+    xp, ldx = _matrix(names[0], x, torch.bfloat16, dev, T, x_cols)
+    c, s, lds = _mx(names[1], mx[0], mx[1], dev, mx_rows, K, fmt)
+    yp, ldy = _matrix(names[2], y, y_dtype, dev, y_rows, y_cols)
+    ws, size = _ws(workspace, dev)
+    rc = fn(raw, T, N, K, xp, ldx, c, s, lds, yp, ldy, beta, ws, size)
+    if rc:
+        _check(rc)
 
 
 def mxfp4_linear(X, codes, scales, Y, beta: float = 0.0, workspace=None, stream=None) -> None:
     """Y <- beta*Y + X W^T. X [T, K], Y [T, N] bf16; W [N, K] as MXFP4 codes
     [N, K/2] and scales [K/32, N or more] (a multiple of 16)."""
-    import torch
-    x, ldx = _rows("X", X, torch.bfloat16)
-    y, ldy = _rows("Y", Y, torch.bfloat16)
-    T, K, N = int(X.shape[0]), int(X.shape[1]), int(Y.shape[1])
-    _shaped("Y", Y, T, N)
-    c, s, lds = _mx("W", codes, scales, N, K, MX_FP4)
-    _check(load_library().tmt_moe_mxfp4_linear(_stream(stream), T, N, K, x, ldx, c, s, lds, y, ldy,
-                                               ctypes.c_float(beta), *_ws(workspace)))
-
-
-def mxfp4_matmul(X_codes, X_scales, codes, scales, Y, beta: float = 0.0, workspace=None, stream=None) -> None:
-    """Y <- beta*Y + X W^T with X [T, K] and W [N, K] both in MXFP4; Y [T, N] bf16."""
-    import torch
-    y, ldy = _rows("Y", Y, torch.bfloat16)
-    T, N, K = int(Y.shape[0]), int(Y.shape[1]), 2 * int(codes.shape[1])
-    xc, xs, xlds = _mx("X", X_codes, X_scales, T, K, MX_FP4)
-    c, s, lds = _mx("W", codes, scales, N, K, MX_FP4)
-    _check(load_library().tmt_moe_mxfp4_matmul(_stream(stream), T, N, K, xc, xs, xlds, c, s, lds, y, ldy,
-                                               ctypes.c_float(beta), *_ws(workspace)))
+    (T, K), N = X.shape, Y.shape[-1]
+    _product(load_library().tmt_moe_mxfp4_linear, T, N, K, X, K, (codes, scales), N, MX_FP4, Y, T, N, X.dtype,
+             ("X", "W", "Y"), beta, workspace, stream)
 
 
 def mxfp4_linear_dx(dY, codes, scales, dX, beta: float = 0.0, workspace=None, stream=None) -> None:
     """dX <- beta*dX + dY W. dY [T, N], dX [T, K] bf16; W as in mxfp4_linear."""
-    import torch
-    x, ldx = _rows("dY", dY, torch.bfloat16)
-    y, ldy = _rows("dX", dX, torch.bfloat16)
-    T, N, K = int(dY.shape[0]), int(dY.shape[1]), int(dX.shape[1])
-    _shaped("dX", dX, T, K)
-    c, s, lds = _mx("W", codes, scales, N, K, MX_FP4)
-    _check(load_library().tmt_moe_mxfp4_linear_dx(_stream(stream), T, N, K, x, ldx, c, s, lds, y, ldy,
-                                                  ctypes.c_float(beta), *_ws(workspace)))
+    (T, N), K = dY.shape, dX.shape[-1]
+    _product(load_library().tmt_moe_mxfp4_linear_dx, T, N, K, dY, N, (codes, scales), N, MX_FP4, dX, T, K, dY.dtype,
+             ("dY", "W", "dX"), beta, workspace, stream)
 
 
 def mxfp8_linear_dw(dY, codes, scales, dW, beta: float = 0.0, workspace=None, stream=None) -> None:
     """dW <- beta*dW + dY^T X from the MXFP8 checkpoint of X [T, K] (codes [T, K],
     scales [K/32, T or more], a multiple of 16). dY [T, N] bf16, dW [N, K] fp32."""
     import torch
-    x, ldx = _rows("dY", dY, torch.bfloat16)
-    y, ldy = _rows("dW", dW, torch.float32)
-    T, N, K = int(dY.shape[0]), int(dY.shape[1]), int(dW.shape[1])
-    _shaped("dW", dW, N, K)
-    c, s, lds = _mx("X", codes, scales, T, K, MX_FP8)
-    _check(load_library().tmt_moe_mxfp8_linear_dw(_stream(stream), T, N, K, x, ldx, c, s, lds, y, ldy,
-                                                  ctypes.c_float(beta), *_ws(workspace)))
+    (T, N), K = dY.shape, dW.shape[-1]
+    _product(load_library().tmt_moe_mxfp8_linear_dw, T, N, K, dY, N, (codes, scales), T, MX_FP8, dW, N, K,
+             torch.float32, ("dY", "X", "dW"), beta, workspace, stream)
+
+
+def mxfp4_matmul(X_codes, X_scales, codes, scales, Y, beta: float = 0.0, workspace=None, stream=None) -> None:
+    """Y <- beta*Y + X W^T with X [T, K] and W [N, K] both in MXFP4; Y [T, N] bf16."""
+    import torch
+    (T, N), K = Y.shape, 2 * codes.shape[-1]
+    dev, raw = _here(stream)
+    xc, xs, xlds = _mx("X", X_codes, X_scales, dev, T, K, MX_FP4)
+    c, s, lds = _mx("W", codes, scales, dev, N, K, MX_FP4)
+    y, ldy = _matrix("Y", Y, torch.bfloat16, dev, T, N)
+    ws, size = _ws(workspace, dev)
+    rc = load_library().tmt_moe_mxfp4_matmul(raw, T, N, K, xc, xs, xlds, c, s, lds, y, ldy, beta, ws, size)
+    if rc:
+        _check(rc)
 
 
 class MoE:
