@@ -26,6 +26,7 @@
 // ahead into a row-contiguous bf16 tile, and fragments are read from that with
 // the transposing ds_read_b64_tr_b16.
 #include <algorithm>
+#include <cmath>
 
 #include "linear.hpp"
 #include "moe_internal.hpp"
@@ -73,7 +74,7 @@ __device__ __forceinline__ void wait_vm() {
 // also wait for the last unit's output stores.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// 8 e2m1 codes with the scale 2^(s - 127) (or NaN) as 8 bf16.
+// 8 e2m1 codes and their scale operand as 8 bf16.
 __device__ __forceinline__ uint4 expand_fp4(uint32_t w, float sc) {
     return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0)),
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1)),
@@ -163,14 +164,20 @@ __device__ __forceinline__ void clear(f32x16 (&acc)[N][N]) {
 __device__ __forceinline__ void wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // out: the wave's first output element, ld its row stride; rows, cols: valid
-// ones. beta times what is there is added in fp32.
-template <int WT, bool F32, int JS>
+// ones. beta times what is there is added in fp32. NT: results are written
+// once and leave the caches to the operands; partial tiles are read again at
+// once.
+template <int WT, bool F32, int JS, bool NT>
 __device__ __forceinline__ void store_wave(f32x16 (&acc)[WT / 32][WT / 32], uint8_t* st, void* out, int64_t ld, int rows,
                                            int cols, float beta) {
     using S = Stage<F32, JS>;
     constexpr int N = WT / 32;
     constexpr int CH = S::ROWB / 16, RPI = 64 / CH;  // 16-byte chunks per staged row, rows per store
-    const int lane = threadIdx.x & 63, lr = lane & 31;
+    // a value of this unit's own: the addresses below are not kept in registers
+    // through the main loop
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int lr = lane & 31;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -216,7 +223,8 @@ __device__ __forceinline__ void store_wave(f32x16 (&acc)[WT / 32][WT / 32], uint
                     float* o = static_cast<float*>(out) + (int64_t)m * ld + c;
                     f32x4 f = __builtin_bit_cast(f32x4, v);
                     if (beta != 0.0f) f = f + beta * *reinterpret_cast<const f32x4*>(o);
-                    st16_nt(o, __builtin_bit_cast(uint4, f));
+                    if (NT) st16_nt(o, __builtin_bit_cast(uint4, f));
+                    else *reinterpret_cast<f32x4*>(o) = f;
                 } else {
                     st16_nt(static_cast<uint16_t*>(out) + (int64_t)m * ld + c, v);
                 }
@@ -238,7 +246,7 @@ __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64],
     if constexpr (SPLIT) {
         float* o = p.part + (int64_t)u.part * TILE * TILE + wrow * TILE + wcol;
         if constexpr (F32) {
-            store_wave<WT, true, JS>(acc, st, o, TILE, rows, cols, 0.0f);
+            store_wave<WT, true, JS, false>(acc, st, o, TILE, rows, cols, 0.0f);
         } else {
             const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -257,8 +265,8 @@ __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64],
         }
     } else {
         const int64_t at = (int64_t)(u.m0 + wrow) * p.ldy + u.c0 + wcol;
-        if constexpr (F32) store_wave<WT, true, JS>(acc, st, static_cast<float*>(p.y) + at, p.ldy, rows, cols, p.beta);
-        else store_wave<WT, false, JS>(acc, st, static_cast<uint16_t*>(p.y) + at, p.ldy, rows, cols, p.beta);
+        if constexpr (F32) store_wave<WT, true, JS, true>(acc, st, static_cast<float*>(p.y) + at, p.ldy, rows, cols, p.beta);
+        else store_wave<WT, false, JS, true>(acc, st, static_cast<uint16_t*>(p.y) + at, p.ldy, rows, cols, p.beta);
     }
 }
 
@@ -273,7 +281,7 @@ struct Fwd {
     static constexpr int A_BYTES = TILE * 128, A_LOADS = A_BYTES / 4096;  // 1 KiB loads per wave
     static constexpr int Q_BYTES = TILE * 32, Q_LOADS = Q_BYTES / 4096;
     static constexpr int B_BYTES = Q_BYTES + 1024;  // codes, then scales (2 * TILE bytes of a 1 KiB load)
-    static constexpr int A0 = 0, B0 = 3 * A_BYTES, ST0 = B0 + 2 * B_BYTES;
+    static constexpr int A0 = 0, B0 = 3 * A_BYTES, ST0 = B0 + 3 * B_BYTES;
     static constexpr int LDS = ST0 + 4 * Stage<false, MI>::BYTES;
     static constexpr int WGS = TILE == 256 ? 1 : 2;
     static_assert(LDS * WGS <= 160 * 1024, "LDS");
@@ -345,7 +353,7 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
         }
     };
     auto next_b = [&]() {
-        slb ^= 1;
+        slb = slb == 2 ? 0 : slb + 1;
         if (kb + 64 < ub.kend) {
             kb += 64;
         } else {
@@ -363,96 +371,100 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
     struct Frag {
         uint4 a[MI], b[MI];
     };
-    auto load_frag = [&](Frag& f, int sa, int sb, int s) {
-        const uint8_t* ta = lds + G::A0 + sa * G::A_BYTES;
-        const uint8_t* tb = lds + G::B0 + sb * G::B_BYTES;
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int r = wrow + 32 * i + (lane & 31), c = (2 * s + (lane >> 5)) ^ ((r >> 1) & 7);
-            f.a[i] = *reinterpret_cast<const uint4*>(ta + r * 128 + c * 16);
-        }
-        // lane: 8 codes k = 16 s + 8 (lane / 32) .. + 7 of row lane % 32
-        const int blk = s >> 1, within = (8 * s + 4 * (lane >> 5)) & 15;
-#pragma unroll
-        for (int j = 0; j < MI; ++j) {
-            const int r = wcol + 32 * j + (lane & 31);
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(tb + r * 32 + ((blk ^ ((r >> 3) & 1)) * 16) + within);
-            f.b[j] = expand_fp4(w, e8m0_value(tb[G::Q_BYTES + blk * TILE + r]));
-        }
+    struct Raw {  // 8 codes and the scale byte of each row block
+        uint32_t q[MI], s[MI];
     };
+    // k16 step s of the K = 64 step in ring slots sa and sb
+    auto read_a = [&](Frag& f, int i, int sa, int s) {
+        const int r = wrow + 32 * i + (lane & 31), c = (2 * s + (lane >> 5)) ^ ((r >> 1) & 7);
+        f.a[i] = *reinterpret_cast<const uint4*>(lds + G::A0 + sa * G::A_BYTES + r * 128 + c * 16);
+    };
+    // lane: 8 codes k = 16 s + 8 (lane / 32) .. + 7 of row lane % 32
+    auto read_codes = [&](Raw& w, int j, int sb, int s) {
+        const uint8_t* tb = lds + G::B0 + sb * G::B_BYTES;
+        const int blk = s >> 1, within = (8 * s + 4 * (lane >> 5)) & 15, r = wcol + 32 * j + (lane & 31);
+        w.q[j] = *reinterpret_cast<const uint32_t*>(tb + r * 32 + ((blk ^ ((r >> 3) & 1)) * 16) + within);
+        w.s[j] = tb[G::Q_BYTES + blk * TILE + r];
+    };
+    auto expand = [&](Frag& f, const Raw& w, int j) { f.b[j] = expand_fp4(w.q[j], e8m0_operand(w.s[j])); };
     f32x16 acc[MI][MI];
-    constexpr int ND = G::A_LOADS + G::Q_LOADS + 1;
-    // MFMAs of one k16 step with loads [d0, d0 + dn) spread over them
-    auto mma = [&](const Frag& f, int d0, int dn) {
-        constexpr int NM = MI * MI;
-        int dq = 0;
+    constexpr int ND = G::A_LOADS + G::Q_LOADS + 1, NM = MI * MI;
+    // MFMAs of one k16 step. Under them, in the slots between two: the reads of
+    // the next step's fragments (f2: k16 step s of ring slots sa, sb), the
+    // conversion of its codes and loads [d0, d0 + dn). A wave's instructions
+    // issue in order and an MFMA takes 32 cycles, so what stands in one slot
+    // is free up to about seven instructions; in a bunch it stalls the matrix
+    // core (T = N = K = 4096: 1.72 us a step with the conversions bunched).
+    auto mma = [&](const Frag& f, Frag& f2, int sa, int sb, int s, int d0, int dn) {
+        constexpr int C0 = NM / 3;  // first slot with conversions: the codes have been read
+        Raw w;
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+        for (int q = 0; q < NM; ++q) {
+            const int i = q / MI, j = q % MI;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.b[j]),
+                                                                __builtin_bit_cast(bf16x8, f.a[i]), acc[i][j], 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < MI; ++j) {
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.b[j]),
-                                                                    __builtin_bit_cast(bf16x8, f.a[i]), acc[i][j], 0, 0, 0);
-                const int q = i * MI + j;
+            for (int r = 0; r < MI; ++r)
+                if (r * NM / (4 * MI) == q) {
+                    read_codes(w, r, sb, s);
+                    read_a(f2, r, sa, s);
+                }
 #pragma unroll
-                for (int rep = 0; rep < 4; ++rep)
-                    if (dq < dn && (q + 1) * dn >= (dq + 1) * NM) {
-                        const int d = d0 + dq;
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (d <= G::Q_LOADS) load_b(d);
-                        else load_a(d - G::Q_LOADS - 1);
-                        __builtin_amdgcn_sched_barrier(0);
-                        ++dq;
-                    }
-            }
+            for (int r = 0; r < MI; ++r)
+                if (C0 + (2 * r + 1) * (NM - C0) / (2 * MI) == q) expand(f2, w, r);
+#pragma unroll
+            for (int d = 0; d < dn; ++d)
+                if ((2 * d + 1) * NM / (2 * dn) == q) {
+                    if (d0 + d <= G::Q_LOADS) load_b(d0 + d);
+                    else load_a(d0 + d - G::Q_LOADS - 1);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
     // ---- stream ----------------------------------------------------------------
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int i = 0; i < G::A_LOADS; ++i) load_a(i);
-    next_a();
+        for (int i = 0; i <= G::Q_LOADS; ++i) load_b(i);
 #pragma unroll
-    for (int i = 0; i <= G::Q_LOADS; ++i) load_b(i);
-    next_b();
-#pragma unroll
-    for (int i = 0; i < G::A_LOADS; ++i) load_a(i);
-    next_a();
-    wait_vm<G::A_LOADS>();
+        for (int i = 0; i < G::A_LOADS; ++i) load_a(i);
+        next_b();
+        next_a();
+    }
+    wait_vm<ND>();
     lds_barrier();
     int sa = 0, sb = 0;  // ring slots being multiplied
     Frag f[2];
-    load_frag(f[0], 0, 0, 0);
+    auto first = [&]() {  // fragments of a unit's first k16 step
+        Raw w;
+#pragma unroll
+        for (int r = 0; r < MI; ++r) {
+            read_codes(w, r, sb, 0);
+            read_a(f[0], r, sa, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < MI; ++r) expand(f[0], w, r);
+    };
+    first();
     uint8_t* st = lds + G::ST0 + wave * Stage<false, MI>::BYTES;
     for (;;) {
         clear(acc);
         for (int k = u.kbeg; k < u.kend; k += 64) {
-            load_frag(f[1], sa, sb, 1);
-            mma(f[0], 0, ND / 3);
-            load_frag(f[0], sa, sb, 2);
-            mma(f[1], ND / 3, 2 * ND / 3 - ND / 3);
-            load_frag(f[1], sa, sb, 3);
-            mma(f[0], 2 * ND / 3, ND - 2 * ND / 3);
+            mma(f[0], f[1], sa, sb, 1, 0, ND / 3);
+            mma(f[1], f[0], sa, sb, 2, ND / 3, 2 * ND / 3 - ND / 3);
+            mma(f[0], f[1], sa, sb, 3, 2 * ND / 3, ND - 2 * ND / 3);
             next_b();
             next_a();
-            // all but the last activation loads: the next step is whole in LDS
-            wait_vm<G::A_LOADS>();
+            wait_vm<ND>();  // all but this step's loads: the next step is whole in LDS
             lds_barrier();
             sa = sa == 2 ? 0 : sa + 1;
-            sb ^= 1;
-            load_frag(f[0], sa, sb, 0);
-            mma(f[1], 0, 0);
-#pragma unroll
-            for (int q = 0; q < MI * MI / 2; ++q) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);  // MFMA
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);  // DS read
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, MI * MI / 2, 1);
-            __builtin_amdgcn_sched_barrier(0);
+            sb = sa;
+            mma(f[1], f[0], sa, sb, 0, 0, 0);
         }
-        __builtin_amdgcn_sched_barrier(0);
         finish_unit<TILE, false, MI, SPLIT>(acc, st, p, u, p.T, p.N, wrow, wcol);
         vb += gridDim.x;
         if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) break;
-        load_frag(f[0], sa, sb, 0);  // again: the fragments' registers served the epilogue
+        first();  // again: the fragments' registers served the epilogue
     }
     wait_vm<0>();  // no load may land in LDS that the next workgroup owns
 }
@@ -504,7 +516,7 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     if (!unit_at<TILE, SPLIT>(pl, R, vb, u)) return;
 
     // ---- cursors: unit and reduction row of the activations and raw codes
-    // loaded next, and of the raw codes expanded next
+    // loaded next, and of the raw codes read for conversion next
     struct Cursor {
         Unit u;
         int vb, k;
@@ -556,78 +568,65 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     set_q();
     int sla = 0, slq = 0;  // ring slots of the next loads
     const int last_sc = (int)(p.wlds < 0x7fffffff ? p.wlds : 0x7fffffff) - 4;
-    auto load_q = [&]() {
+    // Load i of the next raw tile (the last one: its scales). Rows past the end
+    // are zeros.
+    auto load_q = [&](int i) {
         const uint32_t at = lds0 + G::R0 + slq * G::R_BYTES;
-        const uint8_t* base = uniform(p.w + cq.k * rowq);
-        if (cq.k + 32 <= cq.u.kend) {
-#pragma unroll
-            for (int i = 0; i < G::Q_LOADS; ++i) dma16s(base, q_off[i], at + ((wave * G::Q_LOADS + i) % QL) * 1024);
-        } else {  // rows past the end are zeros
-#pragma unroll
-            for (int i = 0; i < G::Q_LOADS; ++i) {
-                const int row = (((wave * G::Q_LOADS + i) % QL) * 64 + lane) / PPR;
-                const void* g = cq.k + row < cq.u.kend ? (const void*)(base + q_off[i]) : (const void*)zero_piece;
-                dma16v(g, at + ((wave * G::Q_LOADS + i) % QL) * 1024);
-            }
+        if (i == G::Q_LOADS) {
+            dma4v(sc_ptr + min(cq.k + 4 * (lane & 7), last_sc), at + G::Q_BYTES);
+            return;
         }
-        dma4v(sc_ptr + min(cq.k + 4 * (lane & 7), last_sc), at + G::Q_BYTES);
-        slq = slq == 2 ? 0 : slq + 1;
-        if (advance(cq)) set_q();
+        const int q = (wave * G::Q_LOADS + i) % QL, row = (q * 64 + lane) / PPR;
+        const uint8_t* g = p.w + cq.k * rowq + q_off[i];
+        dma16v(cq.k + row < cq.u.kend ? (const void*)g : (const void*)zero_piece, at + q * 1024);
     };
-    auto load_a = [&](int half) {  // half: DX, which half of the K = 64 tile
+    // Load i of the next sub-step's activations (DX: `half` of the K = 64 tile).
+    auto load_a = [&](int i, int half) {
         const uint32_t at = lds0 + G::A0 + sla * G::A_BYTES;
         if constexpr (DW) {
-            const uint8_t* base = uniform(p.x + (int64_t)ca.k * p.ldx + ca.u.m0);
-            if (ca.k + 32 <= ca.u.kend) {
-#pragma unroll
-                for (int i = 0; i < G::A_LOADS; ++i) dma16s(base, a_off[i], at + (wave * G::A_LOADS + i) * 1024);
-            } else {
-#pragma unroll
-                for (int i = 0; i < G::A_LOADS; ++i) {
-                    const int k = (64 / AC) * (wave * G::A_LOADS + i) + lane / AC;
-                    const void* g = ca.k + k < ca.u.kend ? (const void*)(base + a_off[i]) : (const void*)zero_piece;
-                    dma16v(g, at + (wave * G::A_LOADS + i) * 1024);
-                }
-            }
-            sla = (sla + 1) & 3;
+            const int k = (64 / AC) * (wave * G::A_LOADS + i) + lane / AC;
+            const uint8_t* g = reinterpret_cast<const uint8_t*>(p.x + (int64_t)ca.k * p.ldx + ca.u.m0) + a_off[i];
+            dma16v(ca.k + k < ca.u.kend ? (const void*)g : (const void*)zero_piece, at + (wave * G::A_LOADS + i) * 1024);
         } else {
-            const int k64 = ca.k - 32 * half;  // first reduction row of the tile
-            const uint8_t* base = uniform(p.x + (int64_t)ca.u.m0 * p.ldx + k64);
-            if (k64 + 64 <= ca.u.kend) {
-#pragma unroll
-                for (int i = 0; i < G::A_LOADS; ++i) {
-                    const int ii = half * G::A_LOADS + i;
-                    dma16s(base, a_off[ii], at + (wave * NA + ii) * 1024);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < G::A_LOADS; ++i) {
-                    const int ii = half * G::A_LOADS + i;
-                    const int r = 8 * (wave * NA + ii) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-                    const void* g = k64 + 8 * c < ca.u.kend ? (const void*)(base + a_off[ii]) : (const void*)zero_piece;
-                    dma16v(g, at + (wave * NA + ii) * 1024);
-                }
-            }
-            if (half == 1) sla = sla == 2 ? 0 : sla + 1;
+            const int k64 = ca.k - 32 * half, ii = half * G::A_LOADS + i;  // k64: first reduction row of the tile
+            const int r = 8 * (wave * NA + ii) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+            const uint8_t* g = reinterpret_cast<const uint8_t*>(p.x + (int64_t)ca.u.m0 * p.ldx + k64) + a_off[ii];
+            dma16v(k64 + 8 * c < ca.u.kend ? (const void*)g : (const void*)zero_piece, at + (wave * NA + ii) * 1024);
         }
+    };
+    constexpr int ND = G::Q_LOADS + 1 + G::A_LOADS;  // loads per wave and sub-step, raw codes first
+    auto load = [&](int d, int half) {
+        if (d <= G::Q_LOADS) load_q(d);
+        else load_a(d - G::Q_LOADS - 1, half);
+    };
+    auto next_loads = [&](int half) {
+        slq = slq == 2 ? 0 : slq + 1;
+        if (advance(cq)) set_q();
+        if (DW) sla = (sla + 1) & 3;
+        else if (half == 1) sla = sla == 2 ? 0 : sla + 1;
         if (advance(ca)) set_a();
     };
-    // Raw slot sr of the expand cursor's rows into bf16 slot sb.
-    auto expand = [&](int sr, int sb) {
+    // The lane's share of a raw tile: EP pieces of 8 codes with their scales,
+    // in registers from one k16 step to the next.
+    constexpr int EP = 32 * AC / 256;
+    const int ec = tid % AC, er = tid / AC;
+    uint2 eq[EP];
+    uint32_t es[EP];
+    int valid = 0;  // reduction rows of them that are not past the end
+    auto read_raw = [&](int q, int sr) {
         const uint8_t* raw = lds + G::R0 + sr * G::R_BYTES;
-        uint8_t* out = lds + G::B0 + sb * G::B_BYTES;
-        const int c = tid % AC, r0 = tid / AC;
-        const int valid = ce.u.kend - ce.k;
-#pragma unroll
-        for (int q = 0; q < 32 * AC / 256; ++q) {
-            const int row = r0 + q * (256 / AC);
-            const float sc = row < valid ? e8m0_value(raw[G::Q_BYTES + (c >> 2) * 32 + row]) : 1.0f;
-            uint4 v;
-            if constexpr (DW) v = expand_fp8(*reinterpret_cast<const uint2*>(raw + row * G::ROWQ + c * 8), sc);
-            else v = expand_fp4(*reinterpret_cast<const uint32_t*>(raw + row * G::ROWQ + c * 4), sc);
-            *reinterpret_cast<uint4*>(out + row * (TILE * 2) + ((c ^ (4 * (row & 3))) * 16)) = v;
-        }
-        advance(ce);
+        const int row = er + q * (256 / AC);
+        if constexpr (DW) eq[q] = *reinterpret_cast<const uint2*>(raw + row * G::ROWQ + ec * 8);
+        else eq[q].x = *reinterpret_cast<const uint32_t*>(raw + row * G::ROWQ + ec * 4);
+        es[q] = raw[G::Q_BYTES + (ec >> 2) * 32 + row];
+    };
+    auto write_piece = [&](int q, int sb) {  // expanded into bf16 slot sb
+        const int row = er + q * (256 / AC);
+        const float unit = e8m0_operand(row < valid ? es[q] : 127);
+        uint4 v;
+        if constexpr (DW) v = expand_fp8(eq[q], unit);
+        else v = expand_fp4(eq[q].x, unit);
+        *reinterpret_cast<uint4*>(lds + G::B0 + sb * G::B_BYTES + row * (TILE * 2) + ((ec ^ (4 * (row & 3))) * 16)) = v;
     };
 
     // ---- fragments -----------------------------------------------------------
@@ -653,75 +652,117 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
     // k16 step s of the sub-step in activation slot sa (DX: half `half` of it)
-    // and bf16 slot sb
-    auto load_frag = [&](Frag& f, int sa, int half, int sb, int s) {
+    // and bf16 slot sb. Read n of 2 MI, in the order in which the MFMAs need
+    // them: a[0], b[0] .., a[1] ..
+    auto read_frag = [&](Frag& f, int n, int sa, int half, int sb, int s) {
         const uint8_t* ta = lds + G::A0 + sa * G::A_BYTES;
         const uint8_t* tb = lds + G::B0 + sb * G::B_BYTES;
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            if constexpr (DW) {
-                f.a[i] = read_across(ta, wrow + 32 * i, s);
-            } else {
-                const int r = wrow + 32 * i + (lane & 31), c = (2 * (2 * half + s) + (lane >> 5)) ^ ((r >> 1) & 7);
-                f.a[i] = *reinterpret_cast<const uint4*>(ta + r * 128 + c * 16);
-            }
+        if (n >= 1 && n <= MI) {
+            f.b[n - 1] = read_across(tb, wcol + 32 * (n - 1), s);
+            return;
         }
-#pragma unroll
-        for (int j = 0; j < MI; ++j) f.b[j] = read_across(tb, wcol + 32 * j, s);
+        const int i = n == 0 ? 0 : n - MI;
+        if constexpr (DW) {
+            f.a[i] = read_across(ta, wrow + 32 * i, s);
+        } else {
+            const int r = wrow + 32 * i + (lane & 31), c = (2 * (2 * half + s) + (lane >> 5)) ^ ((r >> 1) & 7);
+            f.a[i] = *reinterpret_cast<const uint4*>(ta + r * 128 + c * 16);
+        }
     };
     f32x16 acc[MI][MI];
-    auto mma = [&](const Frag& f) {
+    constexpr int NM = MI * MI;
+    // MFMAs of one k16 step; slot(q) stands behind MFMA q (see the forward)
+    auto mma = [&](const Frag& f, auto slot) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < MI; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.b[j]),
-                                                                    __builtin_bit_cast(bf16x8, f.a[i]), acc[i][j], 0, 0, 0);
+        for (int q = 0; q < NM; ++q) {
+            const int i = q / MI, j = q % MI;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.b[j]),
+                                                                __builtin_bit_cast(bf16x8, f.a[i]), acc[i][j], 0, 0, 0);
+            slot(q);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
     // ---- stream ----------------------------------------------------------------
-    load_q();
-    load_q();
-    load_q();
-    load_a(0);
-    load_a(1);
-    load_a(0);
-    if constexpr (!DW) load_a(1);
+    // raw tiles 0 .. 2 and the activations of sub-steps 0 .. 2 (DW) or 0 .. 3
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            if (d > G::Q_LOADS ? !DW || t < 3 : t < 3) load(d, t & 1);
+        if (t < 3) {
+            next_loads(t & 1);
+        } else if constexpr (!DW) {
+            sla = sla == 2 ? 0 : sla + 1;
+            if (advance(ca)) set_a();
+        }
+    }
     wait_vm<0>();
     lds_barrier();
-    expand(0, 0);
+    int sa = 0, sr = 0;  // activation slot multiplied, raw slot read next
+    auto next_raw = [&]() {
+        sr = sr == 2 ? 0 : sr + 1;
+        valid = ce.u.kend - ce.k;
+        advance(ce);
+    };
+#pragma unroll
+    for (int q = 0; q < EP; ++q) read_raw(q, sr);
+    next_raw();
+#pragma unroll
+    for (int q = 0; q < EP; ++q) write_piece(q, 0);
+#pragma unroll
+    for (int q = 0; q < EP; ++q) read_raw(q, sr);
+    next_raw();
     lds_barrier();
-    int sa = 0, sr = 1;  // activation slot multiplied, raw slot expanded next
     Frag f[2];
-    load_frag(f[0], 0, 0, 0, 0);
+    auto first = [&]() {  // fragments of a unit's first k16 step
+#pragma unroll
+        for (int n = 0; n < 2 * MI; ++n) read_frag(f[0], n, sa, 0, 0, 0);
+    };
+    first();
     uint8_t* st = lds + G::ST0 + wave * G::STB;
     for (;;) {
         clear(acc);
         for (int k = u.kbeg; k < u.kend; k += 64) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                load_frag(f[1], sa, h, h, 1);
-                load_q();
-                load_a(h);
-                __builtin_amdgcn_sched_barrier(0);
-                expand(sr, h ^ 1);
-                sr = sr == 2 ? 0 : sr + 1;
-                __builtin_amdgcn_sched_barrier(0);
-                mma(f[0]);
-                // Outstanding at most: the activations of the last sub-step
-                // and all loads of this one. The next sub-step's activations
-                // and the raw codes it expands are in LDS.
+                // first k16 step: the second's fragments are read, the next
+                // sub-step's codes converted, and all loads go out (LDS
+                // accesses early, so that the barrier does not wait for them)
+                mma(f[0], [&](int q) {
+#pragma unroll
+                    for (int n = 0; n < 2 * MI; ++n)
+                        if (n * NM / (4 * MI) == q) read_frag(f[1], n, sa, h, h, 1);
+#pragma unroll
+                    for (int e = 0; e < EP; ++e)
+                        if (NM / 8 + e * 5 * NM / (8 * EP) == q) write_piece(e, h ^ 1);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        if (d * NM / ND == q) load(d, h);
+                });
+                next_loads(h);
+                // Outstanding at most: the activations of the last sub-step and
+                // all loads of this one. The next sub-step's activations and
+                // the raw codes read in this one are in LDS.
                 wait_vm<2 * G::A_LOADS + G::Q_LOADS + 1>();
                 lds_barrier();
                 if (DW || h == 1) sa = sa == G::A_SLOTS - 1 ? 0 : sa + 1;
-                load_frag(f[0], sa, h ^ 1, h ^ 1, 0);
-                mma(f[1]);
+                // second k16 step: the next sub-step's first fragments and the
+                // raw codes of the one after are read
+                mma(f[1], [&](int q) {
+#pragma unroll
+                    for (int n = 0; n < 2 * MI; ++n)
+                        if (n * NM / (4 * MI) == q) read_frag(f[0], n, sa, h ^ 1, h ^ 1, 0);
+#pragma unroll
+                    for (int e = 0; e < EP; ++e)
+                        if (NM / 8 + e * 5 * NM / (8 * EP) == q) read_raw(e, sr);
+                });
+                next_raw();
             }
         }
         finish_unit<TILE, DW, MI / 2, SPLIT>(acc, st, p, u, M, C, wrow, wcol);
         vb += gridDim.x;
         if (!unit_at<TILE, SPLIT>(pl, R, vb, u)) break;
-        load_frag(f[0], sa, 0, 0, 0);  // again: the fragments' registers served the epilogue
+        first();  // again: the fragments' registers served the epilogue
     }
     wait_vm<0>();  // no load may land in LDS that the next workgroup owns
 }
@@ -826,6 +867,118 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
     }
 }
 
+// ---- few tokens -------------------------------------------------------------------
+// A workgroup takes 16 NB output columns (rows of W) and 16 RB tokens; its NW
+// waves deal out the reduction in pieces of K = 128, U pieces in flight. Lane l
+// loads row l % 16's whole block 4 i + l / 16 of a piece straight into
+// registers (16 code bytes, one scale) and takes 8 codes of it to each of four
+// v_mfma_f32_16x16x32_bf16; the activations follow the same order of the
+// reduction. They come through LDS of the wave's own ([16 tokens][256 bytes] a
+// piece, chunks XOR-swizzled by token): fragments straight from memory touch 64
+// lines a load, which bound the kernel (16 tokens, N 1024, K 4096: 6.5 us).
+// The waves' sums meet in LDS and are added in wave order.
+template <int RB, int NB, int NW, int U>
+__global__ __launch_bounds__(64 * NW) void linear_rows_kernel(LinearParams p) {
+    constexpr int OUT = 256 * RB * NB;  // outputs of a workgroup
+    constexpr int XB = U * RB * 4096;   // activation bytes of a wave
+    __shared__ uint4 lds_raw[(NW * (XB > OUT * 4 ? XB : OUT * 4)) / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16 * NB, t0 = blockIdx.y * 16 * RB;
+    const int K = p.K, pieces = (K + 127) / 128;
+    const uint8_t* wq[NB];
+    const uint8_t* wsc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int n = min(n0 + 16 * b + row, p.N - 1);
+        wq[b] = p.w + (int64_t)n * (K / 2) + g * 16;
+        wsc[b] = p.ws + (int64_t)g * p.wlds + n;
+    }
+    const uint8_t* xw = lds + wave * XB;
+    const uint32_t xw0 = lds_u32(xw);
+    f32x4 acc[RB][NB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[r][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = wave; i0 < pieces; i0 += NW * U) {
+        uint4 q[U][NB];
+        uint32_t sc[U][NB];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * NW;
+            const bool in = 4 * i + g < K / 32;  // past the end: zero times zero
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                q[u][b] = in ? *reinterpret_cast<const uint4*>(wq[b] + i * 64) : make_uint4(0, 0, 0, 0);
+                sc[u][b] = in ? wsc[b][(int64_t)(4 * i) * p.wlds] : 127;
+            }
+        }
+        // load d of a piece: tokens 4 d .. 4 d + 3, lane l chunk l % 16
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    if (t0 + 16 * r + 4 * d >= p.T) break;  // tokens past the last: whatever LDS holds, for no output
+                    const int i = i0 + u * NW, t = 4 * d + g, k = i * 128 + 8 * (row ^ t);
+                    const uint16_t* src = p.x + (int64_t)min(t0 + 16 * r + t, p.T - 1) * p.ldx + k;
+                    dma16v(k < K ? (const void*)src : (const void*)zero_piece, xw0 + (u * RB + r) * 4096 + d * 1024);
+                }
+        wait_vm<0>();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            uint4 v[RB][4];
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[r][j] = *reinterpret_cast<const uint4*>(xw + (u * RB + r) * 4096 + row * 256 + ((4 * g + j) ^ row) * 16);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const float unit = e8m0_operand(sc[u][b]);
+                const uint32_t w[4] = {q[u][b].x, q[u][b].y, q[u][b].z, q[u][b].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bf16x8 f = __builtin_bit_cast(bf16x8, expand_fp4(w[j], unit));
+#pragma unroll
+                    for (int r = 0; r < RB; ++r)
+                        acc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8, v[r][j]), acc[r][b], 0, 0, 0);
+                }
+            }
+        }
+        wave_lds_fence();  // the activations are read: the next loads may land
+    }
+    __syncthreads();  // the sums take the activations' place
+    float* red = reinterpret_cast<float*>(lds);
+    // acc[r][b][e]: token 16 r + lane % 16, column 16 b + 4 (lane / 16) + e
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            *reinterpret_cast<f32x4*>(red + wave * OUT + (16 * r + row) * (16 * NB) + 16 * b + 4 * g) = acc[r][b];
+    __syncthreads();
+    for (int o = threadIdx.x * 2; o < OUT; o += 128 * NW) {
+        const int t = t0 + o / (16 * NB), n = n0 + o % (16 * NB);
+        if (t >= p.T || n >= p.N) continue;
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            a += red[w * OUT + o];
+            b += red[w * OUT + o + 1];
+        }
+        uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.y) + (int64_t)t * p.ldy + n);
+        if (p.beta != 0.0f) {
+            const uint32_t old = *y;
+            a += p.beta * bf_lo(old);
+            b += p.beta * bf_hi(old);
+        }
+        *y = pack_bf2(a, b);
+    }
+}
+
 // ---- the last round's sums ------------------------------------------------------
 // Tail tile j is the sum of its partial tiles in part order, plus beta times
 // what is there, rounded once. A thread takes 4 columns of a row.
@@ -883,34 +1036,77 @@ Sizes sizes(LinearOp op, int T, int N, int K) {
 
 // Workgroups that run at a time.
 int64_t tile_slots(int tile) { return (int64_t)cu_count() * (tile == 256 ? 1 : 2); }
+constexpr int kMinSteps = 4;  // K = 64 steps that a part of a split reduction has at least
 
-constexpr int kMinSteps = 8;  // K = 64 steps that a part of a split reduction has at least
-
-LinearPlan plan_tiles(const Sizes& z, int tile) {
+LinearPlan plan_tiles(const Sizes& z, int tile, int64_t parts) {
     LinearPlan pl;
     pl.tile = tile;
     pl.tiles_m = (z.M + tile - 1) / tile;
     pl.tiles_c = (z.C + tile - 1) / tile;
     const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_c;
-    const int64_t slots = tile_slots(tile);
-    const int64_t whole = tiles / slots * slots, rest = tiles - whole;
-    const int nk = (z.R + 63) / 64;
-    const int64_t parts = rest > 0 ? std::min<int64_t>(slots / rest, nk / kMinSteps) : 1;
     pl.whole = (int)tiles;
     if (parts >= 2) {
-        pl.whole = (int)whole;
-        pl.tail = (int)rest;
+        const int nk = (z.R + 63) / 64;
+        pl.whole = (int)(tiles / tile_slots(tile) * tile_slots(tile));
+        pl.tail = (int)(tiles - pl.whole);
         pl.chunk = (int)((nk + 4 * parts - 1) / (4 * parts)) * 256;  // whole steps of every kernel
         pl.parts = (nk * 64 + pl.chunk - 1) / pl.chunk;
     }
     return pl;
 }
 
-LinearPlan linear_plan(LinearOp op, int T, int N, int K) {
+// What a launch takes, in us, from its K = 64 steps. Measured on one MI355X
+// over 16 .. 512 tiles and 4 .. 512 steps:
+//   start  launch, first loads and epilogue of 128 x 128 tiles (256 x 256: 4 more)
+//   one    a step of 128 x 128 tiles, one workgroup per CU (bound by latency)
+//   two    the same with two
+//   large  a step of 256 x 256 tiles (bound by the matrix cores)
+struct StepTimes {
+    double start, one, two, large;
+};
+constexpr StepTimes kTimes[4] = {{4.5, 0.51, 1.1, 1.4}, {3.0, 0.30, 0.48, 0.0}, {5.5, 0.84, 1.4, 1.75}, {5.5, 0.84, 1.4, 1.8}};
+// A split reduction adds a launch for the sums and its partial tiles' way
+// through the last-level cache and back.
+constexpr double kSplitStart = 3.5, kSplitPerMiB = 0.3;
+
+double round_time(const StepTimes& t, int tile, int64_t units, double steps) {
+    if (tile == 256) return 2.0 + steps * t.large;
+    return steps * (units <= cu_count() ? t.one : t.two);
+}
+double plan_time(const StepTimes& t, const Sizes& z, int tile, int64_t parts) {
+    const int64_t slots = tile_slots(tile);
+    const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
+    const int64_t whole = tiles / slots, rest = tiles - whole * slots;
+    const double nk = (z.R + 63) / 64;
+    double us = t.start + (tile == 256 ? 4.0 : 0.0) + whole * round_time(t, tile, slots, nk);
+    if (rest == 0) return us;
+    if (parts < 2) return us + round_time(t, tile, rest, nk);
+    const double mib = (double)(rest * parts) * tile * tile * 4 / (1 << 20);
+    return us + round_time(t, tile, rest * parts, std::ceil(nk / parts)) + (whole > 0 ? t.start : 0.0) + kSplitStart + kSplitPerMiB * mib;
+}
+
+// The tile size and split with the shortest estimate. Measured (us, chosen /
+// others): forward T 777, N 4096, K 1024 14.4 whole 128 x 128 tiles / 23.2 in
+// two parts, 28.4 on 256 x 256; T 777, N 1024, K 4096 21.3 in four parts /
+// 38.2 whole, 51.9 on 256 x 256 in two; dW T 32768, N 4096, K 1024 290 on
+// 256 x 256 tiles in four parts / 373 on 128 x 128 in two, 860 whole.
+LinearPlan linear_plan(LinearOp op, int T, int N, int K, double* us = nullptr) {
     const Sizes z = sizes(op, T, N, K);
-    const int64_t t256 = (int64_t)((z.M + 255) / 256) * ((z.C + 255) / 256);
-    if (op == LINEAR_MATMUL) return plan_tiles(z, 128);
-    return plan_tiles(z, t256 >= cu_count() / 2 ? 256 : 128);
+    const StepTimes& t = kTimes[op];
+    int best_tile = 128;
+    int64_t best_parts = 1;
+    double best = 1e30;
+    for (int tile = 128; tile <= (op == LINEAR_MATMUL ? 128 : 256); tile *= 2) {
+        const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
+        const int64_t rest = tiles % tile_slots(tile);
+        const int64_t most = rest > 0 ? std::min<int64_t>(tile_slots(tile) / rest, (z.R + 63) / 64 / kMinSteps) : 1;
+        for (int64_t parts = 1; parts <= std::max<int64_t>(most, 1); parts += parts < 8 ? 1 : parts / 4) {
+            const double c = plan_time(t, z, tile, parts);
+            if (c < best) best = c, best_tile = tile, best_parts = parts;
+        }
+    }
+    if (us != nullptr) *us = best;
+    return plan_tiles(z, best_tile, best_parts);
 }
 
 template <int OP, int TILE, bool SPLIT>
@@ -929,6 +1125,31 @@ void launch_tiles(const LinearParams& p, const LinearPlan& pl, hipStream_t s) {
         const Sizes z = sizes((LinearOp)OP, p.T, p.N, p.K);
         linear_fixup_kernel<TILE, OP == LINEAR_DW><<<pl.tail * SLABS, 256, 0, s>>>(p, pl, z.M, z.C);
     }
+}
+
+template <int RB, int NB, int NW, int U>
+void launch_rows_as(const LinearParams& p, hipStream_t s) {
+    const dim3 grid((p.N + 16 * NB - 1) / (16 * NB), (p.T + 16 * RB - 1) / (16 * RB));
+    linear_rows_kernel<RB, NB, NW, U><<<grid, 64 * NW, 0, s>>>(p);
+}
+// The kernel for few tokens where its estimate, 3 us and 7.2 us for each 10^9
+// products (measured over T 1 .. 777, N and K 256 .. 4096), is below the
+// tiles'. Blocks of outputs grow with the grid, which fills the chip twice at
+// most: 16 x 16, 16 x 32 (columns), 32 x 32, 64 x 32. Measured (us) 16 x 16 /
+// 16 x 32 / 32 x 32 / 64 x 32: T 16, N 1024, K 4096 4.7 / 6.4 / 7.6 / 8.8; T
+// 64, N 4096, K 1024 4.8 / 4.6 / 4.7 / 6.4; T 256, N 4096, K 1024 13.8 / 11.4 /
+// 11.2 / 10.0. Reductions of more than 8 pieces take 8 waves with two pieces in
+// flight (32 x 32: one), shorter ones 4 waves with two (16 x 16: 8 with one).
+bool launch_rows(const LinearParams& p, double tiles_us, hipStream_t s) {
+    if (3.0 + 7.2e-9 * ((double)p.T * p.N * p.K) > tiles_us) return false;
+    const int64_t most = 2 * (int64_t)cu_count(), n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32;
+    const int64_t t16 = (p.T + 15) / 16, t32 = (p.T + 31) / 32;
+    const bool many = p.K > 1024;
+    if (n16 * t16 <= most) many ? launch_rows_as<1, 1, 8, 2>(p, s) : launch_rows_as<1, 1, 8, 1>(p, s);
+    else if (n32 * t16 <= most) many ? launch_rows_as<1, 2, 8, 2>(p, s) : launch_rows_as<1, 2, 4, 2>(p, s);
+    else if (n32 * t32 <= most) many ? launch_rows_as<2, 2, 8, 1>(p, s) : launch_rows_as<2, 2, 4, 2>(p, s);
+    else launch_rows_as<4, 2, 4, 1>(p, s);
+    return true;
 }
 
 }  // namespace
@@ -957,7 +1178,9 @@ hipError_t launch_linear(LinearOp op, const LinearParams& p, hipStream_t s) {
         linear_scale_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(static_cast<float*>(p.y), p.ldy, p.N, p.K, p.beta);
         return hipGetLastError();
     }
-    const LinearPlan pl = linear_plan(op, p.T, p.N, p.K);
+    double us = 0.0;
+    const LinearPlan pl = linear_plan(op, p.T, p.N, p.K, &us);
+    if (op == LINEAR_FORWARD && launch_rows(p, us, s)) return hipGetLastError();
     const bool big = pl.tile == 256;
     switch (op) {
         case LINEAR_FORWARD: big ? launch_tiles<LINEAR_FORWARD, 256>(p, pl, s) : launch_tiles<LINEAR_FORWARD, 128>(p, pl, s); break;

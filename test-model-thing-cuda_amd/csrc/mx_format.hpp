@@ -12,6 +12,10 @@ __device__ __forceinline__ float e8m0_value(uint32_t s) {
     return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23);
 }
 
+// The scale operand of the scaled conversions, which read its exponent field
+// as an e8m0 byte: 0 is 2^-127 there and 255 NaN.
+__device__ __forceinline__ float e8m0_operand(uint32_t s) { return __uint_as_float(s << 23); }
+
 // Scale byte of a block whose largest |value| has the fp32 bits `amax` (an
 // integer maximum of the bits without the sign, so inf and NaN come out on
 // top). Blocks of zeros take 127; a block with an inf or NaN takes 255.
