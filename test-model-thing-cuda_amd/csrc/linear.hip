@@ -27,6 +27,7 @@
 // the transposing ds_read_b64_tr_b16.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "linear.hpp"
 #include "moe_internal.hpp"
@@ -39,7 +40,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
 // What is read for reduction rows past the end: the products of a step's tail
 // are zero times zero, whatever lies behind the operands.
@@ -142,7 +145,7 @@ __device__ __forceinline__ bool unit_at(const LinearPlan& pl, int R, int vb, Uni
 
 // ---- epilogue ----------------------------------------------------------------
 // acc[i][j][r] = C[m][c] with m = 32 i + lane % 32 and c = 32 j + 8 (r / 4) +
-// 4 (lane / 32) + r % 4 in the wave's WT x WT outputs. 32 rows by 32 JS columns
+// 4 (lane / 32) + r % 4 in the wave's outputs. 32 rows by 32 JS columns
 // at a time go through the wave's own LDS, so that a row's columns leave as one
 // run of 16-byte stores; no barrier.
 template <bool F32, int JS>
@@ -151,12 +154,12 @@ struct Stage {
     static constexpr int BYTES = 32 * ROWB;
 };
 
-template <int N>
-__device__ __forceinline__ void clear(f32x16 (&acc)[N][N]) {
+template <int MI, int NJ>
+__device__ __forceinline__ void clear(f32x16 (&acc)[MI][NJ]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < N; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 }
@@ -167,11 +170,10 @@ __device__ __forceinline__ void wave_lds_fence() { asm volatile("s_waitcnt lgkmc
 // ones. beta times what is there is added in fp32. NT: results are written
 // once and leave the caches to the operands; partial tiles are read again at
 // once.
-template <int WT, bool F32, int JS, bool NT>
-__device__ __forceinline__ void store_wave(f32x16 (&acc)[WT / 32][WT / 32], uint8_t* st, void* out, int64_t ld, int rows,
+template <bool F32, int JS, bool NT, int MI, int NJ>
+__device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, void* out, int64_t ld, int rows,
                                            int cols, float beta) {
     using S = Stage<F32, JS>;
-    constexpr int N = WT / 32;
     constexpr int CH = S::ROWB / 16, RPI = 64 / CH;  // 16-byte chunks per staged row, rows per store
     // a value of this unit's own: the addresses below are not kept in registers
     // through the main loop
@@ -179,14 +181,14 @@ __device__ __forceinline__ void store_wave(f32x16 (&acc)[WT / 32][WT / 32], uint
     asm volatile("" : "+v"(lane));
     const int lr = lane & 31;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int jg = 0; jg < N; jg += JS) {
+        for (int jg = 0; jg < NJ; jg += JS) {
             // the outputs not yet staged stay in the accumulator registers
 #pragma unroll
-            for (int i2 = i; i2 < N; ++i2)
+            for (int i2 = i; i2 < MI; ++i2)
 #pragma unroll
-                for (int j = 0; j < N; ++j)
+                for (int j = 0; j < NJ; ++j)
                     if (i2 > i || j >= jg) asm volatile("" : "+a"(acc[i2][j]));
 #pragma unroll
             for (int j = 0; j < JS; ++j) {
@@ -246,7 +248,7 @@ __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64],
     if constexpr (SPLIT) {
         float* o = p.part + (int64_t)u.part * TILE * TILE + wrow * TILE + wcol;
         if constexpr (F32) {
-            store_wave<WT, true, JS, false>(acc, st, o, TILE, rows, cols, 0.0f);
+            store_wave<true, JS, false>(acc, st, o, TILE, rows, cols, 0.0f);
         } else {
             const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -265,16 +267,15 @@ __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64],
         }
     } else {
         const int64_t at = (int64_t)(u.m0 + wrow) * p.ldy + u.c0 + wcol;
-        if constexpr (F32) store_wave<WT, true, JS, true>(acc, st, static_cast<float*>(p.y) + at, p.ldy, rows, cols, p.beta);
-        else store_wave<WT, false, JS, true>(acc, st, static_cast<uint16_t*>(p.y) + at, p.ldy, rows, cols, p.beta);
+        if constexpr (F32) store_wave<true, JS, true>(acc, st, static_cast<float*>(p.y) + at, p.ldy, rows, cols, p.beta);
+        else store_wave<false, JS, true>(acc, st, static_cast<uint16_t*>(p.y) + at, p.ldy, rows, cols, p.beta);
     }
 }
 
 // ---- forward -------------------------------------------------------------------
-// Per K = 64 step: activations [TILE rows][64] bf16 in a ring of 3 (rows of
-// 128 bytes, 16-byte chunks XOR-swizzled by row / 2), codes [TILE rows][32
-// bytes] and scales [2 blocks][TILE] in a ring of 2. Step s loads the codes of
-// step s + 1 and the activations of step s + 2, spread over its MFMAs.
+// Per K = 64 step: activations [TILE rows][64] bf16 (rows of 128 bytes, 16-byte
+// chunks XOR-swizzled by row / 2), codes [TILE rows][32 bytes] and scales [2
+// blocks][TILE]. Rings of 3: step s loads step s + 2.
 template <int TILE>
 struct Fwd {
     static constexpr int WT = TILE / 2, MI = WT / 32;
@@ -371,33 +372,38 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
     struct Frag {
         uint4 a[MI], b[MI];
     };
-    struct Raw {  // 8 codes and the scale byte of each row block
-        uint32_t q[MI], s[MI];
+    struct Raw {  // the lane's codes of a K = 64 step, 8 for each k16 step, and their scales
+        uint32_t q[MI][4], s[MI][2];
     };
-    // k16 step s of the K = 64 step in ring slots sa and sb
-    auto read_a = [&](Frag& f, int i, int sa, int s) {
+    // k16 step s of the K = 64 step in ring slot sl
+    auto read_a = [&](Frag& f, int i, int sl, int s) {
         const int r = wrow + 32 * i + (lane & 31), c = (2 * s + (lane >> 5)) ^ ((r >> 1) & 7);
-        f.a[i] = *reinterpret_cast<const uint4*>(lds + G::A0 + sa * G::A_BYTES + r * 128 + c * 16);
+        f.a[i] = *reinterpret_cast<const uint4*>(lds + G::A0 + sl * G::A_BYTES + r * 128 + c * 16);
     };
-    // lane: 8 codes k = 16 s + 8 (lane / 32) .. + 7 of row lane % 32
-    auto read_codes = [&](Raw& w, int j, int sb, int s) {
-        const uint8_t* tb = lds + G::B0 + sb * G::B_BYTES;
-        const int blk = s >> 1, within = (8 * s + 4 * (lane >> 5)) & 15, r = wcol + 32 * j + (lane & 31);
-        w.q[j] = *reinterpret_cast<const uint32_t*>(tb + r * 32 + ((blk ^ ((r >> 3) & 1)) * 16) + within);
-        w.s[j] = tb[G::Q_BYTES + blk * TILE + r];
+    // lane: codes k = 16 s + 8 (lane / 32) .. + 7 of row lane % 32
+    auto read_codes = [&](Raw& w, int j, int sl) {
+        const uint8_t* tb = lds + G::B0 + sl * G::B_BYTES;
+        const int r = wcol + 32 * j + (lane & 31);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            w.q[j][s] = *reinterpret_cast<const uint32_t*>(tb + r * 32 + (((s >> 1) ^ ((r >> 3) & 1)) * 16) + 8 * (s & 1) + 4 * (lane >> 5));
+#pragma unroll
+        for (int b = 0; b < 2; ++b) w.s[j][b] = tb[G::Q_BYTES + b * TILE + r];
     };
-    auto expand = [&](Frag& f, const Raw& w, int j) { f.b[j] = expand_fp4(w.q[j], e8m0_operand(w.s[j])); };
+    auto expand = [&](Frag& f, const Raw& w, int j, int s) { f.b[j] = expand_fp4(w.q[j][s], e8m0_operand(w.s[j][s >> 1])); };
     f32x16 acc[MI][MI];
     constexpr int ND = G::A_LOADS + G::Q_LOADS + 1, NM = MI * MI;
     // MFMAs of one k16 step. Under them, in the slots between two: the reads of
-    // the next step's fragments (f2: k16 step s of ring slots sa, sb), the
-    // conversion of its codes and loads [d0, d0 + dn). A wave's instructions
-    // issue in order and an MFMA takes 32 cycles, so what stands in one slot
-    // is free up to about seven instructions; in a bunch it stalls the matrix
-    // core (T = N = K = 4096: 1.72 us a step with the conversions bunched).
-    auto mma = [&](const Frag& f, Frag& f2, int sa, int sb, int s, int d0, int dn) {
-        constexpr int C0 = NM / 3;  // first slot with conversions: the codes have been read
-        Raw w;
+    // the next step's activations (f2: k16 step s of ring slot sl; the first
+    // also reads its K = 64 step's codes, which the others find in registers),
+    // the conversion of its codes and loads [d0, d0 + dn). A wave's
+    // instructions issue in order and an MFMA takes 32 cycles, so what stands
+    // in one slot is free up to about seven instructions; in a bunch it stalls
+    // the matrix core (T = N = K = 4096: 1.72 us a step with the conversions
+    // bunched, 1.43 spread).
+    Raw w;
+    auto mma = [&](const Frag& f, Frag& f2, int sl, int s, int d0, int dn) {
+        const int c0 = s == 0 ? NM / 2 : 0;  // first slot with conversions
 #pragma unroll
         for (int q = 0; q < NM; ++q) {
             const int i = q / MI, j = q % MI;
@@ -406,12 +412,12 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
 #pragma unroll
             for (int r = 0; r < MI; ++r)
                 if (r * NM / (4 * MI) == q) {
-                    read_codes(w, r, sb, s);
-                    read_a(f2, r, sa, s);
+                    if (s == 0) read_codes(w, r, sl);
+                    read_a(f2, r, sl, s);
                 }
 #pragma unroll
             for (int r = 0; r < MI; ++r)
-                if (C0 + (2 * r + 1) * (NM - C0) / (2 * MI) == q) expand(f2, w, r);
+                if (c0 + (2 * r + 1) * (NM - c0) / (2 * MI) == q) expand(f2, w, r, s);
 #pragma unroll
             for (int d = 0; d < dn; ++d)
                 if ((2 * d + 1) * NM / (2 * dn) == q) {
@@ -433,34 +439,33 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
     }
     wait_vm<ND>();
     lds_barrier();
-    int sa = 0, sb = 0;  // ring slots being multiplied
+    int sl = 0;  // ring slot being multiplied
     Frag f[2];
     auto first = [&]() {  // fragments of a unit's first k16 step
-        Raw w;
 #pragma unroll
         for (int r = 0; r < MI; ++r) {
-            read_codes(w, r, sb, 0);
-            read_a(f[0], r, sa, 0);
+            read_codes(w, r, sl);
+            read_a(f[0], r, sl, 0);
         }
 #pragma unroll
-        for (int r = 0; r < MI; ++r) expand(f[0], w, r);
+        for (int r = 0; r < MI; ++r) expand(f[0], w, r, 0);
     };
     first();
     uint8_t* st = lds + G::ST0 + wave * Stage<false, MI>::BYTES;
     for (;;) {
         clear(acc);
         for (int k = u.kbeg; k < u.kend; k += 64) {
-            mma(f[0], f[1], sa, sb, 1, 0, ND / 3);
-            mma(f[1], f[0], sa, sb, 2, ND / 3, 2 * ND / 3 - ND / 3);
-            mma(f[0], f[1], sa, sb, 3, 2 * ND / 3, ND - 2 * ND / 3);
+            mma(f[0], f[1], sl, 1, 0, ND / 3);
+            mma(f[1], f[0], sl, 2, ND / 3, 2 * ND / 3 - ND / 3);
+            mma(f[0], f[1], sl, 3, 2 * ND / 3, ND - 2 * ND / 3);
             next_b();
             next_a();
             wait_vm<ND>();  // all but this step's loads: the next step is whole in LDS
             lds_barrier();
-            sa = sa == 2 ? 0 : sa + 1;
-            sb = sa;
-            mma(f[1], f[0], sa, sb, 0, 0, 0);
+            sl = sl == 2 ? 0 : sl + 1;
+            mma(f[1], f[0], sl, 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
         finish_unit<TILE, false, MI, SPLIT>(acc, st, p, u, p.T, p.N, wrow, wcol);
         vb += gridDim.x;
         if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) break;
@@ -768,15 +773,41 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
 }
 
 // ---- both operands in MXFP4 ------------------------------------------------------
-// 128 x 128 outputs on the scaled matrix instruction, which takes 32 codes of
-// a row and their scale byte from each lane: 32 x 32 outputs over K = 64. Steps
-// of K = 256 make 128-byte row segments (a CU takes a 1 KiB load of those in
-// half the time of 64-byte ones). Ring of 2: codes of both operands [128
-// rows][128 bytes], chunks XOR-swizzled by row / 2, and scales [8 blocks][128]
-// each. A unit's first step is loaded before the previous unit's epilogue,
-// which stages through the other slot; two workgroups per CU, so that one's
-// output stores (what bounds a large product: at K = 1024 an output byte for
-// every byte of codes) drain while the other multiplies.
+// The scaled matrix instruction takes 32 codes of a row and a scale byte from
+// each lane: 32 x 32 outputs over K = 64. Steps of K = 256 make 128-byte row
+// segments (a CU takes a 1 KiB load of those in half the time of 64-byte
+// ones); codes lie in LDS as [rows][128 bytes], chunks XOR-swizzled by row /
+// 2, scales as [16 rows][8 blocks][16 bytes], so that one transposing read
+// gives a lane its row's 8 scales.
+
+// Scales of row `base` + lane % 32 (base a multiple of 32, region `sc`): byte g
+// is that of block 2 g + lane / 32.
+__device__ __forceinline__ int read_scales(const uint8_t* sc, int base, int lane) {
+    const i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (lds_i32x2*)(sc + (base + 16 * ((lane >> 4) & 1)) * 8 + (lane & 15) * 8));
+    return __builtin_amdgcn_perm(v[1], v[0], lane < 32 ? 0x06040200 : 0x07050301);
+}
+// 16 code bytes of block blk of row r.
+__device__ __forceinline__ i32x4 read_block(const uint8_t* codes, int r, int blk) {
+    return *reinterpret_cast<const i32x4*>(codes + r * 128 + ((blk ^ ((r >> 1) & 7)) * 16));
+}
+template <int G>
+__device__ __forceinline__ f32x16 mma_mx(i32x4 w, i32x4 x, f32x16 c, int ws, int xs) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(__builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1),
+                                                           __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4,
+                                                           G, ws, G, xs);
+}
+// The lane's source in a 1 KiB load of 8 row groups' scales (from row r0, a
+// multiple of 16, and block b0): rows past the operand's and blocks past the
+// row's end are clamped.
+__device__ __forceinline__ const uint8_t* scale_source(const uint8_t* s, int64_t lds, int blocks, int64_t r0, int b0) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = r0 + 16 * (lane >> 3);
+    return s + (int64_t)min(b0 + (lane & 7), blocks - 1) * lds + (row < lds - 16 ? row : lds - 16);
+}
+
+// 128 x 128 outputs, ring of 2. A unit's first step is loaded before the
+// previous unit's epilogue, which stages through the other slot.
 struct Mx {
     static constexpr int TILE = 128, WT = 64, MI = 2;
     static constexpr int CODES = TILE * 128, LOADS = CODES / 4096;  // per operand; 1 KiB loads per wave
@@ -813,11 +844,8 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
             dma16s(bw, (uint32_t)min(r, p.N - 1 - n.c0) * (uint32_t)(K / 2) + col, at + G::CODES + q * 1024);
         }
         // waves 0 and 1: the scales of X and W; 2 and 3 the same again
-        const int64_t blk = min(k / 32 + (lane >> 3), K / 32 - 1);
-        const int row = 16 * (lane & 7);
-        const uint8_t* sx = p.xs + blk * p.xlds + min((int64_t)n.m0 + row, p.xlds - 16);
-        const uint8_t* sw = p.ws + blk * p.wlds + min((int64_t)n.c0 + row, p.wlds - 16);
-        dma16v((wave & 1) ? sw : sx, at + 2 * G::CODES + (wave & 1) * 1024);
+        const uint8_t* sc = (wave & 1) ? scale_source(p.ws, p.wlds, K / 32, n.c0, k / 32) : scale_source(p.xs, p.xlds, K / 32, n.m0, k / 32);
+        dma16v(sc, at + 2 * G::CODES + (wave & 1) * 1024);
     };
     f32x16 acc[MI][MI];
     clear(acc);
@@ -833,28 +861,29 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
             else if (more) load_step(n, n.kbeg, slot ^ 1);
             const uint8_t* st = lds + slot * G::SLOT;
             const int groups = min(4, (u.kend - k) / 64);
+            int as[MI], bs[MI];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                if (g >= groups) break;
-                i32x8 a[MI], b[MI];
-                int as[MI], bs[MI];
-                const int blk = 2 * g + (lane >> 5);
+            for (int i = 0; i < MI; ++i) {
+                as[i] = read_scales(st + 2 * G::CODES, wrow + 32 * i, lane);
+                bs[i] = read_scales(st + 2 * G::CODES + 1024, wcol + 32 * i, lane);
+            }
+            auto group = [&](auto g_) {
+                constexpr int g = decltype(g_)::value;
+                i32x4 a[MI], b[MI];
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
-                    const int ra = wrow + 32 * i + (lane & 31), rb = wcol + 32 * i + (lane & 31);
-                    const i32x4 va = *reinterpret_cast<const i32x4*>(st + ra * 128 + ((blk ^ ((ra >> 1) & 7)) * 16));
-                    const i32x4 vw = *reinterpret_cast<const i32x4*>(st + G::CODES + rb * 128 + ((blk ^ ((rb >> 1) & 7)) * 16));
-                    a[i] = __builtin_shufflevector(va, va, 0, 1, 2, 3, -1, -1, -1, -1);
-                    b[i] = __builtin_shufflevector(vw, vw, 0, 1, 2, 3, -1, -1, -1, -1);
-                    as[i] = st[2 * G::CODES + blk * 128 + ra];
-                    bs[i] = st[2 * G::CODES + 1024 + blk * 128 + rb];
+                    a[i] = read_block(st, wrow + 32 * i + (lane & 31), 2 * g + (lane >> 5));
+                    b[i] = read_block(st + G::CODES, wcol + 32 * i + (lane & 31), 2 * g + (lane >> 5));
                 }
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int j = 0; j < MI; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 4, 4, 0, bs[j], 0, as[i]);
-            }
+                    for (int j = 0; j < MI; ++j) acc[i][j] = mma_mx<g>(b[j], a[i], acc[i][j], bs[j], as[i]);
+            };
+            group(std::integral_constant<int, 0>{});
+            if (groups > 1) group(std::integral_constant<int, 1>{});
+            if (groups > 2) group(std::integral_constant<int, 2>{});
+            if (groups > 3) group(std::integral_constant<int, 3>{});
             slot ^= 1;
         }
         lds_barrier();  // the last step's slot is read: the epilogue stages there
@@ -1064,10 +1093,10 @@ LinearPlan plan_tiles(const Sizes& z, int tile, int64_t parts) {
 struct StepTimes {
     double start, one, two, large;
 };
-constexpr StepTimes kTimes[4] = {{4.5, 0.51, 1.1, 1.4}, {3.0, 0.30, 0.48, 0.0}, {5.5, 0.84, 1.4, 1.75}, {5.5, 0.84, 1.4, 1.8}};
+constexpr StepTimes kTimes[4] = {{4.5, 0.60, 1.0, 1.4}, {3.0, 0.30, 0.48, 0.0}, {5.5, 0.90, 1.2, 1.75}, {5.5, 0.90, 1.15, 1.8}};
 // A split reduction adds a launch for the sums and its partial tiles' way
 // through the last-level cache and back.
-constexpr double kSplitStart = 3.5, kSplitPerMiB = 0.3;
+constexpr double kSplitStart = 3.5, kSplitPerMiB = 0.25;
 
 double round_time(const StepTimes& t, int tile, int64_t units, double steps) {
     if (tile == 256) return 2.0 + steps * t.large;
