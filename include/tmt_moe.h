@@ -395,7 +395,8 @@ int tmt_moe_f32_to_bf16(void* stream, const float* in, uint16_t* out, int64_t n)
  * Every product sums exact terms in fp32 (a code times its scale is exact in
  * bf16) and rounds once. Y = beta * Y + ...; with beta == 0 the output is
  * not read. Outputs must not overlap inputs. T any number >= 0, N a multiple
- * of 16, K a multiple of 64. Strides are in elements; bf16 and fp32 rows start
+ * of 16, K a multiple of 64, both and all row strides at most 2^22, scale
+ * strides at most 2^27. Strides are in elements; bf16 and fp32 rows start
  * at 16-byte boundaries (base and stride), codes and scales of a product too
  * (scale strides are multiples of 16). Elements between a row's width and its
  * stride are neither read into a result nor written.

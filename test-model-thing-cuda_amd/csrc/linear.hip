@@ -44,31 +44,35 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
-// What is read for reduction rows past the end: the products of a step's tail
-// are zero times zero, whatever lies behind the operands.
+// What is read past the end of a reduction.
 __device__ __align__(16) const uint32_t zero_piece[4] = {0, 0, 0, 0};
 
+// A window on global memory: loads read zeros past its `bytes`, so that no
+// address has to be clamped and a reduction's tail is zero times zero,
+// whatever lies behind the operands. Wave-uniform.
+struct Window {
+    uint64_t at;
+    uint32_t bytes;
+};
+__device__ __forceinline__ uint64_t address(const void* p) { return reinterpret_cast<uint64_t>(p); }
+__device__ __forceinline__ i32x4 descriptor(const Window& w) {
+    return i32x4{(int)(uint32_t)w.at, (int)(uint32_t)(w.at >> 32), (int)w.bytes, 0x00020000};  // raw buffer
+}
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-// 16 bytes per lane from a wave-uniform base and a 32-bit lane offset into
-// LDS at lds_base + 16 * lane (lds_base wave-uniform); M0 is written.
-__device__ __forceinline__ void dma16s(const void* sbase, uint32_t voff, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "m0");
+// 16 (4) bytes per lane from a window into LDS at lds_base + 16 (4) * lane
+// (lds_base wave-uniform); M0 is written.
+__device__ __forceinline__ void dma16(const Window& w, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(descriptor(w)), "s"(lds_base) : "m0");
 }
-// The same from a 64-bit lane address, and 4 bytes per lane.
+__device__ __forceinline__ void dma4(const Window& w, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(descriptor(w)), "s"(lds_base) : "m0");
+}
+// The same from a lane's 64-bit address.
 __device__ __forceinline__ void dma16v(const void* g, uint32_t lds_base) {
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base) : "m0");
 }
-__device__ __forceinline__ void dma4v(const void* g, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_base) : "m0");
-}
 #pragma clang diagnostic pop
-// A wave-uniform pointer in scalar registers.
-__device__ __forceinline__ const uint8_t* uniform(const void* p) {
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-    return reinterpret_cast<const uint8_t*>(((uint64_t)hi << 32) | lo);
-}
 template <int N>
 __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -138,8 +142,11 @@ __device__ __forceinline__ bool unit_at(const LinearPlan& pl, int R, int vb, Uni
         j = pl.whole + q;
     }
     tile_at(pl, j, mt, ct);
-    u.m0 = mt * TILE;
-    u.c0 = ct * TILE;
+    // the divisions run on the vector unit: back to scalar registers
+    u.m0 = __builtin_amdgcn_readfirstlane(mt * TILE);
+    u.c0 = __builtin_amdgcn_readfirstlane(ct * TILE);
+    u.kbeg = __builtin_amdgcn_readfirstlane(u.kbeg);
+    u.kend = __builtin_amdgcn_readfirstlane(u.kend);
     return true;
 }
 
@@ -304,67 +311,53 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) return;
 
-    // ---- load cursors: the unit and step that the next loads belong to. Past
-    // the last unit they stay on its last step (loaded again, never used).
+    // ---- the next step to load: windows on its operands, and the steps left in
+    // its unit. Past the last unit the windows are empty.
+    Window wa, wq, wsc;
+    int left = 0, vl = vb, sll = 0;
+    auto set = [&](const Unit& n) {
+        wa = {address(p.x + (int64_t)n.m0 * p.ldx + n.kbeg),
+              (uint32_t)(min(p.T - n.m0, TILE) - 1) * (uint32_t)(p.ldx * 2) + (uint32_t)(K - n.kbeg) * 2};
+        wq = {address(p.w + (int64_t)n.c0 * (K / 2) + n.kbeg / 2),
+              (uint32_t)(min(p.N - n.c0, TILE) - 1) * (uint32_t)(K / 2) + (uint32_t)(K - n.kbeg) / 2};
+        wsc = {address(p.ws + (int64_t)(n.kbeg / 32) * p.wlds + n.c0), (uint32_t)(2 * p.wlds) - n.c0};
+        left = (n.kend - n.kbeg) >> 6;
+    };
+    set(u);
     uint32_t a_off[G::A_LOADS], q_off[G::Q_LOADS];
-    const uint8_t *a_base = nullptr, *q_base = nullptr, *sc_ptr = nullptr;
-    Unit ua = u, ub = u;
-    int vba = vb, vbb = vb, ka = u.kbeg, kb = u.kbeg;
-    auto set_a = [&]() {
-        a_base = reinterpret_cast<const uint8_t*>(p.x + (int64_t)ua.m0 * p.ldx);
 #pragma unroll
-        for (int i = 0; i < G::A_LOADS; ++i) {
-            const int r = 8 * (wave * G::A_LOADS + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-            a_off[i] = (uint32_t)min(r, p.T - 1 - ua.m0) * (uint32_t)(p.ldx * 2) + c * 16;
-        }
-    };
-    auto set_b = [&]() {
-        q_base = p.w + (int64_t)ub.c0 * (K / 2);
+    for (int i = 0; i < G::A_LOADS; ++i) {
+        const int r = 8 * (wave * G::A_LOADS + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        a_off[i] = (uint32_t)r * (uint32_t)(p.ldx * 2) + c * 16;
+    }
 #pragma unroll
-        for (int i = 0; i < G::Q_LOADS; ++i) {
-            const int s = (wave * G::Q_LOADS + i) * 64 + lane, m = s >> 1, half = (s & 1) ^ ((m >> 3) & 1);
-            q_off[i] = (uint32_t)min(m, p.N - 1 - ub.c0) * (uint32_t)(K / 2) + half * 16;
+    for (int i = 0; i < G::Q_LOADS; ++i) {
+        const int s = (wave * G::Q_LOADS + i) * 64 + lane, m = s >> 1, half = (s & 1) ^ ((m >> 3) & 1);
+        q_off[i] = (uint32_t)m * (uint32_t)(K / 2) + half * 16;
+    }
+    const uint32_t sc_off = (uint32_t)((lane / (TILE / 16)) & 1) * (uint32_t)p.wlds + 16 * (lane % (TILE / 16));
+    // load d of the step: the codes, the scales, the activations
+    auto load = [&](int d) {
+        const uint32_t a = lds0 + G::A0 + sll * G::A_BYTES, b = lds0 + G::B0 + sll * G::B_BYTES;
+        if (d < G::Q_LOADS) dma16(wq, q_off[d], b + (wave * G::Q_LOADS + d) * 1024);
+        else if (d == G::Q_LOADS) dma16(wsc, sc_off, b + G::Q_BYTES);
+        else dma16(wa, a_off[d - G::Q_LOADS - 1], a + (wave * G::A_LOADS + d - G::Q_LOADS - 1) * 1024);
+    };
+    auto next_loads = [&]() {
+        sll = sll == 2 ? 0 : sll + 1;
+        if (left == 0) return;  // no unit left: the windows stay empty
+        if (--left > 0) {
+            wa = {wa.at + 128, wa.bytes - 128};
+            wq = {wq.at + 32, wq.bytes - 32};
+            wsc.at += 2 * p.wlds;
+            return;
         }
-        constexpr int G16 = TILE / 16;
-        sc_ptr = p.ws + (int64_t)((lane / G16) & 1) * p.wlds + min(ub.c0 + 16 * (lane % G16), p.N - 16);
-    };
-    set_a();
-    set_b();
-    int sla = 0, slb = 0;  // ring slots of the next loads
-    auto load_a = [&](int i) {
-        dma16s(uniform(a_base + (int64_t)ka * 2), a_off[i], lds0 + G::A0 + sla * G::A_BYTES + (wave * G::A_LOADS + i) * 1024);
-    };
-    auto load_b = [&](int i) {
-        const uint32_t at = lds0 + G::B0 + slb * G::B_BYTES;
-        if (i < G::Q_LOADS) dma16s(uniform(q_base + kb / 2), q_off[i], at + (wave * G::Q_LOADS + i) * 1024);
-        else dma16v(sc_ptr + (int64_t)(kb / 32) * p.wlds, at + G::Q_BYTES);
-    };
-    auto next_a = [&]() {
-        sla = sla == 2 ? 0 : sla + 1;
-        if (ka + 64 < ua.kend) {
-            ka += 64;
+        Unit n;
+        vl += gridDim.x;
+        if (unit_at<TILE, SPLIT>(pl, K, vl, n)) {
+            set(n);
         } else {
-            Unit n;
-            if (unit_at<TILE, SPLIT>(pl, K, vba + gridDim.x, n)) {
-                vba += gridDim.x;
-                ua = n;
-                ka = n.kbeg;
-                set_a();
-            }
-        }
-    };
-    auto next_b = [&]() {
-        slb = slb == 2 ? 0 : slb + 1;
-        if (kb + 64 < ub.kend) {
-            kb += 64;
-        } else {
-            Unit n;
-            if (unit_at<TILE, SPLIT>(pl, K, vbb + gridDim.x, n)) {
-                vbb += gridDim.x;
-                ub = n;
-                kb = n.kbeg;
-                set_b();
-            }
+            wa.bytes = wq.bytes = wsc.bytes = 0;
         }
     };
 
@@ -420,10 +413,7 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
                 if (c0 + (2 * r + 1) * (NM - c0) / (2 * MI) == q) expand(f2, w, r, s);
 #pragma unroll
             for (int d = 0; d < dn; ++d)
-                if ((2 * d + 1) * NM / (2 * dn) == q) {
-                    if (d0 + d <= G::Q_LOADS) load_b(d0 + d);
-                    else load_a(d0 + d - G::Q_LOADS - 1);
-                }
+                if ((2 * d + 1) * NM / (2 * dn) == q) load(d0 + d);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -431,11 +421,8 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
     // ---- stream ----------------------------------------------------------------
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int i = 0; i <= G::Q_LOADS; ++i) load_b(i);
-#pragma unroll
-        for (int i = 0; i < G::A_LOADS; ++i) load_a(i);
-        next_b();
-        next_a();
+        for (int d = 0; d < ND; ++d) load(d);
+        next_loads();
     }
     wait_vm<ND>();
     lds_barrier();
@@ -458,8 +445,7 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
             mma(f[0], f[1], sl, 1, 0, ND / 3);
             mma(f[1], f[0], sl, 2, ND / 3, 2 * ND / 3 - ND / 3);
             mma(f[0], f[1], sl, 3, 2 * ND / 3, ND - 2 * ND / 3);
-            next_b();
-            next_a();
+            next_loads();
             wait_vm<ND>();  // all but this step's loads: the next step is whole in LDS
             lds_barrier();
             sl = sl == 2 ? 0 : sl + 1;
@@ -513,103 +499,121 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT;
-    const int M = DW ? p.N : p.T, C = p.K, R = DW ? p.T : p.N;
+    const int M = DW ? p.N : p.T, C = p.K, K = p.K, R = DW ? p.T : p.N;
     const int64_t rowq = DW ? p.K : p.K / 2;  // code bytes per row of the weights / checkpoint
 
     Unit u;
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, R, vb, u)) return;
 
-    // ---- cursors: unit and reduction row of the activations and raw codes
-    // loaded next, and of the raw codes read for conversion next
-    struct Cursor {
-        Unit u;
-        int vb, k;
-    };
-    Cursor ca{u, vb, u.kbeg}, cq{u, vb, u.kbeg}, ce{u, vb, u.kbeg};
-    // 32 rows on (a unit's sub-steps fill its K = 64 steps); true: a new unit.
-    // Past the last unit the cursor stays on its last sub-step.
-    auto advance = [&](Cursor& c) {
-        if (c.k + 32 < c.u.kbeg + ((c.u.kend - c.u.kbeg + 63) & ~63)) {
-            c.k += 32;
-            return false;
-        }
-        Unit n;
-        if (!unit_at<TILE, SPLIT>(pl, R, c.vb + gridDim.x, n)) return false;
-        c.vb += gridDim.x;
-        c.u = n;
-        c.k = n.kbeg;
-        return true;
-    };
+    // ---- the next sub-steps to load, of the activations and of the raw codes:
+    // windows on them, and the sub-steps left in their units (which fill K = 64
+    // steps). Past the last unit the windows are empty.
+    constexpr int AC = TILE / 8;                // 16-byte chunks per row of a tile across the reduction
+    constexpr int PPR = G::ROWQ / 16;           // 16-byte pieces per raw row
+    constexpr int QL = G::Q_BYTES / 1024;       // wave loads of a raw tile (fewer than the waves: loaded twice)
     constexpr int NA = DW ? G::A_LOADS : 2 * G::A_LOADS;
+    const uint32_t ldb = (uint32_t)(p.ldx * 2), rowb = (uint32_t)rowq;
+    Window wa, wq, wsc;
+    int a_left = 0, q_left = 0, va = vb, vq = vb;
+    int a_rows = 0, q_rows = 0;                 // reduction rows not loaded yet (DX: q only)
+    uint32_t a_skip = 0, q_skip = 0;            // bytes of a row outside the window behind the last row
+    int sla = 0, slq = 0;                       // ring slots of the next loads
+    auto rows_window = [](int rows, uint32_t row_bytes, uint32_t skip) {
+        return rows > 0 ? (uint32_t)min(rows, 32) * row_bytes - skip : 0u;
+    };
+    auto substeps = [](const Unit& n) { return ((n.kend - n.kbeg + 63) >> 6) * 2; };
+    auto set_a = [&](const Unit& n) {
+        a_left = substeps(n);
+        if constexpr (DW) {
+            a_rows = n.kend - n.kbeg;
+            a_skip = ldb - (uint32_t)(p.N - n.m0) * 2;
+            wa = {address(p.x + (int64_t)n.kbeg * p.ldx + n.m0), rows_window(a_rows, ldb, a_skip)};
+        } else {
+            wa = {address(p.x + (int64_t)n.m0 * p.ldx + n.kbeg),
+                  (uint32_t)(min(p.T - n.m0, TILE) - 1) * ldb + (uint32_t)(p.N - n.kbeg) * 2};
+        }
+    };
+    auto set_q = [&](const Unit& n) {
+        q_left = substeps(n);
+        q_rows = n.kend - n.kbeg;
+        q_skip = (uint32_t)n.c0 * G::CB / 8;
+        wq = {address(p.w + n.kbeg * rowq + q_skip), rows_window(q_rows, rowb, q_skip)};
+        const int blocks = min(K / 32 - n.c0 / 32, TILE / 32);
+        wsc = {address(p.ws + (int64_t)(n.c0 / 32) * p.wlds + n.kbeg), (uint32_t)(blocks * p.wlds) - n.kbeg};
+    };
+    set_a(u);
+    set_q(u);
     uint32_t a_off[NA], q_off[G::Q_LOADS];
-    const uint8_t* sc_ptr = nullptr;
-    // DW: reduction row and chunk of the lane in load i of a 32-row tile
-    constexpr int AC = TILE / 8;  // chunks per row
-    auto set_a = [&]() {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            if constexpr (DW) {
-                const int k = (64 / AC) * (wave * G::A_LOADS + i) + lane / AC, c = (lane % AC) ^ (4 * (k & 3));
-                a_off[i] = (uint32_t)k * (uint32_t)(p.ldx * 2) + (uint32_t)min(c * 8, p.N - 8 - ca.u.m0) * 2;
-            } else {
-                const int r = 8 * (wave * NA + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-                a_off[i] = (uint32_t)min(r, p.T - 1 - ca.u.m0) * (uint32_t)(p.ldx * 2) + c * 16;
-            }
+    for (int i = 0; i < NA; ++i) {
+        if constexpr (DW) {  // a 32-row tile, row k, chunk c
+            const int k = (64 / AC) * (wave * G::A_LOADS + i) + lane / AC, c = (lane % AC) ^ (4 * (k & 3));
+            a_off[i] = (uint32_t)k * ldb + c * 16;
+        } else {
+            const int r = 8 * (wave * NA + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+            a_off[i] = (uint32_t)r * ldb + c * 16;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < G::Q_LOADS; ++i) {
+        const int s = ((wave * G::Q_LOADS + i) % QL) * 64 + lane;
+        q_off[i] = (uint32_t)(s / PPR) * rowb + (s % PPR) * 16;
+    }
+    const uint32_t sc_off = (uint32_t)(lane >> 3) * (uint32_t)p.wlds + 4 * (lane & 7);
+    constexpr int ND = G::Q_LOADS + 1 + G::A_LOADS;  // loads per wave and sub-step, raw codes first
+    // load d of the next raw tile (codes, scales) or of the next sub-step's
+    // activations (DX: `half` of the rows of a K = 64 tile)
+    auto load = [&](int d, int half) {
+        const uint32_t raw = lds0 + G::R0 + slq * G::R_BYTES, act = lds0 + G::A0 + sla * G::A_BYTES;
+        if (d < G::Q_LOADS) {
+            dma16(wq, q_off[d], raw + ((wave * G::Q_LOADS + d) % QL) * 1024);
+        } else if (d == G::Q_LOADS) {
+            dma4(wsc, sc_off, raw + G::Q_BYTES);
+        } else {
+            const int i = d - G::Q_LOADS - 1 + (DW ? 0 : half * G::A_LOADS);
+            dma16(wa, a_off[i], act + (wave * NA + i) * 1024);
         }
     };
-    constexpr int PPR = G::ROWQ / 16;             // 16-byte pieces per raw row
-    constexpr int QL = G::Q_BYTES / 1024;         // wave loads of a raw tile (fewer than the waves: loaded twice)
-    auto set_q = [&]() {
-#pragma unroll
-        for (int i = 0; i < G::Q_LOADS; ++i) {
-            const int s = ((wave * G::Q_LOADS + i) % QL) * 64 + lane;
-            const int64_t col = (int64_t)cq.u.c0 * G::CB / 8 + (s % PPR) * 16;
-            q_off[i] = (uint32_t)((s / PPR) * rowq + (col < rowq - 16 ? col : rowq - 16));
-        }
-        sc_ptr = p.ws + (int64_t)min(cq.u.c0 / 32 + (lane >> 3), p.K / 32 - 1) * p.wlds;
-    };
-    set_a();
-    set_q();
-    int sla = 0, slq = 0;  // ring slots of the next loads
-    const int last_sc = (int)(p.wlds < 0x7fffffff ? p.wlds : 0x7fffffff) - 4;
-    // Load i of the next raw tile (the last one: its scales). Rows past the end
-    // are zeros.
-    auto load_q = [&](int i) {
-        const uint32_t at = lds0 + G::R0 + slq * G::R_BYTES;
-        if (i == G::Q_LOADS) {
-            dma4v(sc_ptr + min(cq.k + 4 * (lane & 7), last_sc), at + G::Q_BYTES);
+    auto next_q = [&]() {
+        slq = slq == 2 ? 0 : slq + 1;
+        if (q_left == 0) return;  // no unit left: the windows stay empty
+        if (--q_left > 0) {
+            q_rows -= 32;
+            wq = {wq.at + 32 * rowq, rows_window(q_rows, rowb, q_skip)};
+            wsc = {wsc.at + 32, (uint32_t)max((int)wsc.bytes - 32, 0)};
             return;
         }
-        const int q = (wave * G::Q_LOADS + i) % QL, row = (q * 64 + lane) / PPR;
-        const uint8_t* g = p.w + cq.k * rowq + q_off[i];
-        dma16v(cq.k + row < cq.u.kend ? (const void*)g : (const void*)zero_piece, at + q * 1024);
-    };
-    // Load i of the next sub-step's activations (DX: `half` of the K = 64 tile).
-    auto load_a = [&](int i, int half) {
-        const uint32_t at = lds0 + G::A0 + sla * G::A_BYTES;
-        if constexpr (DW) {
-            const int k = (64 / AC) * (wave * G::A_LOADS + i) + lane / AC;
-            const uint8_t* g = reinterpret_cast<const uint8_t*>(p.x + (int64_t)ca.k * p.ldx + ca.u.m0) + a_off[i];
-            dma16v(ca.k + k < ca.u.kend ? (const void*)g : (const void*)zero_piece, at + (wave * G::A_LOADS + i) * 1024);
+        Unit n;
+        vq += gridDim.x;
+        if (unit_at<TILE, SPLIT>(pl, R, vq, n)) {
+            set_q(n);
         } else {
-            const int k64 = ca.k - 32 * half, ii = half * G::A_LOADS + i;  // k64: first reduction row of the tile
-            const int r = 8 * (wave * NA + ii) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-            const uint8_t* g = reinterpret_cast<const uint8_t*>(p.x + (int64_t)ca.u.m0 * p.ldx + k64) + a_off[ii];
-            dma16v(k64 + 8 * c < ca.u.kend ? (const void*)g : (const void*)zero_piece, at + (wave * NA + ii) * 1024);
+            wq.bytes = wsc.bytes = 0;
+            q_rows = 0;
         }
     };
-    constexpr int ND = G::Q_LOADS + 1 + G::A_LOADS;  // loads per wave and sub-step, raw codes first
-    auto load = [&](int d, int half) {
-        if (d <= G::Q_LOADS) load_q(d);
-        else load_a(d - G::Q_LOADS - 1, half);
-    };
-    auto next_loads = [&](int half) {
-        slq = slq == 2 ? 0 : slq + 1;
-        if (advance(cq)) set_q();
+    auto next_a = [&](int half) {
         if (DW) sla = (sla + 1) & 3;
         else if (half == 1) sla = sla == 2 ? 0 : sla + 1;
-        if (advance(ca)) set_a();
+        if (a_left == 0) return;
+        if (--a_left > 0) {
+            if constexpr (DW) {
+                a_rows -= 32;
+                wa = {wa.at + 32 * (uint64_t)ldb, rows_window(a_rows, ldb, a_skip)};
+            } else if (half == 1) {
+                wa = {wa.at + 128, wa.bytes - 128};
+            }
+            return;
+        }
+        Unit n;
+        va += gridDim.x;
+        if (unit_at<TILE, SPLIT>(pl, R, va, n)) {
+            set_a(n);
+        } else {
+            wa.bytes = 0;
+            a_rows = 0;
+        }
     };
     // The lane's share of a raw tile: EP pieces of 8 codes with their scales,
     // in registers from one k16 step to the next.
@@ -617,7 +621,10 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     const int ec = tid % AC, er = tid / AC;
     uint2 eq[EP];
     uint32_t es[EP];
-    int valid = 0;  // reduction rows of them that are not past the end
+    // DW: reduction rows of the raw tiles in LDS that are not past the end, of
+    // the one being multiplied first. (A checkpoint's scales behind its last row
+    // are anything. DX leaves out whole k16 steps instead: N is a multiple of 16.)
+    int valid[3] = {0, 0, 0};
     auto read_raw = [&](int q, int sr) {
         const uint8_t* raw = lds + G::R0 + sr * G::R_BYTES;
         const int row = er + q * (256 / AC);
@@ -625,9 +632,9 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
         else eq[q].x = *reinterpret_cast<const uint32_t*>(raw + row * G::ROWQ + ec * 4);
         es[q] = raw[G::Q_BYTES + (ec >> 2) * 32 + row];
     };
-    auto write_piece = [&](int q, int sb) {  // expanded into bf16 slot sb
+    auto write_piece = [&](int q, int sb, int rows) {  // expanded into bf16 slot sb
         const int row = er + q * (256 / AC);
-        const float unit = e8m0_operand(row < valid ? es[q] : 127);
+        const float unit = e8m0_operand(!DW || row < rows ? es[q] : 127);
         uint4 v;
         if constexpr (DW) v = expand_fp8(eq[q], unit);
         else v = expand_fp4(eq[q].x, unit);
@@ -676,52 +683,63 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     };
     f32x16 acc[MI][MI];
     constexpr int NM = MI * MI;
-    // MFMAs of one k16 step; slot(q) stands behind MFMA q (see the forward)
-    auto mma = [&](const Frag& f, auto slot) {
+    // MFMAs of one k16 step; slot(q) stands behind MFMA q (see the forward). A
+    // step past the reduction's end (DX) is not `on`.
+    auto mma = [&](const Frag& f, bool on, auto slot) {
+        if (DW || on) {
 #pragma unroll
-        for (int q = 0; q < NM; ++q) {
-            const int i = q / MI, j = q % MI;
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.b[j]),
-                                                                __builtin_bit_cast(bf16x8, f.a[i]), acc[i][j], 0, 0, 0);
-            slot(q);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int q = 0; q < NM; ++q) {
+                const int i = q / MI, j = q % MI;
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f.b[j]),
+                                                                    __builtin_bit_cast(bf16x8, f.a[i]), acc[i][j], 0, 0, 0);
+                slot(q);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < NM; ++q) slot(q);
         }
     };
 
     // ---- stream ----------------------------------------------------------------
     // raw tiles 0 .. 2 and the activations of sub-steps 0 .. 2 (DW) or 0 .. 3
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 3; ++t) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-            if (d > G::Q_LOADS ? !DW || t < 3 : t < 3) load(d, t & 1);
-        if (t < 3) {
-            next_loads(t & 1);
-        } else if constexpr (!DW) {
-            sla = sla == 2 ? 0 : sla + 1;
-            if (advance(ca)) set_a();
-        }
+        for (int d = 0; d <= G::Q_LOADS; ++d) load(d, 0);
+        valid[0] = valid[1];
+        valid[1] = valid[2];
+        valid[2] = q_rows;
+        next_q();
+    }
+    for (int t = 0; t < (DW ? 3 : 4); ++t) {
+#pragma unroll
+        for (int d = G::Q_LOADS + 1; d < ND; ++d) load(d, t & 1);
+        next_a(t & 1);
     }
     wait_vm<0>();
     lds_barrier();
     int sa = 0, sr = 0;  // activation slot multiplied, raw slot read next
-    auto next_raw = [&]() {
-        sr = sr == 2 ? 0 : sr + 1;
-        valid = ce.u.kend - ce.k;
-        advance(ce);
-    };
 #pragma unroll
-    for (int q = 0; q < EP; ++q) read_raw(q, sr);
-    next_raw();
+    for (int q = 0; q < EP; ++q) read_raw(q, 0);
 #pragma unroll
-    for (int q = 0; q < EP; ++q) write_piece(q, 0);
+    for (int q = 0; q < EP; ++q) write_piece(q, 0, valid[0]);
 #pragma unroll
-    for (int q = 0; q < EP; ++q) read_raw(q, sr);
-    next_raw();
+    for (int q = 0; q < EP; ++q) read_raw(q, 1);
+    sr = 2;
     lds_barrier();
-    Frag f[2];
-    auto first = [&]() {  // fragments of a unit's first k16 step
+    // 256 x 256 tiles read a k16 step's fragments under the MFMAs of the step
+    // before. A k16 step of a 128 x 128 tile is four MFMAs, shorter than an LDS
+    // read: both steps' fragments are read right behind the barrier, the second
+    // step's into f[1] and f[2] in turn (T 777, N 1024, K 4096, one workgroup
+    // per CU: dX 21.2 us step by step, FASTER).
+    constexpr bool PAIR = MI == 2;
+    Frag f[PAIR ? 3 : 2];
+    auto first = [&]() {  // fragments of a unit's first sub-step, as far as the loop has them there
 #pragma unroll
-        for (int n = 0; n < 2 * MI; ++n) read_frag(f[0], n, sa, 0, 0, 0);
+        for (int n = 0; n < 2 * MI; ++n) {
+            read_frag(f[0], n, sa, 0, 0, 0);
+            if constexpr (PAIR) read_frag(f[1], n, sa, 0, 0, 1);
+        }
     };
     first();
     uint8_t* st = lds + G::ST0 + wave * G::STB;
@@ -730,38 +748,50 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
         for (int k = u.kbeg; k < u.kend; k += 64) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                Frag& second = f[PAIR && h == 1 ? 2 : 1];
                 // first k16 step: the second's fragments are read, the next
                 // sub-step's codes converted, and all loads go out (LDS
                 // accesses early, so that the barrier does not wait for them)
-                mma(f[0], [&](int q) {
+                mma(f[0], k + 32 * h < u.kend, [&](int q) {
+                    if constexpr (!PAIR) {
 #pragma unroll
-                    for (int n = 0; n < 2 * MI; ++n)
-                        if (n * NM / (4 * MI) == q) read_frag(f[1], n, sa, h, h, 1);
+                        for (int n = 0; n < 2 * MI; ++n)
+                            if (n * NM / (4 * MI) == q) read_frag(second, n, sa, h, h, 1);
+                    }
 #pragma unroll
                     for (int e = 0; e < EP; ++e)
-                        if (NM / 8 + e * 5 * NM / (8 * EP) == q) write_piece(e, h ^ 1);
+                        if (NM / 8 + e * 5 * NM / (8 * EP) == q) write_piece(e, h ^ 1, valid[1]);
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
                         if (d * NM / ND == q) load(d, h);
                 });
-                next_loads(h);
+                valid[0] = valid[1];
+                valid[1] = valid[2];
+                valid[2] = q_rows;
+                next_q();
+                next_a(h);
                 // Outstanding at most: the activations of the last sub-step and
                 // all loads of this one. The next sub-step's activations and
                 // the raw codes read in this one are in LDS.
                 wait_vm<2 * G::A_LOADS + G::Q_LOADS + 1>();
                 lds_barrier();
                 if (DW || h == 1) sa = sa == G::A_SLOTS - 1 ? 0 : sa + 1;
-                // second k16 step: the next sub-step's first fragments and the
-                // raw codes of the one after are read
-                mma(f[1], [&](int q) {
+                // second k16 step: the next sub-step's first fragments (PAIR:
+                // all) and the raw codes of the one after are read
+                mma(second, k + 32 * h + 16 < u.kend, [&](int q) {
 #pragma unroll
                     for (int n = 0; n < 2 * MI; ++n)
                         if (n * NM / (4 * MI) == q) read_frag(f[0], n, sa, h ^ 1, h ^ 1, 0);
+                    if constexpr (PAIR) {
+#pragma unroll
+                        for (int n = 0; n < 2 * MI; ++n)
+                            if (NM / 2 + n * NM / (4 * MI) == q) read_frag(f[h == 0 ? 2 : 1], n, sa, h ^ 1, h ^ 1, 1);
+                    }
 #pragma unroll
                     for (int e = 0; e < EP; ++e)
                         if (NM / 8 + e * 5 * NM / (8 * EP) == q) read_raw(e, sr);
                 });
-                next_raw();
+                sr = sr == 2 ? 0 : sr + 1;
             }
         }
         finish_unit<TILE, DW, MI / 2, SPLIT>(acc, st, p, u, M, C, wrow, wcol);
@@ -797,15 +827,6 @@ __device__ __forceinline__ f32x16 mma_mx(i32x4 w, i32x4 x, f32x16 c, int ws, int
                                                            __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4,
                                                            G, ws, G, xs);
 }
-// The lane's source in a 1 KiB load of 8 row groups' scales (from row r0, a
-// multiple of 16, and block b0): rows past the operand's and blocks past the
-// row's end are clamped.
-__device__ __forceinline__ const uint8_t* scale_source(const uint8_t* s, int64_t lds, int blocks, int64_t r0, int b0) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = r0 + 16 * (lane >> 3);
-    return s + (int64_t)min(b0 + (lane & 7), blocks - 1) * lds + (row < lds - 16 ? row : lds - 16);
-}
-
 // 128 x 128 outputs, ring of 2. A unit's first step is loaded before the
 // previous unit's epilogue, which stages through the other slot.
 struct Mx {
@@ -830,35 +851,61 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) return;
 
-    // Step k of unit n into slot `slot`. Pieces past the row's end are clamped
-    // into it (they are not multiplied), rows past the operand's too.
-    auto load_step = [&](const Unit& n, int k, int slot) {
-        const uint32_t at = lds0 + slot * G::SLOT;
-        const uint8_t* ba = uniform(p.xq + (int64_t)n.m0 * (K / 2));
-        const uint8_t* bw = uniform(p.w + (int64_t)n.c0 * (K / 2));
+    // ---- the next step to load: windows on its operands. Pieces past a row's
+    // end are another row's: they are not multiplied.
+    Window wx, wxs, ww, wws;
+    int kn = 0, kend = 0, vn = vb, sl = 0;
+    bool left = true;
+    auto set = [&](const Unit& n) {
+        kn = n.kbeg;
+        kend = n.kend;
+        wx = {address(p.xq + (int64_t)n.m0 * (K / 2) + kn / 2), (uint32_t)(min(p.T - n.m0, TILE) - 1) * (uint32_t)(K / 2) + (K - kn) / 2};
+        ww = {address(p.w + (int64_t)n.c0 * (K / 2) + kn / 2), (uint32_t)(min(p.N - n.c0, TILE) - 1) * (uint32_t)(K / 2) + (K - kn) / 2};
+        const uint32_t blocks = (uint32_t)min(8, (K - kn) / 32);
+        wxs = {address(p.xs + (int64_t)(kn / 32) * p.xlds + n.m0), blocks * (uint32_t)p.xlds - n.m0};
+        wws = {address(p.ws + (int64_t)(kn / 32) * p.wlds + n.c0), blocks * (uint32_t)p.wlds - n.c0};
+    };
+    set(u);
+    uint32_t off[G::LOADS];
+#pragma unroll
+    for (int i = 0; i < G::LOADS; ++i) {
+        const int r = 8 * (wave * G::LOADS + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        off[i] = (uint32_t)r * (uint32_t)(K / 2) + c * 16;
+    }
+    // waves 0 and 1: the scales of X and W; 2 and 3 the same again
+    const uint32_t sc_off = (uint32_t)(lane & 7) * (uint32_t)((wave & 1) ? p.wlds : p.xlds) + 16 * (lane >> 3);
+    auto load_step = [&]() {
+        const uint32_t at = lds0 + sl * G::SLOT;
 #pragma unroll
         for (int i = 0; i < G::LOADS; ++i) {
-            const int q = wave * G::LOADS + i, r = 8 * q + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
-            const uint32_t col = (uint32_t)min(k / 2 + c * 16, K / 2 - 16);
-            dma16s(ba, (uint32_t)min(r, p.T - 1 - n.m0) * (uint32_t)(K / 2) + col, at + q * 1024);
-            dma16s(bw, (uint32_t)min(r, p.N - 1 - n.c0) * (uint32_t)(K / 2) + col, at + G::CODES + q * 1024);
+            dma16(wx, off[i], at + (wave * G::LOADS + i) * 1024);
+            dma16(ww, off[i], at + G::CODES + (wave * G::LOADS + i) * 1024);
         }
-        // waves 0 and 1: the scales of X and W; 2 and 3 the same again
-        const uint8_t* sc = (wave & 1) ? scale_source(p.ws, p.wlds, K / 32, n.c0, k / 32) : scale_source(p.xs, p.xlds, K / 32, n.m0, k / 32);
-        dma16v(sc, at + 2 * G::CODES + (wave & 1) * 1024);
+        dma16((wave & 1) ? wws : wxs, sc_off, at + 2 * G::CODES + (wave & 1) * 1024);
+        sl ^= 1;
+        kn += 256;
+        if (kn < kend) {
+            wx = {wx.at + 128, wx.bytes - 128};
+            ww = {ww.at + 128, ww.bytes - 128};
+            const uint32_t gone = (uint32_t)(8 - min(8, (K - kn) / 32));  // blocks past the end in a last step
+            wxs = {wxs.at + 8 * p.xlds, wxs.bytes - gone * (uint32_t)p.xlds};
+            wws = {wws.at + 8 * p.wlds, wws.bytes - gone * (uint32_t)p.wlds};
+            return;
+        }
+        Unit n;
+        vn += gridDim.x;
+        left = unit_at<TILE, SPLIT>(pl, K, vn, n);
+        if (left) set(n);
     };
     f32x16 acc[MI][MI];
     clear(acc);
     int slot = 0;
-    load_step(u, u.kbeg, 0);
+    load_step();
     for (;;) {
-        Unit n = u;
-        const bool more = unit_at<TILE, SPLIT>(pl, K, vb + gridDim.x, n);
         for (int k = u.kbeg; k < u.kend; k += 256) {
             wait_vm<0>();
             lds_barrier();  // step k is whole in LDS, and the other slot is read
-            if (k + 256 < u.kend) load_step(u, k + 256, slot ^ 1);
-            else if (more) load_step(n, n.kbeg, slot ^ 1);
+            if (left) load_step();
             const uint8_t* st = lds + slot * G::SLOT;
             const int groups = min(4, (u.kend - k) / 64);
             int as[MI], bs[MI];
@@ -889,9 +936,8 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
         lds_barrier();  // the last step's slot is read: the epilogue stages there
         finish_unit<TILE, false, MI, SPLIT>(acc, lds + (slot ^ 1) * G::SLOT + wave * Stage<false, MI>::BYTES, p, u, p.T, p.N,
                                             wrow, wcol);
-        if (!more) break;
-        u = n;
         vb += gridDim.x;
+        if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) break;
         clear(acc);
     }
 }

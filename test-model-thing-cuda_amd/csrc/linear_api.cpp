@@ -30,10 +30,16 @@ int check_rows(int32_t format, int32_t dtype, int32_t rows, int32_t K, const voi
     return TMT_MOE_OK;
 }
 
+// The kernels' offsets inside a tile are 32-bit.
+constexpr int64_t kMaxStride = int64_t(1) << 22;   // elements between rows
+constexpr int64_t kMaxScaleStride = int64_t(1) << 27;
+constexpr int32_t kMaxWidth = 1 << 22;             // N and K
+
 int check_shape(int32_t T, int32_t N, int32_t K) {
     if (T < 0) return fail(TMT_MOE_EINVAL, "T=%d < 0", T);
     if (N <= 0 || N % 16 != 0) return fail(TMT_MOE_EINVAL, "N=%d must be a positive multiple of 16", N);
     if (K <= 0 || K % 64 != 0) return fail(TMT_MOE_EINVAL, "K=%d must be a positive multiple of 64", K);
+    if (N > kMaxWidth || K > kMaxWidth) return fail(TMT_MOE_EINVAL, "N=%d and K=%d must be at most %d", N, K, kMaxWidth);
     return TMT_MOE_OK;
 }
 
@@ -43,6 +49,7 @@ int check_matrix(const char* what, const void* p, int64_t ld, int width, int pie
     if (ld < width || ld % piece != 0)
         return fail(TMT_MOE_EINVAL, "the row stride %lld of %s must be a multiple of %d, at least %d", (long long)ld,
                     what, piece, width);
+    if (ld > kMaxStride) return fail(TMT_MOE_EINVAL, "the row stride %lld of %s is over %lld", (long long)ld, what, (long long)kMaxStride);
     return TMT_MOE_OK;
 }
 
@@ -54,6 +61,8 @@ int check_mx(const char* what, const uint8_t* codes, const uint8_t* scales, int6
     if (lds < rows || lds % 16 != 0)
         return fail(TMT_MOE_EINVAL, "the scale stride %lld of %s must be a multiple of 16, at least %d", (long long)lds,
                     what, rows);
+    if (lds > kMaxScaleStride)
+        return fail(TMT_MOE_EINVAL, "the scale stride %lld of %s is over %lld", (long long)lds, what, (long long)kMaxScaleStride);
     return TMT_MOE_OK;
 }
 
