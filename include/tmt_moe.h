@@ -393,7 +393,8 @@ int tmt_moe_f32_to_bf16(void* stream, const float* in, uint16_t* out, int64_t n)
  * tmt_moe_forward_mxfp4.
  *
  * Every product sums exact terms in fp32 (a code times its scale is exact in
- * bf16) and rounds once. Y = beta * Y + ...; with beta == 0 the output is
+ * bf16; MXFP8 values at scale bytes below 3 are rounded to bf16's subnormals)
+ * and rounds once. Y = beta * Y + ...; with beta == 0 the output is
  * not read. Outputs must not overlap inputs. T any number >= 0, N a multiple
  * of 16, K a multiple of 64, both and all row strides at most 2^22, scale
  * strides at most 2^27. Strides are in elements; bf16 and fp32 rows start

@@ -730,8 +730,8 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     // 256 x 256 tiles read a k16 step's fragments under the MFMAs of the step
     // before. A k16 step of a 128 x 128 tile is four MFMAs, shorter than an LDS
     // read: both steps' fragments are read right behind the barrier, the second
-    // step's into f[1] and f[2] in turn (T 777, N 1024, K 4096, one workgroup
-    // per CU: dX 21.2 us step by step, FASTER).
+    // step's into f[1] and f[2] in turn (step by step / so: dX T 777, N 1024, K
+    // 4096 18.3 / 17.9 us, dW T 2048, N 1280, K 1280 24.7 / 24.1).
     constexpr bool PAIR = MI == 2;
     Frag f[PAIR ? 3 : 2];
     auto first = [&]() {  // fragments of a unit's first sub-step, as far as the loop has them there
@@ -827,6 +827,10 @@ __device__ __forceinline__ f32x16 mma_mx(i32x4 w, i32x4 x, f32x16 c, int ws, int
                                                            __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4,
                                                            G, ws, G, xs);
 }
+// FULL: K is a multiple of 256, and no branch stands between a step's reads and
+// its MFMAs (T 16384, N 4096, K 4096 185 -> 175 us, T 16384, N 16384, K 8192
+// 1319 -> 1201).
+//
 // 128 x 128 outputs, ring of 2. A unit's first step is loaded before the
 // previous unit's epilogue, which stages through the other slot.
 struct Mx {
@@ -836,7 +840,7 @@ struct Mx {
     static constexpr int LDS = 2 * SLOT;
 };
 
-template <bool SPLIT>
+template <bool SPLIT, bool FULL>
 __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, LinearPlan pl) {
     using G = Mx;
     constexpr int MI = G::MI, WT = G::WT, TILE = G::TILE;
@@ -907,30 +911,41 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
             lds_barrier();  // step k is whole in LDS, and the other slot is read
             if (left) load_step();
             const uint8_t* st = lds + slot * G::SLOT;
-            const int groups = min(4, (u.kend - k) / 64);
+            const int groups = FULL ? 4 : min(4, (u.kend - k) / 64);
             int as[MI], bs[MI];
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 as[i] = read_scales(st + 2 * G::CODES, wrow + 32 * i, lane);
                 bs[i] = read_scales(st + 2 * G::CODES + 1024, wcol + 32 * i, lane);
             }
-            auto group = [&](auto g_) {
-                constexpr int g = decltype(g_)::value;
+            struct Frag {
                 i32x4 a[MI], b[MI];
+            } f[2];
+            auto read = [&](Frag& f, int g) {
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
-                    a[i] = read_block(st, wrow + 32 * i + (lane & 31), 2 * g + (lane >> 5));
-                    b[i] = read_block(st + G::CODES, wcol + 32 * i + (lane & 31), 2 * g + (lane >> 5));
+                    f.a[i] = read_block(st, wrow + 32 * i + (lane & 31), 2 * g + (lane >> 5));
+                    f.b[i] = read_block(st + G::CODES, wcol + 32 * i + (lane & 31), 2 * g + (lane >> 5));
                 }
+            };
+            auto mma = [&](auto g_, const Frag& f) {
+                constexpr int g = decltype(g_)::value;
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int j = 0; j < MI; ++j) acc[i][j] = mma_mx<g>(b[j], a[i], acc[i][j], bs[j], as[i]);
+                    for (int j = 0; j < MI; ++j) acc[i][j] = mma_mx<g>(f.b[j], f.a[i], acc[i][j], bs[j], as[i]);
             };
-            group(std::integral_constant<int, 0>{});
-            if (groups > 1) group(std::integral_constant<int, 1>{});
-            if (groups > 2) group(std::integral_constant<int, 2>{});
-            if (groups > 3) group(std::integral_constant<int, 3>{});
+            read(f[0], 0);
+            read(f[1], 1);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(std::integral_constant<int, 0>{}, f[0]);
+            read(f[0], 2);
+            __builtin_amdgcn_sched_barrier(0);
+            if (groups > 1) mma(std::integral_constant<int, 1>{}, f[1]);
+            read(f[1], 3);
+            __builtin_amdgcn_sched_barrier(0);
+            if (groups > 2) mma(std::integral_constant<int, 2>{}, f[0]);
+            if (groups > 3) mma(std::integral_constant<int, 3>{}, f[1]);
             slot ^= 1;
         }
         lds_barrier();  // the last step's slot is read: the epilogue stages there
@@ -1139,7 +1154,7 @@ LinearPlan plan_tiles(const Sizes& z, int tile, int64_t parts) {
 struct StepTimes {
     double start, one, two, large;
 };
-constexpr StepTimes kTimes[4] = {{4.5, 0.60, 1.0, 1.4}, {3.0, 0.30, 0.48, 0.0}, {5.5, 0.90, 1.2, 1.75}, {5.5, 0.90, 1.15, 1.8}};
+constexpr StepTimes kTimes[4] = {{4.5, 0.62, 1.05, 1.45}, {2.5, 0.28, 0.48, 0.0}, {4.2, 0.82, 1.35, 1.75}, {4.2, 0.82, 1.35, 1.8}};
 // A split reduction adds a launch for the sums and its partial tiles' way
 // through the last-level cache and back.
 constexpr double kSplitStart = 3.5, kSplitPerMiB = 0.25;
@@ -1161,10 +1176,11 @@ double plan_time(const StepTimes& t, const Sizes& z, int tile, int64_t parts) {
 }
 
 // The tile size and split with the shortest estimate. Measured (us, chosen /
-// others): forward T 777, N 4096, K 1024 14.4 whole 128 x 128 tiles / 23.2 in
-// two parts, 28.4 on 256 x 256; T 777, N 1024, K 4096 21.3 in four parts /
-// 38.2 whole, 51.9 on 256 x 256 in two; dW T 32768, N 4096, K 1024 290 on
-// 256 x 256 tiles in four parts / 373 on 128 x 128 in two, 860 whole.
+// others): forward T 777, N 4096, K 1024 14.9 on whole 128 x 128 tiles / 23.7 in
+// two parts, 30.2 on 256 x 256; T 777, N 1024, K 4096 20.7 in four parts / 27.2
+// in two, 38.2 whole; dX T 777, N 4096, K 1024 23.9 in four parts / 28.5 in
+// three; dW T 32768, N 1024, K 1024 95 on 256 x 256 tiles in 16 parts / 107 on
+// 128 x 128 in 8; T 16384, N 256, K 256 16.7 in 32 parts / 32 in 8.
 LinearPlan linear_plan(LinearOp op, int T, int N, int K, double* us = nullptr) {
     const Sizes z = sizes(op, T, N, K);
     const StepTimes& t = kTimes[op];
@@ -1187,8 +1203,10 @@ LinearPlan linear_plan(LinearOp op, int T, int N, int K, double* us = nullptr) {
 template <int OP, int TILE, bool SPLIT>
 void launch_units(const LinearParams& p, const LinearPlan& pl, int units, hipStream_t s) {
     const int grid = std::min((units + 7) & ~7, (int)tile_slots(TILE) & ~7);
-    if constexpr (OP == LINEAR_MATMUL) linear_mx_kernel<SPLIT><<<grid, 256, 0, s>>>(p, pl);
-    else if constexpr (OP == LINEAR_FORWARD) linear_fwd_kernel<TILE, SPLIT><<<grid, 256, 0, s>>>(p, pl);
+    if constexpr (OP == LINEAR_MATMUL) {
+        if (p.K % 256 == 0) linear_mx_kernel<SPLIT, true><<<grid, 256, 0, s>>>(p, pl);
+        else linear_mx_kernel<SPLIT, false><<<grid, 256, 0, s>>>(p, pl);
+    } else if constexpr (OP == LINEAR_FORWARD) linear_fwd_kernel<TILE, SPLIT><<<grid, 256, 0, s>>>(p, pl);
     else linear_grad_kernel<OP, TILE, SPLIT><<<grid, 256, 0, s>>>(p, pl);
 }
 template <int OP, int TILE>

@@ -229,14 +229,15 @@ class Problem:
     def magnitude(self):
         return self._product(np.abs(self.A), np.abs(self.B))
 
-    def check(self, y, init=None, beta=0.0):
+    def check(self, y, init=None, beta=0.0, more=0.0):
+        """more: a further absolute tolerance per output."""
         ref, mag = self.reference(), self.magnitude()
         R = {"linear": self.K, "matmul": self.K, "dx": self.N, "dw": self.T}[self.op]
         if init is not None:
             ref = ref + beta * init.astype(np.float64)
             mag = mag + abs(beta) * np.abs(init)
         got = y.double().cpu().numpy()
-        tol = (R + 4) * 2.0 ** -23 * mag + np.abs(ref) * (2.0 ** -24 if self.op == "dw" else 2.0 ** -8)
+        tol = (R + 4) * 2.0 ** -23 * mag + np.abs(ref) * (2.0 ** -24 if self.op == "dw" else 2.0 ** -8) + more
         far = np.abs(got - ref) - tol
         worst = np.unravel_index(np.nanargmax(np.where(np.isnan(far), np.inf, far)), far.shape)
         assert (far <= 0).all(), (worst, got[worst], ref[worst], tol[worst])
@@ -539,3 +540,133 @@ def test_expert_weights_from_the_quantiser():
         outs.append(Y.cpu())
         m.close()
     assert torch.equal(*outs)
+
+
+# ---- dispatch, ends of memory, streams ----------------------------------------------
+
+
+@pytest.mark.parametrize("op,T,N,K,kernels", [
+    ("linear", 1, 4096, 1024, ["linear_rows_kernelILi1ELi1ELi8ELi1E"]),
+    ("linear", 16, 1024, 4096, ["linear_rows_kernelILi1ELi1ELi8ELi2E"]),
+    ("linear", 64, 4096, 1024, ["linear_rows_kernelILi1ELi2ELi4ELi2E"]),
+    ("linear", 64, 4096, 2048, ["linear_rows_kernelILi1ELi2ELi8ELi2E"]),
+    ("linear", 128, 4096, 1024, ["linear_rows_kernelILi2ELi2ELi4ELi2E"]),
+    ("linear", 256, 2048, 2048, ["linear_rows_kernelILi2ELi2ELi8ELi1E"]),
+    ("linear", 600, 1280, 1024, ["linear_rows_kernelILi4ELi2ELi4ELi1E"]),
+    ("linear", 777, 4096, 1024, ["linear_fwd_kernelILi128ELb0E"]),
+    ("linear", 777, 1024, 4096, ["linear_fwd_kernelILi128ELb1E", "linear_fixup_kernelILi128ELb0E"]),
+    ("linear", 16384, 4096, 1024, ["linear_fwd_kernelILi256ELb0E"]),
+    ("matmul", 777, 4096, 1024, ["linear_mx_kernelILb0ELb1E"]),
+    ("matmul", 777, 4096, 960, ["linear_mx_kernelILb0ELb0E"]),
+    ("matmul", 128, 256, 8192, ["linear_mx_kernelILb1ELb1E", "linear_fixup_kernelILi128ELb0E"]),
+    ("matmul", 128, 256, 8128, ["linear_mx_kernelILb1ELb0E", "linear_fixup_kernelILi128ELb0E"]),
+    ("dx", 1024, 256, 256, ["linear_grad_kernelILi2ELi128ELb0E"]),
+    ("dx", 64, 4096, 256, ["linear_grad_kernelILi2ELi128ELb1E", "linear_fixup_kernelILi128ELb0E"]),
+    ("dx", 16384, 1024, 4096, ["linear_grad_kernelILi2ELi256ELb0E"]),
+    ("dw", 128, 1024, 1024, ["linear_grad_kernelILi3ELi128ELb0E"]),
+    ("dw", 2048, 256, 256, ["linear_grad_kernelILi3ELi128ELb1E", "linear_fixup_kernelILi128ELb1E"]),
+    ("dw", 4096, 4096, 4096, ["linear_grad_kernelILi3ELi256ELb0E"]),
+    ("dw", 16384, 4096, 1024, ["linear_grad_kernelILi3ELi256ELb1E", "linear_fixup_kernelILi256ELb1E"]),
+])
+def test_every_kernel_variant(op, T, N, K, kernels):
+    """Each shape reaches the kernels that the plan should choose for it, and
+    its result holds."""
+    from launched_kernels import launched_kernels
+    p = _run(op, T, N, K)
+    _, y = p.output()
+    ws = p.workspace()
+    names = launched_kernels(lambda: p.call(y, ws))
+    assert len(names) == len(kernels), names
+    for want, name in zip(kernels, names):
+        assert want in name, (want, name)
+
+
+@pytest.mark.parametrize("op,T,N,K,kernel", [
+    ("linear", 70 * 256, 1024, 4096, "linear_fwd_kernelILi256E"),
+    ("dx", 70 * 256, 4096, 1024, "linear_grad_kernelILi2ELi256E"),
+])
+def test_whole_rounds_and_a_split_tail(op, T, N, K, kernel):
+    """More tiles than fit at a time: whole ones, then the last round's parts
+    and their sums."""
+    from launched_kernels import launched_kernels
+    p = _run(op, T, N, K)
+    _, y = p.output()
+    ws = p.workspace()
+    names = launched_kernels(lambda: p.call(y, ws))
+    assert [kernel + "Lb0E" in names[0], kernel + "Lb1E" in names[1], "linear_fixup_kernelILi256ELb0E" in names[2]] == [True] * 3, names
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_operands_at_the_end_of_their_memory(op):
+    """Operands that fill their allocations to the last byte (32 MiB, its own
+    mapping), several units to a workgroup: nothing behind them is read."""
+    torch.cuda.empty_cache()
+    T = N = 4096
+    K = 4096
+    big = 16384 if op != "dw" else 4096
+    T = big if op in ("linear", "matmul", "dx") else T
+    N = 1024 if op in ("linear", "matmul", "dx") else N
+    p = Problem(op, T, N, K if op != "dx" else 1024, seed=1)
+    hold = []
+    def own(t):  # t's values at the end of an allocation of whole 2 MiB pages
+        n = t.numel() * t.element_size()
+        page = 2 << 20
+        whole = max((n + page - 1) // page * page, 12 << 20)
+        buf = torch.empty(whole, dtype=torch.uint8, device="cuda")
+        hold.append(buf)
+        view = buf[whole - n:].view(t.dtype).view(t.shape)
+        view.copy_(t)
+        return view
+    p.codes, p.scales = own(p.codes), own(p.scales)
+    if op == "matmul":
+        p.x = (own(p.x[0]), own(p.x[1]))
+    else:
+        p.x = own(p.x.contiguous())
+    _, y = p.output()
+    p.call(y, p.workspace())
+    p.check(y)
+
+
+def test_the_smallest_scales():
+    """Scale byte 0 is 2^-127, in every product. MXFP4 values are multiples of
+    2^-128 there, which bf16 holds (its subnormals are multiples of 2^-133);
+    MXFP8 values are multiples of 2^-136 and each is rounded to a subnormal,
+    off by at most 2^-134: the sum of |dY| times that comes on top."""
+    for op in OPS:
+        p = Problem(op, 20, 32, 128, seed=7, spread=0.1)
+        p.mx_s[:] = 0
+        p.B = mx_ref.dequantize(p.mx_c, p.mx_s, FP8 if op == "dw" else FP4)
+        if op == "matmul":
+            p.xs[:] = 250
+            p.A = mx_ref.dequantize(p.xc, p.xs, FP4)
+        else:
+            p.A = _bf16(p.A * 2.0 ** 100).astype(np.float64)
+        p.upload()
+        _, y = p.output()
+        p.call(y, p.workspace())
+        p.check(y, more=np.abs(p.A).sum(0)[:, None] * 2.0 ** -134 if op == "dw" else 0.0)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams, a workspace each."""
+    ps = [Problem(op, 777, 1024, 2048, seed=s) for s, op in enumerate(("linear", "dw"))]
+    outs, wss = [p.output()[1] for p in ps], [p.workspace() for p in ps]
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for p, y, ws, st in zip(ps, outs, wss, streams):
+            with torch.cuda.stream(st):
+                p.call(y, ws)
+    torch.cuda.synchronize()
+    for p, y in zip(ps, outs):
+        p.check(y)
+
+
+def test_the_stream_argument():
+    p = Problem("linear", 5, 64, 128)
+    _, y = p.output()
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    tmt_moe.mxfp4_linear(p.x, p.codes, p.scales, y, workspace=p.workspace(), stream=st)
+    st.synchronize()
+    p.check(y)
