@@ -506,9 +506,9 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, R, vb, u)) return;
 
-    // ---- the next sub-steps to load, of the activations and of the raw codes:
-    // windows on them, and the sub-steps left in their units (which fill K = 64
-    // steps). Past the last unit the windows are empty.
+    // ---- the next K = 64 steps to load, of the activations and of the raw codes:
+    // windows on them, and the steps left in their units. Past the last unit the
+    // windows are empty.
     constexpr int AC = TILE / 8;                // 16-byte chunks per row of a tile across the reduction
     constexpr int PPR = G::ROWQ / 16;           // 16-byte pieces per raw row
     constexpr int QL = G::Q_BYTES / 1024;       // wave loads of a raw tile (fewer than the waves: loaded twice)
@@ -520,11 +520,11 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     uint32_t a_skip = 0, q_skip = 0;            // bytes of a row outside the window behind the last row
     int sla = 0, slq = 0;                       // ring slots of the next loads
     auto rows_window = [](int rows, uint32_t row_bytes, uint32_t skip) {
-        return rows > 0 ? (uint32_t)min(rows, 32) * row_bytes - skip : 0u;
+        return rows > 0 ? (uint32_t)min(rows, 64) * row_bytes - skip : 0u;
     };
-    auto substeps = [](const Unit& n) { return ((n.kend - n.kbeg + 63) >> 6) * 2; };
+    auto steps = [](const Unit& n) { return (n.kend - n.kbeg + 63) >> 6; };
     auto set_a = [&](const Unit& n) {
-        a_left = substeps(n);
+        a_left = steps(n);
         if constexpr (DW) {
             a_rows = n.kend - n.kbeg;
             a_skip = ldb - (uint32_t)(p.N - n.m0) * 2;
@@ -535,7 +535,7 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
         }
     };
     auto set_q = [&](const Unit& n) {
-        q_left = substeps(n);
+        q_left = steps(n);
         q_rows = n.kend - n.kbeg;
         q_skip = (uint32_t)n.c0 * G::CB / 8;
         wq = {address(p.w + n.kbeg * rowq + q_skip), rows_window(q_rows, rowb, q_skip)};
@@ -544,12 +544,13 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     };
     set_a(u);
     set_q(u);
-    uint32_t a_off[NA], q_off[G::Q_LOADS];
+    // DW and raw codes: [half][load], the lane's piece of a K = 64 step's half
+    uint32_t a_off[2 * G::A_LOADS], q_off[2][G::Q_LOADS];
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
+    for (int i = 0; i < 2 * G::A_LOADS; ++i) {
         if constexpr (DW) {  // a 32-row tile, row k, chunk c
-            const int k = (64 / AC) * (wave * G::A_LOADS + i) + lane / AC, c = (lane % AC) ^ (4 * (k & 3));
-            a_off[i] = (uint32_t)k * ldb + c * 16;
+            const int k = (64 / AC) * (wave * G::A_LOADS + i % G::A_LOADS) + lane / AC, c = (lane % AC) ^ (4 * (k & 3));
+            a_off[i] = (uint32_t)(k + 32 * (i / G::A_LOADS)) * ldb + c * 16;
         } else {
             const int r = 8 * (wave * NA + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
             a_off[i] = (uint32_t)r * ldb + c * 16;
@@ -558,30 +559,32 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
 #pragma unroll
     for (int i = 0; i < G::Q_LOADS; ++i) {
         const int s = ((wave * G::Q_LOADS + i) % QL) * 64 + lane;
-        q_off[i] = (uint32_t)(s / PPR) * rowb + (s % PPR) * 16;
+        q_off[0][i] = (uint32_t)(s / PPR) * rowb + (s % PPR) * 16;
+        q_off[1][i] = q_off[0][i] + 32 * rowb;
     }
     const uint32_t sc_off = (uint32_t)(lane >> 3) * (uint32_t)p.wlds + 4 * (lane & 7);
     constexpr int ND = G::Q_LOADS + 1 + G::A_LOADS;  // loads per wave and sub-step, raw codes first
-    // load d of the next raw tile (codes, scales) or of the next sub-step's
-    // activations (DX: `half` of the rows of a K = 64 tile)
-    auto load = [&](int d, int half) {
+    // Load d of a raw tile (codes, scales) or of a sub-step's activations, which
+    // half of their K = 64 steps they are (DX: which half of the rows).
+    auto load = [&](int d, int q_half, int a_half) {
         const uint32_t raw = lds0 + G::R0 + slq * G::R_BYTES, act = lds0 + G::A0 + sla * G::A_BYTES;
         if (d < G::Q_LOADS) {
-            dma16(wq, q_off[d], raw + ((wave * G::Q_LOADS + d) % QL) * 1024);
+            dma16(wq, q_off[q_half][d], raw + ((wave * G::Q_LOADS + d) % QL) * 1024);
         } else if (d == G::Q_LOADS) {
-            dma4(wsc, sc_off, raw + G::Q_BYTES);
+            dma4(wsc, sc_off + 32 * q_half, raw + G::Q_BYTES);
         } else {
-            const int i = d - G::Q_LOADS - 1 + (DW ? 0 : half * G::A_LOADS);
-            dma16(wa, a_off[i], act + (wave * NA + i) * 1024);
+            const int i = d - G::Q_LOADS - 1;
+            dma16(wa, a_off[a_half * G::A_LOADS + i], act + (wave * NA + i + (DW ? 0 : a_half * G::A_LOADS)) * 1024);
         }
     };
-    auto next_q = [&]() {
+    // behind a raw tile's loads, and behind a sub-step's activations
+    auto next_q = [&](int half) {
         slq = slq == 2 ? 0 : slq + 1;
-        if (q_left == 0) return;  // no unit left: the windows stay empty
+        if (half == 0 || q_left == 0) return;
         if (--q_left > 0) {
-            q_rows -= 32;
-            wq = {wq.at + 32 * rowq, rows_window(q_rows, rowb, q_skip)};
-            wsc = {wsc.at + 32, (uint32_t)max((int)wsc.bytes - 32, 0)};
+            q_rows -= 64;
+            wq = {wq.at + 64 * rowq, rows_window(q_rows, rowb, q_skip)};
+            wsc = {wsc.at + 64, (uint32_t)max((int)wsc.bytes - 64, 0)};
             return;
         }
         Unit n;
@@ -596,12 +599,12 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     auto next_a = [&](int half) {
         if (DW) sla = (sla + 1) & 3;
         else if (half == 1) sla = sla == 2 ? 0 : sla + 1;
-        if (a_left == 0) return;
+        if (half == 0 || a_left == 0) return;
         if (--a_left > 0) {
             if constexpr (DW) {
-                a_rows -= 32;
-                wa = {wa.at + 32 * (uint64_t)ldb, rows_window(a_rows, ldb, a_skip)};
-            } else if (half == 1) {
+                a_rows -= 64;
+                wa = {wa.at + 64 * (uint64_t)ldb, rows_window(a_rows, ldb, a_skip)};
+            } else {
                 wa = {wa.at + 128, wa.bytes - 128};
             }
             return;
@@ -703,17 +706,17 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
 
     // ---- stream ----------------------------------------------------------------
     // raw tiles 0 .. 2 and the activations of sub-steps 0 .. 2 (DW) or 0 .. 3
+#pragma unroll
     for (int t = 0; t < 3; ++t) {
 #pragma unroll
-        for (int d = 0; d <= G::Q_LOADS; ++d) load(d, 0);
-        valid[0] = valid[1];
-        valid[1] = valid[2];
-        valid[2] = q_rows;
-        next_q();
+        for (int d = 0; d <= G::Q_LOADS; ++d) load(d, t & 1, 0);
+        valid[t] = q_rows - 32 * (t & 1);
+        next_q(t & 1);
     }
+#pragma unroll
     for (int t = 0; t < (DW ? 3 : 4); ++t) {
 #pragma unroll
-        for (int d = G::Q_LOADS + 1; d < ND; ++d) load(d, t & 1);
+        for (int d = G::Q_LOADS + 1; d < ND; ++d) load(d, 0, t & 1);
         next_a(t & 1);
     }
     wait_vm<0>();
@@ -763,13 +766,13 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
                         if (NM / 8 + e * 5 * NM / (8 * EP) == q) write_piece(e, h ^ 1, valid[1]);
 #pragma unroll
                     for (int d = 0; d < ND; ++d)
-                        if (d * NM / ND == q) load(d, h);
+                        if (d * NM / ND == q) load(d, h ^ 1, DW ? h ^ 1 : h);
                 });
                 valid[0] = valid[1];
                 valid[1] = valid[2];
-                valid[2] = q_rows;
-                next_q();
-                next_a(h);
+                valid[2] = q_rows - 32 * (h ^ 1);
+                next_q(h ^ 1);
+                next_a(DW ? h ^ 1 : h);
                 // Outstanding at most: the activations of the last sub-step and
                 // all loads of this one. The next sub-step's activations and
                 // the raw codes read in this one are in LDS.
