@@ -395,10 +395,10 @@ int tmt_moe_f32_to_bf16(void* stream, const float* in, uint16_t* out, int64_t n)
  * Every product sums exact terms in fp32 (a code times its scale is exact in
  * bf16; MXFP8 values at scale bytes below 3 are rounded to bf16's subnormals)
  * and rounds once. Y = beta * Y + ...; with beta == 0 the output is
- * not read. Outputs must not overlap inputs. T any number >= 0, N a multiple
+ * not read. Outputs must not overlap inputs. T from 0 to 2^30, N a multiple
  * of 16, K a multiple of 64, both and all row strides at most 2^22, scale
- * strides at most 2^27. Strides are in elements; bf16 and fp32 rows start
- * at 16-byte boundaries (base and stride), codes and scales of a product too
+ * strides at most 2^27, T*N, T*K and N*K at most 2^40. Strides are in elements;
+ * bf16 and fp32 rows start at 16-byte boundaries (base and stride), codes and scales of a product too
  * (scale strides are multiples of 16). Elements between a row's width and its
  * stride are neither read into a result nor written.
  *
@@ -422,7 +422,7 @@ enum { TMT_MOE_BF16 = 0, TMT_MOE_F32 = 1 };
  *           2^-4 of itself or half a step of e4m3's subnormals.
  * Exponents are clamped to [-127, 127]; a block of zeros takes exponent 0; a
  * block with an infinity or a NaN takes s = 255. K a multiple of 32; lds any
- * number >= rows.
+ * number >= rows; rows times K, rounded up to a multiple of 256, under 2^36.
  */
 int tmt_moe_mx_quantize(void* stream, int32_t format, int32_t dtype, const void* X, int64_t ldx, int32_t rows,
                         int32_t K, uint8_t* codes, uint8_t* scales, int64_t lds);

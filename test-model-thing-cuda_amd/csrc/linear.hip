@@ -978,7 +978,8 @@ __global__ __launch_bounds__(64 * NW) void linear_rows_kernel(LinearParams p) {
     uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16 * NB, t0 = blockIdx.y * 16 * RB;
+    const int nb = (p.N + 16 * NB - 1) / (16 * NB);  // blocks of columns, which run fastest
+    const int n0 = (int)(blockIdx.x % nb) * 16 * NB, t0 = (int)(blockIdx.x / nb) * 16 * RB;
     const int K = p.K, pieces = (K + 127) / 128;
     const uint8_t* wq[NB];
     const uint8_t* wsc[NB];
@@ -1109,13 +1110,14 @@ __global__ __launch_bounds__(256) void linear_fixup_kernel(LinearParams p, Linea
     }
 }
 
-// dW = beta dW: the weight gradient over no tokens.
+// dW = beta dW: the weight gradient over no tokens. Four values a thread; the
+// workgroups stride over the matrix.
 __global__ __launch_bounds__(256) void linear_scale_kernel(float* y, int64_t ldy, int rows, int cols, float beta) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int r = (int)(i / cols), c = (int)(i % cols);
-    if (r >= rows) return;
-    float* o = y + (int64_t)r * ldy + c;
-    *o = beta != 0.0f ? beta * *o : 0.0f;
+    const int pieces = cols / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * pieces; i += (int64_t)gridDim.x * 256) {
+        f32x4* o = reinterpret_cast<f32x4*>(y + i / pieces * ldy + i % pieces * 4);
+        *o = beta != 0.0f ? beta * *o : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 }
 
 struct Sizes {
@@ -1225,19 +1227,24 @@ void launch_tiles(const LinearParams& p, const LinearPlan& pl, hipStream_t s) {
 
 template <int RB, int NB, int NW, int U>
 void launch_rows_as(const LinearParams& p, hipStream_t s) {
-    const dim3 grid((p.N + 16 * NB - 1) / (16 * NB), (p.T + 16 * RB - 1) / (16 * RB));
-    linear_rows_kernel<RB, NB, NW, U><<<grid, 64 * NW, 0, s>>>(p);
+    const int64_t grid = (int64_t)((p.N + 16 * NB - 1) / (16 * NB)) * ((p.T + 16 * RB - 1) / (16 * RB));
+    linear_rows_kernel<RB, NB, NW, U><<<(unsigned)grid, 64 * NW, 0, s>>>(p);
 }
-// The kernel for few tokens where its estimate, 3 us and 7.2 us for each 10^9
-// products (measured over T 1 .. 777, N and K 256 .. 4096), is below the
-// tiles'. Blocks of outputs grow with the grid, which fills the chip twice at
-// most: 16 x 16, 16 x 32 (columns), 32 x 32, 64 x 32. Measured (us) 16 x 16 /
-// 16 x 32 / 32 x 32 / 64 x 32: T 16, N 1024, K 4096 4.7 / 6.4 / 7.6 / 8.8; T
-// 64, N 4096, K 1024 4.8 / 4.6 / 4.7 / 6.4; T 256, N 4096, K 1024 13.8 / 11.4 /
-// 11.2 / 10.0. Reductions of more than 8 pieces take 8 waves with two pieces in
-// flight (32 x 32: one), shorter ones 4 waves with two (16 x 16: 8 with one).
-bool launch_rows(const LinearParams& p, double tiles_us, hipStream_t s) {
-    if (3.0 + 7.2e-9 * ((double)p.T * p.N * p.K) > tiles_us) return false;
+// The kernel for few tokens runs where its estimate in us, measured over T 1 ..
+// 777, N and K 256 .. 4096, is not above the tiles'. T 777, N 1024, K 1024 10.1
+// (tiles 13.6), T 512, N 4096, K 1024 17.7 (tiles 14.2).
+// The kernel for few tokens stays below 2^22 workgroups; a launch holds 2^32 threads.
+double rows_time(int T, int N, int K) {
+    if ((int64_t)T * N >= (int64_t)1 << 30) return 1e30;
+    return 3.0 + 7.2e-9 * ((double)T * N * K);
+}
+// Blocks of outputs grow with the grid, which fills the chip twice at most: 16 x
+// 16, 16 x 32 (columns), 32 x 32, 64 x 32. Measured (us) 16 x 16 / 16 x 32 / 32 x
+// 32 / 64 x 32: T 16, N 1024, K 4096 4.7 / 6.4 / 7.6 / 8.8; T 64, N 4096, K 1024
+// 4.8 / 4.6 / 4.7 / 6.4; T 256, N 4096, K 1024 13.8 / 11.4 / 11.2 / 10.0.
+// Reductions of more than 8 pieces take 8 waves with two pieces in flight (32 x
+// 32: one), shorter ones 4 waves with two (16 x 16: 8 with one).
+void launch_rows(const LinearParams& p, hipStream_t s) {
     const int64_t most = 2 * (int64_t)cu_count(), n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32;
     const int64_t t16 = (p.T + 15) / 16, t32 = (p.T + 31) / 32;
     const bool many = p.K > 1024;
@@ -1245,7 +1252,6 @@ bool launch_rows(const LinearParams& p, double tiles_us, hipStream_t s) {
     else if (n32 * t16 <= most) many ? launch_rows_as<1, 2, 8, 2>(p, s) : launch_rows_as<1, 2, 4, 2>(p, s);
     else if (n32 * t32 <= most) many ? launch_rows_as<2, 2, 8, 1>(p, s) : launch_rows_as<2, 2, 4, 2>(p, s);
     else launch_rows_as<4, 2, 4, 1>(p, s);
-    return true;
 }
 
 }  // namespace
@@ -1270,13 +1276,16 @@ hipError_t launch_linear(LinearOp op, const LinearParams& p, hipStream_t s) {
     if (op != LINEAR_DW && p.T <= 0) return hipSuccess;
     if (op == LINEAR_DW && p.T == 0) {
         if (p.beta == 1.0f) return hipSuccess;
-        const int64_t n = (int64_t)p.N * p.K;
-        linear_scale_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(static_cast<float*>(p.y), p.ldy, p.N, p.K, p.beta);
+        const int64_t blocks = std::min<int64_t>(((int64_t)p.N * p.K / 4 + 255) / 256, 16 * (int64_t)cu_count());
+        linear_scale_kernel<<<(unsigned)blocks, 256, 0, s>>>(static_cast<float*>(p.y), p.ldy, p.N, p.K, p.beta);
         return hipGetLastError();
     }
     double us = 0.0;
     const LinearPlan pl = linear_plan(op, p.T, p.N, p.K, &us);
-    if (op == LINEAR_FORWARD && launch_rows(p, us, s)) return hipGetLastError();
+    if (op == LINEAR_FORWARD && rows_time(p.T, p.N, p.K) <= us) {
+        launch_rows(p, s);
+        return hipGetLastError();
+    }
     const bool big = pl.tile == 256;
     switch (op) {
         case LINEAR_FORWARD: big ? launch_tiles<LINEAR_FORWARD, 256>(p, pl, s) : launch_tiles<LINEAR_FORWARD, 128>(p, pl, s); break;

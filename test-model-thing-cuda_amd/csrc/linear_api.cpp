@@ -12,6 +12,8 @@ static_assert((int)TMT_MOE_LINEAR_FORWARD == LINEAR_FORWARD && (int)TMT_MOE_LINE
 
 namespace {
 
+constexpr int64_t kMaxValues = int64_t(1) << 36;  // quantised by one call: a launch holds 2^32 threads
+
 int check_rows(int32_t format, int32_t dtype, int32_t rows, int32_t K, const void* X, int64_t ldx,
                const uint8_t* codes, const uint8_t* scales, int64_t lds) {
     if (format != TMT_MOE_MX_FP4 && format != TMT_MOE_MX_FP8)
@@ -21,6 +23,8 @@ int check_rows(int32_t format, int32_t dtype, int32_t rows, int32_t K, const voi
     if (rows < 0) return fail(TMT_MOE_EINVAL, "rows=%d < 0", rows);
     if (K <= 0 || K % 32 != 0) return fail(TMT_MOE_EINVAL, "K=%d must be a positive multiple of 32", K);
     if (rows == 0) return TMT_MOE_OK;
+    if ((int64_t)rows * ((K + 255LL) / 256 * 256) >= kMaxValues)
+        return fail(TMT_MOE_EINVAL, "rows=%d of K=%d, rounded up to 256, are 2^36 values or more", rows, K);
     const int piece = dtype == TMT_MOE_BF16 ? 8 : 4;  // elements of 16 bytes
     if (ldx < K || ldx % piece != 0)
         return fail(TMT_MOE_EINVAL, "ldx=%lld must be a multiple of %d, at least K=%d", (long long)ldx, piece, K);
@@ -34,12 +38,17 @@ int check_rows(int32_t format, int32_t dtype, int32_t rows, int32_t K, const voi
 constexpr int64_t kMaxStride = int64_t(1) << 22;   // elements between rows
 constexpr int64_t kMaxScaleStride = int64_t(1) << 27;
 constexpr int32_t kMaxWidth = 1 << 22;             // N and K
+constexpr int32_t kMaxTokens = 1 << 30;
+constexpr int64_t kMaxOutputs = int64_t(1) << 40;  // of a product, so that 32 bits count the tiles
 
 int check_shape(int32_t T, int32_t N, int32_t K) {
     if (T < 0) return fail(TMT_MOE_EINVAL, "T=%d < 0", T);
     if (N <= 0 || N % 16 != 0) return fail(TMT_MOE_EINVAL, "N=%d must be a positive multiple of 16", N);
     if (K <= 0 || K % 64 != 0) return fail(TMT_MOE_EINVAL, "K=%d must be a positive multiple of 64", K);
     if (N > kMaxWidth || K > kMaxWidth) return fail(TMT_MOE_EINVAL, "N=%d and K=%d must be at most %d", N, K, kMaxWidth);
+    if ((int64_t)T * N > kMaxOutputs || (int64_t)T * K > kMaxOutputs || (int64_t)N * K > kMaxOutputs)
+        return fail(TMT_MOE_EINVAL, "T=%d, N=%d, K=%d: T*N, T*K and N*K must be at most 2^40", T, N, K);
+    if (T > kMaxTokens) return fail(TMT_MOE_EINVAL, "T=%d is over %d", T, kMaxTokens);
     return TMT_MOE_OK;
 }
 

@@ -297,6 +297,8 @@ def _ws(workspace, dev: int) -> tuple:
         return 0, 0
     if workspace.get_device() != dev:
         raise ValueError(f"workspace is on {workspace.device}, not on the current GPU")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 

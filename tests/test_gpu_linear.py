@@ -670,3 +670,49 @@ def test_the_stream_argument():
     tmt_moe.mxfp4_linear(p.x, p.codes, p.scales, y, workspace=p.workspace(), stream=st)
     st.synchronize()
     p.check(y)
+
+
+def test_more_rows_than_a_grid_dimension_of_blocks():
+    """4.3 million tokens of the narrowest layer: more than 65535 blocks of rows."""
+    T, N, K = 4_300_001, 16, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    X = torch.empty(T, K, dtype=BF16, device="cuda").normal_(generator=g)
+    codes = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device="cuda", generator=g)
+    scales = torch.randint(120, 130, (K // 32, N), dtype=torch.uint8, device="cuda", generator=g)
+    Y = torch.full((T + 1, N), 7.0, dtype=BF16, device="cuda")
+    size = tmt_moe.linear_workspace_size(tmt_moe.LINEAR_FORWARD, T, N, K)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda") if size else None
+    tmt_moe.mxfp4_linear(X, codes, scales, Y[:T], workspace=ws)
+    W = torch.empty(N, K, dtype=torch.float32, device="cuda")
+    tmt_moe.mx_dequantize(codes, scales, W, FP4)
+    for at in (0, 2_097_100, 4_194_200, T - 1000):
+        x, w = X[at:at + 1000].double().cpu(), W.double().cpu()
+        want, most = x @ w.T, x.abs() @ w.abs().T
+        assert ((Y[at:min(at + 1000, T)].double().cpu() - want).abs() <= (K + 2) * 2.0 ** -23 * most + 2.0 ** -8 * want.abs()).all()
+    assert (Y[T] == 7.0).all()
+
+
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_no_tokens_over_a_large_matrix(beta):
+    """dW = beta dW past one pass of the launch's workgroups, rows padded."""
+    N, K, ld = 4112, 4160, 4164
+    buf = torch.full((N + 1, ld), 3.0, device="cuda")
+    dW = buf[:N, :K]
+    if beta == 0.0:
+        dW.fill_(float("nan"))
+    dY = torch.empty(0, N, dtype=BF16, device="cuda")
+    codes = torch.empty(0, K, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(K // 32, 16, dtype=torch.uint8, device="cuda")
+    tmt_moe.mxfp8_linear_dw(dY, codes, scales, dW, beta=beta)
+    assert (dW == 3.0 * beta).all()
+    assert (buf[:N, K:] == 3.0).all() and (buf[N] == 3.0).all()
+
+
+def test_a_strided_workspace_is_refused():
+    X = torch.zeros(16, 64, dtype=BF16, device="cuda")
+    codes = torch.zeros(16, 32, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(2, 16, dtype=torch.uint8, device="cuda")
+    Y = torch.zeros(16, 16, dtype=BF16, device="cuda")
+    ws = torch.zeros(64, 64, dtype=torch.uint8, device="cuda")[:, :32]
+    with pytest.raises(ValueError, match="workspace must be contiguous"):
+        tmt_moe.mxfp4_linear(X, codes, scales, Y, workspace=ws)

@@ -126,3 +126,29 @@ def test_the_reference_rounds_to_the_nearest_code():
     assert a.max() <= 448 and np.all(np.abs(x).reshape(64, 3, 32).max(2) * 2 > 448 * mx_ref.e8m0(scales))
     codes, scales = mx_ref.quantize(x, mx_ref.FP4)
     assert np.array_equal(mx_ref.dequantize(codes, scales, mx_ref.FP4), synthetic.mxfp4_dequantize(codes, scales))
+
+
+@pytest.mark.parametrize("rows,K", [(1 << 28, 32), (1 << 28, 256), (1 << 24, 4096), (2 ** 31 - 1, 4096)])
+def test_rows_past_one_launch_are_refused(rows, K):
+    lib = tmt_moe.load_library()
+    refused(lib.tmt_moe_mx_quantize(None, 0, 0, A, i64(K), rows, K, A, A, i64(rows)), "2^36")
+    refused(lib.tmt_moe_mx_dequantize(None, 1, A, A, i64(rows), rows, K, 1, A, i64(K)), "2^36")
+
+
+@pytest.mark.parametrize("op", ["linear", "dx", "dw"])
+@pytest.mark.parametrize("T,N,K,ld", [
+    (2 ** 31 - 1, 1024, 64, 1024), (2 ** 31 - 1, 16, 1024, 1024), (1, 1 << 22, 1 << 20, 1 << 22),
+])
+def test_outputs_past_32_bit_tile_counts_are_refused(op, T, N, K, ld):
+    q = dict(PRODUCT, T=T, N=N, K=K, ldx=ld, ldy=ld, wlds=1 << 22)
+    refused(_product(op, q), "2^40")
+
+
+@pytest.mark.parametrize("change", [dict(ldx=(1 << 22) + 64), dict(ldy=(1 << 22) + 64), dict(wlds=(1 << 27) + 16)])
+@pytest.mark.parametrize("op", ["linear", "dx", "dw"])
+def test_strides_past_the_limits_are_refused(op, change):
+    refused(_product(op, dict(PRODUCT, **change)), "is over")
+
+
+def test_tokens_past_the_limit_are_refused():
+    refused(_product("linear", dict(PRODUCT, T=(1 << 30) + 1)), "T=1073741825 is over")
