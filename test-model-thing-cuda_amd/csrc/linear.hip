@@ -960,6 +960,168 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
     }
 }
 
+// Large products with K a multiple of 256: 256 x 256 outputs, one workgroup per
+// CU, which halves what a product reads from LDS and L2. Ring of 2. A K = 64
+// group of 16 MFMAs runs on registers; in the slots between them the next
+// group's fragments are read and loads are issued. Behind a step's third group
+// the whole slot is in registers: the barrier stands there, the fourth group
+// reads the next slot's first fragments and the freed slot's loads begin. (us,
+// 128 x 128 / 256 x 256, the latter with loads and reads in a bunch ahead of each
+// step: T 16384, N 4096, K 4096 162 / 147, 166 bunched; T = N = 16384, K 8192
+// 1191 / 1037, 1112 bunched, 4.2 PFLOP/s.) Not the matrix cores alone bound it:
+// what a unit's outputs take, 6.5 us at K 256, adds to its steps' 1.85 us each,
+// with CUs in lockstep or spread over a round, so loads wait behind the chip's
+// stores; with codes of zeros T 65536, N 4096, K 1024 still takes 214 us of 222.
+struct MxLarge {
+    static constexpr int TILE = 256, WT = 128, MI = 4;
+    static constexpr int CODES = TILE * 128, SCALES = TILE * 8;  // bytes per operand
+    static constexpr int LOADS = CODES / 4096, ND = 2 * LOADS + 1, FIRST = 9;
+    static constexpr int SLOT = 2 * CODES + 2 * SCALES, ST0 = 2 * SLOT;
+    static constexpr int LDS = ST0 + 4 * Stage<false, 2>::BYTES;
+    static constexpr int STORES = 32;  // of a wave's full output
+    static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+__global__ __launch_bounds__(256, 1) void linear_mx_large_kernel(LinearParams p, LinearPlan pl) {
+    using G = MxLarge;
+    constexpr int MI = G::MI, WT = G::WT, TILE = G::TILE;
+    __shared__ uint4 lds_raw[G::LDS / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const uint32_t lds0 = lds_u32(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT;
+    const int K = p.K;
+    Unit u;
+    int vb = blockIdx.x;
+    if (!unit_at<TILE, false>(pl, K, vb, u)) return;
+
+    // ---- the next step to load, as in linear_fwd_kernel
+    Window wx, wxs, ww, wws;
+    int left = 0, vl = vb, sll = 0;
+    auto set = [&](const Unit& n) {
+        wx = {address(p.xq + (int64_t)n.m0 * (K / 2)), (uint32_t)min(p.T - n.m0, TILE) * (uint32_t)(K / 2)};
+        ww = {address(p.w + (int64_t)n.c0 * (K / 2)), (uint32_t)min(p.N - n.c0, TILE) * (uint32_t)(K / 2)};
+        wxs = {address(p.xs + n.m0), 8 * (uint32_t)p.xlds - n.m0};
+        wws = {address(p.ws + n.c0), 8 * (uint32_t)p.wlds - n.c0};
+        left = K / 256;
+    };
+    set(u);
+    uint32_t off[G::LOADS];
+#pragma unroll
+    for (int i = 0; i < G::LOADS; ++i) {
+        const int r = 8 * (wave * G::LOADS + i) + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        off[i] = (uint32_t)r * (uint32_t)(K / 2) + c * 16;
+    }
+    // even waves: the scales of X, odd waves: of W; 128 rows each
+    const uint32_t sc_off = (uint32_t)(lane & 7) * (uint32_t)((wave & 1) ? p.wlds : p.xlds) + 16 * (lane >> 3) + 128 * (wave >> 1);
+    auto load = [&](int d) {
+        const uint32_t at = lds0 + sll * G::SLOT;
+        const int i = d >> 1;
+        if (d == 2 * G::LOADS) dma16((wave & 1) ? wws : wxs, sc_off, at + 2 * G::CODES + (wave & 1) * G::SCALES + (wave >> 1) * 1024);
+        else if (d & 1) dma16(ww, off[i], at + G::CODES + (wave * G::LOADS + i) * 1024);
+        else dma16(wx, off[i], at + (wave * G::LOADS + i) * 1024);
+    };
+    auto next_loads = [&]() {
+        sll ^= 1;
+        if (left == 0) return;  // no unit left: the windows stay empty
+        if (--left > 0) {
+            wx = {wx.at + 128, wx.bytes - 128};
+            ww = {ww.at + 128, ww.bytes - 128};
+            wxs.at += 8 * p.xlds;
+            wws.at += 8 * p.wlds;
+            return;
+        }
+        Unit n;
+        vl += gridDim.x;
+        if (unit_at<TILE, false>(pl, K, vl, n)) set(n);
+        else wx.bytes = ww.bytes = wxs.bytes = wws.bytes = 0;
+    };
+
+    // ---- fragments
+    struct Frag {
+        i32x4 a[MI], b[MI];
+    } f[2];
+    int as[MI], bs[MI], as2[MI], bs2[MI];
+    auto read = [&](Frag& t, int r, int sl, int g) {  // r: A blocks, then B blocks
+        const uint8_t* st = lds + sl * G::SLOT;
+        if (r < MI) t.a[r] = read_block(st, wrow + 32 * r + (lane & 31), 2 * g + (lane >> 5));
+        else t.b[r - MI] = read_block(st + G::CODES, wcol + 32 * (r - MI) + (lane & 31), 2 * g + (lane >> 5));
+    };
+    auto scales = [&](int r, int sl) {
+        const uint8_t* sc = lds + sl * G::SLOT + 2 * G::CODES;
+        if (r < MI) as2[r] = read_scales(sc, wrow + 32 * r, lane);
+        else bs2[r - MI] = read_scales(sc + G::SCALES, wcol + 32 * (r - MI), lane);
+    };
+    f32x16 acc[MI][MI];
+    // group g; reads group (g + 1) % 4 of slot sl; issues loads [d0, d0 + dn)
+    auto mma = [&](auto g_, const Frag& t, Frag& t2, int sl, int d0, int dn) {
+        constexpr int g = decltype(g_)::value;
+#pragma unroll
+        for (int q = 0; q < MI * MI; ++q) {
+            const int i = q / MI, j = q % MI;
+            acc[i][j] = mma_mx<g>(t.b[j], t.a[i], acc[i][j], bs[j], as[i]);
+            if (q < 2 * MI) read(t2, q, sl, (g + 1) & 3);
+            else if (g == 3) scales(q - 2 * MI, sl);
+#pragma unroll
+            for (int d = 0; d < dn; ++d)
+                if ((2 * d + 1) * MI * MI / (2 * dn) == q) load(d0 + d);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto take_scales = [&]() {
+#pragma unroll
+        for (int r = 0; r < MI; ++r) as[r] = as2[r], bs[r] = bs2[r];
+    };
+
+    // ---- stream
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int d = 0; d < G::ND; ++d) load(d);
+        next_loads();
+    }
+    wait_vm<G::ND>();
+    lds_barrier();
+    int sl = 0;
+#pragma unroll
+    for (int r = 0; r < 2 * MI; ++r) {
+        read(f[0], r, 0, 0);
+        scales(r, 0);
+    }
+    take_scales();
+    bool stored = false;  // the last unit's outputs fill the wave's part: STORES stores behind the loads
+    uint8_t* st = lds + G::ST0 + wave * Stage<false, 2>::BYTES;
+    for (;;) {
+        clear(acc);
+        for (int k = 0; k < K; k += 256) {
+            if (k == 0) {
+                mma(std::integral_constant<int, 0>{}, f[0], f[1], sl, 0, 0);
+            } else {
+                mma(std::integral_constant<int, 0>{}, f[0], f[1], sl, G::FIRST, G::ND - G::FIRST);
+                next_loads();
+            }
+            mma(std::integral_constant<int, 1>{}, f[1], f[0], sl, 0, 0);
+            mma(std::integral_constant<int, 2>{}, f[0], f[1], sl, 0, 0);
+            if (k == 0 && stored) wait_vm<G::STORES>();
+            else wait_vm<0>();
+            lds_barrier();  // this slot is read, the other one is whole
+            sl ^= 1;
+            mma(std::integral_constant<int, 3>{}, f[1], f[0], sl, 0, G::FIRST);
+            take_scales();
+        }
+        // the next unit's second step: its loads stand before the stores
+#pragma unroll
+        for (int d = G::FIRST; d < G::ND; ++d) load(d);
+        next_loads();
+        __builtin_amdgcn_sched_barrier(0);
+        finish_unit<TILE, false, 2, false>(acc, st, p, u, p.T, p.N, wrow, wcol);
+        stored = p.T - u.m0 - wrow >= WT && p.N - u.c0 - wcol >= WT;
+        vb += gridDim.x;
+        if (!unit_at<TILE, false>(pl, K, vb, u)) break;
+    }
+    wait_vm<0>();  // no load may land in LDS that the next workgroup owns
+}
+
 // ---- few tokens -------------------------------------------------------------------
 // A workgroup takes 16 NB output columns (rows of W) and 16 RB tokens; its NW
 // waves deal out the reduction in pieces of K = 128, U pieces in flight. Lane l
@@ -1225,6 +1387,23 @@ void launch_tiles(const LinearParams& p, const LinearPlan& pl, hipStream_t s) {
     }
 }
 
+// Whether 256 x 256 tiles of MXFP4 x MXFP4 are estimated to be faster: their
+// rounds of one tile per CU against two rounds' worth of 128 x 128 tiles at two
+// per CU, from two such rounds on. Measured (us, 128 / 256): T 65536, N 4096, K
+// 512 164 / 164, K 1024 230 / 222; T 16384, N 4096, K 1024 59 / 61; T 65536, N
+// 1024, K 4096 164 / 149; T 20011, N 2736, K 768 47 / 64.
+bool mx_large(int T, int N, int K) {
+    const int64_t small = (int64_t)((T + 127) / 128) * ((N + 127) / 128), big = (int64_t)((T + 255) / 256) * ((N + 255) / 256);
+    if (K % 256 != 0 || small < 2 * tile_slots(128)) return false;
+    const double steps = K / 256, slots2 = (double)tile_slots(128), slots1 = (double)tile_slots(256);
+    return 4.0 + std::ceil(big / slots1) * (6.5 + 1.85 * steps) < std::ceil(small / slots2) * (2.75 + 1.12 * steps);
+}
+void launch_mx_large(const LinearParams& p, hipStream_t s) {
+    const LinearPlan pl = plan_tiles(sizes(LINEAR_MATMUL, p.T, p.N, p.K), 256, 1);
+    const int grid = std::min((pl.whole + 7) & ~7, (int)tile_slots(256) & ~7);
+    linear_mx_large_kernel<<<grid, 256, 0, s>>>(p, pl);
+}
+
 template <int RB, int NB, int NW, int U>
 void launch_rows_as(const LinearParams& p, hipStream_t s) {
     const int64_t grid = (int64_t)((p.N + 16 * NB - 1) / (16 * NB)) * ((p.T + 16 * RB - 1) / (16 * RB));
@@ -1289,7 +1468,10 @@ hipError_t launch_linear(LinearOp op, const LinearParams& p, hipStream_t s) {
     const bool big = pl.tile == 256;
     switch (op) {
         case LINEAR_FORWARD: big ? launch_tiles<LINEAR_FORWARD, 256>(p, pl, s) : launch_tiles<LINEAR_FORWARD, 128>(p, pl, s); break;
-        case LINEAR_MATMUL: launch_tiles<LINEAR_MATMUL, 128>(p, pl, s); break;
+        case LINEAR_MATMUL:
+            if (mx_large(p.T, p.N, p.K)) launch_mx_large(p, s);
+            else launch_tiles<LINEAR_MATMUL, 128>(p, pl, s);
+            break;
         case LINEAR_DX: big ? launch_tiles<LINEAR_DX, 256>(p, pl, s) : launch_tiles<LINEAR_DX, 128>(p, pl, s); break;
         case LINEAR_DW: big ? launch_tiles<LINEAR_DW, 256>(p, pl, s) : launch_tiles<LINEAR_DW, 128>(p, pl, s); break;
         default: return hipErrorInvalidValue;

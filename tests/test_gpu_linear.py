@@ -716,3 +716,19 @@ def test_a_strided_workspace_is_refused():
     ws = torch.zeros(64, 64, dtype=torch.uint8, device="cuda")[:, :32]
     with pytest.raises(ValueError, match="workspace must be contiguous"):
         tmt_moe.mxfp4_linear(X, codes, scales, Y, workspace=ws)
+
+
+@pytest.mark.parametrize("T,N,K,pad,beta", [
+    (8192, 2048, 4096, 0, 0.0), (8100, 2000, 4096, 16, 0.5), (16300, 2000, 2048, 8, 0.0), (4081, 4080, 8192, 0, 0.0),
+    (16384, 2048, 2048, 0, -1.0),
+])
+def test_large_matmul_tiles(T, N, K, pad, beta):
+    """MXFP4 x MXFP4 on 256 x 256 tiles: one round and two, whole and ragged."""
+    from launched_kernels import launched_kernels
+    p = _run("matmul", T, N, K, pad=pad, beta=beta)
+    ws, outs = p.workspace(), [p.output()[1] for _ in range(3)]
+    names = launched_kernels(lambda: p.call(outs[0], ws))
+    assert len(names) == 1 and "linear_mx_large_kernel" in names[0], names
+    for y in outs:
+        p.call(y, ws)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
