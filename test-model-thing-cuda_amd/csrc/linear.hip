@@ -41,6 +41,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
@@ -172,81 +174,111 @@ __device__ __forceinline__ void clear(f32x16 (&acc)[MI][NJ]) {
 }
 
 __device__ __forceinline__ void wave_lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// Keeps the compiler from moving a wave's LDS accesses across.
+__device__ __forceinline__ void wave_lds_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 // out: the wave's first output element, ld its row stride; rows, cols: valid
-// ones. beta times what is there is added in fp32. NT: results are written
-// once and leave the caches to the operands; partial tiles are read again at
-// once.
-template <bool F32, int JS, bool NT, int MI, int NJ>
+// ones. The outputs are a window: rows past its end are dropped by the hardware,
+// columns past the end get an offset past it. BETA: beta times what is there is
+// added in fp32. NT: results are written once and leave the caches to the
+// operands; partial tiles are read again at once.
+//
+// With one wave per SIMD this is bound by its instructions, so it has few: one
+// addition and one store per 1 KiB, no branch (MXFP4 x MXFP4, T 65536, N 4096, K
+// 1024: 222 us with addresses, branches and a sum with beta = 0, 210 without). A
+// slice is converted while the one
+// before comes back from LDS, and its own way through LDS needs no wait: a wave's
+// LDS accesses run in order.
+template <bool F32, int JS, bool NT, bool BETA, int MI, int NJ>
 __device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, void* out, int64_t ld, int rows,
                                            int cols, float beta) {
     using S = Stage<F32, JS>;
     constexpr int CH = S::ROWB / 16, RPI = 64 / CH;  // 16-byte chunks per staged row, rows per store
+    constexpr int JG = NJ / JS, SLICES = MI * JG, SIZE = F32 ? 4 : 2;
+    constexpr uint32_t FAR = 0x80000000u;
     // a value of this unit's own: the addresses below are not kept in registers
     // through the main loop
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
-    const int lr = lane & 31;
+    const int lr = lane & 31, cl = lane % CH;
+    const uint32_t row = (uint32_t)(ld * SIZE);
+    rows = min(rows, 32 * MI);
+    cols = min(cols, 32 * NJ);
+    const __amdgpu_buffer_rsrc_t win =
+        __builtin_amdgcn_make_buffer_rsrc(out, 0, (int)((uint32_t)(rows - 1) * row + (uint32_t)cols * SIZE), 0x00020000);
+    uint4 v[32 / RPI];  // rows of a slice
+    auto store = [&](int n) {
+        const int c = 32 * JS * (n % JG) + cl * (16 / SIZE);
+        uint32_t at = c < cols ? (uint32_t)(32 * (n / JG) + lane / CH) * row + (uint32_t)c * SIZE : FAR;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+        for (int k = 0; k < 32 / RPI; ++k) {
+            if constexpr (F32 && BETA)
+                v[k] = __builtin_bit_cast(uint4, __builtin_bit_cast(f32x4, v[k]) + beta * __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(win, (int)at, 0, 0)));
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), win, (int)at, 0, NT ? 2 : 0);
+            at += RPI * row;
+        }
+    };
 #pragma unroll
-        for (int jg = 0; jg < NJ; jg += JS) {
-            // the outputs not yet staged stay in the accumulator registers
+    for (int n = 0; n < SLICES; ++n) {
+        const int i = n / JG, jg = n % JG * JS;
+        // the outputs not yet staged stay in the accumulator registers
 #pragma unroll
-            for (int i2 = i; i2 < MI; ++i2)
+        for (int i2 = i; i2 < MI; ++i2)
 #pragma unroll
-                for (int j = 0; j < NJ; ++j)
-                    if (i2 > i || j >= jg) asm volatile("" : "+a"(acc[i2][j]));
+            for (int j = 0; j < NJ; ++j)
+                if (i2 > i || j >= jg) asm volatile("" : "+a"(acc[i2][j]));
+        uint2 half[JS][4];
+        if constexpr (!F32) {
 #pragma unroll
-            for (int j = 0; j < JS; ++j) {
-                const f32x16& a = acc[i][jg + j];
-                uint2 old[4] = {};  // bf16 outputs that are added to
-                if (!F32 && beta != 0.0f) {
-                    const uint16_t* y = static_cast<const uint16_t*>(out) + (int64_t)min(32 * i + lr, rows - 1) * ld;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        old[q] = *reinterpret_cast<const uint2*>(y + min(32 * (jg + j) + 8 * q + 4 * (lane >> 5), cols - 4));
-                }
+            for (int j = 0; j < JS; ++j)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    if constexpr (F32) {
-                        const int ch = j * 8 + 2 * q + (lane >> 5);
-                        *reinterpret_cast<f32x4*>(st + lr * S::ROWB + ((ch ^ (lr & (CH - 1))) * 16)) =
-                            f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
-                    } else {
-                        const int ch = j * 4 + q;
-                        *reinterpret_cast<uint2*>(st + lr * S::ROWB + ((ch ^ (lr & (CH - 1))) * 16) + (lane >> 5) * 8) =
-                            make_uint2(pack_bf2(a[4 * q] + beta * bf_lo(old[q].x), a[4 * q + 1] + beta * bf_hi(old[q].x)),
-                                       pack_bf2(a[4 * q + 2] + beta * bf_lo(old[q].y), a[4 * q + 3] + beta * bf_hi(old[q].y)));
+                    const f32x16& a = acc[i][jg + j];
+                    f32x4 f = {a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+                    if constexpr (BETA) {
+                        const int c = 32 * (jg + j) + 8 * q + 4 * (lane >> 5);
+                        const u32x2 old = __builtin_amdgcn_raw_buffer_load_b64(
+                            win, c < cols ? (int)((uint32_t)(32 * i + lr) * row + (uint32_t)c * SIZE) : (int)FAR, 0, 0);
+                        f = f + beta * f32x4{bf_lo(old[0]), bf_hi(old[0]), bf_lo(old[1]), bf_hi(old[1])};
                     }
+                    half[j][q] = make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]));
                 }
-            }
-            wave_lds_fence();
-            const int cl = lane % CH, c = 32 * jg + cl * (F32 ? 4 : 8);
-#pragma unroll
-            for (int k = 0; k < 32 / RPI; ++k) {
-                const int rr = lane / CH + RPI * k, m = 32 * i + rr;
-                const uint4 v = *reinterpret_cast<const uint4*>(st + rr * S::ROWB + ((cl ^ (rr & (CH - 1))) * 16));
-                if (m >= rows || c >= cols) continue;
-                if constexpr (F32) {
-                    float* o = static_cast<float*>(out) + (int64_t)m * ld + c;
-                    f32x4 f = __builtin_bit_cast(f32x4, v);
-                    if (beta != 0.0f) f = f + beta * *reinterpret_cast<const f32x4*>(o);
-                    if (NT) st16_nt(o, __builtin_bit_cast(uint4, f));
-                    else *reinterpret_cast<f32x4*>(o) = f;
-                } else {
-                    st16_nt(static_cast<uint16_t*>(out) + (int64_t)m * ld + c, v);
-                }
-            }
-            wave_lds_fence();
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (n > 0) store(n - 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < JS; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if constexpr (F32) {
+                    const f32x16& a = acc[i][jg + j];
+                    const int ch = j * 8 + 2 * q + (lane >> 5);
+                    *reinterpret_cast<f32x4*>(st + lr * S::ROWB + ((ch ^ (lr & (CH - 1))) * 16)) =
+                        f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+                } else {
+                    const int ch = j * 4 + q;
+                    *reinterpret_cast<uint2*>(st + lr * S::ROWB + ((ch ^ (lr & (CH - 1))) * 16) + (lane >> 5) * 8) = half[j][q];
+                }
+            }
+        wave_lds_order();
+#pragma unroll
+        for (int k = 0; k < 32 / RPI; ++k) {
+            const int rr = lane / CH + RPI * k;
+            v[k] = *reinterpret_cast<const uint4*>(st + rr * S::ROWB + ((cl ^ (rr & (CH - 1))) * 16));
+        }
+        wave_lds_order();
+    }
+    store(SLICES - 1);
 }
 
 // Writes a unit's wave outputs: to the result or, SPLIT, as a partial tile
 // (fp32; bf16 results' partial tiles leave from the registers, whose LDS holds
 // no fp32 rows).
-template <int TILE, bool F32, int JS, bool SPLIT>
+template <int TILE, bool F32, int JS, bool SPLIT, bool BETA>
 __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64], uint8_t* st, const LinearParams& p,
                                             const Unit& u, int M, int C, int wrow, int wcol) {
     constexpr int WT = TILE / 2;
@@ -255,7 +287,7 @@ __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64],
     if constexpr (SPLIT) {
         float* o = p.part + (int64_t)u.part * TILE * TILE + wrow * TILE + wcol;
         if constexpr (F32) {
-            store_wave<true, JS, false>(acc, st, o, TILE, rows, cols, 0.0f);
+            store_wave<true, JS, false, false>(acc, st, o, TILE, rows, cols, 0.0f);
         } else {
             const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -273,9 +305,9 @@ __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64],
             }
         }
     } else {
-        const int64_t at = (int64_t)(u.m0 + wrow) * p.ldy + u.c0 + wcol;
-        if constexpr (F32) store_wave<true, JS, true>(acc, st, static_cast<float*>(p.y) + at, p.ldy, rows, cols, p.beta);
-        else store_wave<false, JS, true>(acc, st, static_cast<uint16_t*>(p.y) + at, p.ldy, rows, cols, p.beta);
+        using Out = std::conditional_t<F32, float, uint16_t>;
+        Out* o = static_cast<Out*>(p.y) + (int64_t)(u.m0 + wrow) * p.ldy + u.c0 + wcol;
+        store_wave<F32, JS, true, BETA>(acc, st, o, p.ldy, rows, cols, p.beta);
     }
 }
 
@@ -295,7 +327,7 @@ struct Fwd {
     static_assert(LDS * WGS <= 160 * 1024, "LDS");
 };
 
-template <int TILE, bool SPLIT>
+template <int TILE, bool SPLIT, bool BETA>
 __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(LinearParams p, LinearPlan pl) {
     using G = Fwd<TILE>;
     constexpr int MI = G::MI, WT = G::WT;
@@ -452,7 +484,7 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
             mma(f[1], f[0], sl, 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        finish_unit<TILE, false, MI, SPLIT>(acc, st, p, u, p.T, p.N, wrow, wcol);
+        finish_unit<TILE, false, MI, SPLIT, BETA>(acc, st, p, u, p.T, p.N, wrow, wcol);
         vb += gridDim.x;
         if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) break;
         first();  // again: the fragments' registers served the epilogue
@@ -488,7 +520,7 @@ struct Grad {
 };
 
 
-template <int OP, int TILE, bool SPLIT>
+template <int OP, int TILE, bool SPLIT, bool BETA>
 __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel(LinearParams p, LinearPlan pl) {
     using G = Grad<OP, TILE>;
     constexpr bool DW = G::DW;
@@ -797,7 +829,7 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
                 sr = sr == 2 ? 0 : sr + 1;
             }
         }
-        finish_unit<TILE, DW, MI / 2, SPLIT>(acc, st, p, u, M, C, wrow, wcol);
+        finish_unit<TILE, DW, MI / 2, SPLIT, BETA>(acc, st, p, u, M, C, wrow, wcol);
         vb += gridDim.x;
         if (!unit_at<TILE, SPLIT>(pl, R, vb, u)) break;
         first();  // again: the fragments' registers served the epilogue
@@ -843,7 +875,7 @@ struct Mx {
     static constexpr int LDS = 2 * SLOT;
 };
 
-template <bool SPLIT, bool FULL>
+template <bool SPLIT, bool FULL, bool BETA>
 __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, LinearPlan pl) {
     using G = Mx;
     constexpr int MI = G::MI, WT = G::WT, TILE = G::TILE;
@@ -952,7 +984,7 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
             slot ^= 1;
         }
         lds_barrier();  // the last step's slot is read: the epilogue stages there
-        finish_unit<TILE, false, MI, SPLIT>(acc, lds + (slot ^ 1) * G::SLOT + wave * Stage<false, MI>::BYTES, p, u, p.T, p.N,
+        finish_unit<TILE, false, MI, SPLIT, BETA>(acc, lds + (slot ^ 1) * G::SLOT + wave * Stage<false, MI>::BYTES, p, u, p.T, p.N,
                                             wrow, wcol);
         vb += gridDim.x;
         if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) break;
@@ -968,10 +1000,10 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
 // reads the next slot's first fragments and the freed slot's loads begin. (us,
 // 128 x 128 / 256 x 256, the latter with loads and reads in a bunch ahead of each
 // step: T 16384, N 4096, K 4096 162 / 147, 166 bunched; T = N = 16384, K 8192
-// 1191 / 1037, 1112 bunched, 4.2 PFLOP/s.) Not the matrix cores alone bound it:
-// what a unit's outputs take, 6.5 us at K 256, adds to its steps' 1.85 us each,
-// with CUs in lockstep or spread over a round, so loads wait behind the chip's
-// stores; with codes of zeros T 65536, N 4096, K 1024 still takes 214 us of 222.
+// 1191 / 1037, 1112 bunched, 4.2 PFLOP/s.)
+// At small K the outputs bound it: a unit takes 5.8 us for its 128 KiB of outputs
+// (the chip's stores alone: 5.6 us at 6 TB/s) and 1.8 us a step, one behind the
+// other, with the CUs' epilogues together or spread over a round.
 struct MxLarge {
     static constexpr int TILE = 256, WT = 128, MI = 4;
     static constexpr int CODES = TILE * 128, SCALES = TILE * 8;  // bytes per operand
@@ -982,6 +1014,7 @@ struct MxLarge {
     static_assert(LDS <= 160 * 1024, "LDS");
 };
 
+template <bool BETA>
 __global__ __launch_bounds__(256, 1) void linear_mx_large_kernel(LinearParams p, LinearPlan pl) {
     using G = MxLarge;
     constexpr int MI = G::MI, WT = G::WT, TILE = G::TILE;
@@ -1114,7 +1147,7 @@ __global__ __launch_bounds__(256, 1) void linear_mx_large_kernel(LinearParams p,
         for (int d = G::FIRST; d < G::ND; ++d) load(d);
         next_loads();
         __builtin_amdgcn_sched_barrier(0);
-        finish_unit<TILE, false, 2, false>(acc, st, p, u, p.T, p.N, wrow, wcol);
+        finish_unit<TILE, false, 2, false, BETA>(acc, st, p, u, p.T, p.N, wrow, wcol);
         stored = p.T - u.m0 - wrow >= WT && p.N - u.c0 - wcol >= WT;
         vb += gridDim.x;
         if (!unit_at<TILE, false>(pl, K, vb, u)) break;
@@ -1367,20 +1400,25 @@ LinearPlan linear_plan(LinearOp op, int T, int N, int K, double* us = nullptr) {
     return plan_tiles(z, best_tile, best_parts);
 }
 
-template <int OP, int TILE, bool SPLIT>
+// BETA: a kernel that adds to what is there. Apart, since two epilogues in one
+// kernel spill the accumulators.
+template <int OP, int TILE, bool SPLIT, bool BETA>
 void launch_units(const LinearParams& p, const LinearPlan& pl, int units, hipStream_t s) {
     const int grid = std::min((units + 7) & ~7, (int)tile_slots(TILE) & ~7);
     if constexpr (OP == LINEAR_MATMUL) {
-        if (p.K % 256 == 0) linear_mx_kernel<SPLIT, true><<<grid, 256, 0, s>>>(p, pl);
-        else linear_mx_kernel<SPLIT, false><<<grid, 256, 0, s>>>(p, pl);
-    } else if constexpr (OP == LINEAR_FORWARD) linear_fwd_kernel<TILE, SPLIT><<<grid, 256, 0, s>>>(p, pl);
-    else linear_grad_kernel<OP, TILE, SPLIT><<<grid, 256, 0, s>>>(p, pl);
+        if (p.K % 256 == 0) linear_mx_kernel<SPLIT, true, BETA><<<grid, 256, 0, s>>>(p, pl);
+        else linear_mx_kernel<SPLIT, false, BETA><<<grid, 256, 0, s>>>(p, pl);
+    } else if constexpr (OP == LINEAR_FORWARD) linear_fwd_kernel<TILE, SPLIT, BETA><<<grid, 256, 0, s>>>(p, pl);
+    else linear_grad_kernel<OP, TILE, SPLIT, BETA><<<grid, 256, 0, s>>>(p, pl);
 }
 template <int OP, int TILE>
 void launch_tiles(const LinearParams& p, const LinearPlan& pl, hipStream_t s) {
-    if (pl.whole > 0) launch_units<OP, TILE, false>(p, pl, pl.whole, s);
+    if (pl.whole > 0) {
+        if (p.beta == 0.0f) launch_units<OP, TILE, false, false>(p, pl, pl.whole, s);
+        else launch_units<OP, TILE, false, true>(p, pl, pl.whole, s);
+    }
     if (pl.tail > 0) {
-        launch_units<OP, TILE, true>(p, pl, pl.tail * pl.parts, s);
+        launch_units<OP, TILE, true, false>(p, pl, pl.tail * pl.parts, s);  // the sums add what is there
         constexpr int SLABS = TILE / (256 / (TILE / 4));
         const Sizes z = sizes((LinearOp)OP, p.T, p.N, p.K);
         linear_fixup_kernel<TILE, OP == LINEAR_DW><<<pl.tail * SLABS, 256, 0, s>>>(p, pl, z.M, z.C);
@@ -1401,7 +1439,8 @@ bool mx_large(int T, int N, int K) {
 void launch_mx_large(const LinearParams& p, hipStream_t s) {
     const LinearPlan pl = plan_tiles(sizes(LINEAR_MATMUL, p.T, p.N, p.K), 256, 1);
     const int grid = std::min((pl.whole + 7) & ~7, (int)tile_slots(256) & ~7);
-    linear_mx_large_kernel<<<grid, 256, 0, s>>>(p, pl);
+    if (p.beta == 0.0f) linear_mx_large_kernel<false><<<grid, 256, 0, s>>>(p, pl);
+    else linear_mx_large_kernel<true><<<grid, 256, 0, s>>>(p, pl);
 }
 
 template <int RB, int NB, int NW, int U>
