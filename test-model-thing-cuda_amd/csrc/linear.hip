@@ -1001,8 +1001,8 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
 // 128 x 128 / 256 x 256, the latter with loads and reads in a bunch ahead of each
 // step: T 16384, N 4096, K 4096 162 / 147, 166 bunched; T = N = 16384, K 8192
 // 1191 / 1037, 1112 bunched, 4.2 PFLOP/s.)
-// At small K the outputs bound it: a unit takes 5.8 us for its 128 KiB of outputs
-// (the chip's stores alone: 5.6 us at 6 TB/s) and 1.8 us a step, one behind the
+// At small K the outputs bound it: a unit takes 5.0 us for its 128 KiB of outputs
+// (the chip's stores alone: 5.0 to 5.6 us, 6 to 6.7 TB/s) and 1.9 us a step, one behind the
 // other, with the CUs' epilogues together or spread over a round.
 struct MxLarge {
     static constexpr int TILE = 256, WT = 128, MI = 4;
@@ -1425,16 +1425,17 @@ void launch_tiles(const LinearParams& p, const LinearPlan& pl, hipStream_t s) {
     }
 }
 
-// Whether 256 x 256 tiles of MXFP4 x MXFP4 are estimated to be faster: their
-// rounds of one tile per CU against two rounds' worth of 128 x 128 tiles at two
-// per CU, from two such rounds on. Measured (us, 128 / 256): T 65536, N 4096, K
-// 512 164 / 164, K 1024 230 / 222; T 16384, N 4096, K 1024 59 / 61; T 65536, N
-// 1024, K 4096 164 / 149; T 20011, N 2736, K 768 47 / 64.
+// Whether 256 x 256 tiles of MXFP4 x MXFP4 are estimated to be faster: rounds of
+// one tile per CU, 5.0 us and 1.9 a step (K = 256), against rounds of 128 x 128
+// tiles at two per CU, 1.95 and 1.13, from two of those on. Measured (us, 128 /
+// 256): T 65536, N 4096, K 512 134 / 137, K 1024 226 / 206; T 16384, N 4096, K
+// 1024 53 / 55, K 2048 87 / 84; T 65536, N 1024, K 4096 152 / 143; T 20011, N
+// 2736, K 768 47 / 64.
 bool mx_large(int T, int N, int K) {
     const int64_t small = (int64_t)((T + 127) / 128) * ((N + 127) / 128), big = (int64_t)((T + 255) / 256) * ((N + 255) / 256);
     if (K % 256 != 0 || small < 2 * tile_slots(128)) return false;
     const double steps = K / 256, slots2 = (double)tile_slots(128), slots1 = (double)tile_slots(256);
-    return 4.0 + std::ceil(big / slots1) * (6.5 + 1.85 * steps) < std::ceil(small / slots2) * (2.75 + 1.12 * steps);
+    return 3.0 + std::ceil(big / slots1) * (5.0 + 1.9 * steps) < std::ceil(small / slots2) * (1.95 + 1.13 * steps);
 }
 void launch_mx_large(const LinearParams& p, hipStream_t s) {
     const LinearPlan pl = plan_tiles(sizes(LINEAR_MATMUL, p.T, p.N, p.K), 256, 1);
@@ -1451,7 +1452,7 @@ void launch_rows_as(const LinearParams& p, hipStream_t s) {
 // The kernel for few tokens runs where its estimate in us, measured over T 1 ..
 // 777, N and K 256 .. 4096, is not above the tiles'. T 777, N 1024, K 1024 10.1
 // (tiles 13.6), T 512, N 4096, K 1024 17.7 (tiles 14.2).
-// The kernel for few tokens stays below 2^22 workgroups; a launch holds 2^32 threads.
+// It stays below 2^21 workgroups; a launch holds 2^32 threads.
 double rows_time(int T, int N, int K) {
     if ((int64_t)T * N >= (int64_t)1 << 30) return 1e30;
     return 3.0 + 7.2e-9 * ((double)T * N * K);
