@@ -216,7 +216,8 @@ __device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, v
 #pragma unroll
         for (int k = 0; k < 32 / RPI; ++k) {
             if constexpr (F32 && BETA)
-                v[k] = __builtin_bit_cast(uint4, __builtin_bit_cast(f32x4, v[k]) + beta * __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(win, (int)at, 0, 0)));
+                v[k] = __builtin_bit_cast(uint4, __builtin_bit_cast(f32x4, v[k]) +
+                                                     beta * __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(win, (int)at, 0, 0)));
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), win, (int)at, 0, NT ? 2 : 0);
             at += RPI * row;
         }

@@ -8,7 +8,8 @@
 //   pointwise.hip combine, combine/router backward, router dW, dX scatter
 //   norm.hip      LayerNorm forward / backward in front of the block
 //   adamw.hip     multi-tensor AdamW with global-norm clipping
-// The host orchestration lives in moe_api.cpp.
+// The host orchestration lives in moe_api.cpp. The linear layer on microscaled
+// numbers (mx_quant.hip, linear.hip, linear_api.cpp) is declared in linear.hpp.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
