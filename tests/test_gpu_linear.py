@@ -732,3 +732,11 @@ def test_large_matmul_tiles(T, N, K, pad, beta):
     for y in outs:
         p.call(y, ws)
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("op", OPS)
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_the_widest_rows(op, beta):
+    """Row strides of 2^22 elements: offsets inside a tile close to 2^31 bytes."""
+    T, N, K = 300, 256, 320
+    _run(op, T, N, K, pad=(1 << 22) - K, beta=beta)
