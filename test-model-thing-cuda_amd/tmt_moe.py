@@ -266,26 +266,29 @@ def _here(stream) -> tuple:
 def _matrix(what: str, t, dtype, dev: int, rows: int, cols: int) -> tuple:
     """(pointer, row stride) of a [rows, cols] matrix on GPU `dev` whose rows
     are contiguous."""
+    if t.dtype is dtype and t.shape == (rows, cols) and t.get_device() == dev:
+        ld, one = t.stride()
+        if one == 1 or cols <= 1:
+            return t.data_ptr(), ld if rows > 1 else cols
     if t.dtype is not dtype or t.dim() != 2:
         raise ValueError(f"{what} must be a matrix of {dtype}, not {list(t.shape)} of {t.dtype}")
     if t.get_device() != dev:
         raise ValueError(f"{what} is on {t.device}, not on the current GPU")
     if t.shape != (rows, cols):
         raise ValueError(f"{what} must be [{rows}, {cols}], not {list(t.shape)}")
-    ld, one = t.stride()
-    if one != 1 and cols > 1:
-        raise ValueError(f"the rows of {what} must be contiguous")
-    return t.data_ptr(), ld if rows > 1 else cols
+    raise ValueError(f"the rows of {what} must be contiguous")
 
 
 def _mx(what: str, codes, scales, dev: int, rows: int, K: int, fmt: int) -> tuple:
     """(codes, scales, scale stride) of a microscaled matrix [rows, K]."""
     import torch
-    width = K if fmt == MX_FP8 else K // 2
-    c, ld = _matrix("codes of " + what, codes, torch.uint8, dev, rows, width)
-    if ld != width:
-        raise ValueError(f"the codes of {what} must be contiguous")
-    n = scales.shape[-1]
+    width, n = K if fmt == MX_FP8 else K // 2, scales.shape[-1]
+    if codes.dtype is torch.uint8 and codes.shape == (rows, width) and codes.get_device() == dev and codes.is_contiguous():
+        c = codes.data_ptr()
+    else:
+        c, ld = _matrix("codes of " + what, codes, torch.uint8, dev, rows, width)
+        if ld != width:
+            raise ValueError(f"the codes of {what} must be contiguous")
     if n < rows:
         raise ValueError(f"scales of {what} must be [{K // 32}, {rows} or more], not {list(scales.shape)}")
     s, lds = _matrix("scales of " + what, scales, torch.uint8, dev, K // 32, n)
@@ -299,7 +302,7 @@ def _ws(workspace, dev: int) -> tuple:
         raise ValueError(f"workspace is on {workspace.device}, not on the current GPU")
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.nbytes
 
 
 def _mx_rows(X, codes, scales, fmt, stream):
