@@ -1326,10 +1326,12 @@ Sizes sizes(LinearOp op, int T, int N, int K) {
 }
 
 // Workgroups that run at a time.
-int64_t tile_slots(int tile) { return (int64_t)cu_count() * (tile == 256 ? 1 : 2); }
+// (cus: compute units, asked for once a call; each question costs the host 30 ns,
+// and a plan of many candidates would ask 100 times.)
+int64_t tile_slots(int tile, int cus) { return (int64_t)cus * (tile == 256 ? 1 : 2); }
 constexpr int kMinSteps = 4;  // K = 64 steps that a part of a split reduction has at least
 
-LinearPlan plan_tiles(const Sizes& z, int tile, int64_t parts) {
+LinearPlan plan_tiles(const Sizes& z, int tile, int64_t parts, int cus) {
     LinearPlan pl;
     pl.tile = tile;
     pl.tiles_m = (z.M + tile - 1) / tile;
@@ -1338,7 +1340,7 @@ LinearPlan plan_tiles(const Sizes& z, int tile, int64_t parts) {
     pl.whole = (int)tiles;
     if (parts >= 2) {
         const int nk = (z.R + 63) / 64;
-        pl.whole = (int)(tiles / tile_slots(tile) * tile_slots(tile));
+        pl.whole = (int)(tiles / tile_slots(tile, cus) * tile_slots(tile, cus));
         pl.tail = (int)(tiles - pl.whole);
         pl.chunk = (int)((nk + 4 * parts - 1) / (4 * parts)) * 256;  // whole steps of every kernel
         pl.parts = (nk * 64 + pl.chunk - 1) / pl.chunk;
@@ -1360,20 +1362,20 @@ constexpr StepTimes kTimes[4] = {{4.5, 0.62, 1.05, 1.45}, {2.5, 0.28, 0.48, 0.0}
 // through the last-level cache and back.
 constexpr double kSplitStart = 3.5, kSplitPerMiB = 0.25;
 
-double round_time(const StepTimes& t, int tile, int64_t units, double steps) {
+double round_time(const StepTimes& t, int tile, int64_t units, double steps, int cus) {
     if (tile == 256) return 2.0 + steps * t.large;
-    return steps * (units <= cu_count() ? t.one : t.two);
+    return steps * (units <= cus ? t.one : t.two);
 }
-double plan_time(const StepTimes& t, const Sizes& z, int tile, int64_t parts) {
-    const int64_t slots = tile_slots(tile);
+double plan_time(const StepTimes& t, const Sizes& z, int tile, int64_t parts, int cus) {
+    const int64_t slots = tile_slots(tile, cus);
     const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
     const int64_t whole = tiles / slots, rest = tiles - whole * slots;
     const double nk = (z.R + 63) / 64;
-    double us = t.start + (tile == 256 ? 4.0 : 0.0) + whole * round_time(t, tile, slots, nk);
+    double us = t.start + (tile == 256 ? 4.0 : 0.0) + whole * round_time(t, tile, slots, nk, cus);
     if (rest == 0) return us;
-    if (parts < 2) return us + round_time(t, tile, rest, nk);
+    if (parts < 2) return us + round_time(t, tile, rest, nk, cus);
     const double mib = (double)(rest * parts) * tile * tile * 4 / (1 << 20);
-    return us + round_time(t, tile, rest * parts, std::ceil(nk / parts)) + (whole > 0 ? t.start : 0.0) + kSplitStart + kSplitPerMiB * mib;
+    return us + round_time(t, tile, rest * parts, std::ceil(nk / parts), cus) + (whole > 0 ? t.start : 0.0) + kSplitStart + kSplitPerMiB * mib;
 }
 
 // The tile size and split with the shortest estimate. Measured (us, chosen /
@@ -1382,7 +1384,7 @@ double plan_time(const StepTimes& t, const Sizes& z, int tile, int64_t parts) {
 // in two, 38.2 whole; dX T 777, N 4096, K 1024 23.9 in four parts / 28.5 in
 // three; dW T 32768, N 1024, K 1024 95 on 256 x 256 tiles in 16 parts / 107 on
 // 128 x 128 in 8; T 16384, N 256, K 256 16.7 in 32 parts / 32 in 8.
-LinearPlan linear_plan(LinearOp op, int T, int N, int K, double* us = nullptr) {
+LinearPlan linear_plan(LinearOp op, int T, int N, int K, int cus, double* us) {
     const Sizes z = sizes(op, T, N, K);
     const StepTimes& t = kTimes[op];
     int best_tile = 128;
@@ -1390,22 +1392,22 @@ LinearPlan linear_plan(LinearOp op, int T, int N, int K, double* us = nullptr) {
     double best = 1e30;
     for (int tile = 128; tile <= (op == LINEAR_MATMUL ? 128 : 256); tile *= 2) {
         const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
-        const int64_t rest = tiles % tile_slots(tile);
-        const int64_t most = rest > 0 ? std::min<int64_t>(tile_slots(tile) / rest, (z.R + 63) / 64 / kMinSteps) : 1;
+        const int64_t rest = tiles % tile_slots(tile, cus);
+        const int64_t most = rest > 0 ? std::min<int64_t>(tile_slots(tile, cus) / rest, (z.R + 63) / 64 / kMinSteps) : 1;
         for (int64_t parts = 1; parts <= std::max<int64_t>(most, 1); parts += parts < 8 ? 1 : parts / 4) {
-            const double c = plan_time(t, z, tile, parts);
+            const double c = plan_time(t, z, tile, parts, cus);
             if (c < best) best = c, best_tile = tile, best_parts = parts;
         }
     }
-    if (us != nullptr) *us = best;
-    return plan_tiles(z, best_tile, best_parts);
+    *us = best;
+    return plan_tiles(z, best_tile, best_parts, cus);
 }
 
 // BETA: a kernel that adds to what is there. Apart, since two epilogues in one
 // kernel spill the accumulators.
 template <int OP, int TILE, bool SPLIT, bool BETA>
-void launch_units(const LinearParams& p, const LinearPlan& pl, int units, hipStream_t s) {
-    const int grid = std::min((units + 7) & ~7, (int)tile_slots(TILE) & ~7);
+void launch_units(const LinearParams& p, const LinearPlan& pl, int units, int cus, hipStream_t s) {
+    const int grid = std::min((units + 7) & ~7, (int)tile_slots(TILE, cus) & ~7);
     if constexpr (OP == LINEAR_MATMUL) {
         if (p.K % 256 == 0) linear_mx_kernel<SPLIT, true, BETA><<<grid, 256, 0, s>>>(p, pl);
         else linear_mx_kernel<SPLIT, false, BETA><<<grid, 256, 0, s>>>(p, pl);
@@ -1413,13 +1415,13 @@ void launch_units(const LinearParams& p, const LinearPlan& pl, int units, hipStr
     else linear_grad_kernel<OP, TILE, SPLIT, BETA><<<grid, 256, 0, s>>>(p, pl);
 }
 template <int OP, int TILE>
-void launch_tiles(const LinearParams& p, const LinearPlan& pl, hipStream_t s) {
+void launch_tiles(const LinearParams& p, const LinearPlan& pl, int cus, hipStream_t s) {
     if (pl.whole > 0) {
-        if (p.beta == 0.0f) launch_units<OP, TILE, false, false>(p, pl, pl.whole, s);
-        else launch_units<OP, TILE, false, true>(p, pl, pl.whole, s);
+        if (p.beta == 0.0f) launch_units<OP, TILE, false, false>(p, pl, pl.whole, cus, s);
+        else launch_units<OP, TILE, false, true>(p, pl, pl.whole, cus, s);
     }
     if (pl.tail > 0) {
-        launch_units<OP, TILE, true, false>(p, pl, pl.tail * pl.parts, s);  // the sums add what is there
+        launch_units<OP, TILE, true, false>(p, pl, pl.tail * pl.parts, cus, s);  // the sums add what is there
         constexpr int SLABS = TILE / (256 / (TILE / 4));
         const Sizes z = sizes((LinearOp)OP, p.T, p.N, p.K);
         linear_fixup_kernel<TILE, OP == LINEAR_DW><<<pl.tail * SLABS, 256, 0, s>>>(p, pl, z.M, z.C);
@@ -1432,15 +1434,15 @@ void launch_tiles(const LinearParams& p, const LinearPlan& pl, hipStream_t s) {
 // 256): T 65536, N 4096, K 512 134 / 137, K 1024 226 / 206; T 16384, N 4096, K
 // 1024 53 / 55, K 2048 87 / 84; T 65536, N 1024, K 4096 152 / 143; T 20011, N
 // 2736, K 768 47 / 64.
-bool mx_large(int T, int N, int K) {
+bool mx_large(int T, int N, int K, int cus) {
     const int64_t small = (int64_t)((T + 127) / 128) * ((N + 127) / 128), big = (int64_t)((T + 255) / 256) * ((N + 255) / 256);
-    if (K % 256 != 0 || small < 2 * tile_slots(128)) return false;
-    const double steps = K / 256, slots2 = (double)tile_slots(128), slots1 = (double)tile_slots(256);
+    if (K % 256 != 0 || small < 2 * tile_slots(128, cus)) return false;
+    const double steps = K / 256, slots2 = (double)tile_slots(128, cus), slots1 = (double)tile_slots(256, cus);
     return 3.0 + std::ceil(big / slots1) * (5.0 + 1.9 * steps) < std::ceil(small / slots2) * (1.95 + 1.13 * steps);
 }
-void launch_mx_large(const LinearParams& p, hipStream_t s) {
-    const LinearPlan pl = plan_tiles(sizes(LINEAR_MATMUL, p.T, p.N, p.K), 256, 1);
-    const int grid = std::min((pl.whole + 7) & ~7, (int)tile_slots(256) & ~7);
+void launch_mx_large(const LinearParams& p, int cus, hipStream_t s) {
+    const LinearPlan pl = plan_tiles(sizes(LINEAR_MATMUL, p.T, p.N, p.K), 256, 1, cus);
+    const int grid = std::min((pl.whole + 7) & ~7, (int)tile_slots(256, cus) & ~7);
     if (p.beta == 0.0f) linear_mx_large_kernel<false><<<grid, 256, 0, s>>>(p, pl);
     else linear_mx_large_kernel<true><<<grid, 256, 0, s>>>(p, pl);
 }
@@ -1464,8 +1466,8 @@ double rows_time(int T, int N, int K) {
 // 4.8 / 4.6 / 4.7 / 6.4; T 256, N 4096, K 1024 13.8 / 11.4 / 11.2 / 10.0.
 // Reductions of more than 8 pieces take 8 waves with two pieces in flight (32 x
 // 32: one), shorter ones 4 waves with two (16 x 16: 8 with one).
-void launch_rows(const LinearParams& p, hipStream_t s) {
-    const int64_t most = 2 * (int64_t)cu_count(), n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32;
+void launch_rows(const LinearParams& p, int cus, hipStream_t s) {
+    const int64_t most = 2 * (int64_t)cus, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32;
     const int64_t t16 = (p.T + 15) / 16, t32 = (p.T + 31) / 32;
     const bool many = p.K > 1024;
     if (n16 * t16 <= most) many ? launch_rows_as<1, 1, 8, 2>(p, s) : launch_rows_as<1, 1, 8, 1>(p, s);
@@ -1481,40 +1483,43 @@ void launch_rows(const LinearParams& p, hipStream_t s) {
 // neither tiles nor parts fall with T.
 size_t linear_workspace(LinearOp op, int T, int N, int K) {
     const Sizes z = sizes(op, T, N, K);
+    const int cus = cu_count();
     size_t most = 0;
     for (int tile = 128; tile <= 256; tile *= 2) {
         const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
         const int64_t parts = (z.R + 63) / 64 / kMinSteps;
         if (parts < 2) continue;
-        const int64_t units = std::min(tiles * parts, tile_slots(tile));
+        const int64_t units = std::min(tiles * parts, tile_slots(tile, cus));
         most = std::max(most, (size_t)units * tile * tile * 4);
     }
     return most;
 }
 
 hipError_t launch_linear(LinearOp op, const LinearParams& p, hipStream_t s) {
+    const int cus = cu_count();
     if (op != LINEAR_DW && p.T <= 0) return hipSuccess;
     if (op == LINEAR_DW && p.T == 0) {
         if (p.beta == 1.0f) return hipSuccess;
-        const int64_t blocks = std::min<int64_t>(((int64_t)p.N * p.K / 4 + 255) / 256, 16 * (int64_t)cu_count());
+        const int64_t blocks = std::min<int64_t>(((int64_t)p.N * p.K / 4 + 255) / 256, 16 * (int64_t)cus);
         linear_scale_kernel<<<(unsigned)blocks, 256, 0, s>>>(static_cast<float*>(p.y), p.ldy, p.N, p.K, p.beta);
         return hipGetLastError();
     }
+    if (op == LINEAR_MATMUL && mx_large(p.T, p.N, p.K, cus)) {
+        launch_mx_large(p, cus, s);
+        return hipGetLastError();
+    }
     double us = 0.0;
-    const LinearPlan pl = linear_plan(op, p.T, p.N, p.K, &us);
+    const LinearPlan pl = linear_plan(op, p.T, p.N, p.K, cus, &us);
     if (op == LINEAR_FORWARD && rows_time(p.T, p.N, p.K) <= us) {
-        launch_rows(p, s);
+        launch_rows(p, cus, s);
         return hipGetLastError();
     }
     const bool big = pl.tile == 256;
     switch (op) {
-        case LINEAR_FORWARD: big ? launch_tiles<LINEAR_FORWARD, 256>(p, pl, s) : launch_tiles<LINEAR_FORWARD, 128>(p, pl, s); break;
-        case LINEAR_MATMUL:
-            if (mx_large(p.T, p.N, p.K)) launch_mx_large(p, s);
-            else launch_tiles<LINEAR_MATMUL, 128>(p, pl, s);
-            break;
-        case LINEAR_DX: big ? launch_tiles<LINEAR_DX, 256>(p, pl, s) : launch_tiles<LINEAR_DX, 128>(p, pl, s); break;
-        case LINEAR_DW: big ? launch_tiles<LINEAR_DW, 256>(p, pl, s) : launch_tiles<LINEAR_DW, 128>(p, pl, s); break;
+        case LINEAR_FORWARD: big ? launch_tiles<LINEAR_FORWARD, 256>(p, pl, cus, s) : launch_tiles<LINEAR_FORWARD, 128>(p, pl, cus, s); break;
+        case LINEAR_MATMUL: launch_tiles<LINEAR_MATMUL, 128>(p, pl, cus, s); break;
+        case LINEAR_DX: big ? launch_tiles<LINEAR_DX, 256>(p, pl, cus, s) : launch_tiles<LINEAR_DX, 128>(p, pl, cus, s); break;
+        case LINEAR_DW: big ? launch_tiles<LINEAR_DW, 256>(p, pl, cus, s) : launch_tiles<LINEAR_DW, 128>(p, pl, cus, s); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
