@@ -213,18 +213,41 @@ __device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, v
     auto store = [&](int n) {
         const int c = 32 * JS * (n % JG) + cl * (16 / SIZE);
         uint32_t at = c < cols ? (uint32_t)(32 * (n / JG) + lane / CH) * row + (uint32_t)c * SIZE : FAR;
+        if constexpr (F32 && BETA) {
+            u32x4 was[32 / RPI];
+#pragma unroll
+            for (int k = 0; k < 32 / RPI; ++k) was[k] = __builtin_amdgcn_raw_buffer_load_b128(win, (int)(at + k * RPI * row), 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 32 / RPI; ++k)
+                v[k] = __builtin_bit_cast(uint4, __builtin_bit_cast(f32x4, v[k]) + beta * __builtin_bit_cast(f32x4, was[k]));
+        }
 #pragma unroll
         for (int k = 0; k < 32 / RPI; ++k) {
-            if constexpr (F32 && BETA)
-                v[k] = __builtin_bit_cast(uint4, __builtin_bit_cast(f32x4, v[k]) +
-                                                     beta * __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(win, (int)at, 0, 0)));
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), win, (int)at, 0, NT ? 2 : 0);
             at += RPI * row;
         }
     };
+    // bf16 outputs that are added to: a slice's are loaded while the one before is
+    // converted, ahead of the stores, which a later load would wait for
+    u32x2 old[2][JS][4];
+    auto load_old = [&](int n) {
+#pragma unroll
+        for (int j = 0; j < JS; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = 32 * (n % JG * JS + j) + 8 * q + 4 * (lane >> 5);
+                old[n & 1][j][q] = __builtin_amdgcn_raw_buffer_load_b64(
+                    win, c < cols ? (int)((uint32_t)(32 * (n / JG) + lr) * row + (uint32_t)c * SIZE) : (int)FAR, 0, 0);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (!F32 && BETA) load_old(0);
 #pragma unroll
     for (int n = 0; n < SLICES; ++n) {
         const int i = n / JG, jg = n % JG * JS;
+        if constexpr (!F32 && BETA)
+            if (n + 1 < SLICES) load_old(n + 1);
         // the outputs not yet staged stay in the accumulator registers
 #pragma unroll
         for (int i2 = i; i2 < MI; ++i2)
@@ -240,10 +263,8 @@ __device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, v
                     const f32x16& a = acc[i][jg + j];
                     f32x4 f = {a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
                     if constexpr (BETA) {
-                        const int c = 32 * (jg + j) + 8 * q + 4 * (lane >> 5);
-                        const u32x2 old = __builtin_amdgcn_raw_buffer_load_b64(
-                            win, c < cols ? (int)((uint32_t)(32 * i + lr) * row + (uint32_t)c * SIZE) : (int)FAR, 0, 0);
-                        f = f + beta * f32x4{bf_lo(old[0]), bf_hi(old[0]), bf_lo(old[1]), bf_hi(old[1])};
+                        const u32x2 o = old[n & 1][j][q];
+                        f = f + beta * f32x4{bf_lo(o[0]), bf_hi(o[0]), bf_lo(o[1]), bf_hi(o[1])};
                     }
                     half[j][q] = make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]));
                 }
@@ -1117,12 +1138,15 @@ __global__ __launch_bounds__(256, 1) void linear_mx_large_kernel(LinearParams p,
     wait_vm<G::ND>();
     lds_barrier();
     int sl = 0;
+    auto first = [&]() {  // a unit's first fragments
 #pragma unroll
-    for (int r = 0; r < 2 * MI; ++r) {
-        read(f[0], r, 0, 0);
-        scales(r, 0);
-    }
-    take_scales();
+        for (int r = 0; r < 2 * MI; ++r) {
+            read(f[0], r, sl, 0);
+            scales(r, sl);
+        }
+        take_scales();
+    };
+    first();
     bool stored = false;  // the last unit's outputs fill the wave's part: STORES stores behind the loads
     uint8_t* st = lds + G::ST0 + wave * Stage<false, 2>::BYTES;
     for (;;) {
@@ -1152,6 +1176,7 @@ __global__ __launch_bounds__(256, 1) void linear_mx_large_kernel(LinearParams p,
         stored = p.T - u.m0 - wrow >= WT && p.N - u.c0 - wcol >= WT;
         vb += gridDim.x;
         if (!unit_at<TILE, false>(pl, K, vb, u)) break;
+        if constexpr (BETA) first();  // again: what is there took the fragments' registers
     }
     wait_vm<0>();  // no load may land in LDS that the next workgroup owns
 }
