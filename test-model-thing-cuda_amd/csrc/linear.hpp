@@ -15,6 +15,17 @@ struct MxRowsParams {
     uint8_t* scales;  // [K/32][lds]
     int64_t lds;
 };
+// Their launch: tiles of kMxTile values, as wide as K fills, a workgroup each.
+constexpr int kMxTile = 4096;
+__host__ __device__ inline int mx_tile_log2_cols(int K) { return K >= 256 ? 8 : K >= 128 ? 7 : 6; }
+__host__ __device__ inline int mx_tiles_per_row(int K) {
+    const int lg = mx_tile_log2_cols(K);
+    return (int)(((uint32_t)K + (1u << lg) - 1) >> lg);  // K + 255 may pass 31 bits
+}
+inline int64_t mx_tiles(int rows, int K) {
+    const int rt = kMxTile >> mx_tile_log2_cols(K);
+    return ((int64_t)rows + rt - 1) / rt * mx_tiles_per_row(K);
+}
 hipError_t launch_mx_rows(bool quantize, int format, bool f32, const MxRowsParams& p, hipStream_t s);
 
 // The products. M output rows, C output columns, R the reduction length:

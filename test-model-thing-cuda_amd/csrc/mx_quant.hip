@@ -24,9 +24,7 @@ namespace {
 
 constexpr int kPieces = 2;                        // pieces of 8 values per lane
 constexpr int kTile = kPieces * 8 * kThreads;     // values per workgroup
-
-// Tile geometry for a row length.
-__host__ __device__ inline int tile_log2_cols(int K) { return K >= 256 ? 8 : K >= 128 ? 7 : 6; }
+static_assert(kTile == kMxTile, "the launch's tiles are the kernels'");
 
 __device__ __forceinline__ void load8(const void* x, bool f32, int64_t at, float* f) {
     if (f32) {
@@ -42,8 +40,8 @@ __device__ __forceinline__ void load8(const void* x, bool f32, int64_t at, float
 template <int FMT, bool F32>
 __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(MxRowsParams p) {
     __shared__ uint8_t sc[kTile / 32];  // [column block][row]
-    const int lg = tile_log2_cols(p.K), rt = kTile >> lg, lanes = 1 << (lg - 3);  // pieces per row
-    const int tc = (p.K + (1 << lg) - 1) >> lg;
+    const int lg = mx_tile_log2_cols(p.K), rt = kTile >> lg, lanes = 1 << (lg - 3);  // pieces per row
+    const int tc = mx_tiles_per_row(p.K);
     const int64_t r0 = (int64_t)(blockIdx.x / tc) * rt;
     const int c0 = (int)(blockIdx.x % tc) << lg;
     const int pc = threadIdx.x & (lanes - 1), pr = threadIdx.x >> (lg - 3);
@@ -89,8 +87,8 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(MxRowsParams p) {
 template <int FMT, bool F32>
 __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(MxRowsParams p) {
     __shared__ uint8_t sc[kTile / 32];
-    const int lg = tile_log2_cols(p.K), rt = kTile >> lg, lanes = 1 << (lg - 3);
-    const int tc = (p.K + (1 << lg) - 1) >> lg;
+    const int lg = mx_tile_log2_cols(p.K), rt = kTile >> lg, lanes = 1 << (lg - 3);
+    const int tc = mx_tiles_per_row(p.K);
     const int64_t r0 = (int64_t)(blockIdx.x / tc) * rt;
     const int c0 = (int)(blockIdx.x % tc) << lg;
     const int pc = threadIdx.x & (lanes - 1), pr = threadIdx.x >> (lg - 3);
@@ -141,8 +139,7 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(MxRowsParams p)
 hipError_t launch_mx_rows(bool quantize, int format, bool f32, const MxRowsParams& p, hipStream_t s) {
     if (p.rows <= 0) return hipSuccess;
     if (p.K <= 0 || p.K % 32 != 0 || (format != MX_FP4 && format != MX_FP8)) return hipErrorInvalidValue;
-    const int lg = tile_log2_cols(p.K), rt = kTile >> lg;
-    const int64_t grid = ((int64_t)p.rows + rt - 1) / rt * ((p.K + (1 << lg) - 1) >> lg);
+    const int64_t grid = mx_tiles(p.rows, p.K);
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
     const unsigned g = (unsigned)grid;
 #define TMT_MX(FMT_, F32_)                                                        \
