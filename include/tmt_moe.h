@@ -422,7 +422,8 @@ enum { TMT_MOE_BF16 = 0, TMT_MOE_F32 = 1 };
  *           2^-4 of itself or half a step of e4m3's subnormals.
  * Exponents are clamped to [-127, 127]; a block of zeros takes exponent 0; a
  * block with an infinity or a NaN takes s = 255. K a multiple of 32; lds any
- * number >= rows; rows times K, rounded up to a multiple of 256, under 2^36.
+ * number >= rows; rows times K, rounded up to multiples of 16 (32 where K < 256)
+ * and of 256, under 2^36.
  */
 int tmt_moe_mx_quantize(void* stream, int32_t format, int32_t dtype, const void* X, int64_t ldx, int32_t rows,
                         int32_t K, uint8_t* codes, uint8_t* scales, int64_t lds);

@@ -12,7 +12,9 @@ static_assert((int)TMT_MOE_LINEAR_FORWARD == LINEAR_FORWARD && (int)TMT_MOE_LINE
 
 namespace {
 
-constexpr int64_t kMaxValues = int64_t(1) << 36;  // quantised by one call: a launch holds 2^32 threads
+// Values quantised by one call: a launch holds less than 2^32 threads, 2^24
+// workgroups of a tile each. Matrices that round up to as many are refused too.
+constexpr int64_t kMaxValues = int64_t(1) << 36;
 
 int check_rows(int32_t format, int32_t dtype, int32_t rows, int32_t K, const void* X, int64_t ldx,
                const uint8_t* codes, const uint8_t* scales, int64_t lds) {
@@ -23,8 +25,8 @@ int check_rows(int32_t format, int32_t dtype, int32_t rows, int32_t K, const voi
     if (rows < 0) return fail(TMT_MOE_EINVAL, "rows=%d < 0", rows);
     if (K <= 0 || K % 32 != 0) return fail(TMT_MOE_EINVAL, "K=%d must be a positive multiple of 32", K);
     if (rows == 0) return TMT_MOE_OK;
-    if ((int64_t)rows * ((K + 255LL) / 256 * 256) >= kMaxValues)
-        return fail(TMT_MOE_EINVAL, "rows=%d of K=%d, rounded up to 256, are 2^36 values or more", rows, K);
+    if ((int64_t)rows * ((K + 255LL) / 256 * 256) >= kMaxValues || mx_tiles(rows, K) >= kMaxValues / kMxTile)
+        return fail(TMT_MOE_EINVAL, "rows=%d of K=%d, rounded up to whole tiles, are 2^36 values or more", rows, K);
     const int piece = dtype == TMT_MOE_BF16 ? 8 : 4;  // elements of 16 bytes
     if (ldx < K || ldx % piece != 0)
         return fail(TMT_MOE_EINVAL, "ldx=%lld must be a multiple of %d, at least K=%d", (long long)ldx, piece, K);

@@ -1,11 +1,16 @@
 """Launch arithmetic of the microscaled linear layer on the host, from the
 header that its kernels and launchers use, with the compiler's check of signed
 overflow, which ends the program."""
+import ctypes
 import os
 import shutil
 import subprocess
 
 import pytest
+
+import tmt_moe
+
+A, i64 = 0x10000, ctypes.c_int64  # a 16-byte aligned address, never followed
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "test-model-thing-cuda_amd", "csrc")
@@ -48,3 +53,38 @@ int main() {
 def test_tiles_of_the_widest_rows(tmp_path):
     """Rows of any multiple of 32 columns that 32 bits hold."""
     _run(tmp_path, WIDEST)
+
+
+@pytest.mark.parametrize("rows,K", [((1 << 28) - 1, 256), ((1 << 28) - 15, 256), ((1 << 28) - 15, 224), ((1 << 24) - 1, 4096),
+                                    ((1 << 27) - 1, 512)])
+def test_rows_that_fill_a_launch_are_refused(rows, K):
+    """A tile is 16 or 32 rows: with those of the last one, 2^24 workgroups of
+    256 threads, more than one launch holds."""
+    lib = tmt_moe.load_library()
+    for rc in (lib.tmt_moe_mx_quantize(None, 0, 0, A, i64(K), rows, K, A, A, i64(rows)),
+               lib.tmt_moe_mx_dequantize(None, 1, A, A, i64(rows), rows, K, 1, A, i64(K))):
+        assert rc == -1 and "2^36" in tmt_moe.last_error()
+
+
+LARGEST = r"""
+#include <cstdio>
+#include "linear.hpp"
+int main() {  // accepted: rows and columns, rounded up, under 2^36 values
+    for (int64_t K = 32; K < (1ll << 31); K = K < 512 ? K + 32 : K * 2 - 32) {
+        const int64_t cols = (K + 255) / 256 * 256, tile = K < 256 ? 32 : 16;
+        const int64_t most = ((1ll << 36) - 1) / cols / tile * tile;
+        const int rows = (int)(most < (1ll << 31) - 1 ? most : (1ll << 31) - 1);
+        for (int r : {rows, rows > 7 ? rows - 7 : rows, rows / 2 + 1})
+            if (r > 0 && tmt::mx_tiles(r, (int)K) >= 1 << 24) {
+                std::printf("rows %d, K %lld: %lld tiles\n", r, (long long)K, (long long)tmt::mx_tiles(r, (int)K));
+                return 1;
+            }
+    }
+    std::printf("ok\n");
+    return 0;
+}
+"""
+
+
+def test_the_most_rows_fit_a_launch(tmp_path):
+    _run(tmp_path, LARGEST)
