@@ -263,6 +263,10 @@ def _here(stream) -> tuple:
     return dev, stream.cuda_stream
 
 
+def _past_int32(*sizes) -> None:
+    raise ValueError(f"sizes {list(sizes)} do not fit the 32 bits that the library takes")
+
+
 def _matrix(what: str, t, dtype, dev: int, rows: int, cols: int) -> tuple:
     """(pointer, row stride) of a [rows, cols] matrix on GPU `dev` whose rows
     are contiguous."""
@@ -315,6 +319,8 @@ def _mx_rows(X, codes, scales, fmt, stream):
         raise ValueError(f"X must be bfloat16 or float32, not {X.dtype}")
     dev, raw = _here(stream)
     rows, K = X.shape
+    if (rows | K) >> 31:
+        _past_int32(rows, K)
     x, ldx = _matrix("X", X, X.dtype, dev, rows, K)
     return (raw, dtype, x, ldx, rows, K) + _mx("X", codes, scales, dev, rows, K, fmt)
 
@@ -342,6 +348,8 @@ def mx_dequantize(codes, scales, X, fmt: int = MX_FP4, stream=None) -> None:
 def linear_workspace_size(op: int, T: int, N: int, K: int) -> int:
     """Bytes of device workspace that the product `op` (LINEAR_FORWARD,
     LINEAR_MATMUL, LINEAR_DX, LINEAR_DW) needs for up to T tokens."""
+    if any(n >> 31 not in (0, -1) for n in (op, T, N, K)):
+        _past_int32(op, T, N, K)
     out = ctypes.c_size_t(0)
     _check(load_library().tmt_moe_linear_workspace_size(op, T, N, K, ctypes.byref(out)))
     return int(out.value)
@@ -350,6 +358,8 @@ def linear_workspace_size(op: int, T: int, N: int, K: int) -> int:
 def _product(fn, T, N, K, x, x_cols, mx, mx_rows, fmt, y, y_rows, y_cols, y_dtype, names, beta, workspace, stream):
     """One product of a bf16 matrix x with a microscaled one."""
     import torch
+    if (T | N | K) >> 31:
+        _past_int32(T, N, K)
     dev, raw = _here(stream)
     xp, ldx = _matrix(names[0], x, torch.bfloat16, dev, T, x_cols)
     c, s, lds = _mx(names[1], mx[0], mx[1], dev, mx_rows, K, fmt)
@@ -388,6 +398,8 @@ def mxfp4_matmul(X_codes, X_scales, codes, scales, Y, beta: float = 0.0, workspa
     """Y <- beta*Y + X W^T with X [T, K] and W [N, K] both in MXFP4; Y [T, N] bf16."""
     import torch
     (T, N), K = Y.shape, 2 * codes.shape[-1]
+    if (T | N | K) >> 31:
+        _past_int32(T, N, K)
     dev, raw = _here(stream)
     xc, xs, xlds = _mx("X", X_codes, X_scales, dev, T, K, MX_FP4)
     c, s, lds = _mx("W", codes, scales, dev, N, K, MX_FP4)
