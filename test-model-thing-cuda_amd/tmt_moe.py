@@ -260,6 +260,8 @@ def _here(stream) -> tuple:
     dev = torch.cuda.current_device()
     if stream is None:
         return dev, torch._C._cuda_getCurrentRawStream(dev)
+    if stream.device_index != dev:
+        raise ValueError(f"stream is on cuda:{stream.device_index}, not on the current GPU")
     return dev, stream.cuda_stream
 
 

@@ -90,3 +90,20 @@ def test_workspace_sizes_past_32_bits_are_refused(sizes):
     for op in range(4):
         with pytest.raises(ValueError, match="32 bits"):
             tmt_moe.linear_workspace_size(op, *sizes)
+
+
+class Queue:
+    """A torch.cuda.Stream as the binding sees it."""
+
+    def __init__(self, device):
+        self.cuda_stream, self.device_index, self.device = 0x7000, device, torch.device("cuda", device)
+
+
+@pytest.mark.parametrize("entry", ENTRIES)
+def test_a_stream_of_another_gpu_is_refused(lib, entry):
+    """Work goes to the current GPU, whose memory the operands are in."""
+    _calls(48, 32, 128, stream=Queue(0))[entry]()
+    assert len(lib.calls) == 1 and lib.calls[0][1][0] == 0x7000
+    with pytest.raises(ValueError, match="stream is on cuda:1"):
+        _calls(48, 32, 128, stream=Queue(1))[entry]()
+    assert len(lib.calls) == 1
