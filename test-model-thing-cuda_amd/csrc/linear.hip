@@ -26,10 +26,9 @@
 // ahead into a row-contiguous bf16 tile, and fragments are read from that with
 // the transposing ds_read_b64_tr_b16.
 #include <algorithm>
-#include <cmath>
 #include <type_traits>
 
-#include "linear.hpp"
+#include "linear_plan.hpp"
 #include "moe_internal.hpp"
 #include "mx_format.hpp"
 
@@ -49,14 +48,6 @@ typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 // What is read past the end of a reduction.
 __device__ __align__(16) const uint32_t zero_piece[4] = {0, 0, 0, 0};
 
-// A window on global memory: loads read zeros past its `bytes`, so that no
-// address has to be clamped and a reduction's tail is zero times zero,
-// whatever lies behind the operands. Wave-uniform.
-struct Window {
-    uint64_t at;
-    uint32_t bytes;
-};
-__device__ __forceinline__ uint64_t address(const void* p) { return reinterpret_cast<uint64_t>(p); }
 __device__ __forceinline__ i32x4 descriptor(const Window& w) {
     return i32x4{(int)(uint32_t)w.at, (int)(uint32_t)(w.at >> 32), (int)w.bytes, 0x00020000};  // raw buffer
 }
@@ -96,60 +87,6 @@ __device__ __forceinline__ uint4 expand_fp8(uint2 w, float sc) {
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, sc, true)),
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, false)),
                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, sc, true)));
-}
-
-// ---- units -----------------------------------------------------------------
-// tiles_m x tiles_c output tiles. The first `whole` are units of their own;
-// the `tail` others, the last round's, are cut into `parts` along the
-// reduction, `chunk` (a multiple of 256) each: a launch of its own writes
-// their fp32 partial tiles, which linear_fixup_kernel adds in part order.
-struct LinearPlan {
-    int tile = 256, tiles_m = 0, tiles_c = 0, whole = 0, tail = 0, parts = 1, chunk = 0;
-};
-struct Unit {
-    int m0, c0, kbeg, kend, part;
-};
-// Consecutive tiles go down 4 rows of tiles (or what 32 tiles leave where
-// there are few columns), then to the next column, so that the 32 tiles that
-// an XCD works on share operand slices in its L2.
-__device__ __forceinline__ void tile_at(const LinearPlan& pl, int j, int& mt, int& ct) {
-    const int rows = pl.tiles_c >= 8 ? 4 : 32 / pl.tiles_c;
-    const int blk = j / (rows * pl.tiles_c), rem = j - blk * (rows * pl.tiles_c);
-    const int in = min(rows, pl.tiles_m - blk * rows);
-    ct = rem / in;
-    mt = blk * rows + (rem - ct * in);
-}
-// Unit of the workgroup's slot vb (blockIdx.x, + gridDim.x, ...). The hardware
-// hands workgroup b to XCD b % 8 and the grid is a multiple of 8 where a
-// workgroup takes several slots; each XCD takes runs of consecutive units.
-template <int TILE, bool SPLIT>
-__device__ __forceinline__ bool unit_at(const LinearPlan& pl, int R, int vb, Unit& u) {
-    const int n = SPLIT ? pl.tail * pl.parts : pl.whole, whole = n & ~255, per = (n - whole + 7) / 8;
-    int j;
-    if (vb < whole) {
-        j = (((vb >> 8) << 3) + (vb & 7)) * 32 + ((vb >> 3) & 31);
-    } else {
-        const int i = (vb - whole) >> 3;
-        j = whole + (vb & 7) * per + i;
-        if (i >= per || j >= n) return false;
-    }
-    int mt, ct;
-    u.kbeg = 0;
-    u.kend = R;
-    u.part = j;
-    if constexpr (SPLIT) {
-        const int q = j / pl.parts;
-        u.kbeg = (j - q * pl.parts) * pl.chunk;
-        u.kend = min(R, u.kbeg + pl.chunk);
-        j = pl.whole + q;
-    }
-    tile_at(pl, j, mt, ct);
-    // the divisions run on the vector unit: back to scalar registers
-    u.m0 = __builtin_amdgcn_readfirstlane(mt * TILE);
-    u.c0 = __builtin_amdgcn_readfirstlane(ct * TILE);
-    u.kbeg = __builtin_amdgcn_readfirstlane(u.kbeg);
-    u.kend = __builtin_amdgcn_readfirstlane(u.kend);
-    return true;
 }
 
 // ---- epilogue ----------------------------------------------------------------
@@ -208,7 +145,7 @@ __device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, v
     rows = min(rows, 32 * MI);
     cols = min(cols, 32 * NJ);
     const __amdgpu_buffer_rsrc_t win =
-        __builtin_amdgcn_make_buffer_rsrc(out, 0, (int)((uint32_t)(rows - 1) * row + (uint32_t)cols * SIZE), 0x00020000);
+        __builtin_amdgcn_make_buffer_rsrc(out, 0, (int)output_window(rows, row, cols, SIZE), 0x00020000);
     uint4 v[32 / RPI];  // rows of a slice
     auto store = [&](int n) {
         const int c = 32 * JS * (n % JG) + cl * (16 / SIZE);
@@ -297,6 +234,8 @@ __device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, v
     store(SLICES - 1);
 }
 
+constexpr auto workgroups = [] __device__() { return (int)gridDim.x; };
+
 // Writes a unit's wave outputs: to the result or, SPLIT, as a partial tile
 // (fp32; bf16 results' partial tiles leave from the registers, whose LDS holds
 // no fp32 rows).
@@ -365,19 +304,11 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) return;
 
-    // ---- the next step to load: windows on its operands, and the steps left in
-    // its unit. Past the last unit the windows are empty.
-    Window wa, wq, wsc;
-    int left = 0, vl = vb, sll = 0;
-    auto set = [&](const Unit& n) {
-        wa = {address(p.x + (int64_t)n.m0 * p.ldx + n.kbeg),
-              (uint32_t)(min(p.T - n.m0, TILE) - 1) * (uint32_t)(p.ldx * 2) + (uint32_t)(K - n.kbeg) * 2};
-        wq = {address(p.w + (int64_t)n.c0 * (K / 2) + n.kbeg / 2),
-              (uint32_t)(min(p.N - n.c0, TILE) - 1) * (uint32_t)(K / 2) + (uint32_t)(K - n.kbeg) / 2};
-        wsc = {address(p.ws + (int64_t)(n.kbeg / 32) * p.wlds + n.c0), (uint32_t)(2 * p.wlds) - n.c0};
-        left = (n.kend - n.kbeg) >> 6;
-    };
-    set(u);
+    // ---- the next step to load
+    FwdCursor<TILE, SPLIT> at;
+    at.vl = vb;
+    at.set(p, u);
+    int sll = 0;
     uint32_t a_off[G::A_LOADS], q_off[G::Q_LOADS];
 #pragma unroll
     for (int i = 0; i < G::A_LOADS; ++i) {
@@ -393,26 +324,13 @@ __global__ __launch_bounds__(256, (Fwd<TILE>::WGS)) void linear_fwd_kernel(Linea
     // load d of the step: the codes, the scales, the activations
     auto load = [&](int d) {
         const uint32_t a = lds0 + G::A0 + sll * G::A_BYTES, b = lds0 + G::B0 + sll * G::B_BYTES;
-        if (d < G::Q_LOADS) dma16(wq, q_off[d], b + (wave * G::Q_LOADS + d) * 1024);
-        else if (d == G::Q_LOADS) dma16(wsc, sc_off, b + G::Q_BYTES);
-        else dma16(wa, a_off[d - G::Q_LOADS - 1], a + (wave * G::A_LOADS + d - G::Q_LOADS - 1) * 1024);
+        if (d < G::Q_LOADS) dma16(at.wq, q_off[d], b + (wave * G::Q_LOADS + d) * 1024);
+        else if (d == G::Q_LOADS) dma16(at.wsc, sc_off, b + G::Q_BYTES);
+        else dma16(at.wa, a_off[d - G::Q_LOADS - 1], a + (wave * G::A_LOADS + d - G::Q_LOADS - 1) * 1024);
     };
     auto next_loads = [&]() {
         sll = sll == 2 ? 0 : sll + 1;
-        if (left == 0) return;  // no unit left: the windows stay empty
-        if (--left > 0) {
-            wa = {wa.at + 128, wa.bytes - 128};
-            wq = {wq.at + 32, wq.bytes - 32};
-            wsc.at += 2 * p.wlds;
-            return;
-        }
-        Unit n;
-        vl += gridDim.x;
-        if (unit_at<TILE, SPLIT>(pl, K, vl, n)) {
-            set(n);
-        } else {
-            wa.bytes = wq.bytes = wsc.bytes = 0;
-        }
+        at.next(p, pl, workgroups);
     };
 
     // ---- fragments -----------------------------------------------------------
@@ -528,7 +446,7 @@ struct Grad {
     static constexpr int WT = TILE / 2, MI = WT / 32;
     static constexpr int A_BYTES = DW ? TILE * 64 : TILE * 128, A_SLOTS = DW ? 4 : 3;
     static constexpr int A_LOADS = TILE * 64 / 4096;  // 1 KiB loads per wave and sub-step
-    static constexpr int CB = DW ? 8 : 4;             // code bytes of 8 columns
+    static constexpr int CB = GradCodesCursor<OP, TILE, false>::CB;
     static constexpr int ROWQ = TILE / 8 * CB;        // code bytes per raw row
     static constexpr int Q_BYTES = 32 * ROWQ;
     static constexpr int Q_LOADS = (Q_BYTES + 4095) / 4096;
@@ -553,51 +471,25 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT;
-    const int M = DW ? p.N : p.T, C = p.K, K = p.K, R = DW ? p.T : p.N;
-    const int64_t rowq = DW ? p.K : p.K / 2;  // code bytes per row of the weights / checkpoint
+    const int M = DW ? p.N : p.T, C = p.K, R = DW ? p.T : p.N;
 
     Unit u;
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, R, vb, u)) return;
 
-    // ---- the next K = 64 steps to load, of the activations and of the raw codes:
-    // windows on them, and the steps left in their units. Past the last unit the
-    // windows are empty.
+    // ---- the next K = 64 steps to load, of the activations and of the raw codes
     constexpr int AC = TILE / 8;                // 16-byte chunks per row of a tile across the reduction
     constexpr int PPR = G::ROWQ / 16;           // 16-byte pieces per raw row
     constexpr int QL = G::Q_BYTES / 1024;       // wave loads of a raw tile (fewer than the waves: loaded twice)
     constexpr int NA = DW ? G::A_LOADS : 2 * G::A_LOADS;
-    const uint32_t ldb = (uint32_t)(p.ldx * 2), rowb = (uint32_t)rowq;
-    Window wa, wq, wsc;
-    int a_left = 0, q_left = 0, va = vb, vq = vb;
-    int a_rows = 0, q_rows = 0;                 // reduction rows not loaded yet (DX: q only)
-    uint32_t a_skip = 0, q_skip = 0;            // bytes of a row outside the window behind the last row
+    using Codes = GradCodesCursor<OP, TILE, SPLIT>;
+    const uint32_t ldb = (uint32_t)(p.ldx * 2), rowb = (uint32_t)Codes::row_bytes(p);
+    GradRowsCursor<OP, TILE, SPLIT> ca;
+    Codes cq;
+    ca.vl = cq.vl = vb;
+    ca.set(p, u);
+    cq.set(p, u);
     int sla = 0, slq = 0;                       // ring slots of the next loads
-    auto rows_window = [](int rows, uint32_t row_bytes, uint32_t skip) {
-        return rows > 0 ? (uint32_t)min(rows, 64) * row_bytes - skip : 0u;
-    };
-    auto steps = [](const Unit& n) { return (n.kend - n.kbeg + 63) >> 6; };
-    auto set_a = [&](const Unit& n) {
-        a_left = steps(n);
-        if constexpr (DW) {
-            a_rows = n.kend - n.kbeg;
-            a_skip = ldb - (uint32_t)(p.N - n.m0) * 2;
-            wa = {address(p.x + (int64_t)n.kbeg * p.ldx + n.m0), rows_window(a_rows, ldb, a_skip)};
-        } else {
-            wa = {address(p.x + (int64_t)n.m0 * p.ldx + n.kbeg),
-                  (uint32_t)(min(p.T - n.m0, TILE) - 1) * ldb + (uint32_t)(p.N - n.kbeg) * 2};
-        }
-    };
-    auto set_q = [&](const Unit& n) {
-        q_left = steps(n);
-        q_rows = n.kend - n.kbeg;
-        q_skip = (uint32_t)n.c0 * G::CB / 8;
-        wq = {address(p.w + n.kbeg * rowq + q_skip), rows_window(q_rows, rowb, q_skip)};
-        const int blocks = min(K / 32 - n.c0 / 32, TILE / 32);
-        wsc = {address(p.ws + (int64_t)(n.c0 / 32) * p.wlds + n.kbeg), (uint32_t)(blocks * p.wlds) - n.kbeg};
-    };
-    set_a(u);
-    set_q(u);
     // DW and raw codes: [half][load], the lane's piece of a K = 64 step's half
     uint32_t a_off[2 * G::A_LOADS], q_off[2][G::Q_LOADS];
 #pragma unroll
@@ -623,54 +515,23 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     auto load = [&](int d, int q_half, int a_half) {
         const uint32_t raw = lds0 + G::R0 + slq * G::R_BYTES, act = lds0 + G::A0 + sla * G::A_BYTES;
         if (d < G::Q_LOADS) {
-            dma16(wq, q_off[q_half][d], raw + ((wave * G::Q_LOADS + d) % QL) * 1024);
+            dma16(cq.wq, q_off[q_half][d], raw + ((wave * G::Q_LOADS + d) % QL) * 1024);
         } else if (d == G::Q_LOADS) {
-            dma4(wsc, sc_off + 32 * q_half, raw + G::Q_BYTES);
+            dma4(cq.wsc, sc_off + 32 * q_half, raw + G::Q_BYTES);
         } else {
             const int i = d - G::Q_LOADS - 1;
-            dma16(wa, a_off[a_half * G::A_LOADS + i], act + (wave * NA + i + (DW ? 0 : a_half * G::A_LOADS)) * 1024);
+            dma16(ca.wa, a_off[a_half * G::A_LOADS + i], act + (wave * NA + i + (DW ? 0 : a_half * G::A_LOADS)) * 1024);
         }
     };
     // behind a raw tile's loads, and behind a sub-step's activations
     auto next_q = [&](int half) {
         slq = slq == 2 ? 0 : slq + 1;
-        if (half == 0 || q_left == 0) return;
-        if (--q_left > 0) {
-            q_rows -= 64;
-            wq = {wq.at + 64 * rowq, rows_window(q_rows, rowb, q_skip)};
-            wsc = {wsc.at + 64, (uint32_t)max((int)wsc.bytes - 64, 0)};
-            return;
-        }
-        Unit n;
-        vq += gridDim.x;
-        if (unit_at<TILE, SPLIT>(pl, R, vq, n)) {
-            set_q(n);
-        } else {
-            wq.bytes = wsc.bytes = 0;
-            q_rows = 0;
-        }
+        if (half == 1) cq.next(p, pl, workgroups);
     };
     auto next_a = [&](int half) {
         if (DW) sla = (sla + 1) & 3;
         else if (half == 1) sla = sla == 2 ? 0 : sla + 1;
-        if (half == 0 || a_left == 0) return;
-        if (--a_left > 0) {
-            if constexpr (DW) {
-                a_rows -= 64;
-                wa = {wa.at + 64 * (uint64_t)ldb, rows_window(a_rows, ldb, a_skip)};
-            } else {
-                wa = {wa.at + 128, wa.bytes - 128};
-            }
-            return;
-        }
-        Unit n;
-        va += gridDim.x;
-        if (unit_at<TILE, SPLIT>(pl, R, va, n)) {
-            set_a(n);
-        } else {
-            wa.bytes = 0;
-            a_rows = 0;
-        }
+        if (half == 1) ca.next(p, pl, workgroups);
     };
     // The lane's share of a raw tile: EP pieces of 8 codes with their scales,
     // in registers from one k16 step to the next.
@@ -764,7 +625,7 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
     for (int t = 0; t < 3; ++t) {
 #pragma unroll
         for (int d = 0; d <= G::Q_LOADS; ++d) load(d, t & 1, 0);
-        valid[t] = q_rows - 32 * (t & 1);
+        valid[t] = cq.rows - 32 * (t & 1);
         next_q(t & 1);
     }
 #pragma unroll
@@ -824,7 +685,7 @@ __global__ __launch_bounds__(256, (Grad<OP, TILE>::WGS)) void linear_grad_kernel
                 });
                 valid[0] = valid[1];
                 valid[1] = valid[2];
-                valid[2] = q_rows - 32 * (h ^ 1);
+                valid[2] = cq.rows - 32 * (h ^ 1);
                 next_q(h ^ 1);
                 next_a(DW ? h ^ 1 : h);
                 // Outstanding at most: the activations of the last sub-step and
@@ -912,21 +773,12 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, K, vb, u)) return;
 
-    // ---- the next step to load: windows on its operands. Pieces past a row's
-    // end are another row's: they are not multiplied.
-    Window wx, wxs, ww, wws;
-    int kn = 0, kend = 0, vn = vb, sl = 0;
-    bool left = true;
-    auto set = [&](const Unit& n) {
-        kn = n.kbeg;
-        kend = n.kend;
-        wx = {address(p.xq + (int64_t)n.m0 * (K / 2) + kn / 2), (uint32_t)(min(p.T - n.m0, TILE) - 1) * (uint32_t)(K / 2) + (K - kn) / 2};
-        ww = {address(p.w + (int64_t)n.c0 * (K / 2) + kn / 2), (uint32_t)(min(p.N - n.c0, TILE) - 1) * (uint32_t)(K / 2) + (K - kn) / 2};
-        const uint32_t blocks = (uint32_t)min(8, (K - kn) / 32);
-        wxs = {address(p.xs + (int64_t)(kn / 32) * p.xlds + n.m0), blocks * (uint32_t)p.xlds - n.m0};
-        wws = {address(p.ws + (int64_t)(kn / 32) * p.wlds + n.c0), blocks * (uint32_t)p.wlds - n.c0};
-    };
-    set(u);
+    // ---- the next step to load
+    MxCursor<TILE, SPLIT> at;
+    at.vl = vb;
+    at.of_w = wave & 1;
+    at.set(p, u);
+    int sl = 0;
     uint32_t off[G::LOADS];
 #pragma unroll
     for (int i = 0; i < G::LOADS; ++i) {
@@ -936,27 +788,15 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
     // waves 0 and 1: the scales of X and W; 2 and 3 the same again
     const uint32_t sc_off = (uint32_t)(lane & 7) * (uint32_t)((wave & 1) ? p.wlds : p.xlds) + 16 * (lane >> 3);
     auto load_step = [&]() {
-        const uint32_t at = lds0 + sl * G::SLOT;
+        const uint32_t to = lds0 + sl * G::SLOT;
 #pragma unroll
         for (int i = 0; i < G::LOADS; ++i) {
-            dma16(wx, off[i], at + (wave * G::LOADS + i) * 1024);
-            dma16(ww, off[i], at + G::CODES + (wave * G::LOADS + i) * 1024);
+            dma16(at.wx, off[i], to + (wave * G::LOADS + i) * 1024);
+            dma16(at.ww, off[i], to + G::CODES + (wave * G::LOADS + i) * 1024);
         }
-        dma16((wave & 1) ? wws : wxs, sc_off, at + 2 * G::CODES + (wave & 1) * 1024);
+        dma16(at.wsc, sc_off, to + 2 * G::CODES + (wave & 1) * 1024);
         sl ^= 1;
-        kn += 256;
-        if (kn < kend) {
-            wx = {wx.at + 128, wx.bytes - 128};
-            ww = {ww.at + 128, ww.bytes - 128};
-            const uint32_t gone = (uint32_t)(8 - min(8, (K - kn) / 32));  // blocks past the end in a last step
-            wxs = {wxs.at + 8 * p.xlds, wxs.bytes - gone * (uint32_t)p.xlds};
-            wws = {wws.at + 8 * p.wlds, wws.bytes - gone * (uint32_t)p.wlds};
-            return;
-        }
-        Unit n;
-        vn += gridDim.x;
-        left = unit_at<TILE, SPLIT>(pl, K, vn, n);
-        if (left) set(n);
+        at.next(p, pl, workgroups);
     };
     f32x16 acc[MI][MI];
     clear(acc);
@@ -966,7 +806,7 @@ __global__ __launch_bounds__(256, 2) void linear_mx_kernel(LinearParams p, Linea
         for (int k = u.kbeg; k < u.kend; k += 256) {
             wait_vm<0>();
             lds_barrier();  // step k is whole in LDS, and the other slot is read
-            if (left) load_step();
+            if (at.left) load_step();
             const uint8_t* st = lds + slot * G::SLOT;
             const int groups = FULL ? 4 : min(4, (u.kend - k) / 64);
             int as[MI], bs[MI];
@@ -1051,17 +891,12 @@ __global__ __launch_bounds__(256, 1) void linear_mx_large_kernel(LinearParams p,
     int vb = blockIdx.x;
     if (!unit_at<TILE, false>(pl, K, vb, u)) return;
 
-    // ---- the next step to load, as in linear_fwd_kernel
-    Window wx, wxs, ww, wws;
-    int left = 0, vl = vb, sll = 0;
-    auto set = [&](const Unit& n) {
-        wx = {address(p.xq + (int64_t)n.m0 * (K / 2)), (uint32_t)min(p.T - n.m0, TILE) * (uint32_t)(K / 2)};
-        ww = {address(p.w + (int64_t)n.c0 * (K / 2)), (uint32_t)min(p.N - n.c0, TILE) * (uint32_t)(K / 2)};
-        wxs = {address(p.xs + n.m0), 8 * (uint32_t)p.xlds - n.m0};
-        wws = {address(p.ws + n.c0), 8 * (uint32_t)p.wlds - n.c0};
-        left = K / 256;
-    };
-    set(u);
+    // ---- the next step to load
+    MxLargeCursor<TILE> at;
+    at.vl = vb;
+    at.of_w = wave & 1;
+    at.set(p, u);
+    int sll = 0;
     uint32_t off[G::LOADS];
 #pragma unroll
     for (int i = 0; i < G::LOADS; ++i) {
@@ -1071,26 +906,15 @@ __global__ __launch_bounds__(256, 1) void linear_mx_large_kernel(LinearParams p,
     // even waves: the scales of X, odd waves: of W; 128 rows each
     const uint32_t sc_off = (uint32_t)(lane & 7) * (uint32_t)((wave & 1) ? p.wlds : p.xlds) + 16 * (lane >> 3) + 128 * (wave >> 1);
     auto load = [&](int d) {
-        const uint32_t at = lds0 + sll * G::SLOT;
+        const uint32_t to = lds0 + sll * G::SLOT;
         const int i = d >> 1;
-        if (d == 2 * G::LOADS) dma16((wave & 1) ? wws : wxs, sc_off, at + 2 * G::CODES + (wave & 1) * G::SCALES + (wave >> 1) * 1024);
-        else if (d & 1) dma16(ww, off[i], at + G::CODES + (wave * G::LOADS + i) * 1024);
-        else dma16(wx, off[i], at + (wave * G::LOADS + i) * 1024);
+        if (d == 2 * G::LOADS) dma16(at.wsc, sc_off, to + 2 * G::CODES + (wave & 1) * G::SCALES + (wave >> 1) * 1024);
+        else if (d & 1) dma16(at.ww, off[i], to + G::CODES + (wave * G::LOADS + i) * 1024);
+        else dma16(at.wx, off[i], to + (wave * G::LOADS + i) * 1024);
     };
     auto next_loads = [&]() {
         sll ^= 1;
-        if (left == 0) return;  // no unit left: the windows stay empty
-        if (--left > 0) {
-            wx = {wx.at + 128, wx.bytes - 128};
-            ww = {ww.at + 128, ww.bytes - 128};
-            wxs.at += 8 * p.xlds;
-            wws.at += 8 * p.wlds;
-            return;
-        }
-        Unit n;
-        vl += gridDim.x;
-        if (unit_at<TILE, false>(pl, K, vl, n)) set(n);
-        else wx.bytes = ww.bytes = wxs.bytes = wws.bytes = 0;
+        at.next(p, pl, workgroups);
     };
 
     // ---- fragments
@@ -1341,98 +1165,11 @@ __global__ __launch_bounds__(256) void linear_scale_kernel(float* y, int64_t ldy
     }
 }
 
-struct Sizes {
-    int M, C, R;  // output rows and columns, reduction length
-};
-Sizes sizes(LinearOp op, int T, int N, int K) {
-    if (op == LINEAR_DX) return {T, K, N};
-    if (op == LINEAR_DW) return {N, K, T};
-    return {T, N, K};
-}
-
-// Workgroups that run at a time.
-// (cus: compute units, asked for once a call; each question costs the host 30 ns,
-// and a plan of many candidates would ask 100 times.)
-int64_t tile_slots(int tile, int cus) { return (int64_t)cus * (tile == 256 ? 1 : 2); }
-constexpr int kMinSteps = 4;  // K = 64 steps that a part of a split reduction has at least
-
-LinearPlan plan_tiles(const Sizes& z, int tile, int64_t parts, int cus) {
-    LinearPlan pl;
-    pl.tile = tile;
-    pl.tiles_m = (z.M + tile - 1) / tile;
-    pl.tiles_c = (z.C + tile - 1) / tile;
-    const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_c;
-    pl.whole = (int)tiles;
-    if (parts >= 2) {
-        const int nk = (z.R + 63) / 64;
-        pl.whole = (int)(tiles / tile_slots(tile, cus) * tile_slots(tile, cus));
-        pl.tail = (int)(tiles - pl.whole);
-        pl.chunk = (int)((nk + 4 * parts - 1) / (4 * parts)) * 256;  // whole steps of every kernel
-        pl.parts = (nk * 64 + pl.chunk - 1) / pl.chunk;
-    }
-    return pl;
-}
-
-// What a launch takes, in us, from its K = 64 steps. Measured on one MI355X
-// over 16 .. 512 tiles and 4 .. 512 steps:
-//   start  launch, first loads and epilogue of 128 x 128 tiles (256 x 256: 4 more)
-//   one    a step of 128 x 128 tiles, one workgroup per CU (bound by latency)
-//   two    the same with two
-//   large  a step of 256 x 256 tiles (bound by the matrix cores)
-struct StepTimes {
-    double start, one, two, large;
-};
-constexpr StepTimes kTimes[4] = {{4.5, 0.62, 1.05, 1.45}, {2.5, 0.28, 0.48, 0.0}, {4.2, 0.82, 1.35, 1.75}, {4.2, 0.82, 1.35, 1.8}};
-// A split reduction adds a launch for the sums and its partial tiles' way
-// through the last-level cache and back.
-constexpr double kSplitStart = 3.5, kSplitPerMiB = 0.25;
-
-double round_time(const StepTimes& t, int tile, int64_t units, double steps, int cus) {
-    if (tile == 256) return 2.0 + steps * t.large;
-    return steps * (units <= cus ? t.one : t.two);
-}
-double plan_time(const StepTimes& t, const Sizes& z, int tile, int64_t parts, int cus) {
-    const int64_t slots = tile_slots(tile, cus);
-    const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
-    const int64_t whole = tiles / slots, rest = tiles - whole * slots;
-    const double nk = (z.R + 63) / 64;
-    double us = t.start + (tile == 256 ? 4.0 : 0.0) + whole * round_time(t, tile, slots, nk, cus);
-    if (rest == 0) return us;
-    if (parts < 2) return us + round_time(t, tile, rest, nk, cus);
-    const double mib = (double)(rest * parts) * tile * tile * 4 / (1 << 20);
-    return us + round_time(t, tile, rest * parts, std::ceil(nk / parts), cus) + (whole > 0 ? t.start : 0.0) + kSplitStart + kSplitPerMiB * mib;
-}
-
-// The tile size and split with the shortest estimate. Measured (us, chosen /
-// others): forward T 777, N 4096, K 1024 14.9 on whole 128 x 128 tiles / 23.7 in
-// two parts, 30.2 on 256 x 256; T 777, N 1024, K 4096 20.7 in four parts / 27.2
-// in two, 38.2 whole; dX T 777, N 4096, K 1024 23.9 in four parts / 28.5 in
-// three; dW T 32768, N 1024, K 1024 95 on 256 x 256 tiles in 16 parts / 107 on
-// 128 x 128 in 8; T 16384, N 256, K 256 16.7 in 32 parts / 32 in 8.
-LinearPlan linear_plan(LinearOp op, int T, int N, int K, int cus, double* us) {
-    const Sizes z = sizes(op, T, N, K);
-    const StepTimes& t = kTimes[op];
-    int best_tile = 128;
-    int64_t best_parts = 1;
-    double best = 1e30;
-    for (int tile = 128; tile <= (op == LINEAR_MATMUL ? 128 : 256); tile *= 2) {
-        const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
-        const int64_t rest = tiles % tile_slots(tile, cus);
-        const int64_t most = rest > 0 ? std::min<int64_t>(tile_slots(tile, cus) / rest, (z.R + 63) / 64 / kMinSteps) : 1;
-        for (int64_t parts = 1; parts <= std::max<int64_t>(most, 1); parts += parts < 8 ? 1 : parts / 4) {
-            const double c = plan_time(t, z, tile, parts, cus);
-            if (c < best) best = c, best_tile = tile, best_parts = parts;
-        }
-    }
-    *us = best;
-    return plan_tiles(z, best_tile, best_parts, cus);
-}
-
 // BETA: a kernel that adds to what is there. Apart, since two epilogues in one
 // kernel spill the accumulators.
 template <int OP, int TILE, bool SPLIT, bool BETA>
 void launch_units(const LinearParams& p, const LinearPlan& pl, int units, int cus, hipStream_t s) {
-    const int grid = std::min((units + 7) & ~7, (int)tile_slots(TILE, cus) & ~7);
+    const int grid = unit_grid(TILE, units, cus);
     if constexpr (OP == LINEAR_MATMUL) {
         if (p.K % 256 == 0) linear_mx_kernel<SPLIT, true, BETA><<<grid, 256, 0, s>>>(p, pl);
         else linear_mx_kernel<SPLIT, false, BETA><<<grid, 256, 0, s>>>(p, pl);
@@ -1453,21 +1190,9 @@ void launch_tiles(const LinearParams& p, const LinearPlan& pl, int cus, hipStrea
     }
 }
 
-// Whether 256 x 256 tiles of MXFP4 x MXFP4 are estimated to be faster: rounds of
-// one tile per CU, 5.0 us and 1.9 a step (K = 256), against rounds of 128 x 128
-// tiles at two per CU, 1.95 and 1.13, from two of those on. Measured (us, 128 /
-// 256): T 65536, N 4096, K 512 134 / 137, K 1024 226 / 206; T 16384, N 4096, K
-// 1024 53 / 55, K 2048 87 / 84; T 65536, N 1024, K 4096 152 / 143; T 20011, N
-// 2736, K 768 47 / 64.
-bool mx_large(int T, int N, int K, int cus) {
-    const int64_t small = (int64_t)((T + 127) / 128) * ((N + 127) / 128), big = (int64_t)((T + 255) / 256) * ((N + 255) / 256);
-    if (K % 256 != 0 || small < 2 * tile_slots(128, cus)) return false;
-    const double steps = K / 256, slots2 = (double)tile_slots(128, cus), slots1 = (double)tile_slots(256, cus);
-    return 3.0 + std::ceil(big / slots1) * (5.0 + 1.9 * steps) < std::ceil(small / slots2) * (1.95 + 1.13 * steps);
-}
 void launch_mx_large(const LinearParams& p, int cus, hipStream_t s) {
     const LinearPlan pl = plan_tiles(sizes(LINEAR_MATMUL, p.T, p.N, p.K), 256, 1, cus);
-    const int grid = std::min((pl.whole + 7) & ~7, (int)tile_slots(256, cus) & ~7);
+    const int grid = unit_grid(256, pl.whole, cus);
     if (p.beta == 0.0f) linear_mx_large_kernel<false><<<grid, 256, 0, s>>>(p, pl);
     else linear_mx_large_kernel<true><<<grid, 256, 0, s>>>(p, pl);
 }
@@ -1476,14 +1201,6 @@ template <int RB, int NB, int NW, int U>
 void launch_rows_as(const LinearParams& p, hipStream_t s) {
     const int64_t grid = (int64_t)((p.N + 16 * NB - 1) / (16 * NB)) * ((p.T + 16 * RB - 1) / (16 * RB));
     linear_rows_kernel<RB, NB, NW, U><<<(unsigned)grid, 64 * NW, 0, s>>>(p);
-}
-// The kernel for few tokens runs where its estimate in us, measured over T 1 ..
-// 777, N and K 256 .. 4096, is not above the tiles'. T 777, N 1024, K 1024 10.1
-// (tiles 13.6), T 512, N 4096, K 1024 17.7 (tiles 14.2).
-// It stays below 2^21 workgroups; a launch holds 2^32 threads.
-double rows_time(int T, int N, int K) {
-    if ((int64_t)T * N >= (int64_t)1 << 30) return 1e30;
-    return 3.0 + 7.2e-9 * ((double)T * N * K);
 }
 // Blocks of outputs grow with the grid, which fills the chip twice at most: 16 x
 // 16, 16 x 32 (columns), 32 x 32, 64 x 32. Measured (us) 16 x 16 / 16 x 32 / 32 x
@@ -1503,22 +1220,7 @@ void launch_rows(const LinearParams& p, int cus, hipStream_t s) {
 
 }  // namespace
 
-// An upper bound over all token counts up to T, so that a workspace for T
-// serves fewer: tail tiles times parts fill at most the workgroup slots, and
-// neither tiles nor parts fall with T.
-size_t linear_workspace(LinearOp op, int T, int N, int K) {
-    const Sizes z = sizes(op, T, N, K);
-    const int cus = cu_count();
-    size_t most = 0;
-    for (int tile = 128; tile <= 256; tile *= 2) {
-        const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
-        const int64_t parts = (z.R + 63) / 64 / kMinSteps;
-        if (parts < 2) continue;
-        const int64_t units = std::min(tiles * parts, tile_slots(tile, cus));
-        most = std::max(most, (size_t)units * tile * tile * 4);
-    }
-    return most;
-}
+size_t linear_workspace(LinearOp op, int T, int N, int K) { return workspace_bound(op, T, N, K, cu_count()); }
 
 hipError_t launch_linear(LinearOp op, const LinearParams& p, hipStream_t s) {
     const int cus = cu_count();

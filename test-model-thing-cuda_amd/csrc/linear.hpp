@@ -33,6 +33,9 @@ hipError_t launch_mx_rows(bool quantize, int format, bool f32, const MxRowsParam
 //   MATMUL   the same with x in MXFP4
 //   DX       y[t][k] = sum_n x[t][n] w[n][k]   M = T, C = K, R = N
 //   DW       y[n][k] = sum_t x[t][n] w[t][k]   M = N, C = K, R = T; w in MXFP8, y fp32
+// The kernels' offsets inside a tile are 32-bit.
+constexpr int64_t kMaxStride = int64_t(1) << 22;   // elements between rows
+constexpr int64_t kMaxScaleStride = int64_t(1) << 27;
 enum LinearOp { LINEAR_FORWARD = 0, LINEAR_MATMUL = 1, LINEAR_DX = 2, LINEAR_DW = 3 };
 struct LinearParams {
     int T, N, K;

@@ -36,9 +36,6 @@ int check_rows(int32_t format, int32_t dtype, int32_t rows, int32_t K, const voi
     return TMT_MOE_OK;
 }
 
-// The kernels' offsets inside a tile are 32-bit.
-constexpr int64_t kMaxStride = int64_t(1) << 22;   // elements between rows
-constexpr int64_t kMaxScaleStride = int64_t(1) << 27;
 constexpr int32_t kMaxWidth = 1 << 22;             // N and K
 constexpr int32_t kMaxTokens = 1 << 30;
 constexpr int64_t kMaxOutputs = int64_t(1) << 40;  // of a product, so that 32 bits count the tiles
