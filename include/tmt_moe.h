@@ -438,6 +438,7 @@ enum {
     TMT_MOE_LINEAR_DX = 2,       /* tmt_moe_mxfp4_linear_dx */
     TMT_MOE_LINEAR_DW = 3        /* tmt_moe_mxfp8_linear_dw */
 };
+/* Bytes for calls of up to T tokens; 0 for tmt_moe_mxfp4_linear of few. */
 int tmt_moe_linear_workspace_size(int32_t op, int32_t T, int32_t N, int32_t K, size_t* bytes);
 
 /* Y [T][ldy] = beta * Y + X W^T: X [T][ldx] bf16, W [N][K] MXFP4, Y bf16. */

@@ -386,11 +386,16 @@ inline double rows_time(int T, int N, int K) {
 
 // An upper bound over all token counts up to T, so that a workspace for T
 // serves fewer: tail tiles times parts fill at most the workgroup slots, and
-// neither tiles nor parts fall with T.
+// neither tiles nor parts fall with T. Both operands in MXFP4 are split on 128 x
+// 128 tiles only. A split reduction's estimate is at least its start and end
+// and the fewest steps of a part: where the kernel for few tokens is estimated to
+// take no longer, no call of up to T tokens is split.
 inline size_t workspace_bound(LinearOp op, int T, int N, int K, int cus) {
     const Sizes z = sizes(op, T, N, K);
+    const StepTimes& t = kTimes[op];
+    if (op == LINEAR_FORWARD && rows_time(T, N, K) <= t.start + kMinSteps * t.one + kSplitStart) return 0;
     size_t most = 0;
-    for (int tile = 128; tile <= 256; tile *= 2) {
+    for (int tile = 128; tile <= (op == LINEAR_MATMUL ? 128 : 256); tile *= 2) {
         const int64_t tiles = (int64_t)((z.M + tile - 1) / tile) * ((z.C + tile - 1) / tile);
         const int64_t parts = (z.R + 63) / 64 / kMinSteps;
         if (parts < 2) continue;
