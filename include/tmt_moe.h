@@ -392,15 +392,19 @@ int tmt_moe_f32_to_bf16(void* stream, const float* in, uint16_t* out, int64_t n)
  * An MXFP4 matrix with lds == rows is a W_up[e] / W_down[e] of
  * tmt_moe_forward_mxfp4.
  *
- * Every product sums exact terms in fp32 (a code times its scale is exact in
- * bf16; MXFP8 values at scale bytes below 3 are rounded to bf16's subnormals)
- * and rounds once. Y = beta * Y + ...; with beta == 0 the output is
- * not read. Outputs must not overlap inputs. T from 0 to 2^30, N a multiple
- * of 16, K a multiple of 64, both and all row strides at most 2^22, scale
- * strides at most 2^27, T*N, T*K and N*K at most 2^40. Strides are in elements;
- * bf16 and fp32 rows start at 16-byte boundaries (base and stride), codes and scales of a product too
- * (scale strides are multiples of 16). Elements between a row's width and its
- * stride are neither read into a result nor written.
+ * Every product sums exact terms in fp32 and rounds once. Where an operand
+ * goes through bf16 (all but both in MXFP4), a code times its scale is exact
+ * there, except that MXFP8 values at scale bytes below 3 are rounded to bf16's
+ * subnormals and values of 2^128 or more (MXFP4 codes at scale bytes 253 and
+ * 254, which tmt_moe_mx_quantize never writes) are infinite. Y = beta * Y +
+ * ...; with beta == 0 the output is not read. Outputs must not overlap inputs.
+ * T from 0 to 2^30, N a multiple of 16, K a multiple of 64, both and all row
+ * strides at most 2^22, scale strides at most 2^27 (which bounds T where X is
+ * microscaled), T*N, T*K and N*K at most 2^40. Strides are in elements; bf16
+ * and fp32 rows start at 16-byte boundaries (base and stride), codes and
+ * scales of a product too (scale strides are multiples of 16). Elements
+ * between a row's width and its stride are neither read into a result nor
+ * written.
  *
  * All calls enqueue on `stream` on the current device, allocate nothing and
  * do not synchronise. The products take a workspace of
@@ -419,7 +423,9 @@ enum { TMT_MOE_BF16 = 0, TMT_MOE_F32 = 1 };
  *           the even code), saturating at 6: the format of the expert weights;
  *   MX_FP8  the smallest exponent with amax <= 448 * 2^e, nearest e4m3 value
  *           (ties to even): nothing saturates, so a value is off by at most
- *           2^-4 of itself or half a step of e4m3's subnormals.
+ *           2^-4 of itself or half a step of e4m3's subnormals. Values of
+ *           1.9375 * 2^127 or more round to 2^128, which is infinite in bf16
+ *           and fp32.
  * Exponents are clamped to [-127, 127]; a block of zeros takes exponent 0; a
  * block with an infinity or a NaN takes s = 255. K a multiple of 32; lds any
  * number >= rows; rows times K, rounded up to multiples of 16 (32 where K < 256)

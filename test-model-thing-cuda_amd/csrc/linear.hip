@@ -1,8 +1,9 @@
 // linear.hip -- products of the linear layer on microscaled numbers.
 //
-// Every operand value is exact in bf16 (an e2m1 code has two significant
-// bits, an e4m3 code four, and scales are powers of two), so a product with
-// bf16 rows is one bf16 matrix product with fp32 sums of exact terms.
+// Every operand value inside bf16's range is exact in bf16 (an e2m1 code has
+// two significant bits, an e4m3 code four, and scales are powers of two), so a
+// product with bf16 rows is one bf16 matrix product with fp32 sums of exact
+// terms.
 //
 //   FORWARD  Y[t][n] = sum_k X[t][k] W[n][k]     X and the codes along k
 //   MATMUL   the same with X in MXFP4, on the scaled matrix instructions
