@@ -1225,7 +1225,6 @@ size_t linear_workspace(LinearOp op, int T, int N, int K) { return workspace_bou
 
 hipError_t launch_linear(LinearOp op, const LinearParams& p, hipStream_t s) {
     const int cus = cu_count();
-    if (op != LINEAR_DW && p.T <= 0) return hipSuccess;
     if (op == LINEAR_DW && p.T == 0) {
         if (p.beta == 1.0f) return hipSuccess;
         const int64_t blocks = std::min<int64_t>(((int64_t)p.N * p.K / 4 + 255) / 256, 16 * (int64_t)cus);

@@ -26,6 +26,7 @@ inline int64_t mx_tiles(int rows, int K) {
     const int rt = kMxTile >> mx_tile_log2_cols(K);
     return ((int64_t)rows + rt - 1) / rt * mx_tiles_per_row(K);
 }
+// Arguments as the C ABI has checked them, rows > 0.
 hipError_t launch_mx_rows(bool quantize, int format, bool f32, const MxRowsParams& p, hipStream_t s);
 
 // The products. M output rows, C output columns, R the reduction length:
@@ -53,6 +54,7 @@ struct LinearParams {
     float* part;          // workspace: split reductions' partial sums
 };
 size_t linear_workspace(LinearOp op, int T, int N, int K);
+// Arguments as the C ABI has checked them; T == 0 for DW only.
 hipError_t launch_linear(LinearOp op, const LinearParams& p, hipStream_t s);
 
 }  // namespace tmt

@@ -32,11 +32,8 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t amax) {
     const int s = FMT == MX_FP4 ? be - 2 : be - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
     return (uint32_t)max(s, 0);
 }
-// 1 / 2^(s - 127) for the scales that mx_scale gives (0 .. 252, or 255: then
-// the codes are those of 0).
-__device__ __forceinline__ float mx_inverse(uint32_t s) {
-    return s == 255 ? 0.0f : __uint_as_float((254 - s) << 23);
-}
+// 1 / 2^(s - 127) for the scales that mx_scale gives a finite block (0 .. 252).
+__device__ __forceinline__ float mx_inverse(uint32_t s) { return __uint_as_float((254 - s) << 23); }
 
 // Eight scaled values to e2m1 codes, element i in bits 4i .. 4i + 3.
 __device__ __forceinline__ uint32_t to_e2m1(const float* v) {
