@@ -746,6 +746,8 @@ __device__ __forceinline__ f32x16 mma_mx(i32x4 w, i32x4 x, f32x16 c, int ws, int
                                                            __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4,
                                                            G, ws, G, xs);
 }
+// Few tokens take a tile's 128 rows too: N 1024, K 4096, split in parts, T 1 / 16
+// / 64 6.0 / 6.7 / 8.0 us (bf16 activations, T 16: 5.1).
 // FULL: K is a multiple of 256, and no branch stands between a step's reads and
 // its MFMAs (T 16384, N 4096, K 4096 185 -> 175 us, T 16384, N 16384, K 8192
 // 1319 -> 1201).
@@ -1209,6 +1211,9 @@ void launch_rows_as(const LinearParams& p, hipStream_t s) {
 // 4.8 / 4.6 / 4.7 / 6.4; T 256, N 4096, K 1024 13.8 / 11.4 / 11.2 / 10.0.
 // Reductions of more than 8 pieces take 8 waves with two pieces in flight (32 x
 // 32: one), shorter ones 4 waves with two (16 x 16: 8 with one).
+// Measured to N 4096. Layers so wide that blocks of 32 x 32 fill the chip more
+// than twice take blocks of 64 tokens however few there are, and lose by it: one
+// token, K 4096: N 16384 10.9 us, N 32768 38, where the codes alone take 14.
 void launch_rows(const LinearParams& p, int cus, hipStream_t s) {
     const int64_t most = 2 * (int64_t)cus, n16 = (p.N + 15) / 16, n32 = (p.N + 31) / 32;
     const int64_t t16 = (p.T + 15) / 16, t32 = (p.T + 31) / 32;
