@@ -469,6 +469,96 @@ int tmt_moe_mxfp8_linear_dw(void* stream, int32_t T, int32_t N, int32_t K, const
                             const uint8_t* X, const uint8_t* X_scale, int64_t ldxs, float* dW, int64_t lddw,
                             float beta, void* workspace, size_t workspace_bytes);
 
+/*
+ * A linear layer in 8-bit floating point and the root-mean-square norm in front
+ * of it, next to the microscaled layer above: both operands are e4m3 codes, with
+ * one fp32 scale for each block of 128 values. No handle; the reference has
+ * neither. A training step of the layer:
+ *   forward   rmsnorm_forward (residual added, out in codes), fp8_matmul with the
+ *             weight's codes;
+ *   backward  fp8_quantize of dY, in its own order and transposed; dX = dY W:
+ *             fp8_matmul with the weight's transposed codes; dW = dY^T X:
+ *             fp8_matmul of the transposed codes of dY and X, fp32 out;
+ *             rmsnorm_backward;
+ *   weights   fp8_quantize of the fp32 masters in tiles, both ways.
+ *
+ * Blocks: with m the largest magnitude of a block, and at least 2^-100,
+ *   code = e4m3(x * (448 / m)),  scale = m / 448,
+ * each operation rounded to fp32 once and the code to nearest, ties to even. A
+ * value is off by at most 2^-4 of itself, or by half a step of e4m3's subnormals
+ * (m / 448 * 2^-10). A block with an infinity or a NaN has a NaN for its scale and
+ * codes of zero: every product with it is NaN.
+ *   FP8_ROWS   1 x 128: codes [rows][ldc], scales [ceil(K / 128)][lds], lds >= rows
+ *   FP8_TILES  128 x 128: codes [rows][ldc], scales [ceil(rows / 128)][lds],
+ *              lds >= ceil(K / 128)
+ * The last block of a row (a tile's last rows and columns) may be short. Code rows
+ * start at 16-byte boundaries (base and ldc); the bytes from K to the next
+ * multiple of 16 are part of every row, the last one too: the calls here write
+ * zeros there, and a product needs them to be zeros. Bytes past that, and the
+ * scales' columns past the last row, are neither written nor read into a result.
+ *
+ * bf16 and fp32 rows start at 16-byte boundaries (base and stride), fp32 vectors
+ * too; scales and rstd need 4 bytes. Rows are at most 2^30, row strides 2^22,
+ * scale strides 2^31 elements. Outputs must not overlap inputs, but for what is
+ * said below. All calls enqueue on `stream` on the current device, allocate
+ * nothing and do not synchronise. A workspace (device memory, 256-byte aligned,
+ * NULL where its size is 0) is used only inside the call: calls that share one
+ * must be ordered by the caller; its size for T or M rows serves fewer. Results
+ * are the same, bit for bit, from run to run.
+ */
+enum { TMT_MOE_FP8_ROWS = 0, TMT_MOE_FP8_TILES = 1 };
+
+/*
+ * Norm of the residual stream, per row of d values (1 to 16384):
+ *   S = X + R, rounded to the stream's type `dtype` (R and S; X is bf16)
+ *   rstd = 1 / sqrt(mean(S^2) + eps),  y = (S * rstd) * gamma
+ * y is written as bf16 to Y, and in blocks of rows (FP8_ROWS) from its fp32
+ * values to codes and scales. Without R, S is X (dtype is then TMT_MOE_BF16);
+ * without X, it is R. S, Y, codes (with scales) and rstd [T] may each be NULL,
+ * not all of them. S may be X or R itself (the same address and stride), where it
+ * has its type. Squares are summed in fp32: a row's must stay below 2^128.
+ */
+int tmt_moe_rmsnorm_forward(void* stream, int32_t T, int32_t d, int32_t dtype, const uint16_t* X, int64_t ldx,
+                            const void* R, int64_t ldr, const float* gamma, float eps, void* S, int64_t lds, uint16_t* Y,
+                            int64_t ldy, uint8_t* codes, int64_t ldc, float* scales, int64_t ldsc, float* rstd);
+/*
+ * Its gradient from dY [T][lddy] bf16, the gradient at y (codes pass it on as if
+ * they were y), with S and rstd as the forward wrote them:
+ *   g = dY * gamma, xh = S * rstd, c = mean(g * xh)
+ *   dS = dR + rstd * (g - xh * c),  dgamma = sum over rows of dY * xh
+ * dR, the gradient that reaches S by the residual stream itself, may be NULL; dR
+ * and dS have the stream's type. dS is the gradient at X and at R alike; it may be
+ * dR itself. dgamma [d] is overwritten (T == 0: zeros), its sum in a fixed order.
+ */
+int tmt_moe_rmsnorm_workspace_size(int32_t T, int32_t d, size_t* bytes);
+int tmt_moe_rmsnorm_backward(void* stream, int32_t T, int32_t d, int32_t dtype, const uint16_t* dY, int64_t lddy,
+                             const void* S, int64_t lds, const float* gamma, const float* rstd, const void* dR,
+                             int64_t lddr, void* dS, int64_t ldds, float* dgamma, void* workspace, size_t workspace_bytes);
+
+/*
+ * X [rows][ldx] (bf16 or fp32, `dtype`) to codes and scales and, in the same
+ * pass, X^T [K][rows] to codes_t [K][ldct] and scales_t. Either side may be NULL.
+ * In rows, the blocks of the two sides differ (128 values of a row, of a column);
+ * in tiles they are the same. rows and K any, fewer than 2^24 tiles of 128 x 128.
+ */
+int tmt_moe_fp8_quantize(void* stream, int32_t blocks, int32_t dtype, const void* X, int64_t ldx, int32_t rows,
+                         int32_t K, uint8_t* codes, int64_t ldc, float* scales, int64_t lds, uint8_t* codes_t,
+                         int64_t ldct, float* scales_t, int64_t ldst);
+
+/*
+ * Y [M][ldy] = beta * Y + A B^T: A [M][K] in rows, B [N][K] in rows or tiles
+ * (`b_blocks`), Y bf16 or fp32 (`dtype`). A block's products are summed in fp32,
+ * multiplied by its two scales and added in fp32; Y is rounded once. N a multiple
+ * of 8, at most 2^22 as K is; M*N at most 2^40. With beta == 0 Y is not read;
+ * M == 0 or N == 0 is no work and K == 0 gives beta * Y. Where the product of two
+ * scales is past fp32's range, the outputs may be infinite or NaN.
+ */
+int tmt_moe_fp8_workspace_size(int32_t b_blocks, int32_t M, int32_t N, int32_t K, size_t* bytes);
+int tmt_moe_fp8_matmul(void* stream, int32_t b_blocks, int32_t dtype, int32_t M, int32_t N, int32_t K, const uint8_t* A,
+                       int64_t lda, const float* A_scale, int64_t ldas, const uint8_t* B, int64_t ldb,
+                       const float* B_scale, int64_t ldbs, void* Y, int64_t ldy, float beta, void* workspace,
+                       size_t workspace_bytes);
+
 /* Thread-local message of the last failing call on this thread. */
 const char* tmt_moe_last_error(void);
 

@@ -1,0 +1,183 @@
+// fp8_quant.hip -- a matrix of bf16 or fp32 to e4m3 codes with one fp32 scale
+// for every 128 values, in its own order, transposed, or both in one pass.
+//
+//   rows   blocks of 1 x 128: scales of X's rows, and of the rows of X^T
+//          (columns of X in blocks of 128 rows);
+//   tiles  blocks of 128 x 128, the same both ways.
+//
+// Bound by memory: 2 or 4 bytes a value read, one written a side. A workgroup
+// owns a tile of 128 x 128 values, held in registers, 8 columns a piece, so that
+// the input is read once for both sides. A row's block is found in 16 lanes by
+// DPP, a column's through the waves' maxima in LDS. Codes of X leave straight from
+// the registers (128 bytes a row and tile). Codes of X^T go through LDS: a thread
+// holds the same columns of 4 neighbouring rows, so that a dword holds 4 codes of
+// a column, and the dwords of a column are XOR-swizzled.
+#include "fp8.hpp"
+#include "fp8_format.hpp"
+#include "moe_internal.hpp"
+
+namespace tmt {
+namespace {
+
+constexpr int kTile = kFp8Block;
+
+// Pieces of 8 columns a thread: of rows 4 (t / 16) .. + 3 of each 64.
+template <int THREADS>
+struct Quant {
+    static constexpr int P = kTile * 16 / THREADS;    // pieces
+    static constexpr int SPAN = THREADS / 4;          // rows of 4 pieces
+    static constexpr int WAVES = THREADS / 64;
+};
+
+template <bool TILES, bool F32, int THREADS>
+__global__ __launch_bounds__(THREADS) void fp8_quantize_kernel(Fp8QuantParams p, int tiles_k) {
+    using Q = Quant<THREADS>;
+    __shared__ uint32_t most[Q::WAVES][kTile];        // largest magnitudes: a wave's columns, or [wave][0]
+    __shared__ float row_scale[kTile];
+    __shared__ uint4 codes_t[kTile * kTile / 16];     // [column][row]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int a = tid & 15, c0 = (int)(blockIdx.x % tiles_k) * kTile;
+    const int64_t r0 = (int64_t)(blockIdx.x / tiles_k) * kTile;
+    const int rows = (int)min((int64_t)kTile, p.rows - r0), cols = min(kTile, p.K - c0);
+    auto row_of = [&](int i) { return (i >> 2) * Q::SPAN + (tid >> 4) * 4 + (i & 3); };
+
+    float v[Q::P][8];
+#pragma unroll
+    for (int i = 0; i < Q::P; ++i) {
+        const int row = row_of(i);
+        if (row < rows && 8 * a + 8 <= cols) {
+            const int64_t at = (r0 + row) * p.ldx + c0 + 8 * a;
+            if constexpr (F32) {
+                const f32x4* x = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.x) + at);
+                const f32x4 lo = x[0], hi = x[1];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i][j] = lo[j], v[i][j + 4] = hi[j];
+            } else {
+                unpack8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + at), v[i]);
+            }
+        } else {  // a row's last columns, one by one
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t at = (r0 + row) * p.ldx + c0 + 8 * a + j;
+                v[i][j] = 0.0f;
+                if (row < rows && 8 * a + j < cols)
+                    v[i][j] = F32 ? static_cast<const float*>(p.x)[at] : bf1(static_cast<const uint16_t*>(p.x)[at]);
+            }
+        }
+    }
+
+    // largest magnitudes
+    if constexpr (TILES) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < Q::P; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[i][j]));
+        m = max(m, xor_lane_u32<1>(m));
+        m = max(m, xor_lane_u32<2>(m));
+        m = max(m, xor_lane_u32<4>(m));
+        m = max(m, xor_lane_u32<8>(m));
+        m = max(m, xor_lane_u32<16>(m));
+        m = max(m, xor_lane_u32<32>(m));
+        if (lane == 0) most[wave][0] = m;
+    } else if (p.codes_t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < Q::P; ++i) m = max(m, abs_bits(v[i][j]));
+            m = max(m, xor_lane_u32<16>(m));
+            m = max(m, xor_lane_u32<32>(m));
+            if (lane < 16) most[wave][8 * a + j] = m;
+        }
+    }
+    if (TILES || p.codes_t) __syncthreads();
+    Fp8Scale tile{};
+    if constexpr (TILES) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int w = 0; w < Q::WAVES; ++w) m = max(m, most[w][0]);
+        tile = fp8_scale(m);
+        if (tid == 0) {
+            const int64_t rb = r0 / kTile, kb = c0 / kTile;
+            if (p.codes) p.scales[rb * p.lds + kb] = tile.scale;
+            if (p.codes_t) p.scales_t[kb * p.ldst + rb] = tile.scale;
+        }
+    }
+
+    // in X's order
+    if (p.codes) {
+        const int width = min(kTile, ((p.K + 15) & ~15) - c0);  // up to the 16 bytes' end: zeros
+#pragma unroll
+        for (int i = 0; i < Q::P; ++i) {
+            const int row = row_of(i);
+            Fp8Scale q = tile;
+            if constexpr (!TILES) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[i][j]));
+                m = max(m, xor_lane_u32<1>(m));
+                m = max(m, xor_lane_u32<2>(m));
+                m = max(m, xor_lane_u32<4>(m));
+                m = max(m, xor_lane_u32<8>(m));
+                q = fp8_scale(m);
+                if (a == 0) row_scale[row] = q.scale;
+            }
+            if (row < rows && 8 * a < width)
+                *reinterpret_cast<uint2*>(p.codes + (r0 + row) * p.ldc + c0 + 8 * a) =
+                    make_uint2(fp8_codes(v[i], q.inv), fp8_codes(v[i] + 4, q.inv));
+        }
+    }
+
+    // transposed
+    if (p.codes_t) {
+        uint8_t* ct = reinterpret_cast<uint8_t*>(codes_t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            Fp8Scale q = tile;
+            const int col = 8 * a + j;
+            if constexpr (!TILES) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int w = 0; w < Q::WAVES; ++w) m = max(m, most[w][col]);
+                q = fp8_scale(m);
+                if (tid < 16 && col < cols) p.scales_t[r0 / kTile * p.ldst + c0 + col] = q.scale;
+            }
+#pragma unroll
+            for (int h = 0; h < Q::P; h += 4) {
+                const float f[4] = {v[h][j], v[h + 1][j], v[h + 2][j], v[h + 3][j]};
+                const int dword = (h >> 2) * (Q::SPAN / 4) + (tid >> 4);
+                *reinterpret_cast<uint32_t*>(ct + col * kTile + ((dword ^ ((a & 7) * 4)) * 4)) = fp8_codes(f, q.inv);
+            }
+        }
+    }
+    __syncthreads();
+    if (!TILES && p.codes)
+        for (int i = tid; i < rows; i += THREADS) p.scales[(int64_t)(c0 / kTile) * p.lds + r0 + i] = row_scale[i];
+    if (p.codes_t) {
+        const uint8_t* ct = reinterpret_cast<const uint8_t*>(codes_t);
+        const int height = (int)min((int64_t)kTile, ((p.rows + 15LL) & ~15LL) - r0);
+#pragma unroll
+        for (int i = 0; i < kTile * 8 / THREADS; ++i) {
+            const int col = i * (THREADS / 8) + tid / 8, chunk = tid & 7;
+            if (col < cols && 16 * chunk < height)
+                *reinterpret_cast<uint4*>(p.codes_t + (int64_t)(c0 + col) * p.ldct + r0 + 16 * chunk) =
+                    *reinterpret_cast<const uint4*>(ct + col * kTile + ((chunk ^ ((col >> 3) & 7)) * 16));
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_fp8_quantize(bool tiles, bool f32, const Fp8QuantParams& p, hipStream_t s) {
+    const int tiles_k = (p.K + kTile - 1) / kTile;
+    const unsigned grid = (unsigned)((((int64_t)p.rows + kTile - 1) / kTile) * tiles_k);
+    constexpr int THREADS = 256;
+    if (tiles) f32 ? fp8_quantize_kernel<true, true, THREADS><<<grid, THREADS, 0, s>>>(p, tiles_k)
+                   : fp8_quantize_kernel<true, false, THREADS><<<grid, THREADS, 0, s>>>(p, tiles_k);
+    else f32 ? fp8_quantize_kernel<false, true, THREADS><<<grid, THREADS, 0, s>>>(p, tiles_k)
+             : fp8_quantize_kernel<false, false, THREADS><<<grid, THREADS, 0, s>>>(p, tiles_k);
+    return hipGetLastError();
+}
+
+}  // namespace tmt

@@ -409,7 +409,8 @@ hipError_t launch_ln_fwd(const LayerNormParams& p, hipStream_t s);
 hipError_t launch_ln_bwd(const LayerNormParams& p, hipStream_t s);
 // Fixed-order column sums of in [nrows][ncols] (ncols % 4 == 0): columns
 // [0, split) to out_lo, [split, ncols) to out_hi, each of which receives its
-// first `width` columns (width <= split, ncols - split).
+// first `width` columns (width <= split, ncols - split); split == ncols: out_lo
+// alone.
 hipError_t launch_colsum(const float* in, int nrows, int ncols, int split, int width, float* out_lo,
                          float* out_hi, hipStream_t s);
 

@@ -433,7 +433,7 @@ int ln_chunks(int T) {
 
 hipError_t launch_colsum(const float* in, int nrows, int ncols, int split, int width, float* out_lo,
                          float* out_hi, hipStream_t s) {
-    if (ncols % 4 != 0 || split % 4 != 0 || width > split || width > ncols - split) return hipErrorInvalidValue;
+    if (ncols % 4 != 0 || split % 4 != 0 || width > split || (split < ncols && width > ncols - split)) return hipErrorInvalidValue;
     colsum_kernel<<<(ncols + kColCols - 1) / kColCols, kColThreads, 0, s>>>(in, nrows, ncols, split, width, out_lo,
                                                                           out_hi);
     return hipGetLastError();

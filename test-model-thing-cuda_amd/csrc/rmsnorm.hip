@@ -1,0 +1,360 @@
+// rmsnorm.hip -- root-mean-square norm with the residual's addition, out in
+// bf16 and in 8 bits, and its backward.
+//
+//   forward   s = x + r, rounded to the stream's type; rstd = 1 / sqrt(mean(s^2) + eps);
+//             y = (s * rstd) * gamma, to bf16 and to e4m3 codes with a scale for
+//             every 128 columns (the codes from y in fp32, not from bf16)
+//   backward  g = dy gamma, xh = s rstd, c = mean(g xh);
+//             ds = dr + rstd (g - xh c); dgamma = sum over rows of dy xh
+//
+// Bound by memory. A row belongs to one wave (d <= 1024), to a workgroup of four
+// (d <= 4096) or of sixteen, and is held in registers between its statistics and
+// its outputs, so each value is read once and written once; V = 8 or 16
+// values a lane in pieces of 16 bytes of the stream (8 bf16 or 4 fp32 values:
+// with 8 fp32 values a wave's store would cover every second 16 bytes). A wave's
+// pieces are consecutive, so 16 (32) neighbouring lanes own a block of 128
+// columns and find its maximum by DPP.
+//
+// Sums are in fp32 over the values of a lane, then, for the forward's squares, in
+// 64 bits over the lanes (a butterfly) and the waves (in order): rstd moves a whole
+// row, and with it which way its codes round (32768 x 1024, codes against 64 bits in
+// norm: with the butterfly in fp32 2.2 times as far off as with this). The backward's waves keep dgamma of their columns in
+// registers over the rows that they walk; a workgroup's sums are added in wave
+// order into one row of the workspace, and those rows by launch_colsum: no
+// atomics, the same bits every time.
+#include <algorithm>
+
+#include "fp8.hpp"
+#include "fp8_format.hpp"
+#include "moe_internal.hpp"
+
+namespace tmt {
+namespace {
+
+// N consecutive elements of a row from k0 on (16-byte aligned where a piece is
+// whole); TAIL: d is not a multiple of N, and elements from d on are zeros.
+template <int N, bool TAIL>
+__device__ __forceinline__ void load_piece(const float* row, int k0, int d, float* v) {
+    if (!TAIL || k0 + N <= d) {
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(row + k0 + q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[q + i] = a[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = k0 + i < d ? row[k0 + i] : 0.0f;
+    }
+}
+template <int N, bool TAIL>
+__device__ __forceinline__ void load_piece(const uint16_t* row, int k0, int d, float* v) {
+    if (!TAIL || k0 + N <= d) {
+        if constexpr (N == 8) {
+            unpack8(*reinterpret_cast<const uint4*>(row + k0), v);
+        } else {
+            const uint2 a = *reinterpret_cast<const uint2*>(row + k0);
+            v[0] = bf_lo(a.x), v[1] = bf_hi(a.x), v[2] = bf_lo(a.y), v[3] = bf_hi(a.y);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = k0 + i < d ? bf1(row[k0 + i]) : 0.0f;
+    }
+}
+template <int N, bool TAIL>
+__device__ __forceinline__ void store_piece(float* row, int k0, int d, const float* v) {
+    if (!TAIL || k0 + N <= d) {
+#pragma unroll
+        for (int q = 0; q < N; q += 4)
+            *reinterpret_cast<f32x4*>(row + k0 + q) = f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (k0 + i < d) row[k0 + i] = v[i];
+    }
+}
+template <int N, bool TAIL>
+__device__ __forceinline__ void store_piece(uint16_t* row, int k0, int d, const float* v) {
+    if (!TAIL || k0 + N <= d) {
+        if constexpr (N == 8) *reinterpret_cast<uint4*>(row + k0) = pack8(v);
+        else *reinterpret_cast<uint2*>(row + k0) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (k0 + i < d) row[k0 + i] = f2bf(v[i]);
+    }
+}
+
+template <bool F32>
+struct StreamType {
+    using T = uint16_t;
+};
+template <>
+struct StreamType<true> {
+    using T = float;
+};
+
+// The shape of a launch: WAVES per row, V values a lane, rows per workgroup.
+template <bool F32, int WAVES, int V>
+struct Shape {
+    static constexpr int N = F32 ? 4 : 8;             // values of a piece
+    static constexpr int C = V / N;                   // pieces a lane
+    static constexpr int THREADS = WAVES < 4 ? 256 : 64 * WAVES;
+    static constexpr int ROWS = THREADS / (64 * WAVES);
+    static constexpr int STRIDE = 64 * WAVES * N;     // columns between a lane's pieces
+};
+
+// gamma of a lane's columns; zeros past the last one.
+template <class S, bool TAIL, int C, int N>
+__device__ __forceinline__ void load_gamma(const float* gamma, int lane, int d, float (&g)[C][N]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int k0 = c * S::STRIDE + lane * N;
+        if (k0 < d) load_piece<N, TAIL>(gamma, k0, d, g[c]);
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[c][i] = 0.0f;
+    }
+}
+
+template <int OFF>
+__device__ __forceinline__ double add_xor_lane(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t o = ((uint64_t)xor_lane_u32<OFF>((uint32_t)(b >> 32)) << 32) | xor_lane_u32<OFF>((uint32_t)b);
+    return v + __builtin_bit_cast(double, o);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = add_xor_lane<32>(v);
+    v = add_xor_lane<16>(v);
+    v = add_xor_lane<8>(v);
+    v = add_xor_lane<4>(v);
+    v = add_xor_lane<2>(v);
+    return add_xor_lane<1>(v);
+}
+// Sum over the row's waves; `red` is the workgroup's, one of two in turn, so
+// that one barrier a row is enough.
+template <int WAVES, class F>
+__device__ __forceinline__ F row_sum(F v, F* red, int wave) {
+    v = wave_sum(v);
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) red[wave] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += red[w];
+    }
+    return v;
+}
+
+template <bool F32, bool TAIL, int WAVES, int V>
+__global__ __launch_bounds__((Shape<F32, WAVES, V>::THREADS)) void rms_fwd_kernel(RmsParams p, int rows_per_block) {
+    using S = Shape<F32, WAVES, V>;
+    using E = typename StreamType<F32>::T;
+    constexpr int N = S::N, C = S::C;
+    __shared__ double red[2][WAVES];
+    const int wave = threadIdx.x >> 6, d = p.d;
+    const int sub = wave / WAVES, lane = threadIdx.x - sub * (64 * WAVES);
+    const int first = blockIdx.x * rows_per_block, last = min(p.T, first + rows_per_block);
+    float g[C][N];
+    load_gamma<S, TAIL>(p.gamma, lane, d, g);
+    int turn = 0;
+    for (int r = first + sub; r < last; r += S::ROWS) {
+        float v[C][N];
+        float sq = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int k0 = c * S::STRIDE + lane * N;
+            if (k0 < d) {
+                float x[N];
+                if (p.R) load_piece<N, TAIL>(static_cast<const E*>(p.R) + (int64_t)r * p.ldr, k0, d, v[c]);
+                if (p.X) load_piece<N, TAIL>(p.X + (int64_t)r * p.ldx, k0, d, x);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    v[c][i] = p.R ? (p.X ? x[i] + v[c][i] : v[c][i]) : x[i];
+                    if constexpr (!F32) v[c][i] = bf1(f2bf(v[c][i]));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[c][i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) sq = __builtin_fmaf(v[c][i], v[c][i], sq);
+        }
+        const double sum = row_sum<WAVES>((double)sq, red[turn], wave);
+        turn ^= 1;
+        const float rstd = (float)(1.0 / sqrt(sum / d + p.eps));
+        if (p.rstd && lane == 0) p.rstd[r] = rstd;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int k0 = c * S::STRIDE + lane * N;
+            if (k0 < d) {
+                if (p.S) store_piece<N, TAIL>(static_cast<E*>(p.S) + (int64_t)r * p.lds, k0, d, v[c]);
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[c][i] = v[c][i] * rstd * g[c][i];
+                if (p.Y) store_piece<N, TAIL>(p.Y + (int64_t)r * p.ldy, k0, d, v[c]);
+            }
+            if (p.codes) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) m = max(m, abs_bits(v[c][i]));
+                m = max(m, xor_lane_u32<1>(m));
+                m = max(m, xor_lane_u32<2>(m));
+                m = max(m, xor_lane_u32<4>(m));
+                m = max(m, xor_lane_u32<8>(m));
+                if constexpr (N == 4) m = max(m, xor_lane_u32<16>(m));
+                const Fp8Scale q = fp8_scale(m);
+                if (lane % (kFp8Block / N) == 0 && k0 < d) p.scales[(int64_t)(k0 / kFp8Block) * p.ldsc + r] = q.scale;
+                if (k0 < ((d + 15) & ~15)) {  // up to the 16 bytes' end: zeros
+                    uint8_t* o = p.codes + (int64_t)r * p.ldc + k0;
+                    if constexpr (N == 8) *reinterpret_cast<uint2*>(o) = make_uint2(fp8_codes(v[c], q.inv), fp8_codes(v[c] + 4, q.inv));
+                    else *reinterpret_cast<uint32_t*>(o) = fp8_codes(v[c], q.inv);
+                }
+            }
+        }
+    }
+}
+
+template <bool F32, bool TAIL, int WAVES, int V>
+__global__ __launch_bounds__((Shape<F32, WAVES, V>::THREADS)) void rms_bwd_kernel(RmsParams p, int rows_per_block) {
+    using S = Shape<F32, WAVES, V>;
+    using E = typename StreamType<F32>::T;
+    constexpr int N = S::N, C = S::C;
+    __shared__ float red[2][WAVES];
+    const int wave = threadIdx.x >> 6, d = p.d;
+    const int sub = wave / WAVES, lane = threadIdx.x - sub * (64 * WAVES);
+    const int first = blockIdx.x * rows_per_block, last = min(p.T, first + rows_per_block);
+    const float over = 1.0f / (float)d;
+    float dg[C][N], g[C][N];
+    load_gamma<S, TAIL>(p.gamma, lane, d, g);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < N; ++i) dg[c][i] = 0.0f;
+    int turn = 0;
+    for (int r = first + sub; r < last; r += S::ROWS) {
+        float dy[C][N], xh[C][N];
+        float dot = 0.0f;
+        const float rstd = p.rstd[r];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int k0 = c * S::STRIDE + lane * N;
+            if (k0 < d) {
+                load_piece<N, TAIL>(p.dY + (int64_t)r * p.lddy, k0, d, dy[c]);
+                load_piece<N, TAIL>(static_cast<const E*>(p.S) + (int64_t)r * p.lds, k0, d, xh[c]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) dy[c][i] = xh[c][i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                xh[c][i] *= rstd;
+                dg[c][i] = __builtin_fmaf(dy[c][i], xh[c][i], dg[c][i]);
+                dy[c][i] *= g[c][i];
+                dot = __builtin_fmaf(dy[c][i], xh[c][i], dot);
+            }
+        }
+        const float mean = row_sum<WAVES>(dot, red[turn], wave) * over;
+        turn ^= 1;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int k0 = c * S::STRIDE + lane * N;
+            if (k0 < d) {
+                float o[N];
+                if (p.dR) load_piece<N, TAIL>(static_cast<const E*>(p.dR) + (int64_t)r * p.lddr, k0, d, o);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float t = rstd * __builtin_fmaf(-xh[c][i], mean, dy[c][i]);
+                    o[i] = p.dR ? o[i] + t : t;
+                }
+                store_piece<N, TAIL>(static_cast<E*>(p.dS) + (int64_t)r * p.ldds, k0, d, o);
+            }
+        }
+    }
+    // the workgroup's rows of sums, in wave order
+    const int w4 = ln_width4(d);
+    float* out = p.partial + (int64_t)blockIdx.x * w4;
+    if constexpr (S::ROWS == 1) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int k0 = c * S::STRIDE + lane * N;
+#pragma unroll
+            for (int q = 0; q < N; q += 4)
+                if (k0 + q < w4) *reinterpret_cast<f32x4*>(out + k0 + q) = f32x4{dg[c][q], dg[c][q + 1], dg[c][q + 2], dg[c][q + 3]};
+        }
+    } else {
+        __shared__ float sum[S::ROWS][V * 64];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int q = 0; q < N; q += 4)
+                *reinterpret_cast<f32x4*>(&sum[sub][c * S::STRIDE + lane * N + q]) = f32x4{dg[c][q], dg[c][q + 1], dg[c][q + 2], dg[c][q + 3]};
+        __syncthreads();
+        for (int k = threadIdx.x * 4; k < w4; k += S::THREADS * 4) {
+            f32x4 t = *reinterpret_cast<f32x4*>(&sum[0][k]);
+#pragma unroll
+            for (int w = 1; w < S::ROWS; ++w) t += *reinterpret_cast<f32x4*>(&sum[w][k]);
+            *reinterpret_cast<f32x4*>(out + k) = t;
+        }
+    }
+}
+
+// Waves per row for a width; V follows.
+int waves_of(int d) { return d <= 1024 ? 1 : d <= 4096 ? 4 : 16; }
+// Rows of a workgroup so that the chip runs the launch in about one round.
+int rows_per_block(int T, int d, int cus, int per_cu) {
+    const int rows = d <= 1024 ? 4 : 1;
+    const int64_t blocks = (int64_t)cus * per_cu;
+    const int64_t each = ((int64_t)T + blocks - 1) / blocks;
+    return (int)((each + rows - 1) / rows * rows);
+}
+constexpr int kFwdPerCu[3] = {8, 8, 2}, kBwdPerCu[3] = {4, 4, 1};
+int per_cu(const int* of, int d) { return of[waves_of(d) == 1 ? 0 : waves_of(d) == 4 ? 1 : 2]; }
+
+template <bool F32, bool TAIL, int WAVES, int V>
+void launch(bool fwd, const RmsParams& p, int grid, int rpb, hipStream_t s) {
+    constexpr int threads = Shape<F32, WAVES, V>::THREADS;
+    if (fwd) rms_fwd_kernel<F32, TAIL, WAVES, V><<<grid, threads, 0, s>>>(p, rpb);
+    else rms_bwd_kernel<F32, TAIL, WAVES, V><<<grid, threads, 0, s>>>(p, rpb);
+}
+template <bool F32, bool TAIL>
+void launch_width(bool fwd, const RmsParams& p, int grid, int rpb, hipStream_t s) {
+    const int d = p.d;
+    if (d <= 512) launch<F32, TAIL, 1, 8>(fwd, p, grid, rpb, s);
+    else if (d <= 1024) launch<F32, TAIL, 1, 16>(fwd, p, grid, rpb, s);
+    else if (d <= 2048) launch<F32, TAIL, 4, 8>(fwd, p, grid, rpb, s);
+    else if (d <= 4096) launch<F32, TAIL, 4, 16>(fwd, p, grid, rpb, s);
+    else if (d <= 8192) launch<F32, TAIL, 16, 8>(fwd, p, grid, rpb, s);
+    else launch<F32, TAIL, 16, 16>(fwd, p, grid, rpb, s);
+}
+void launch_rms(bool fwd, const RmsParams& p, int grid, int rpb, hipStream_t s) {
+    const bool tail = p.d % (p.f32 ? 4 : 8) != 0;
+    if (p.f32) tail ? launch_width<true, true>(fwd, p, grid, rpb, s) : launch_width<true, false>(fwd, p, grid, rpb, s);
+    else tail ? launch_width<false, true>(fwd, p, grid, rpb, s) : launch_width<false, false>(fwd, p, grid, rpb, s);
+}
+
+}  // namespace
+
+int rms_partials(int T, int d, int cus) {
+    const int rpb = rows_per_block(T, d, cus, per_cu(kBwdPerCu, d));
+    return rpb > 0 ? (T + rpb - 1) / rpb : 0;
+}
+
+int rms_partials_max(int d, int cus) { return cus * per_cu(kBwdPerCu, d); }
+
+hipError_t launch_rms_fwd(const RmsParams& p, hipStream_t s) {
+    const int rpb = rows_per_block(p.T, p.d, cu_count(), per_cu(kFwdPerCu, p.d));
+    launch_rms(true, p, (p.T + rpb - 1) / rpb, rpb, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_rms_bwd(const RmsParams& p, hipStream_t s) {
+    const int cus = cu_count(), rpb = rows_per_block(p.T, p.d, cus, per_cu(kBwdPerCu, p.d));
+    const int grid = rms_partials(p.T, p.d, cus), w4 = ln_width4(p.d);
+    if (grid > 0) launch_rms(false, p, grid, rpb, s);
+    return launch_colsum(p.partial, grid, w4, w4, p.d, p.dgamma, nullptr, s);
+}
+
+}  // namespace tmt

@@ -60,6 +60,12 @@ EXPORTED = (
     "tmt_moe_mxfp4_matmul",
     "tmt_moe_mxfp4_linear_dx",
     "tmt_moe_mxfp8_linear_dw",
+    "tmt_moe_rmsnorm_forward",
+    "tmt_moe_rmsnorm_workspace_size",
+    "tmt_moe_rmsnorm_backward",
+    "tmt_moe_fp8_quantize",
+    "tmt_moe_fp8_workspace_size",
+    "tmt_moe_fp8_matmul",
     "tmt_moe_set_profiling",
     "tmt_moe_read_profile",
     "tmt_moe_phase_name",
@@ -72,6 +78,8 @@ LINEAR_FORWARD = 0
 LINEAR_MATMUL = 1
 LINEAR_DX = 2
 LINEAR_DW = 3
+FP8_ROWS = 0
+FP8_TILES = 1
 
 NPHASES = 15
 
@@ -135,6 +143,14 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     for name in ("tmt_moe_mxfp4_linear", "tmt_moe_mxfp4_linear_dx", "tmt_moe_mxfp8_linear_dw"):
         getattr(lib, name).argtypes = [vp, i32, i32, i32, vp, i64, vp, vp, i64, vp, i64, f32, vp, size]
     lib.tmt_moe_mxfp4_matmul.argtypes = [vp, i32, i32, i32, vp, vp, i64, vp, vp, i64, vp, i64, f32, vp, size]
+    lib.tmt_moe_rmsnorm_forward.argtypes = [vp, i32, i32, i32, vp, i64, vp, i64, vp, f32, vp, i64, vp, i64, vp, i64, vp,
+                                            i64, vp]
+    lib.tmt_moe_rmsnorm_workspace_size.argtypes = [i32, i32, ctypes.POINTER(size)]
+    lib.tmt_moe_rmsnorm_backward.argtypes = [vp, i32, i32, i32, vp, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, size]
+    lib.tmt_moe_fp8_quantize.argtypes = [vp, i32, i32, vp, i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64]
+    lib.tmt_moe_fp8_workspace_size.argtypes = [i32, i32, i32, i32, ctypes.POINTER(size)]
+    lib.tmt_moe_fp8_matmul.argtypes = [vp, i32, i32, i32, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, f32, vp,
+                                       size]
     lib.tmt_moe_read_stats.argtypes = [vp, vp, vp, vp, vp]
     lib.tmt_moe_stats_device_ptr.argtypes = [vp, pp]
     lib.tmt_moe_read_routing.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp]
@@ -408,6 +424,177 @@ def mxfp4_matmul(X_codes, X_scales, codes, scales, Y, beta: float = 0.0, workspa
     y, ldy = _matrix("Y", Y, torch.bfloat16, dev, T, N)
     ws, size = _ws(workspace, dev)
     rc = load_library().tmt_moe_mxfp4_matmul(raw, T, N, K, xc, xs, xlds, c, s, lds, y, ldy, beta, ws, size)
+    if rc:
+        _check(rc)
+
+
+def _rows(what: str, t, dtype, dev: int, rows: int, cols: int, unit: int) -> tuple:
+    """(pointer, row stride) of a matrix whose rows take whole units of `unit`
+    elements (16 bytes); a single row's stride does not matter."""
+    if t.dtype is dtype and t.shape == (rows, cols) and t.get_device() == dev:
+        ld, one = t.stride()
+        if one == 1 or cols <= 1:
+            return t.data_ptr(), cols if rows == 1 and cols % unit == 0 else ld
+    return _matrix(what, t, dtype, dev, rows, cols)  # says what is wrong
+
+
+def _fp8_codes(what: str, t, dev: int, rows: int, cols: int) -> tuple:
+    """The same of e4m3 codes (uint8 or float8_e4m3fn), whose rows end at a multiple of 16 bytes."""
+    import torch
+    dtype = t.dtype
+    if dtype is not torch.float8_e4m3fn and dtype is not torch.uint8:
+        raise ValueError(f"{what} must be uint8 or float8_e4m3fn, not {dtype}")
+    ptr, ld = _rows(what, t, dtype, dev, rows, cols, 16)
+    if cols % 16 and rows and t.storage_offset() + (rows - 1) * ld + (cols + 15) // 16 * 16 > t.untyped_storage().nbytes():
+        raise ValueError(f"the last row of {what} must extend to a multiple of 16 bytes")
+    return ptr, ld
+
+
+def _fp8_scales(what: str, t, dev: int, blocks: int, cols: int) -> tuple:
+    """(pointer, stride) of scales [blocks, cols or more]."""
+    import torch
+    n = t.shape[-1]
+    if n < cols:
+        raise ValueError(f"{what} must be [{blocks}, {cols} or more], not {list(t.shape)}")
+    return _rows(what, t, torch.float32, dev, blocks, n, 1)
+
+
+def _vector(what: str, t, dev: int, n: int) -> int:
+    import torch
+    if t.dtype is torch.float32 and t.shape == (n,) and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    if t.get_device() != dev:
+        raise ValueError(f"{what} is on {t.device}, not on the current GPU")
+    raise ValueError(f"{what} must be [{n}] contiguous float32, not {list(t.shape)} of {t.dtype}")
+
+
+def _blocks_of(n: int) -> int:
+    return (n + 127) // 128
+
+
+def _stream_dtype(t) -> tuple:
+    """(the library's constant, elements of 16 bytes) of a residual stream's type."""
+    import torch
+    if t.dtype is torch.bfloat16:
+        return 0, 8
+    if t.dtype is torch.float32:
+        return 1, 4
+    raise ValueError(f"the stream must be bfloat16 or float32, not {t.dtype}")
+
+
+def rmsnorm_forward(X, R, gamma, S=None, Y=None, codes=None, scales=None, rstd=None, eps: float = 1e-5,
+                    stream=None) -> None:
+    """S = X + R (X [T, d] bf16; R, S bf16 or fp32; either of X and R may be
+    None), rstd [T] = 1/sqrt(mean(S^2) + eps), y = S * rstd * gamma, out as
+    Y (bf16) and as codes [T, d] (e4m3) with scales [d/128, T or more]."""
+    import torch
+    if X is None and R is None:
+        raise ValueError("X and R are both None")
+    if codes is not None and scales is None:
+        raise ValueError("codes need scales")
+    T, d = (X if R is None else R).shape
+    if (T | d) >> 31:
+        _past_int32(T, d)
+    dev, raw = _here(stream)
+    dtype, piece = _stream_dtype(X if R is None else R)
+    stream_type = torch.float32 if dtype else torch.bfloat16
+    none = (0, 0)
+    x, ldx = none if X is None else _rows("X", X, torch.bfloat16, dev, T, d, 8)
+    r, ldr = none if R is None else _rows("R", R, stream_type, dev, T, d, piece)
+    s, lds = none if S is None else _rows("S", S, stream_type, dev, T, d, piece)
+    y, ldy = none if Y is None else _rows("Y", Y, torch.bfloat16, dev, T, d, 8)
+    c, ldc = none if codes is None else _fp8_codes("codes", codes, dev, T, d)
+    q, ldq = none if codes is None else _fp8_scales("scales", scales, dev, _blocks_of(d), T)
+    rc = load_library().tmt_moe_rmsnorm_forward(
+        raw, T, d, dtype, x, ldx, r, ldr, _vector("gamma", gamma, dev, d), eps, s, lds, y, ldy, c, ldc, q, ldq,
+        0 if rstd is None else _vector("rstd", rstd, dev, T))
+    if rc:
+        _check(rc)
+
+
+def rmsnorm_workspace_size(T: int, d: int) -> int:
+    """Bytes of device workspace that rmsnorm_backward needs for up to T rows."""
+    if any(n >> 31 not in (0, -1) for n in (T, d)):
+        _past_int32(T, d)
+    out = ctypes.c_size_t(0)
+    _check(load_library().tmt_moe_rmsnorm_workspace_size(T, d, ctypes.byref(out)))
+    return int(out.value)
+
+
+def rmsnorm_backward(dY, S, gamma, rstd, dS, dgamma, workspace, dR=None, stream=None) -> None:
+    """dS = dR + the gradient at S of the norm, dgamma [d], from dY [T, d] bf16;
+    S and rstd as rmsnorm_forward wrote them; S, dR (or None) and dS of the
+    stream's type. dS may be dR itself."""
+    import torch
+    T, d = S.shape
+    if (T | d) >> 31:
+        _past_int32(T, d)
+    dev, raw = _here(stream)
+    dtype, piece = _stream_dtype(S)
+    dy, lddy = _rows("dY", dY, torch.bfloat16, dev, T, d, 8)
+    s, lds = _rows("S", S, S.dtype, dev, T, d, piece)
+    r, lddr = (0, 0) if dR is None else _rows("dR", dR, S.dtype, dev, T, d, piece)
+    ds, ldds = _rows("dS", dS, S.dtype, dev, T, d, piece)
+    ws, size = _ws(workspace, dev)
+    rc = load_library().tmt_moe_rmsnorm_backward(
+        raw, T, d, dtype, dy, lddy, s, lds, _vector("gamma", gamma, dev, d), _vector("rstd", rstd, dev, T), r, lddr, ds,
+        ldds, _vector("dgamma", dgamma, dev, d), ws, size)
+    if rc:
+        _check(rc)
+
+
+def fp8_quantize(X, codes=None, scales=None, codes_t=None, scales_t=None, blocks: int = FP8_ROWS, stream=None) -> None:
+    """X [rows, K] (bf16 or fp32) to e4m3 codes [rows, K] and scales, and X^T to
+    codes_t [K, rows] and scales_t, in one pass; either side may be None. Scales:
+    FP8_ROWS [K/128, rows or more] ([rows/128, K or more] transposed), FP8_TILES
+    [rows/128, K/128 or more] ([K/128, rows/128 or more])."""
+    rows, K = X.shape
+    if (rows | K) >> 31:
+        _past_int32(rows, K)
+    if (codes is None) != (scales is None) or (codes_t is None) != (scales_t is None):
+        raise ValueError("codes and their scales go together")
+    dev, raw = _here(stream)
+    dtype, piece = _stream_dtype(X)
+    x, ldx = _rows("X", X, X.dtype, dev, rows, K, piece)
+    rb, kb, tiles = _blocks_of(rows), _blocks_of(K), blocks == FP8_TILES
+    none = (0, 0)
+    c, ldc = none if codes is None else _fp8_codes("codes", codes, dev, rows, K)
+    s, lds = none if codes is None else _fp8_scales("scales", scales, dev, rb if tiles else kb, kb if tiles else rows)
+    ct, ldct = none if codes_t is None else _fp8_codes("codes_t", codes_t, dev, K, rows)
+    st, ldst = none if codes_t is None else _fp8_scales("scales_t", scales_t, dev, kb if tiles else rb, rb if tiles else K)
+    rc = load_library().tmt_moe_fp8_quantize(raw, blocks, dtype, x, ldx, rows, K, c, ldc, s, lds, ct, ldct, st, ldst)
+    if rc:
+        _check(rc)
+
+
+def fp8_workspace_size(M: int, N: int, K: int, blocks: int = FP8_TILES) -> int:
+    """Bytes of device workspace that fp8_matmul needs for up to M rows."""
+    if any(n >> 31 not in (0, -1) for n in (M, N, K, blocks)):
+        _past_int32(M, N, K, blocks)
+    out = ctypes.c_size_t(0)
+    _check(load_library().tmt_moe_fp8_workspace_size(blocks, M, N, K, ctypes.byref(out)))
+    return int(out.value)
+
+
+def fp8_matmul(A, A_scales, B, B_scales, Y, beta: float = 0.0, blocks: int = FP8_TILES, workspace=None,
+               stream=None) -> None:
+    """Y <- beta*Y + A B^T. A [M, K] e4m3 codes in rows (scales [K/128, M or
+    more]), B [N, K] in `blocks` (FP8_TILES: scales [N/128, K/128 or more],
+    FP8_ROWS: [K/128, N or more]), Y [M, N] bf16 or fp32."""
+    (M, K), N = A.shape, B.shape[0]
+    if (M | N | K) >> 31:
+        _past_int32(M, N, K)
+    dev, raw = _here(stream)
+    dtype, piece = _stream_dtype(Y)
+    kb, tiles = _blocks_of(K), blocks == FP8_TILES
+    a, lda = _fp8_codes("A", A, dev, M, K)
+    sa, ldas = _fp8_scales("A_scales", A_scales, dev, kb, M)
+    b, ldb = _fp8_codes("B", B, dev, N, K)
+    sb, ldbs = _fp8_scales("B_scales", B_scales, dev, _blocks_of(N) if tiles else kb, kb if tiles else N)
+    y, ldy = _rows("Y", Y, Y.dtype, dev, M, N, piece)
+    ws, size = _ws(workspace, dev)
+    rc = load_library().tmt_moe_fp8_matmul(raw, blocks, dtype, M, N, K, a, lda, sa, ldas, b, ldb, sb, ldbs, y, ldy, beta,
+                                           ws, size)
     if rc:
         _check(rc)
 
