@@ -23,8 +23,8 @@
 // lane's values belong to one row m, whose scale it holds, and to neighbouring
 // columns n. The instruction's order of the reduction does not matter as long as
 // both operands are laid out alike.
-#include "fp8.hpp"
 #include "fp8_format.hpp"
+#include "fp8_plan.hpp"
 #include "moe_internal.hpp"
 #include "tile_stream.hpp"
 
@@ -142,19 +142,200 @@ __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8Params p) {
     }
 }
 
+// ---- tiles -------------------------------------------------------------------------
+// The 32 x 32 sums of a block of 128 from LDS rows of 128 bytes, whose chunks of 16
+// are XOR-swizzled by row / 2: lane l holds 64 codes of row l % 32, chunks 2 h, 2 h
+// + 1, 4 + 2 h and 5 + 2 h with h = l / 32.
+struct Codes {
+    i32x8 q[2];
+};
+__device__ __forceinline__ Codes read_codes(const uint8_t* t, int r, int h) {
+    auto at = [&](int c) { return *reinterpret_cast<const uint4*>(t + r * 128 + ((c ^ ((r >> 1) & 7)) * 16)); };
+    return {{join(at(2 * h), at(2 * h + 1)), join(at(4 + 2 * h), at(5 + 2 * h))}};
+}
+__device__ __forceinline__ f32x16 zero16() {
+    return f32x16{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+}
+struct Wide {
+    bf16x8 v[8];
+};
+__device__ __forceinline__ Wide widen(const Codes& c) {
+    Wide w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.v[i] = widen(c.q[i >> 2][2 * (i & 3)], c.q[i >> 2][2 * (i & 3) + 1]);
+    return w;
+}
+__device__ __forceinline__ f32x16 mma32(const Codes& b, const Codes& a) {
+    const f32x16 d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b.q[0], a.q[0], zero16(), 0, 0, 0, 0, 0, 0);
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b.q[1], a.q[1], d, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(const Wide& b, const Wide& a) {
+    f32x16 d = zero16();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b.v[i], a.v[i], d, 0, 0, 0);
+    return d;
+}
+
+// A step's place in LDS: codes of a and b, the scales of a's rows and of b's (tiles:
+// one for each 128 columns, 256 bytes apart).
+template <int TILE>
+struct Slot {
+    static constexpr int CODES = TILE * 128, LOADS = CODES / 4096;  // per operand; 1 KiB loads per wave
+    static constexpr int SA = 2 * CODES, SB = SA + TILE * 4, BYTES = SB + TILE * 4;
+    static constexpr int ND = 2 * LOADS + 2;                        // loads per wave and step
+};
+
+// The loads of a tiled kernel's wave: load(d) issues load d of the next step.
+template <int TILE, bool TILES, bool SPLIT>
+struct Loader {
+    using S = Slot<TILE>;
+    Fp8Cursor<TILE, TILES, SPLIT> at;
+    uint32_t a_off[S::LOADS], b_off[S::LOADS], sc_off;
+    int wave, chunk, lim = 0;
+    __device__ void init(const Fp8Params& p, int wave_, int lane, int nb) {
+        wave = wave_;
+        at.nb = nb;
+        chunk = (lane & 7) ^ (lane >> 4);  // of even loads; odd ones': ^ 4
+#pragma unroll
+        for (int i = 0; i < S::LOADS; ++i) {
+            const int r = 8 * (wave * S::LOADS + i) + (lane >> 3), c = chunk ^ (4 * (i & 1));
+            a_off[i] = (uint32_t)r * (uint32_t)p.lda + c * 16;
+            b_off[i] = (uint32_t)r * (uint32_t)p.ldb + c * 16;
+        }
+        sc_off = 4 * (uint32_t)(64 * (TILE == 256 ? wave : wave & 1) + lane);
+    }
+    __device__ void load(const Fp8Params& p, int d, uint32_t slot) {
+        constexpr uint32_t FAR = 0x80000000u;  // past any window
+        if (d == 0) lim = at.chunks(p);
+        if (d < 2 * S::LOADS) {
+            const int i = d >> 1;
+            const bool in = (chunk ^ (4 * (i & 1))) < lim;
+            if (d & 1) dma16(at.wb, in ? b_off[i] : FAR, slot + S::CODES + (wave * S::LOADS + i) * 1024);
+            else dma16(at.wa, in ? a_off[i] : FAR, slot + (wave * S::LOADS + i) * 1024);
+        } else if (d == 2 * S::LOADS) {
+            dma4(at.wsa, sc_off, slot + S::SA + 256 * (TILE == 256 ? wave : wave & 1));
+        } else if constexpr (TILES) {
+            dma4(at.wsb, sc_off & 255, slot + S::SB + 256 * at.nb);
+        } else {
+            dma4(at.wsb, sc_off, slot + S::SB + 256 * (TILE == 256 ? wave : wave & 1));
+        }
+    }
+};
+
+// 128 x 128 outputs of 4 waves, a wave 64 x 64; ring of 2, two workgroups per CU. A
+// unit's first step is loaded before the previous unit's epilogue, which stages
+// through the other slot.
+template <bool TILES, bool F32, bool SPLIT, bool BETA>
+__global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPlan pl) {
+    constexpr int TILE = 128, WT = 64, MI = 2;
+    using S = Slot<TILE>;
+    using Operand = std::conditional_t<F32, Wide, Codes>;
+    static_assert(4 * Stage<F32, MI>::BYTES <= S::BYTES, "the epilogue stages in a slot");
+    __shared__ uint4 lds_raw[2 * S::BYTES / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const uint32_t lds0 = lds_u32(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT, row = lane & 31, h = lane >> 5;
+    Unit u;
+    int vb = blockIdx.x;
+    if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) return;
+    Loader<TILE, TILES, SPLIT> ld;
+    ld.init(p, wave, lane, 0);
+    ld.at.vl = vb;
+    ld.at.set(p, u);
+    int sl = 0, slot = 0;
+    auto load_step = [&]() {
+#pragma unroll
+        for (int d = 0; d < S::ND; ++d) ld.load(p, d, lds0 + sl * S::BYTES);
+        sl ^= 1;
+        ld.at.next(p, pl, workgroups);
+    };
+    auto operand = [&](const uint8_t* t, int r) {
+        if constexpr (F32) return widen(read_codes(t, r, h));
+        else return read_codes(t, r, h);
+    };
+    f32x16 acc[MI][MI];
+    clear(acc);
+    load_step();
+    for (;;) {
+        for (int k = u.kbeg; k < u.kend; k += kFp8Block) {
+            wait_vm<0>();
+            lds_barrier();  // step k is whole in LDS, and the other slot is read
+            load_step();    // past the last unit: zeros
+            const uint8_t* t = lds + slot * S::BYTES;
+            const float* sa = reinterpret_cast<const float*>(t + S::SA);
+            const float* sb = reinterpret_cast<const float*>(t + S::SB);
+            Operand a[MI];
+            float s[MI];
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                a[i] = operand(t, wrow + 32 * i + row);
+                s[i] = sa[wrow + 32 * i + row];
+                if constexpr (TILES) s[i] *= sb[0];
+            }
+#pragma unroll
+            for (int j = 0; j < MI; ++j) {
+                const Operand b = operand(t + S::CODES, wcol + 32 * j + row);
+                f32x4 sn[4];
+                if constexpr (!TILES)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) sn[q] = *reinterpret_cast<const f32x4*>(sb + wcol + 32 * j + 8 * q + 4 * h);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const f32x16 d = mma32(b, a[i]);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        acc[i][j][r] = __builtin_fmaf(d[r], TILES ? s[i] : s[i] * sn[r >> 2][r & 3], acc[i][j][r]);
+                }
+            }
+            slot ^= 1;
+        }
+        lds_barrier();  // the last step's slot is read: the epilogue stages there
+        finish_unit<TILE, F32, MI, SPLIT, BETA, false>(acc, lds + (slot ^ 1) * S::BYTES + wave * Stage<F32, MI>::BYTES, p, u, p.M, p.N,
+                                                wrow, wcol);
+        vb += gridDim.x;
+        if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) break;
+        clear(acc);
+    }
+    wait_vm<0>();  // no load may land in LDS that the next workgroup owns
+}
+
 template <bool TILES, bool F32>
 void launch_rows(const Fp8Params& p, hipStream_t s) {
     const int64_t grid = (int64_t)((p.N + 31) / 32) * ((p.M + 31) / 32);
     fp8_rows_kernel<TILES, F32, 2, 2, 4><<<(unsigned)grid, 256, 0, s>>>(p);
 }
 
+template <bool TILES, bool F32>
+void launch_tiles(const Fp8Params& p, const LinearPlan& pl, int cus, hipStream_t s) {
+    const auto grid = [&](int units) { return unit_grid(128, units, cus); };
+    if (pl.whole > 0) {
+        if (p.beta == 0.0f) fp8_tile_kernel<TILES, F32, false, false><<<grid(pl.whole), 256, 0, s>>>(p, pl);
+        else fp8_tile_kernel<TILES, F32, false, true><<<grid(pl.whole), 256, 0, s>>>(p, pl);
+    }
+    if (pl.tail > 0) {
+        fp8_tile_kernel<TILES, F32, true, false><<<grid(pl.tail * pl.parts), 256, 0, s>>>(p, pl);  // the sums add what is there
+        constexpr int SLABS = 128 / (256 / (128 / 4));
+        linear_fixup_kernel<128, F32><<<pl.tail * SLABS, 256, 0, s>>>(p, pl, p.M, p.N);
+    }
+}
+
+template <bool TILES, bool F32>
+void launch(const Fp8Params& p, hipStream_t s) {
+    const int cus = cu_count();
+    const Fp8Plan pl = fp8_plan(F32, p.M, p.N, p.K, cus);
+    if (pl.rows) launch_rows<TILES, F32>(p, s);
+    else launch_tiles<TILES, F32>(p, pl.tiles, cus, s);
+}
+
 }  // namespace
 
-size_t fp8_workspace(bool tiles, int M, int N, int K) { return 0; }
+size_t fp8_workspace(bool tiles, int M, int N, int K) { return fp8_workspace_bound(M, N, K, cu_count()); }
 
 hipError_t launch_fp8_matmul(bool tiles, bool f32, const Fp8Params& p, hipStream_t s) {
-    if (tiles) f32 ? launch_rows<true, true>(p, s) : launch_rows<true, false>(p, s);
-    else f32 ? launch_rows<false, true>(p, s) : launch_rows<false, false>(p, s);
+    if (tiles) f32 ? launch<true, true>(p, s) : launch<true, false>(p, s);
+    else f32 ? launch<false, true>(p, s) : launch<false, false>(p, s);
     return hipGetLastError();
 }
 

@@ -916,43 +916,6 @@ __global__ __launch_bounds__(64 * NW) void linear_rows_kernel(LinearParams p) {
     }
 }
 
-// ---- the last round's sums ------------------------------------------------------
-// Tail tile j is the sum of its partial tiles in part order, plus beta times
-// what is there, rounded once. A thread takes 4 columns of a row.
-template <int TILE, bool F32>
-__global__ __launch_bounds__(256) void linear_fixup_kernel(LinearParams p, LinearPlan pl, int M, int C) {
-    constexpr int TPR = TILE / 4, RPW = 256 / TPR, SLABS = TILE / RPW;
-    const int j = blockIdx.x / SLABS, slab = blockIdx.x % SLABS;
-    int mt, ct;
-    tile_at(pl, pl.whole + j, mt, ct);
-    const int r = slab * RPW + threadIdx.x / TPR, c = (threadIdx.x % TPR) * 4;
-    const int m = mt * TILE + r, col = ct * TILE + c;
-    if (m >= M || col >= C) return;
-    const float* src = p.part + (int64_t)j * pl.parts * TILE * TILE + r * TILE + c;
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int q0 = 0; q0 < pl.parts; q0 += 8) {  // up to 8 loads in flight
-        f32x4 v[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const f32x4*>(src + (int64_t)min(q0 + q, pl.parts - 1) * TILE * TILE);
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-            if (q0 + q < pl.parts) sum = sum + v[q];
-    }
-    const int64_t at = (int64_t)m * p.ldy + col;
-    if constexpr (F32) {
-        f32x4* y = reinterpret_cast<f32x4*>(static_cast<float*>(p.y) + at);
-        if (p.beta != 0.0f) sum = sum + p.beta * *y;
-        *y = sum;
-    } else {
-        uint2* y = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at);
-        if (p.beta != 0.0f) {
-            const uint2 old = *y;
-            sum = sum + p.beta * f32x4{bf_lo(old.x), bf_hi(old.x), bf_lo(old.y), bf_hi(old.y)};
-        }
-        *y = make_uint2(pack_bf2(sum[0], sum[1]), pack_bf2(sum[2], sum[3]));
-    }
-}
-
 // dW = beta dW: the weight gradient over no tokens. Four values a thread; the
 // workgroups stride over the matrix.
 __global__ __launch_bounds__(256) void linear_scale_kernel(float* y, int64_t ldy, int rows, int cols, float beta) {

@@ -78,7 +78,8 @@ __device__ __forceinline__ void wave_lds_order() {
 // slice is converted while the one
 // before comes back from LDS, and its own way through LDS needs no wait: a wave's
 // LDS accesses run in order.
-template <bool F32, int JS, bool NT, bool BETA, int MI, int NJ>
+// AGPR: the sums are the matrix instructions' own, else the vector unit's.
+template <bool F32, int JS, bool NT, bool BETA, bool AGPR, int MI, int NJ>
 __device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, void* out, int64_t ld, int rows,
                                            int cols, float beta) {
     using S = Stage<F32, JS>;
@@ -135,11 +136,13 @@ __device__ __forceinline__ void store_wave(f32x16 (&acc)[MI][NJ], uint8_t* st, v
         if constexpr (!F32 && BETA)
             if (n + 1 < SLICES) load_old(n + 1);
         // the outputs not yet staged stay in the accumulator registers
+        if constexpr (AGPR) {
 #pragma unroll
-        for (int i2 = i; i2 < MI; ++i2)
+            for (int i2 = i; i2 < MI; ++i2)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-                if (i2 > i || j >= jg) asm volatile("" : "+a"(acc[i2][j]));
+                for (int j = 0; j < NJ; ++j)
+                    if (i2 > i || j >= jg) asm volatile("" : "+a"(acc[i2][j]));
+        }
         uint2 half[JS][4];
         if constexpr (!F32) {
 #pragma unroll
@@ -188,7 +191,7 @@ constexpr auto workgroups = [] __device__() { return (int)gridDim.x; };
 // Writes a unit's wave outputs: to the result (p.y, p.ldy, p.beta) or, SPLIT, as a partial tile
 // (fp32; bf16 results' partial tiles leave from the registers, whose LDS holds
 // no fp32 rows).
-template <int TILE, bool F32, int JS, bool SPLIT, bool BETA, class Params>
+template <int TILE, bool F32, int JS, bool SPLIT, bool BETA, bool AGPR = true, class Params>
 __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64], uint8_t* st, const Params& p,
                                             const Unit& u, int M, int C, int wrow, int wcol) {
     constexpr int WT = TILE / 2;
@@ -197,7 +200,7 @@ __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64],
     if constexpr (SPLIT) {
         float* o = p.part + (int64_t)u.part * TILE * TILE + wrow * TILE + wcol;
         if constexpr (F32) {
-            store_wave<true, JS, false, false>(acc, st, o, TILE, rows, cols, 0.0f);
+            store_wave<true, JS, false, false, AGPR>(acc, st, o, TILE, rows, cols, 0.0f);
         } else {
             const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -217,7 +220,44 @@ __device__ __forceinline__ void finish_unit(f32x16 (&acc)[TILE / 64][TILE / 64],
     } else {
         using Out = std::conditional_t<F32, float, uint16_t>;
         Out* o = static_cast<Out*>(p.y) + (int64_t)(u.m0 + wrow) * p.ldy + u.c0 + wcol;
-        store_wave<F32, JS, true, BETA>(acc, st, o, p.ldy, rows, cols, p.beta);
+        store_wave<F32, JS, true, BETA, AGPR>(acc, st, o, p.ldy, rows, cols, p.beta);
+    }
+}
+
+// ---- the last round's sums ------------------------------------------------------
+// Tail tile j is the sum of its partial tiles in part order, plus beta times
+// what is there, rounded once. A thread takes 4 columns of a row.
+template <int TILE, bool F32, class Params>
+__global__ __launch_bounds__(256) void linear_fixup_kernel(Params p, LinearPlan pl, int M, int C) {
+    constexpr int TPR = TILE / 4, RPW = 256 / TPR, SLABS = TILE / RPW;
+    const int j = blockIdx.x / SLABS, slab = blockIdx.x % SLABS;
+    int mt, ct;
+    tile_at(pl, pl.whole + j, mt, ct);
+    const int r = slab * RPW + threadIdx.x / TPR, c = (threadIdx.x % TPR) * 4;
+    const int m = mt * TILE + r, col = ct * TILE + c;
+    if (m >= M || col >= C) return;
+    const float* src = p.part + (int64_t)j * pl.parts * TILE * TILE + r * TILE + c;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q0 = 0; q0 < pl.parts; q0 += 8) {  // up to 8 loads in flight
+        f32x4 v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const f32x4*>(src + (int64_t)min(q0 + q, pl.parts - 1) * TILE * TILE);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q0 + q < pl.parts) sum = sum + v[q];
+    }
+    const int64_t at = (int64_t)m * p.ldy + col;
+    if constexpr (F32) {
+        f32x4* y = reinterpret_cast<f32x4*>(static_cast<float*>(p.y) + at);
+        if (p.beta != 0.0f) sum = sum + p.beta * *y;
+        *y = sum;
+    } else {
+        uint2* y = reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + at);
+        if (p.beta != 0.0f) {
+            const uint2 old = *y;
+            sum = sum + p.beta * f32x4{bf_lo(old.x), bf_hi(old.x), bf_lo(old.y), bf_hi(old.y)};
+        }
+        *y = make_uint2(pack_bf2(sum[0], sum[1]), pack_bf2(sum[2], sum[3]));
     }
 }
 
