@@ -178,17 +178,18 @@ __device__ __forceinline__ f32x16 mma32(const Wide& b, const Wide& a) {
 
 // A step's place in LDS: codes of a and b, the scales of a's rows and of b's (tiles:
 // one for each 128 columns, 256 bytes apart).
-template <int TILE>
+template <int TILE, int WAVES>
 struct Slot {
-    static constexpr int CODES = TILE * 128, LOADS = CODES / 4096;  // per operand; 1 KiB loads per wave
+    static constexpr int CODES = TILE * 128, LOADS = CODES / (1024 * WAVES);  // per operand; 1 KiB loads per wave
     static constexpr int SA = 2 * CODES, SB = SA + TILE * 4, BYTES = SB + TILE * 4;
     static constexpr int ND = 2 * LOADS + 2;                        // loads per wave and step
 };
 
 // The loads of a tiled kernel's wave: load(d) issues load d of the next step.
-template <int TILE, bool TILES, bool SPLIT>
+template <int TILE, int WAVES, bool TILES, bool SPLIT>
 struct Loader {
-    using S = Slot<TILE>;
+    using S = Slot<TILE, WAVES>;
+    static_assert(S::LOADS % 2 == 0, "a lane's chunk goes by the load's parity");
     Fp8Cursor<TILE, TILES, SPLIT> at;
     uint32_t a_off[S::LOADS], b_off[S::LOADS], sc_off;
     int wave, chunk, lim = 0;
@@ -202,7 +203,7 @@ struct Loader {
             a_off[i] = (uint32_t)r * (uint32_t)p.lda + c * 16;
             b_off[i] = (uint32_t)r * (uint32_t)p.ldb + c * 16;
         }
-        sc_off = 4 * (uint32_t)(64 * (TILE == 256 ? wave : wave & 1) + lane);
+        sc_off = 4 * (uint32_t)(64 * (wave & (TILE / 64 - 1)) + lane);
     }
     __device__ void load(const Fp8Params& p, int d, uint32_t slot) {
         constexpr uint32_t FAR = 0x80000000u;  // past any window
@@ -213,11 +214,11 @@ struct Loader {
             if (d & 1) dma16(at.wb, in ? b_off[i] : FAR, slot + S::CODES + (wave * S::LOADS + i) * 1024);
             else dma16(at.wa, in ? a_off[i] : FAR, slot + (wave * S::LOADS + i) * 1024);
         } else if (d == 2 * S::LOADS) {
-            dma4(at.wsa, sc_off, slot + S::SA + 256 * (TILE == 256 ? wave : wave & 1));
+            dma4(at.wsa, sc_off, slot + S::SA + 256 * (wave & (TILE / 64 - 1)));
         } else if constexpr (TILES) {
             dma4(at.wsb, sc_off & 255, slot + S::SB + 256 * at.nb);
         } else {
-            dma4(at.wsb, sc_off, slot + S::SB + 256 * (TILE == 256 ? wave : wave & 1));
+            dma4(at.wsb, sc_off, slot + S::SB + 256 * (wave & (TILE / 64 - 1)));
         }
     }
 };
@@ -228,7 +229,7 @@ struct Loader {
 template <bool TILES, bool F32, bool SPLIT, bool BETA>
 __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPlan pl) {
     constexpr int TILE = 128, WT = 64, MI = 2;
-    using S = Slot<TILE>;
+    using S = Slot<TILE, 4>;
     using Operand = std::conditional_t<F32, Wide, Codes>;
     static_assert(4 * Stage<F32, MI>::BYTES <= S::BYTES, "the epilogue stages in a slot");
     __shared__ uint4 lds_raw[2 * S::BYTES / 16];
@@ -240,7 +241,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPla
     Unit u;
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) return;
-    Loader<TILE, TILES, SPLIT> ld;
+    Loader<TILE, 4, TILES, SPLIT> ld;
     ld.init(p, wave, lane, 0);
     ld.at.vl = vb;
     ld.at.set(p, u);
@@ -301,6 +302,212 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPla
     wait_vm<0>();  // no load may land in LDS that the next workgroup owns
 }
 
+// ---- large products ------------------------------------------------------------------
+// acc[i][j][e] = C[m][c] with m = 16 i + lane % 16 and c = 16 j + 4 (lane / 16) + e
+// in the wave's outputs. 16 rows at a time go through the wave's own LDS, so that
+// a row's 64 columns leave as one run of 16-byte stores; no barrier. `out` is the
+// wave's first output; rows and columns past the last ones are dropped by the
+// hardware's bounds.
+template <bool BETA, int MI>
+__device__ __forceinline__ void store_wave16(f32x4 (&acc)[MI][4], uint8_t* st, uint16_t* out, int64_t ld, int rows, int cols,
+                                             float beta) {
+    constexpr uint32_t FAR = 0x80000000u;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // the addresses below are not kept through the main loop
+    const int lr = lane & 15, g = lane >> 4, cl = lane & 7;
+    const uint32_t row = (uint32_t)(ld * 2);
+    rows = min(rows, 16 * MI);
+    cols = min(cols, 64);
+    const __amdgpu_buffer_rsrc_t win = __builtin_amdgcn_make_buffer_rsrc(out, 0, (int)output_window(rows, row, cols, 2), 0x00020000);
+    u32x2 old[2][4];
+    auto load_old = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = 16 * j + 4 * g;
+            old[i & 1][j] = __builtin_amdgcn_raw_buffer_load_b64(win, c < cols ? (int)((uint32_t)(16 * i + lr) * row + 2 * c) : (int)FAR, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (BETA) load_old(0);
+    uint4 v[2];
+    auto store = [&](int i) {
+        uint32_t at = 8 * cl < cols ? (uint32_t)(16 * i + (lane >> 3)) * row + 16 * cl : FAR;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), win, (int)at, 0, 2);
+            at += 8 * row;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        if constexpr (BETA)
+            if (i + 1 < MI) load_old(i + 1);
+        uint2 half[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f32x4 f = acc[i][j];
+            if constexpr (BETA) {
+                const u32x2 o = old[i & 1][j];
+                f = f + beta * f32x4{bf_lo(o[0]), bf_hi(o[0]), bf_lo(o[1]), bf_hi(o[1])};
+            }
+            half[j] = make_uint2(pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (i > 0) store(i - 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint2*>(st + lr * 128 + (((2 * j + (g >> 1)) ^ (lr & 7)) * 16) + (g & 1) * 8) = half[j];
+        wave_lds_order();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int r = (lane >> 3) + 8 * k;
+            v[k] = *reinterpret_cast<const uint4*>(st + r * 128 + ((cl ^ (r & 7)) * 16));
+        }
+        wave_lds_order();
+    }
+    store(MI - 1);
+}
+
+// 256 x 256 outputs of 8 waves, a wave 128 x 64; one workgroup, two waves per SIMD.
+// Half the reads from L2 of 128 x 128. The sums have to be vector registers, since
+// the vector unit scales and adds: 128 a wave.
+// 16 x 16 sums, whose instruction takes a whole block of 128: four of them are in
+// flight, and the vector unit adds the one issued three before while the next run,
+// so that neither waits for the other (32 x 32 sums, two instructions a block, with
+// one in flight: T 32768, N 4096, K 1024 162 us).
+// Ring of 2. A wave holds a step's b and streams its a. Behind the last but one
+// read the whole slot is in registers: the barrier stands there; the last sums cover
+// the next slot's first reads, and the freed slot's loads begin. The stream does not
+// stop between units: their outputs go through LDS of its own, behind the next
+// unit's loads.
+struct Large {
+    static constexpr int TILE = 256, WAVES = 8, MI = 8, NJ = 4, DEPTH = 3;
+    using S = Slot<TILE, WAVES>;
+    static constexpr int ST0 = 2 * S::BYTES, STB = 16 * 128, LDS = ST0 + WAVES * STB;
+    static constexpr int STORES = 2 * MI;  // of a wave's outputs
+    static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+template <bool BETA>
+__global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPlan pl) {
+    using G = Large;
+    using S = G::S;
+    constexpr int MI = G::MI, NJ = G::NJ, TILE = G::TILE, DEPTH = G::DEPTH, NQ = MI * NJ;
+    __shared__ uint4 lds_raw[G::LDS / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const uint32_t lds0 = lds_u32(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wrow = (wave >> 2) * 128, wcol = (wave & 3) * 64, row = lane & 15, g = lane >> 4;
+    const int nb = (wave & 3) >> 1;
+    Unit u;
+    int vb = blockIdx.x;
+    if (!unit_at<TILE, false>(pl, p.K, vb, u)) return;
+    Loader<TILE, G::WAVES, true, false> ld;
+    ld.init(p, wave, lane, nb);
+    ld.at.vl = vb;
+    ld.at.set(p, u);
+    int sll = 0;  // slot of the next loads
+    auto load = [&](int d) { ld.load(p, d, lds0 + sll * S::BYTES); };
+    auto next_loads = [&]() {
+        sll ^= 1;
+        ld.at.next(p, pl, workgroups);
+    };
+
+    // chunks g and g + 4 of row r
+    auto read = [&](const uint8_t* t, int r) {
+        const int sw = (row >> 1) & 7;
+        return join(*reinterpret_cast<const uint4*>(t + r * 128 + ((g ^ sw) * 16)),
+                    *reinterpret_cast<const uint4*>(t + r * 128 + (((g + 4) ^ sw) * 16)));
+    };
+    i32x8 a[2], b[NJ];
+    float s[MI], s2[MI];
+    auto read_a = [&](int i, int sl) { a[i & 1] = read(lds + sl * S::BYTES, wrow + 16 * i + row); };
+    auto read_b = [&](int j, int sl) { b[j] = read(lds + sl * S::BYTES + S::CODES, wcol + 16 * j + row); };
+    auto read_scales = [&](int sl) {
+        const uint8_t* t = lds + sl * S::BYTES;
+        const float sb = *reinterpret_cast<const float*>(t + S::SB + 256 * nb);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) s2[i] = sb * reinterpret_cast<const float*>(t + S::SA)[wrow + 16 * i + row];
+    };
+    f32x4 acc[MI][NJ], d[DEPTH + 1];
+    float last = 0.0f;  // the scale of the sums still in flight from the step before
+#pragma unroll
+    for (int q = 0; q <= DEPTH; ++q) d[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // sums q of this step (q < 0: the step before) are scaled and added
+    auto add = [&](int q) {
+        f32x4& t = acc[(q + NQ) % NQ / NJ][(q + NQ) % NQ % NJ];
+        const float by = q < 0 ? last : s[q / NJ];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = __builtin_fmaf(d[(q + NQ) & DEPTH][e], by, t[e]);
+        asm volatile("" : "+v"(t));  // here, not later: the sums in flight are few
+    };
+
+    // ---- stream
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int n = 0; n < S::ND; ++n) load(n);
+        next_loads();
+    }
+    wait_vm<S::ND>();
+    lds_barrier();
+    int sl = 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) read_b(j, sl);
+    read_a(0, sl);
+    read_scales(sl);
+    bool stored = false;  // the last unit's outputs are STORES stores behind the loads
+    uint8_t* st = lds + G::ST0 + wave * G::STB;
+    for (;;) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                asm volatile("" : "+v"(acc[i][j]));  // no first step of its own
+            }
+        last = 0.0f;
+        for (int k = 0; k < p.K; k += kFp8Block) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i) s[i] = s2[i];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                const int i = q / NJ, j = q % NJ;
+                if (q == NQ - NJ) {
+                    if (stored) wait_vm<G::STORES>();
+                    else wait_vm<0>();
+                    stored = false;
+                    lds_barrier();  // this slot is read, the other one is whole
+                    sl ^= 1;
+                }
+                d[q & DEPTH] = mma16<false>(b[j], a[i & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (j == 0) read_a((i + 1) % MI, sl);
+                if (q == NQ - NJ + 1) read_scales(sl);
+                if (i == MI - 1) read_b(j, sl);
+                if (i == MI - 1)
+#pragma unroll
+                    for (int n = j; n < S::ND; n += NJ) load(n);
+                add(q - DEPTH);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            next_loads();
+            last = s[MI - 1];
+        }
+#pragma unroll
+        for (int q = -DEPTH; q < 0; ++q) add(q);
+        const int rows = p.M - u.m0 - wrow, cols = p.N - u.c0 - wcol;
+        stored = rows > 0 && cols > 0;
+        if (stored)
+            store_wave16<BETA>(acc, st, static_cast<uint16_t*>(p.y) + (int64_t)(u.m0 + wrow) * p.ldy + u.c0 + wcol, p.ldy, rows, cols,
+                               p.beta);
+        vb += gridDim.x;
+        if (!unit_at<TILE, false>(pl, p.K, vb, u)) break;
+    }
+    wait_vm<0>();  // no load may land in LDS that the next workgroup owns
+}
+
 template <bool TILES, bool F32>
 void launch_rows(const Fp8Params& p, hipStream_t s) {
     const int64_t grid = (int64_t)((p.N + 31) / 32) * ((p.M + 31) / 32);
@@ -321,11 +528,19 @@ void launch_tiles(const Fp8Params& p, const LinearPlan& pl, int cus, hipStream_t
     }
 }
 
+void launch_large(const Fp8Params& p, int cus, hipStream_t s) {
+    const LinearPlan pl = fp8_tiles(p.M, p.N, p.K, 256, 1, cus);
+    const int grid = unit_grid(256, pl.whole, cus);
+    if (p.beta == 0.0f) fp8_large_kernel<false><<<grid, 512, 0, s>>>(p, pl);
+    else fp8_large_kernel<true><<<grid, 512, 0, s>>>(p, pl);
+}
+
 template <bool TILES, bool F32>
 void launch(const Fp8Params& p, hipStream_t s) {
     const int cus = cu_count();
     const Fp8Plan pl = fp8_plan(F32, p.M, p.N, p.K, cus);
     if (pl.rows) launch_rows<TILES, F32>(p, s);
+    else if (TILES && !F32 && fp8_large(p.M, p.N, p.K, cus)) launch_large(p, cus, s);
     else launch_tiles<TILES, F32>(p, pl.tiles, cus, s);
 }
 

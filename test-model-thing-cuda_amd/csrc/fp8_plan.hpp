@@ -85,6 +85,10 @@ inline Fp8Plan fp8_plan(bool f32, int M, int N, int K, int cus) {
     pl.tiles = fp8_tiles(M, N, K, 128, (int)std::max<int64_t>(most, 1), cus);
     return pl;
 }
+inline bool fp8_large(int M, int N, int K, int cus) {
+    const int64_t big = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
+    return big >= tile_slots(256, cus);
+}
 // An upper bound over all row counts up to M: partial tiles fill at most the
 // workgroup slots, and neither tiles nor parts fall with M.
 inline size_t fp8_workspace_bound(int M, int N, int K, int cus) {

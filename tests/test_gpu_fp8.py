@@ -163,6 +163,27 @@ def test_product_to_the_bit(M, N, K, tiles, dtype):
     _product(M, N, K, tiles, dtype)
 
 
+def _launched(M, N, K, tiles, dtype):
+    """The kernels that a product of these sizes launches."""
+    from launched_kernels import launched_kernels
+    b = ref.blocks_of
+    e = lambda r, c: torch.zeros(r, ref.up(c, 16), dtype=ref.FP8, device="cuda")[:, :c]  # noqa: E731
+    size = tmt_moe.fp8_workspace_size(M, N, K, TILES if tiles else ROWS)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda") if size else None
+    args = (e(M, K), torch.ones(b(K), M, device="cuda"), e(N, K),
+            torch.ones((b(N), b(K)) if tiles else (b(K), N), device="cuda"), torch.empty(M, N, dtype=dtype, device="cuda"))
+    return launched_kernels(lambda: tmt_moe.fp8_matmul(*args, blocks=TILES if tiles else ROWS, workspace=ws))
+
+
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 128), (4000, 4200, 200), (4090, 4104, 1000), (8200, 4096, 256), (33000, 512, 400)])
+def test_large_products(M, N, K):
+    """256 x 256 tiles: whole and ragged, several to a workgroup, a short last block, added to."""
+    assert any("fp8_large" in k for k in _launched(M, N, K, True, BF16))
+    _product(M, N, K, True, BF16)
+    _product(M, N, K, True, BF16, beta=0.5, ldy=N + 40)
+    _product(M, N, K, True, BF16, exact=False)
+
+
 @pytest.mark.parametrize("tiles", [True, False])
 @pytest.mark.parametrize("M,N,K", [(7, 64, 200), (200, 264, 1024), (777, 512, 2048)])
 def test_product_added(M, N, K, tiles):
