@@ -185,7 +185,8 @@ struct Slot {
     static constexpr int ND = 2 * LOADS + 2;                        // loads per wave and step
 };
 
-// The loads of a tiled kernel's wave: load(d) issues load d of the next step.
+// The loads of a tiled kernel's wave: load(d) issues load d of the next step; those
+// of b's codes come first, then the scales', then those of a's codes.
 template <int TILE, int WAVES, bool TILES, bool SPLIT>
 struct Loader {
     using S = Slot<TILE, WAVES>;
@@ -208,12 +209,12 @@ struct Loader {
     __device__ void load(const Fp8Params& p, int d, uint32_t slot) {
         constexpr uint32_t FAR = 0x80000000u;  // past any window
         if (d == 0) lim = at.chunks(p);
-        if (d < 2 * S::LOADS) {
-            const int i = d >> 1;
-            const bool in = (chunk ^ (4 * (i & 1))) < lim;
-            if (d & 1) dma16(at.wb, in ? b_off[i] : FAR, slot + S::CODES + (wave * S::LOADS + i) * 1024);
-            else dma16(at.wa, in ? a_off[i] : FAR, slot + (wave * S::LOADS + i) * 1024);
-        } else if (d == 2 * S::LOADS) {
+        if (d < S::LOADS) {
+            dma16(at.wb, (chunk ^ (4 * (d & 1))) < lim ? b_off[d] : FAR, slot + S::CODES + (wave * S::LOADS + d) * 1024);
+        } else if (d >= S::LOADS + 2) {
+            const int i = d - S::LOADS - 2;
+            dma16(at.wa, (chunk ^ (4 * (i & 1))) < lim ? a_off[i] : FAR, slot + (wave * S::LOADS + i) * 1024);
+        } else if (d == S::LOADS) {
             dma4(at.wsa, sc_off, slot + S::SA + 256 * (wave & (TILE / 64 - 1)));
         } else if constexpr (TILES) {
             dma4(at.wsb, sc_off & 255, slot + S::SB + 256 * at.nb);
@@ -385,7 +386,8 @@ struct Large {
     static constexpr int TILE = 256, WAVES = 8, MI = 8, NJ = 4, DEPTH = 3;
     using S = Slot<TILE, WAVES>;
     static constexpr int ST0 = 2 * S::BYTES, STB = 16 * 128, LDS = ST0 + WAVES * STB;
-    static constexpr int STORES = 2 * MI;  // of a wave's outputs
+    static constexpr int STORES = 2 * MI;      // of a wave's outputs
+    static constexpr int EARLY = S::LOADS + 2; // a step's loads ahead of its a
     static_assert(LDS <= 160 * 1024, "LDS");
 };
 
@@ -474,11 +476,12 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
                 const int i = q / NJ, j = q % NJ;
+                if (q == NJ) lds_barrier();  // this slot's b and scales are read
                 if (q == NQ - NJ) {
-                    if (stored) wait_vm<G::STORES>();
-                    else wait_vm<0>();
+                    if (stored) wait_vm<G::STORES + G::EARLY>();
+                    else wait_vm<G::EARLY>();
                     stored = false;
-                    lds_barrier();  // this slot is read, the other one is whole
+                    lds_barrier();  // all of this slot is read, the other one is whole
                     sl ^= 1;
                 }
                 d[q & DEPTH] = mma16<false>(b[j], a[i & 1]);
@@ -486,9 +489,8 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
                 if (j == 0) read_a((i + 1) % MI, sl);
                 if (q == NQ - NJ + 1) read_scales(sl);
                 if (i == MI - 1) read_b(j, sl);
-                if (i == MI - 1)
-#pragma unroll
-                    for (int n = j; n < S::ND; n += NJ) load(n);
+                if (i > 0 && i <= G::EARLY && j == 1) load(i - 1);
+                if (i == MI - 1) load(G::EARLY + j);
                 add(q - DEPTH);
                 __builtin_amdgcn_sched_barrier(0);
             }
