@@ -187,7 +187,8 @@ struct Slot {
 
 // The loads of a tiled kernel's wave: load(d) issues load d of the next step; those
 // of b's codes come first, then the scales', then those of a's codes.
-template <int TILE, int WAVES, bool TILES, bool SPLIT>
+// FULL: K is a multiple of 128, and no chunk lies behind a row's end.
+template <int TILE, int WAVES, bool TILES, bool SPLIT, bool FULL>
 struct Loader {
     using S = Slot<TILE, WAVES>;
     static_assert(S::LOADS % 2 == 0, "a lane's chunk goes by the load's parity");
@@ -208,12 +209,12 @@ struct Loader {
     }
     __device__ void load(const Fp8Params& p, int d, uint32_t slot) {
         constexpr uint32_t FAR = 0x80000000u;  // past any window
-        if (d == 0) lim = at.chunks(p);
+        if (!FULL && d == 0) lim = at.chunks(p);
         if (d < S::LOADS) {
-            dma16(at.wb, (chunk ^ (4 * (d & 1))) < lim ? b_off[d] : FAR, slot + S::CODES + (wave * S::LOADS + d) * 1024);
+            dma16(at.wb, FULL || (chunk ^ (4 * (d & 1))) < lim ? b_off[d] : FAR, slot + S::CODES + (wave * S::LOADS + d) * 1024);
         } else if (d >= S::LOADS + 2) {
             const int i = d - S::LOADS - 2;
-            dma16(at.wa, (chunk ^ (4 * (i & 1))) < lim ? a_off[i] : FAR, slot + (wave * S::LOADS + i) * 1024);
+            dma16(at.wa, FULL || (chunk ^ (4 * (i & 1))) < lim ? a_off[i] : FAR, slot + (wave * S::LOADS + i) * 1024);
         } else if (d == S::LOADS) {
             dma4(at.wsa, sc_off, slot + S::SA + 256 * (wave & (TILE / 64 - 1)));
         } else if constexpr (TILES) {
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPla
     Unit u;
     int vb = blockIdx.x;
     if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) return;
-    Loader<TILE, 4, TILES, SPLIT> ld;
+    Loader<TILE, 4, TILES, SPLIT, false> ld;
     ld.init(p, wave, lane, 0);
     ld.at.vl = vb;
     ld.at.set(p, u);
@@ -391,7 +392,7 @@ struct Large {
     static_assert(LDS <= 160 * 1024, "LDS");
 };
 
-template <bool BETA>
+template <bool FULL, bool BETA>
 __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPlan pl) {
     using G = Large;
     using S = G::S;
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
     Unit u;
     int vb = blockIdx.x;
     if (!unit_at<TILE, false>(pl, p.K, vb, u)) return;
-    Loader<TILE, G::WAVES, true, false> ld;
+    Loader<TILE, G::WAVES, true, false, FULL> ld;
     ld.init(p, wave, lane, nb);
     ld.at.vl = vb;
     ld.at.set(p, u);
@@ -424,14 +425,18 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
                     *reinterpret_cast<const uint4*>(t + r * 128 + (((g + 4) ^ sw) * 16)));
     };
     i32x8 a[2], b[NJ];
-    float s[MI], s2[MI];
+    float s[MI], next[2];
     auto read_a = [&](int i, int sl) { a[i & 1] = read(lds + sl * S::BYTES, wrow + 16 * i + row); };
     auto read_b = [&](int j, int sl) { b[j] = read(lds + sl * S::BYTES + S::CODES, wcol + 16 * j + row); };
+    // the next step's scales, while the last two rows' are still in use
     auto read_scales = [&](int sl) {
         const uint8_t* t = lds + sl * S::BYTES;
         const float sb = *reinterpret_cast<const float*>(t + S::SB + 256 * nb);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) s2[i] = sb * reinterpret_cast<const float*>(t + S::SA)[wrow + 16 * i + row];
+        for (int i = 0; i < MI; ++i) {
+            float& to = i < MI - 2 ? s[i] : next[i - MI + 2];
+            to = sb * reinterpret_cast<const float*>(t + S::SA)[wrow + 16 * i + row];
+        }
     };
     f32x4 acc[MI][NJ], d[DEPTH + 1];
     float last = 0.0f;  // the scale of the sums still in flight from the step before
@@ -471,8 +476,8 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
             }
         last = 0.0f;
         for (int k = 0; k < p.K; k += kFp8Block) {
-#pragma unroll
-            for (int i = 0; i < MI; ++i) s[i] = s2[i];
+            s[MI - 2] = next[0];
+            s[MI - 1] = next[1];
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
                 const int i = q / NJ, j = q % NJ;
@@ -533,8 +538,9 @@ void launch_tiles(const Fp8Params& p, const LinearPlan& pl, int cus, hipStream_t
 void launch_large(const Fp8Params& p, int cus, hipStream_t s) {
     const LinearPlan pl = fp8_tiles(p.M, p.N, p.K, 256, 1, cus);
     const int grid = unit_grid(256, pl.whole, cus);
-    if (p.beta == 0.0f) fp8_large_kernel<false><<<grid, 512, 0, s>>>(p, pl);
-    else fp8_large_kernel<true><<<grid, 512, 0, s>>>(p, pl);
+    const bool full = p.K % kFp8Block == 0;
+    if (p.beta == 0.0f) full ? fp8_large_kernel<true, false><<<grid, 512, 0, s>>>(p, pl) : fp8_large_kernel<false, false><<<grid, 512, 0, s>>>(p, pl);
+    else full ? fp8_large_kernel<true, true><<<grid, 512, 0, s>>>(p, pl) : fp8_large_kernel<false, true><<<grid, 512, 0, s>>>(p, pl);
 }
 
 template <bool TILES, bool F32>
