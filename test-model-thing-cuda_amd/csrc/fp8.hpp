@@ -79,7 +79,7 @@ struct Fp8Params {
     float beta;
     float* part;          // workspace: split reductions' partial sums
 };
-size_t fp8_workspace(bool tiles, int M, int N, int K);
+size_t fp8_workspace(int M, int N, int K);
 // Arguments as the C ABI has checked them, M and N > 0, K >= 0.
 hipError_t launch_fp8_matmul(bool tiles, bool f32, const Fp8Params& p, hipStream_t s);
 

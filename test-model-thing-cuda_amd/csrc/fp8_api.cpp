@@ -161,7 +161,7 @@ int tmt_moe_fp8_workspace_size(int32_t b_blocks, int32_t M, int32_t N, int32_t K
     int rc = check_blocks(b_blocks);
     if (rc || (rc = check_product_shape(M, N, K))) return rc;
     if (!bytes) return fail(TMT_MOE_EINVAL, "bytes is NULL");
-    *bytes = M == 0 || N == 0 ? 0 : fp8_workspace(b_blocks == TMT_MOE_FP8_TILES, M, N, K);
+    *bytes = M == 0 || N == 0 ? 0 : fp8_workspace(M, N, K);
     return TMT_MOE_OK;
 }
 
@@ -178,7 +178,7 @@ int tmt_moe_fp8_matmul(void* stream, int32_t b_blocks, int32_t dtype, int32_t M,
                   (rc = check_scales("B_scale", B_scale, ldbs, tiles ? blocks_of(K) : N))))
         return rc;
     if ((rc = check_rows("Y", Y, ldy, N, dtype == TMT_MOE_BF16 ? 8 : 4))) return rc;
-    if ((rc = check_workspace(workspace, workspace_bytes, fp8_workspace(tiles, M, N, K)))) return rc;
+    if ((rc = check_workspace(workspace, workspace_bytes, fp8_workspace(M, N, K)))) return rc;
     Fp8Params p{};
     p.M = M; p.N = N; p.K = K; p.a = A; p.lda = lda; p.as = A_scale; p.ldas = ldas; p.b = B; p.ldb = ldb;
     p.bs = B_scale; p.ldbs = ldbs; p.y = Y; p.ldy = ldy; p.beta = beta; p.part = static_cast<float*>(workspace);

@@ -58,8 +58,9 @@ __device__ __forceinline__ f32x4 mma16(i32x8 b, i32x8 a) {
 // ---- few rows ----------------------------------------------------------------------
 // A workgroup takes 16 NB columns and 16 RB rows of y; its NW waves deal out the
 // reduction in blocks of 128. Lane l loads chunks l / 16 and l / 16 + 4 (16 codes
-// each) of row l % 16 of a block straight into registers, of both operands. The
-// waves' sums meet in LDS and are added in wave order.
+// each) of row l % 16 of a block straight into registers, of both operands: 64
+// bytes of 16 rows a load. The waves' sums meet in LDS and are added in wave order.
+// Bound by a launch and a trip to memory, then by the loads themselves.
 template <bool TILES, bool F32, int RB, int NB, int NW>
 __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8Params p) {
     constexpr int OUT = 256 * RB * NB;
@@ -69,42 +70,61 @@ __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8Params p) {
     const int nb = (p.N + 16 * NB - 1) / (16 * NB);  // blocks of columns, which run fastest
     const int n0 = (int)(blockIdx.x % nb) * 16 * NB, m0 = (int)(blockIdx.x / nb) * 16 * RB;
     const int blocks = (p.K + kFp8Block - 1) / kFp8Block;
+    // windows: rows past the last one, and chunks past a row's end, read zeros
+    constexpr uint32_t FAR = 0x80000000u;
+    const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u;
+    const __amdgpu_buffer_rsrc_t wa = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.a) + (int64_t)m0 * p.lda, 0, (int)((uint32_t)(min(p.M - m0, 16 * RB) - 1) * (uint32_t)p.lda + k16), 0x00020000);
+    const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.b) + (int64_t)n0 * p.ldb, 0, (int)((uint32_t)(min(p.N - n0, 16 * NB) - 1) * (uint32_t)p.ldb + k16), 0x00020000);
+    const float *psa[RB], *psb[NB];  // past the last row: its scale again, for no output
+#pragma unroll
+    for (int r = 0; r < RB; ++r) psa[r] = p.as + min(m0 + 16 * r + row, p.M - 1);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        // rows: the columns 4 g .. + 3 of 16, which are in or out together (N is a multiple of 8)
+        if constexpr (TILES) psb[i] = p.bs + (int64_t)(min(n0 + 16 * i, p.N - 1) / kFp8Block) * p.ldbs;
+        else psb[i] = p.bs + min(n0 + 16 * i + 4 * g, p.N - 4);
+    }
     f32x4 acc[RB][NB];
 #pragma unroll
     for (int r = 0; r < RB; ++r)
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[r][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto chunk = [&](const uint8_t* codes, int k) {
-        return k < p.K ? *reinterpret_cast<const uint4*>(codes + k) : make_uint4(0, 0, 0, 0);
-    };
     for (int kb = wave; kb < blocks; kb += NW) {
-        const int k = kb * kFp8Block + 16 * g;
-        i32x8 b[NB], a[RB];
+        i32x8 a[RB], b[NB];
+        float sa[RB], st[NB];
         f32x4 sb[NB];
-        float sa[RB];
+        const int k = kb * kFp8Block + 16 * g;
+        const uint32_t lo = k < p.K ? (uint32_t)k : FAR, hi = k + 64 < p.K ? (uint32_t)(k + 64) : FAR;
+        auto chunks = [&](__amdgpu_buffer_rsrc_t w, uint32_t at) {
+            return join(__builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, (int)(at + lo), 0, 0)),
+                        __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, (int)(at + hi), 0, 0)));
+        };
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const uint8_t* q = p.b + (int64_t)min(n0 + 16 * i + row, p.N - 1) * p.ldb;
-            b[i] = join(chunk(q, k), chunk(q, k + 64));
+            b[i] = chunks(wb, (uint32_t)(16 * i + row) * (uint32_t)p.ldb);
             if constexpr (TILES) {
-                const float s = p.bs[(int64_t)(min(n0 + 16 * i, p.N - 1) / kFp8Block) * p.ldbs + kb];
-                sb[i] = f32x4{s, s, s, s};
+                st[i] = psb[i][kb];
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sb[i][e] = p.bs[(int64_t)kb * p.ldbs + min(n0 + 16 * i + 4 * g + e, p.N - 1)];
+                for (int e = 0; e < 4; ++e) sb[i][e] = psb[i][(int64_t)kb * p.ldbs + e];
             }
         }
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
-            const int m = min(m0 + 16 * r + row, p.M - 1);
-            const uint8_t* q = p.a + (int64_t)m * p.lda;
-            a[r] = join(chunk(q, k), chunk(q, k + 64));
-            sa[r] = p.as[(int64_t)kb * p.ldas + m];
+            a[r] = chunks(wa, (uint32_t)(16 * r + row) * (uint32_t)p.lda);
+            sa[r] = psa[r][(int64_t)kb * p.ldas];
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < RB; ++r)
 #pragma unroll
-            for (int i = 0; i < NB; ++i) acc[r][i] += mma16<F32>(b[i], a[r]) * (sb[i] * sa[r]);
+            for (int i = 0; i < NB; ++i) {
+                const f32x4 d = mma16<F32>(b[i], a[r]);
+                if constexpr (TILES) acc[r][i] += d * (st[i] * sa[r]);
+                else acc[r][i] += d * (sb[i] * sa[r]);
+            }
     }
     // acc[r][i][e]: row 16 r + lane % 16, column 16 i + 4 (lane / 16) + e
 #pragma unroll
@@ -191,17 +211,17 @@ struct Slot {
 template <int TILE, int WAVES, bool TILES, bool SPLIT, bool FULL>
 struct Loader {
     using S = Slot<TILE, WAVES>;
-    static_assert(S::LOADS % 2 == 0, "a lane's chunk goes by the load's parity");
     Fp8Cursor<TILE, TILES, SPLIT> at;
     uint32_t a_off[S::LOADS], b_off[S::LOADS], sc_off;
     int wave, chunk, lim = 0;
+    __device__ int chunk_of(int i) const { return chunk ^ (4 * ((wave * S::LOADS + i) & 1)); }
     __device__ void init(const Fp8Params& p, int wave_, int lane, int nb) {
         wave = wave_;
         at.nb = nb;
-        chunk = (lane & 7) ^ (lane >> 4);  // of even loads; odd ones': ^ 4
+        chunk = (lane & 7) ^ (lane >> 4);  // of the even loads
 #pragma unroll
         for (int i = 0; i < S::LOADS; ++i) {
-            const int r = 8 * (wave * S::LOADS + i) + (lane >> 3), c = chunk ^ (4 * (i & 1));
+            const int r = 8 * (wave * S::LOADS + i) + (lane >> 3), c = chunk_of(i);
             a_off[i] = (uint32_t)r * (uint32_t)p.lda + c * 16;
             b_off[i] = (uint32_t)r * (uint32_t)p.ldb + c * 16;
         }
@@ -211,10 +231,10 @@ struct Loader {
         constexpr uint32_t FAR = 0x80000000u;  // past any window
         if (!FULL && d == 0) lim = at.chunks(p);
         if (d < S::LOADS) {
-            dma16(at.wb, FULL || (chunk ^ (4 * (d & 1))) < lim ? b_off[d] : FAR, slot + S::CODES + (wave * S::LOADS + d) * 1024);
+            dma16(at.wb, FULL || chunk_of(d) < lim ? b_off[d] : FAR, slot + S::CODES + (wave * S::LOADS + d) * 1024);
         } else if (d >= S::LOADS + 2) {
             const int i = d - S::LOADS - 2;
-            dma16(at.wa, FULL || (chunk ^ (4 * (i & 1))) < lim ? a_off[i] : FAR, slot + (wave * S::LOADS + i) * 1024);
+            dma16(at.wa, FULL || chunk_of(i) < lim ? a_off[i] : FAR, slot + (wave * S::LOADS + i) * 1024);
         } else if (d == S::LOADS) {
             dma4(at.wsa, sc_off, slot + S::SA + 256 * (wave & (TILE / 64 - 1)));
         } else if constexpr (TILES) {
@@ -225,15 +245,14 @@ struct Loader {
     }
 };
 
-// 128 x 128 outputs of 4 waves, a wave 64 x 64; ring of 2, two workgroups per CU. A
-// unit's first step is loaded before the previous unit's epilogue, which stages
-// through the other slot.
-template <bool TILES, bool F32, bool SPLIT, bool BETA>
-__global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPlan pl) {
+// fp32 results, many units: 128 x 128 outputs of 4 waves, a wave 64 x 64; ring of 2, two workgroups
+// per CU, which cover each other's waits. A unit's first step is loaded before the
+// previous unit's epilogue, which stages through the other slot.
+template <bool TILES, bool SPLIT, bool BETA>
+__global__ __launch_bounds__(256, 2) void fp8_wide_kernel(Fp8Params p, LinearPlan pl) {
     constexpr int TILE = 128, WT = 64, MI = 2;
     using S = Slot<TILE, 4>;
-    using Operand = std::conditional_t<F32, Wide, Codes>;
-    static_assert(4 * Stage<F32, MI>::BYTES <= S::BYTES, "the epilogue stages in a slot");
+    static_assert(4 * Stage<true, MI>::BYTES <= S::BYTES, "the epilogue stages in a slot");
     __shared__ uint4 lds_raw[2 * S::BYTES / 16];
     uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
     const uint32_t lds0 = lds_u32(lds);
@@ -254,22 +273,19 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPla
         sl ^= 1;
         ld.at.next(p, pl, workgroups);
     };
-    auto operand = [&](const uint8_t* t, int r) {
-        if constexpr (F32) return widen(read_codes(t, r, h));
-        else return read_codes(t, r, h);
-    };
+    auto operand = [&](const uint8_t* t, int r) { return widen(read_codes(t, r, h)); };
     f32x16 acc[MI][MI];
     clear(acc);
     load_step();
     for (;;) {
         for (int k = u.kbeg; k < u.kend; k += kFp8Block) {
             wait_vm<0>();
-            lds_barrier();  // step k is whole in LDS, and the other slot is read
+            lds_barrier();  // step k is whole in LDS, and the slot before is read
             load_step();    // past the last unit: zeros
             const uint8_t* t = lds + slot * S::BYTES;
             const float* sa = reinterpret_cast<const float*>(t + S::SA);
             const float* sb = reinterpret_cast<const float*>(t + S::SB);
-            Operand a[MI];
+            Wide a[MI];
             float s[MI];
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
@@ -279,7 +295,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPla
             }
 #pragma unroll
             for (int j = 0; j < MI; ++j) {
-                const Operand b = operand(t + S::CODES, wcol + 32 * j + row);
+                const Wide b = operand(t + S::CODES, wcol + 32 * j + row);
                 f32x4 sn[4];
                 if constexpr (!TILES)
 #pragma unroll
@@ -295,7 +311,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPla
             slot ^= 1;
         }
         lds_barrier();  // the last step's slot is read: the epilogue stages there
-        finish_unit<TILE, F32, MI, SPLIT, BETA, false>(acc, lds + (slot ^ 1) * S::BYTES + wave * Stage<F32, MI>::BYTES, p, u, p.M, p.N,
+        finish_unit<TILE, true, MI, SPLIT, BETA, false>(acc, lds + (slot ^ 1) * S::BYTES + wave * Stage<true, MI>::BYTES, p, u, p.M, p.N,
                                                 wrow, wcol);
         vb += gridDim.x;
         if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) break;
@@ -304,49 +320,169 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Params p, LinearPla
     wait_vm<0>();  // no load may land in LDS that the next workgroup owns
 }
 
-// ---- large products ------------------------------------------------------------------
+// fp32 results, few units, and bf16 results on 64 x 64 tiles: TILE x TILE outputs of 4
+// waves, a wave a quarter of them; a ring of 4, filled ahead, whose steps' operands
+// are read one step ahead too. A step of 64 x 64 is bound by its instructions, of
+// which one 32 x 32 sum a wave has the fewest (T 777, N 1024, K 4096 15.1 us; with
+// 16 x 16 sums, four in flight, 17.4 on 4 waves and 16.3 on 8). The stream does not
+// stop between units; the epilogue stages through the slot whose step is in registers
+// already.
+template <int TILE, bool TILES, bool F32, bool SPLIT, bool BETA>
+__global__ __launch_bounds__(256, (TILE == 128 ? 1 : 2)) void fp8_quarter_kernel(Fp8Params p, LinearPlan pl) {
+    constexpr int WT = TILE / 2, MI = WT / 32, RING = 4;
+    using S = Slot<TILE, 4>;
+    static_assert(4 * Stage<F32, MI>::BYTES <= S::BYTES, "the epilogue stages in a slot");
+    __shared__ uint4 lds_raw[RING * S::BYTES / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const uint32_t lds0 = lds_u32(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT, row = lane & 31, h = lane >> 5;
+    Unit u;
+    int vb = blockIdx.x;
+    if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) return;
+    Loader<TILE, 4, TILES, SPLIT, false> ld;
+    ld.init(p, wave, lane, 0);
+    ld.at.vl = vb;
+    ld.at.set(p, u);
+    int sl = 0, slot = 0;  // of the next loads, of the step in registers
+    auto load_step = [&]() {
+#pragma unroll
+        for (int d = 0; d < S::ND; ++d) ld.load(p, d, lds0 + sl * S::BYTES);
+        sl = (sl + 1) & (RING - 1);
+        ld.at.next(p, pl, workgroups);
+    };
+    struct Step {
+        Codes a[MI], b[MI];
+        float s[MI];
+        f32x4 sn[MI][4];
+    } f[2];
+    auto read_step = [&](Step& t, int slot) {
+        const uint8_t* at = lds + slot * S::BYTES;
+        const float* sa = reinterpret_cast<const float*>(at + S::SA);
+        const float* sb = reinterpret_cast<const float*>(at + S::SB);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            t.a[i] = read_codes(at, wrow + 32 * i + row, h);
+            t.b[i] = read_codes(at + S::CODES, wcol + 32 * i + row, h);
+            t.s[i] = sa[wrow + 32 * i + row];
+            if constexpr (TILES) {
+                t.s[i] *= sb[0];
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) t.sn[i][q] = *reinterpret_cast<const f32x4*>(sb + wcol + 32 * i + 8 * q + 4 * h);
+            }
+        }
+    };
+    f32x16 acc[MI][MI];
+    clear(acc);
+    // multiplies the step in t and reads the next one into t2
+    auto step = [&](const Step& t, Step& t2) {
+        wait_vm<(RING - 2) * S::ND>();
+        lds_barrier();  // the next step is whole in LDS, and this one's slot is read
+        load_step();    // past the last unit: zeros
+        slot = (slot + 1) & (RING - 1);
+        read_step(t2, slot);
+        __builtin_amdgcn_sched_barrier(0);
+        using Operand = std::conditional_t<F32, Wide, Codes>;
+        auto operand = [](const Codes& c) {
+            if constexpr (F32) return widen(c);
+            else return c;
+        };
+        Operand a[MI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a[i] = operand(t.a[i]);
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+            const Operand b = operand(t.b[j]);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                const f32x16 d = mma32(b, a[i]);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    acc[i][j][r] = __builtin_fmaf(d[r], TILES ? t.s[i] : t.s[i] * t.sn[j][r >> 2][r & 3], acc[i][j][r]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int n = 0; n < RING; ++n) load_step();
+    wait_vm<(RING - 1) * S::ND>();
+    lds_barrier();
+    read_step(f[0], 0);
+    for (;;) {
+        int left = (u.kend - u.kbeg + kFp8Block - 1) / kFp8Block;
+        for (; left >= 2; left -= 2) {
+            step(f[0], f[1]);
+            step(f[1], f[0]);
+        }
+        if (left > 0) {
+            step(f[0], f[1]);
+            f[0] = f[1];
+        }
+        lds_barrier();  // the slot of the step in registers is read: the epilogue stages there
+        finish_unit<TILE, F32, MI, SPLIT, BETA, false>(acc, lds + slot * S::BYTES + wave * Stage<F32, MI>::BYTES, p, u, p.M, p.N, wrow, wcol);
+        vb += gridDim.x;
+        if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) break;
+        clear(acc);
+    }
+    wait_vm<0>();  // no load may land in LDS that the next workgroup owns
+}
+
+// ---- sums of 16 x 16 ---------------------------------------------------------------
 // acc[i][j][e] = C[m][c] with m = 16 i + lane % 16 and c = 16 j + 4 (lane / 16) + e
-// in the wave's outputs. 16 rows at a time go through the wave's own LDS, so that
-// a row's 64 columns leave as one run of 16-byte stores; no barrier. `out` is the
-// wave's first output; rows and columns past the last ones are dropped by the
-// hardware's bounds.
-template <bool BETA, int MI>
-__device__ __forceinline__ void store_wave16(f32x4 (&acc)[MI][4], uint8_t* st, uint16_t* out, int64_t ld, int rows, int cols,
+// in a wave's outputs.
+
+// Operand rows of 16, from LDS rows of 128 bytes whose chunks of 16 are
+// XOR-swizzled by row / 2: lane l holds chunks g and g + 4 of row l % 16, g = l / 16.
+__device__ __forceinline__ i32x8 read_codes16(const uint8_t* t, int r, int g) {
+    const int sw = (r >> 1) & 7;
+    return join(*reinterpret_cast<const uint4*>(t + r * 128 + ((g ^ sw) * 16)),
+                *reinterpret_cast<const uint4*>(t + r * 128 + (((g + 4) ^ sw) * 16)));
+}
+
+// Outputs to memory: 16 rows at a time go through the wave's own LDS (NJ * 512
+// bytes), so that a row's 16 NJ columns leave as one run of 16-byte stores; no
+// barrier. `out` is the wave's first output; rows and columns past the last ones are
+// dropped by the hardware's bounds.
+template <bool BETA, int MI, int NJ>
+__device__ __forceinline__ void store_wave16(f32x4 (&acc)[MI][NJ], uint8_t* st, uint16_t* out, int64_t ld, int rows, int cols,
                                              float beta) {
     constexpr uint32_t FAR = 0x80000000u;
+    constexpr int CH = 2 * NJ, RPI = 64 / CH, K = 16 / RPI;  // chunks of a staged row, rows per store, stores
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));  // the addresses below are not kept through the main loop
-    const int lr = lane & 15, g = lane >> 4, cl = lane & 7;
+    const int lr = lane & 15, g = lane >> 4, cl = lane % CH;
     const uint32_t row = (uint32_t)(ld * 2);
     rows = min(rows, 16 * MI);
-    cols = min(cols, 64);
+    cols = min(cols, 16 * NJ);
     const __amdgpu_buffer_rsrc_t win = __builtin_amdgcn_make_buffer_rsrc(out, 0, (int)output_window(rows, row, cols, 2), 0x00020000);
-    u32x2 old[2][4];
+    u32x2 old[2][NJ];
     auto load_old = [&](int i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NJ; ++j) {
             const int c = 16 * j + 4 * g;
             old[i & 1][j] = __builtin_amdgcn_raw_buffer_load_b64(win, c < cols ? (int)((uint32_t)(16 * i + lr) * row + 2 * c) : (int)FAR, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
     if constexpr (BETA) load_old(0);
-    uint4 v[2];
+    uint4 v[K];
     auto store = [&](int i) {
-        uint32_t at = 8 * cl < cols ? (uint32_t)(16 * i + (lane >> 3)) * row + 16 * cl : FAR;
+        uint32_t at = 8 * cl < cols ? (uint32_t)(16 * i + lane / CH) * row + 16 * cl : FAR;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < K; ++k) {
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), win, (int)at, 0, 2);
-            at += 8 * row;
+            at += RPI * row;
         }
     };
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         if constexpr (BETA)
             if (i + 1 < MI) load_old(i + 1);
-        uint2 half[4];
+        uint2 half[NJ];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NJ; ++j) {
             f32x4 f = acc[i][j];
             if constexpr (BETA) {
                 const u32x2 o = old[i & 1][j];
@@ -358,19 +494,154 @@ __device__ __forceinline__ void store_wave16(f32x4 (&acc)[MI][4], uint8_t* st, u
         if (i > 0) store(i - 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint2*>(st + lr * 128 + (((2 * j + (g >> 1)) ^ (lr & 7)) * 16) + (g & 1) * 8) = half[j];
+        for (int j = 0; j < NJ; ++j)
+            *reinterpret_cast<uint2*>(st + lr * (16 * CH) + (((2 * j + (g >> 1)) ^ (lr & (CH - 1))) * 16) + (g & 1) * 8) = half[j];
         wave_lds_order();
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int r = (lane >> 3) + 8 * k;
-            v[k] = *reinterpret_cast<const uint4*>(st + r * 128 + ((cl ^ (r & 7)) * 16));
+        for (int k = 0; k < K; ++k) {
+            const int r = lane / CH + RPI * k;
+            v[k] = *reinterpret_cast<const uint4*>(st + r * (16 * CH) + ((cl ^ (r & (CH - 1))) * 16));
         }
         wave_lds_order();
     }
     store(MI - 1);
 }
 
+// bf16 results, not many units: 128 x 128 outputs of 8 waves, a wave 64 x 32; a ring of
+// 4 steps, filled ahead, whose operands are read one step ahead too, so that a step
+// waits for neither. Sums of 16 x 16, four of them in flight as in the kernel for
+// large products. A step takes 0.6 us (0.85 on 4 waves, with 32 x 32 sums or 16 x 16,
+// whatever its loads did: a lone wave per SIMD is bound by its instructions). The
+// stream does not stop between units; the epilogue stages through the slot whose step
+// is in registers already.
+template <bool TILES, bool SPLIT, bool BETA>
+__global__ __launch_bounds__(512, 2) void fp8_deep_kernel(Fp8Params p, LinearPlan pl) {
+    constexpr int TILE = 128, RING = 4, MI = 4, NJ = 2, NQ = MI * NJ, DEPTH = 3;
+    using S = Slot<TILE, 8>;
+    static_assert(8 * NJ * 512 <= S::BYTES && (RING - 1) * S::ND < 64, "the epilogue stages in a slot; what a wait counts");
+    __shared__ uint4 lds_raw[RING * S::BYTES / 16];
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
+    const uint32_t lds0 = lds_u32(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wrow = (wave >> 2) * 64, wcol = (wave & 3) * 32, row = lane & 15, g = lane >> 4;
+    Unit u;
+    int vb = blockIdx.x;
+    if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) return;
+    Loader<TILE, 8, TILES, SPLIT, false> ld;
+    ld.init(p, wave, lane, 0);
+    ld.at.vl = vb;
+    ld.at.set(p, u);
+    int sl = 0, slot = 0;  // of the next loads, of the step in registers
+    auto load_step = [&]() {
+#pragma unroll
+        for (int d = 0; d < S::ND; ++d) ld.load(p, d, lds0 + sl * S::BYTES);
+        sl = (sl + 1) & (RING - 1);
+        ld.at.next(p, pl, workgroups);
+    };
+    struct Scales {
+        float m[MI];   // of a's rows (tiles: times b's)
+        f32x4 n[NJ];   // rows: of b's
+    };
+    struct Step {
+        i32x8 a[MI], b[NJ];
+        Scales s;
+    } f[2];
+    Scales before;  // of the step whose last sums are still in flight
+    auto read_step = [&](Step& t, int slot) {
+        const uint8_t* at = lds + slot * S::BYTES;
+        const float* sa = reinterpret_cast<const float*>(at + S::SA);
+        const float* sb = reinterpret_cast<const float*>(at + S::SB);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            t.a[i] = read_codes16(at, wrow + 16 * i + row, g);
+            t.s.m[i] = sa[wrow + 16 * i + row];
+            if constexpr (TILES) t.s.m[i] *= sb[0];
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            t.b[j] = read_codes16(at + S::CODES, wcol + 16 * j + row, g);
+            if constexpr (!TILES) t.s.n[j] = *reinterpret_cast<const f32x4*>(sb + wcol + 16 * j + 4 * g);
+        }
+    };
+    f32x4 acc[MI][NJ], d[DEPTH + 1];
+    auto start = [&]() {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            before.m[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) before.n[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q <= DEPTH; ++q) d[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    // sums q are scaled and added
+    auto add = [&](const Scales& s, int q) {
+        const int i = q / NJ, j = q % NJ;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(d[q & DEPTH][e], TILES ? s.m[i] : s.m[i] * s.n[j][e], acc[i][j][e]);
+        asm volatile("" : "+v"(acc[i][j]));  // here, not later: the sums in flight are few
+    };
+    // multiplies the step in t and reads the next one into t2
+    auto step = [&](const Step& t, Step& t2) {
+        wait_vm<(RING - 2) * S::ND>();
+        lds_barrier();  // the next step is whole in LDS, and this one's slot is read
+        load_step();    // past the last unit: zeros
+        slot = (slot + 1) & (RING - 1);
+        read_step(t2, slot);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            d[q & DEPTH] = mma16<false>(t.b[q % NJ], t.a[q / NJ]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (q < DEPTH) add(before, NQ - DEPTH + q);
+            else add(t.s, q - DEPTH);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        before = t.s;
+    };
+#pragma unroll
+    for (int n = 0; n < RING; ++n) load_step();
+    wait_vm<(RING - 1) * S::ND>();
+    lds_barrier();
+    read_step(f[0], 0);
+    for (;;) {
+        start();
+        int left = (u.kend - u.kbeg + kFp8Block - 1) / kFp8Block;
+        for (; left >= 2; left -= 2) {
+            step(f[0], f[1]);
+            step(f[1], f[0]);
+        }
+        if (left > 0) {
+            step(f[0], f[1]);
+            f[0] = f[1];
+        }
+#pragma unroll
+        for (int q = NQ - DEPTH; q < NQ; ++q) add(before, q);
+        lds_barrier();  // the slot of the step in registers is read: the epilogue stages there
+        const int rows = p.M - u.m0 - wrow, cols = p.N - u.c0 - wcol;
+        if (rows > 0 && cols > 0) {
+            if constexpr (SPLIT) {
+                float* o = p.part + (int64_t)u.part * TILE * TILE + (wrow + row) * TILE + wcol + 4 * g;
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+                        if (16 * i + row < rows && 16 * j + 4 * g < cols) *reinterpret_cast<f32x4*>(o + 16 * i * TILE + 16 * j) = acc[i][j];
+            } else {
+                store_wave16<BETA>(acc, lds + slot * S::BYTES + wave * NJ * 512,
+                                   static_cast<uint16_t*>(p.y) + (int64_t)(u.m0 + wrow) * p.ldy + u.c0 + wcol, p.ldy, rows, cols, p.beta);
+            }
+        }
+        vb += gridDim.x;
+        if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) break;
+    }
+    wait_vm<0>();  // no load may land in LDS that the next workgroup owns
+}
+
+// ---- large products ------------------------------------------------------------------
 // 256 x 256 outputs of 8 waves, a wave 128 x 64; one workgroup, two waves per SIMD.
 // Half the reads from L2 of 128 x 128. The sums have to be vector registers, since
 // the vector unit scales and adds: 128 a wave.
@@ -418,16 +689,10 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
         ld.at.next(p, pl, workgroups);
     };
 
-    // chunks g and g + 4 of row r
-    auto read = [&](const uint8_t* t, int r) {
-        const int sw = (row >> 1) & 7;
-        return join(*reinterpret_cast<const uint4*>(t + r * 128 + ((g ^ sw) * 16)),
-                    *reinterpret_cast<const uint4*>(t + r * 128 + (((g + 4) ^ sw) * 16)));
-    };
     i32x8 a[2], b[NJ];
     float s[MI], next[2];
-    auto read_a = [&](int i, int sl) { a[i & 1] = read(lds + sl * S::BYTES, wrow + 16 * i + row); };
-    auto read_b = [&](int j, int sl) { b[j] = read(lds + sl * S::BYTES + S::CODES, wcol + 16 * j + row); };
+    auto read_a = [&](int i, int sl) { a[i & 1] = read_codes16(lds + sl * S::BYTES, wrow + 16 * i + row, g); };
+    auto read_b = [&](int j, int sl) { b[j] = read_codes16(lds + sl * S::BYTES + S::CODES, wcol + 16 * j + row, g); };
     // the next step's scales, while the last two rows' are still in use
     auto read_scales = [&](int sl) {
         const uint8_t* t = lds + sl * S::BYTES;
@@ -515,29 +780,84 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
     wait_vm<0>();  // no load may land in LDS that the next workgroup owns
 }
 
-template <bool TILES, bool F32>
-void launch_rows(const Fp8Params& p, hipStream_t s) {
-    const int64_t grid = (int64_t)((p.N + 31) / 32) * ((p.M + 31) / 32);
-    fp8_rows_kernel<TILES, F32, 2, 2, 4><<<(unsigned)grid, 256, 0, s>>>(p);
+template <bool TILES, bool F32, int RB, int NB, int NW, int U>
+void launch_rows_as(const Fp8Params& p, hipStream_t s) {
+    const int64_t grid = (int64_t)((p.N + 16 * NB - 1) / (16 * NB)) * ((p.M + 16 * RB - 1) / (16 * RB));
+    fp8_rows_kernel<TILES, F32, RB, NB, NW, U><<<(unsigned)grid, 64 * NW, 0, s>>>(p);
+}
+// y = beta y, where the reduction is empty: 16 bytes a thread, by strides.
+template <bool F32>
+__global__ __launch_bounds__(256) void fp8_scale_kernel(Fp8Params p) {
+    constexpr int PER = F32 ? 4 : 8;
+    const int pieces = p.N / PER;
+    const int64_t all = (int64_t)p.M * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int64_t at = i / pieces * p.ldy + i % pieces * PER;
+        if constexpr (F32) {
+            f32x4* y = reinterpret_cast<f32x4*>(static_cast<float*>(p.y) + at);
+            *y = p.beta != 0.0f ? p.beta * *y : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        } else {
+            uint4* y = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) + at);
+            float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.beta != 0.0f) {
+                unpack8(*y, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= p.beta;
+            }
+            *y = pack8(v);
+        }
+    }
 }
 
+// Blocks of outputs are the largest of which there are enough for 3/4 of the CUs,
+// and 16 x 16 otherwise: a larger block reads its operands less often, but a CU
+// without one is idle. us with 16 x 16 / 16 x 32 (columns) / 32 x 32 / 64 x 64:
+// M 1, N 4096, K 1024 3.0 / 3.7 / 4.0 / 7.6; M 64, N 1024, K 4096 6.1 / 8.0 / 9.8 /
+// 19.0; M 128, N 1024, K 4096 10.0 / 7.8 / 10.1 / 19.2; M 128, N 4096, K 1024 9.8 / 8.1
+// / 6.6 / 8.8; M 256, N 4096, K 1024 17.5 / 13.6 / 10.7 / 9.4. Eight waves, one block of
+// 128 in flight each: with two or four the times are the same.
+template <bool TILES, bool F32, int RB, int NB>
+void launch_rows_as(const Fp8Params& p, hipStream_t s) {
+    const int64_t grid = (int64_t)((p.N + 16 * NB - 1) / (16 * NB)) * ((p.M + 16 * RB - 1) / (16 * RB));
+    fp8_rows_kernel<TILES, F32, RB, NB, 8><<<(unsigned)grid, 512, 0, s>>>(p);
+}
 template <bool TILES, bool F32>
+void launch_rows(const Fp8Params& p, int cus, hipStream_t s) {
+    switch (fp8_rows_block(p.M, p.N, cus)) {
+        case 64: launch_rows_as<TILES, F32, 4, 4>(p, s); break;
+        case 32: launch_rows_as<TILES, F32, 2, 2>(p, s); break;
+        case 24: launch_rows_as<TILES, F32, 1, 2>(p, s); break;
+        default: launch_rows_as<TILES, F32, 1, 1>(p, s); break;
+    }
+}
+
+template <int TILE, bool TILES, bool F32, bool SPLIT, bool BETA>
+void launch_units(const Fp8Params& p, const LinearPlan& pl, int units, int cus, hipStream_t s) {
+    const int grid = fp8_grid(TILE, F32, units, cus);
+    if constexpr (F32 && TILE == 128) {
+        if (units > cus) {
+            fp8_wide_kernel<TILES, SPLIT, BETA><<<grid, 256, 0, s>>>(p, pl);
+            return;
+        }
+    }
+    if constexpr (F32 || TILE == 64) fp8_quarter_kernel<TILE, TILES, F32, SPLIT, BETA><<<grid, 256, 0, s>>>(p, pl);
+    else fp8_deep_kernel<TILES, SPLIT, BETA><<<grid, 512, 0, s>>>(p, pl);
+}
+template <int TILE, bool TILES, bool F32>
 void launch_tiles(const Fp8Params& p, const LinearPlan& pl, int cus, hipStream_t s) {
-    const auto grid = [&](int units) { return unit_grid(128, units, cus); };
     if (pl.whole > 0) {
-        if (p.beta == 0.0f) fp8_tile_kernel<TILES, F32, false, false><<<grid(pl.whole), 256, 0, s>>>(p, pl);
-        else fp8_tile_kernel<TILES, F32, false, true><<<grid(pl.whole), 256, 0, s>>>(p, pl);
+        if (p.beta == 0.0f) launch_units<TILE, TILES, F32, false, false>(p, pl, pl.whole, cus, s);
+        else launch_units<TILE, TILES, F32, false, true>(p, pl, pl.whole, cus, s);
     }
     if (pl.tail > 0) {
-        fp8_tile_kernel<TILES, F32, true, false><<<grid(pl.tail * pl.parts), 256, 0, s>>>(p, pl);  // the sums add what is there
-        constexpr int SLABS = 128 / (256 / (128 / 4));
-        linear_fixup_kernel<128, F32><<<pl.tail * SLABS, 256, 0, s>>>(p, pl, p.M, p.N);
+        launch_units<TILE, TILES, F32, true, false>(p, pl, pl.tail * pl.parts, cus, s);  // the sums add what is there
+        constexpr int SLABS = TILE / (256 / (TILE / 4));
+        linear_fixup_kernel<TILE, F32><<<pl.tail * SLABS, 256, 0, s>>>(p, pl, p.M, p.N);
     }
 }
 
-void launch_large(const Fp8Params& p, int cus, hipStream_t s) {
-    const LinearPlan pl = fp8_tiles(p.M, p.N, p.K, 256, 1, cus);
-    const int grid = unit_grid(256, pl.whole, cus);
+void launch_large(const Fp8Params& p, const LinearPlan& pl, int cus, hipStream_t s) {
+    const int grid = fp8_grid(256, false, pl.whole, cus);
     const bool full = p.K % kFp8Block == 0;
     if (p.beta == 0.0f) full ? fp8_large_kernel<true, false><<<grid, 512, 0, s>>>(p, pl) : fp8_large_kernel<false, false><<<grid, 512, 0, s>>>(p, pl);
     else full ? fp8_large_kernel<true, true><<<grid, 512, 0, s>>>(p, pl) : fp8_large_kernel<false, true><<<grid, 512, 0, s>>>(p, pl);
@@ -546,15 +866,21 @@ void launch_large(const Fp8Params& p, int cus, hipStream_t s) {
 template <bool TILES, bool F32>
 void launch(const Fp8Params& p, hipStream_t s) {
     const int cus = cu_count();
-    const Fp8Plan pl = fp8_plan(F32, p.M, p.N, p.K, cus);
-    if (pl.rows) launch_rows<TILES, F32>(p, s);
-    else if (TILES && !F32 && fp8_large(p.M, p.N, p.K, cus)) launch_large(p, cus, s);
-    else launch_tiles<TILES, F32>(p, pl.tiles, cus, s);
+    if (p.K == 0) {
+        const int64_t blocks = std::min<int64_t>(((int64_t)p.M * (p.N / 4) + 255) / 256, 16 * (int64_t)cus);
+        fp8_scale_kernel<F32><<<(unsigned)blocks, 256, 0, s>>>(p);
+        return;
+    }
+    const Fp8Plan pl = fp8_plan(TILES, F32, p.M, p.N, p.K, cus);
+    if (pl.kernel == FP8_ROWS_KERNEL) launch_rows<TILES, F32>(p, cus, s);
+    else if (pl.kernel == FP8_LARGE_KERNEL) launch_large(p, pl.tiles, cus, s);
+    else if (pl.tiles.tile == 64) launch_tiles<64, TILES, F32>(p, pl.tiles, cus, s);
+    else launch_tiles<128, TILES, F32>(p, pl.tiles, cus, s);
 }
 
 }  // namespace
 
-size_t fp8_workspace(bool tiles, int M, int N, int K) { return fp8_workspace_bound(M, N, K, cu_count()); }
+size_t fp8_workspace(int M, int N, int K) { return fp8_workspace_bound(M, N, K, cu_count()); }
 
 hipError_t launch_fp8_matmul(bool tiles, bool f32, const Fp8Params& p, hipStream_t s) {
     if (tiles) f32 ? launch<true, true>(p, s) : launch<true, false>(p, s);

@@ -53,14 +53,26 @@ struct Fp8Cursor {
 };
 
 // ---- plan ----------------------------------------------------------------------
+// The kernel for few rows, 64 x 64 or 128 x 128 tiles (whole, or the last round's cut
+// along the reduction), or 256 x 256 tiles: the one with the shortest estimate.
+enum Fp8Kernel { FP8_ROWS_KERNEL, FP8_TILES_KERNEL, FP8_LARGE_KERNEL };
 struct Fp8Plan {
-    bool rows = false;  // the kernel for few rows
+    Fp8Kernel kernel = FP8_ROWS_KERNEL;
     LinearPlan tiles;
 };
+constexpr int kFp8FewRows = 64;  // up to these the kernel for few rows, which needs no workspace
 constexpr int kFp8MinSteps = 4;  // blocks of 128 that a part of a split reduction has at least
 
-// Tiles of 128 x 128 whole, the rest (fewer tiles than run at a time) in `parts`.
-inline LinearPlan fp8_tiles(int M, int N, int K, int tile, int parts, int cus) {
+inline int fp8_steps(int K) { return (int)(((int64_t)K + kFp8Block - 1) / kFp8Block); }
+inline int64_t fp8_count(int M, int N, int m, int n) { return (((int64_t)M + m - 1) / m) * (((int64_t)N + n - 1) / n); }
+// Workgroups of a tile size that run at a time: 128 x 128 tiles of bf16 results and
+// 256 x 256 tiles fill a CU.
+inline int fp8_slots(int tile, bool f32, int cus) { return tile == 256 || (tile == 128 && !f32) ? cus : 2 * cus; }
+// Workgroups of a launch of `units`, a multiple of 8: one for each XCD.
+inline int fp8_grid(int tile, bool f32, int units, int cus) { return std::min((units + 7) & ~7, fp8_slots(tile, f32, cus) & ~7); }
+
+// Tiles whole or, parts >= 2, the rest of the last round's in parts.
+inline LinearPlan fp8_tiles(bool f32, int M, int N, int K, int tile, int parts, int cus) {
     LinearPlan pl;
     pl.tile = tile;
     pl.tiles_m = (M + tile - 1) / tile;
@@ -68,33 +80,93 @@ inline LinearPlan fp8_tiles(int M, int N, int K, int tile, int parts, int cus) {
     const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_c;
     pl.whole = (int)tiles;
     if (parts >= 2) {
-        const int steps = (K + kFp8Block - 1) / kFp8Block;
-        pl.whole = (int)(tiles / tile_slots(tile, cus) * tile_slots(tile, cus));
+        const int steps = fp8_steps(K), slots = fp8_slots(tile, f32, cus);
+        pl.whole = (int)(tiles / slots * slots);
         pl.tail = (int)(tiles - pl.whole);
         pl.chunk = (steps + parts - 1) / parts * kFp8Block;
-        pl.parts = (K + pl.chunk - 1) / pl.chunk;
+        pl.parts = (int)(((int64_t)K + pl.chunk - 1) / pl.chunk);
     }
     return pl;
 }
-inline Fp8Plan fp8_plan(bool f32, int M, int N, int K, int cus) {
-    Fp8Plan pl;
-    pl.rows = M <= 64 || K == 0;
-    if (pl.rows) return pl;
-    const int64_t tiles = (int64_t)((M + 127) / 128) * ((N + 127) / 128), slots = tile_slots(128, cus), rest = tiles % slots;
-    const int64_t most = rest > 0 ? std::min<int64_t>(slots / rest, (K + kFp8Block - 1) / kFp8Block / kFp8MinSteps) : 1;
-    pl.tiles = fp8_tiles(M, N, K, 128, (int)std::max<int64_t>(most, 1), cus);
-    return pl;
+
+// Outputs of a workgroup of the kernel for few rows: 64 x 64, 32 x 32, 16 x 32 (24)
+// or 16 x 16.
+inline int fp8_rows_block(int M, int N, int cus) {
+    const int64_t enough = 3 * (int64_t)cus / 4;
+    return fp8_count(M, N, 64, 64) >= enough ? 64 : fp8_count(M, N, 32, 32) >= enough ? 32 : fp8_count(M, N, 16, 32) >= enough ? 24 : 16;
 }
-inline bool fp8_large(int M, int N, int K, int cus) {
-    const int64_t big = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
-    return big >= tile_slots(256, cus);
+// us, measured on one MI355X over M 1 .. 2048, N and K 256 .. 4096: a CU takes 33 ns
+// for a KiB of operand rows, and blocks of 64 x 64 run one to a CU and take 2 us more.
+inline double fp8_rows_time(int M, int N, int K, int cus) {
+    const int b = fp8_rows_block(M, N, cus), m = b == 24 ? 16 : b, n = b == 24 ? 32 : b;
+    const double kib = (m + n) * (double)K / 1024, groups = (double)fp8_count(M, N, m, n) / cus;
+    return 2.5 + (b == 64 ? std::ceil(groups) * (0.033 * kib + 2.0) : std::max(1.0, groups) * 0.033 * kib);
 }
-// An upper bound over all row counts up to M: partial tiles fill at most the
-// workgroup slots, and neither tiles nor parts fall with M.
+// us of tiles: start of a launch, a step with one workgroup per CU and with two.
+struct Fp8Times {
+    double start, one, two;
+};
+constexpr Fp8Times kFp8Times[2][2] = {{{3.4, 0.36, 0.53}, {4.2, 0.66, 0.66}},   // bf16 results: 64, 128
+                                      {{3.2, 0.53, 0.87}, {4.2, 1.32, 2.35}}};  // fp32
+inline double fp8_launch_time(const Fp8Times& t, int64_t units, int slots, double steps, int cus) {
+    if (units == 0) return 0.0;
+    const int64_t rounds = units / slots, rest = units % slots;
+    return t.start + rounds * (steps * t.two + 0.5) + (rest == 0 ? 0.0 : steps * (rest <= cus ? t.one : t.two) + 0.5);
+}
+// A split reduction adds a launch for the sums and its partial tiles' way through the
+// last-level cache and back.
+inline double fp8_tiles_time(bool f32, const LinearPlan& pl, int K, int cus) {
+    const Fp8Times& t = kFp8Times[f32][pl.tile == 128];
+    const int slots = fp8_slots(pl.tile, f32, cus);
+    double us = fp8_launch_time(t, pl.whole, slots, fp8_steps(K), cus);
+    if (pl.tail > 0) {
+        const double mib = (double)pl.tail * pl.parts * pl.tile * pl.tile * 4 / (1 << 20);
+        us += fp8_launch_time(t, (int64_t)pl.tail * pl.parts, slots, pl.chunk / kFp8Block, cus) + 2.2 + 0.35 * mib;
+    }
+    return us;
+}
+inline double fp8_large_time(int M, int N, int K, int cus) {
+    const double tiles = (double)fp8_count(M, N, 256, 256), fill = std::min(1.0, tiles / cus);
+    return 6.0 + std::ceil(tiles / cus) * (fp8_steps(K) * (1.25 + 0.35 * fill) + 3.0);
+}
+
+// Measured (us, chosen / others): M 128, N 1024, K 4096 8.3 in the kernel for few rows
+// / 10.2 on 64 x 64 tiles in four parts; M 777, N 1024, K 1024 6.3 on 64 x 64 / 8.9
+// few rows, 9.3 on 128 x 128; M 777, N 1024, K 4096 15.3 on 64 x 64 / 17.4 on 128 x 128
+// in four parts; M 777, N 4096, K 1024 10.4 on 128 x 128 / 13.2 on 64 x 64; M = N = 4096,
+// K 1024 22.5 on 256 x 256 / 31.4 on 128 x 128. fp32: T 2048, N = K = 1280 17.6 on 64 x
+// 64 / 22.3 on 128 x 128 in four parts; T 32768, N = K = 1024 90.6 on 128 x 128 in
+// eight parts / 113 on 64 x 64 in two; T 16384, N = K = 256 14.9 on 64 x 64 in eight
+// parts / 18.1 few rows.
+inline Fp8Plan fp8_plan(bool tiles, bool f32, int M, int N, int K, int cus) {
+    Fp8Plan best;
+    if (M <= kFp8FewRows) return best;
+    // a launch holds 2^32 threads
+    double us = fp8_count(M, N, 16, 16) < (1 << 22) ? fp8_rows_time(M, N, K, cus) : 1e30;
+    if (tiles && !f32) {
+        const double t = fp8_large_time(M, N, K, cus);
+        if (t < us) us = t, best = {FP8_LARGE_KERNEL, fp8_tiles(f32, M, N, K, 256, 1, cus)};
+    }
+    for (int tile = 64; tile <= 128; tile *= 2) {
+        const int64_t slots = fp8_slots(tile, f32, cus), rest = fp8_count(M, N, tile, tile) % slots;
+        const int64_t most = rest > 0 ? std::min<int64_t>(slots / rest, fp8_steps(K) / kFp8MinSteps) : 1;
+        for (int64_t parts = 1; parts <= std::max<int64_t>(most, 1); parts += parts < 8 ? 1 : parts / 4) {
+            const LinearPlan pl = fp8_tiles(f32, M, N, K, tile, (int)parts, cus);
+            const double t = fp8_tiles_time(f32, pl, K, cus);
+            if (t < us) us = t, best = {FP8_TILES_KERNEL, pl};
+        }
+    }
+    return best;
+}
+// An upper bound over both result types and all row counts up to M: partial tiles
+// fill at most the workgroup slots, and neither tiles nor parts fall with M.
 inline size_t fp8_workspace_bound(int M, int N, int K, int cus) {
-    const int64_t tiles = (int64_t)((M + 127) / 128) * ((N + 127) / 128), parts = (K + kFp8Block - 1) / kFp8Block / kFp8MinSteps;
-    if (M <= 64 || parts < 2) return 0;
-    return (size_t)std::min(tiles * parts, tile_slots(128, cus)) * 128 * 128 * 4;
+    const int64_t parts = fp8_steps(K) / kFp8MinSteps;
+    if (M <= kFp8FewRows || parts < 2) return 0;
+    size_t most = 0;
+    for (int tile = 64; tile <= 128; tile *= 2)
+        most = std::max(most, (size_t)std::min<int64_t>(fp8_count(M, N, tile, tile) * parts, fp8_slots(tile, true, cus)) * tile * tile * 4);
+    return most;
 }
 
 }  // namespace

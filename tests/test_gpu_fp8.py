@@ -175,13 +175,39 @@ def _launched(M, N, K, tiles, dtype):
     return launched_kernels(lambda: tmt_moe.fp8_matmul(*args, blocks=TILES if tiles else ROWS, workspace=ws))
 
 
-@pytest.mark.parametrize("M,N,K", [(4096, 4096, 128), (4000, 4200, 200), (4090, 4104, 1000), (8200, 4096, 256), (33000, 512, 400)])
-def test_large_products(M, N, K):
-    """256 x 256 tiles: whole and ragged, several to a workgroup, a short last block, added to."""
-    assert any("fp8_large" in k for k in _launched(M, N, K, True, BF16))
-    _product(M, N, K, True, BF16)
-    _product(M, N, K, True, BF16, beta=0.5, ldy=N + 40)
-    _product(M, N, K, True, BF16, exact=False)
+# Sizes that reach every kernel, whole and split, a part of a round and several, with the
+# (mangled) names that must be launched: template numbers are L<type><value>E.
+ROW = "fp8_rows_kernelILb%dELb%dELi%dELi%dE"
+KERNELS = [
+    (5, 40, 300, True, BF16, [ROW % (1, 0, 1, 1)]), (64, 2048, 140, True, BF16, [ROW % (1, 0, 1, 2)]),
+    (64, 4096, 130, False, BF16, [ROW % (0, 0, 2, 2)]), (63, 12288, 129, True, BF16, [ROW % (1, 0, 4, 4)]),
+    (30, 64, 1000, False, F32, [ROW % (0, 1, 1, 1)]), (64, 4096, 200, True, F32, [ROW % (1, 1, 2, 2)]),
+    (700, 1032, 2064, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb0E"]), (1000, 2048, 1000, False, BF16, ["fp8_quarter_kernelILi64ELb0ELb0ELb0E"]),
+    (777, 256, 4096, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb1E", "linear_fixup_kernelILi64ELb0E"]),
+    (1500, 2048, 400, True, BF16, ["fp8_deep_kernelILb1ELb0E"]), (1100, 4000, 700, False, BF16, ["fp8_deep_kernelILb0ELb0E"]),
+    (500, 1000, 20000, True, BF16, ["fp8_deep_kernelILb1ELb1E", "linear_fixup_kernelILi128ELb0E"]),
+    (2304, 1896, 6451, False, BF16, ["fp8_deep_kernelILb0ELb0E", "fp8_deep_kernelILb0ELb1E", "linear_fixup_kernelILi128ELb0E"]),
+    (4096, 4096, 640, True, BF16, ["fp8_large_kernelILb1E"]), (4090, 4096, 1100, True, BF16, ["fp8_large_kernelILb0E"]),
+    (8190, 4088, 700, True, BF16, ["fp8_large_kernelILb0E"]), (8200, 4096, 768, True, BF16, ["fp8_large_kernelILb1E"]),
+    (32700, 504, 1300, True, BF16, ["fp8_large_kernelILb0E"]),
+    (1100, 4000, 700, False, F32, ["fp8_quarter_kernelILi64ELb0ELb1ELb0E"]),
+    (300, 264, 9000, True, F32, ["fp8_quarter_kernelILi64ELb1ELb1ELb1E", "linear_fixup_kernelILi64ELb1E"]),
+    (2304, 1896, 6451, False, F32, ["fp8_quarter_kernelILi64ELb0ELb1ELb0E", "fp8_quarter_kernelILi64ELb0ELb1ELb1E", "linear_fixup_kernelILi64ELb1E"]),
+    (2048, 2048, 1000, False, F32, ["fp8_quarter_kernelILi128ELb0ELb1ELb0E"]),
+    (1000, 1000, 16000, False, F32, ["fp8_quarter_kernelILi128ELb0ELb1ELb1E", "linear_fixup_kernelILi128ELb1E"]),
+    (1100, 1304, 9000, True, F32, ["fp8_wide_kernelILb1ELb1E", "linear_fixup_kernelILi128ELb1E"]),
+    (4096, 4200, 1100, False, F32, ["fp8_wide_kernelILb0ELb0E"]),
+]
+
+
+@pytest.mark.parametrize("M,N,K,tiles,dtype,names", KERNELS)
+def test_every_kernel(M, N, K, tiles, dtype, names):
+    """To the bit, stored and added to, with room behind the rows; then random values."""
+    launched = _launched(M, N, K, tiles, dtype)
+    assert len(launched) == len(names) and all(any(n in k for k in launched) for n in names), launched
+    _product(M, N, K, tiles, dtype)
+    _product(M, N, K, tiles, dtype, beta=0.5, ldy=N + 40)
+    _product(M, N, K, tiles, dtype, exact=False)
 
 
 @pytest.mark.parametrize("tiles", [True, False])
