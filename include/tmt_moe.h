@@ -539,7 +539,7 @@ int tmt_moe_rmsnorm_backward(void* stream, int32_t T, int32_t d, int32_t dtype, 
  * X [rows][ldx] (bf16 or fp32, `dtype`) to codes and scales and, in the same
  * pass, X^T [K][rows] to codes_t [K][ldct] and scales_t. Either side may be NULL.
  * In rows, the blocks of the two sides differ (128 values of a row, of a column);
- * in tiles they are the same. rows and K any, fewer than 2^24 tiles of 128 x 128.
+ * in tiles they are the same. rows and K any, fewer than 2^23 tiles of 128 x 128.
  */
 int tmt_moe_fp8_quantize(void* stream, int32_t blocks, int32_t dtype, const void* X, int64_t ldx, int32_t rows,
                          int32_t K, uint8_t* codes, int64_t ldc, float* scales, int64_t lds, uint8_t* codes_t,

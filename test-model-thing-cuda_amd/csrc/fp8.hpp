@@ -38,9 +38,8 @@ struct RmsParams {
     float* dgamma;        // [d]
     float* partial;       // workspace: [rms_partials][d rounded up to 4]
 };
-// Workgroups of the backward, each of which leaves one row of partial dgamma.
-int rms_partials(int T, int d, int cus);
-int rms_partials_max(int d, int cus);  // of any T
+// The most workgroups of the backward, each of which leaves one row of partial dgamma.
+int rms_partials_max(int d, int cus);
 // Arguments as the C ABI has checked them, T > 0.
 hipError_t launch_rms_fwd(const RmsParams& p, hipStream_t s);
 hipError_t launch_rms_bwd(const RmsParams& p, hipStream_t s);

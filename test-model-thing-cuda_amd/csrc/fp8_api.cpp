@@ -15,7 +15,7 @@ namespace {
 constexpr int32_t kMaxRows = 1 << 30;
 constexpr int64_t kMaxScales = int64_t(1) << 31;   // stride of scales
 constexpr int64_t kMaxOutputs = int64_t(1) << 40;  // of a product, so that 32 bits count the tiles
-constexpr int64_t kMaxGrid = int64_t(1) << 24;     // workgroups: a launch holds less than 2^32 threads
+constexpr int64_t kMaxGrid = int64_t(1) << 23;     // workgroups of 512: a launch holds less than 2^32 threads
 
 int64_t blocks_of(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 
@@ -142,7 +142,7 @@ int tmt_moe_fp8_quantize(void* stream, int32_t blocks, int32_t dtype, const void
     if (!codes && !codes_t) return fail(TMT_MOE_EINVAL, "codes and codes_t are both NULL");
     const bool tiles = blocks == TMT_MOE_FP8_TILES;
     if (blocks_of(rows) * blocks_of(K) >= kMaxGrid)
-        return fail(TMT_MOE_EINVAL, "rows=%d of K=%d are 2^24 tiles of 128 x 128 or more", rows, K);
+        return fail(TMT_MOE_EINVAL, "rows=%d of K=%d are 2^23 tiles of 128 x 128 or more", rows, K);
     if ((rc = check_rows("X", X, ldx, K, dtype == TMT_MOE_BF16 ? 8 : 4))) return rc;
     if (codes && ((rc = check_rows("codes", codes, ldc, K, 16)) ||
                   (rc = check_scales("scales", scales, lds, tiles ? blocks_of(K) : rows))))

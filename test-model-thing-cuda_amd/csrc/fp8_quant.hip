@@ -20,6 +20,9 @@ namespace tmt {
 namespace {
 
 constexpr int kTile = kFp8Block;
+// 512 threads of 4 pieces, whose loads are all in flight at once (32768 x 4096 bf16, rows
+// both ways: 117 us; 256 threads of 8 127).
+constexpr int kThreads8 = 512;
 
 // Pieces of 8 columns a thread: of rows 4 (t / 16) .. + 3 of each 64.
 template <int THREADS>
@@ -29,8 +32,9 @@ struct Quant {
     static constexpr int WAVES = THREADS / 64;
 };
 
-template <bool TILES, bool F32, int THREADS>
-__global__ __launch_bounds__(THREADS) void fp8_quantize_kernel(Fp8QuantParams p, int tiles_k) {
+template <bool TILES, bool F32, bool NT>
+__global__ __launch_bounds__(kThreads8) void fp8_quantize_kernel(Fp8QuantParams p, int tiles_k) {
+    constexpr int THREADS = kThreads8;
     using Q = Quant<THREADS>;
     __shared__ uint32_t most[Q::WAVES][kTile];        // largest magnitudes: a wave's columns, or [wave][0]
     __shared__ float row_scale[kTile];
@@ -45,8 +49,11 @@ __global__ __launch_bounds__(THREADS) void fp8_quantize_kernel(Fp8QuantParams p,
 #pragma unroll
     for (int i = 0; i < Q::P; ++i) {
         const int row = row_of(i);
-        if (row < rows && 8 * a + 8 <= cols) {
-            const int64_t at = (r0 + row) * p.ldx + c0 + 8 * a;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        if (row >= rows || 8 * a >= cols) continue;
+        const int64_t at = (r0 + row) * p.ldx + c0 + 8 * a;
+        if (8 * a + 8 <= cols) {
             if constexpr (F32) {
                 const f32x4* x = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.x) + at);
                 const f32x4 lo = x[0], hi = x[1];
@@ -57,12 +64,8 @@ __global__ __launch_bounds__(THREADS) void fp8_quantize_kernel(Fp8QuantParams p,
             }
         } else {  // a row's last columns, one by one
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t at = (r0 + row) * p.ldx + c0 + 8 * a + j;
-                v[i][j] = 0.0f;
-                if (row < rows && 8 * a + j < cols)
-                    v[i][j] = F32 ? static_cast<const float*>(p.x)[at] : bf1(static_cast<const uint16_t*>(p.x)[at]);
-            }
+            for (int j = 0; j < 8; ++j)
+                if (8 * a + j < cols) v[i][j] = F32 ? static_cast<const float*>(p.x)[at + j] : bf1(static_cast<const uint16_t*>(p.x)[at + j]);
         }
     }
 
@@ -124,8 +127,7 @@ __global__ __launch_bounds__(THREADS) void fp8_quantize_kernel(Fp8QuantParams p,
                 if (a == 0) row_scale[row] = q.scale;
             }
             if (row < rows && 8 * a < width)
-                *reinterpret_cast<uint2*>(p.codes + (r0 + row) * p.ldc + c0 + 8 * a) =
-                    make_uint2(fp8_codes(v[i], q.inv), fp8_codes(v[i] + 4, q.inv));
+                put<NT>(p.codes + (r0 + row) * p.ldc + c0 + 8 * a, u32x2_t{fp8_codes(v[i], q.inv), fp8_codes(v[i] + 4, q.inv)});
         }
     }
 
@@ -161,8 +163,8 @@ __global__ __launch_bounds__(THREADS) void fp8_quantize_kernel(Fp8QuantParams p,
         for (int i = 0; i < kTile * 8 / THREADS; ++i) {
             const int col = i * (THREADS / 8) + tid / 8, chunk = tid & 7;
             if (col < cols && 16 * chunk < height)
-                *reinterpret_cast<uint4*>(p.codes_t + (int64_t)(c0 + col) * p.ldct + r0 + 16 * chunk) =
-                    *reinterpret_cast<const uint4*>(ct + col * kTile + ((chunk ^ ((col >> 3) & 7)) * 16));
+                put<NT>(p.codes_t + (int64_t)(c0 + col) * p.ldct + r0 + 16 * chunk,
+                        *reinterpret_cast<const u32x4_t*>(ct + col * kTile + ((chunk ^ ((col >> 3) & 7)) * 16)));
         }
     }
 }
@@ -172,11 +174,15 @@ __global__ __launch_bounds__(THREADS) void fp8_quantize_kernel(Fp8QuantParams p,
 hipError_t launch_fp8_quantize(bool tiles, bool f32, const Fp8QuantParams& p, hipStream_t s) {
     const int tiles_k = (p.K + kTile - 1) / kTile;
     const unsigned grid = (unsigned)((((int64_t)p.rows + kTile - 1) / kTile) * tiles_k);
-    constexpr int THREADS = 256;
-    if (tiles) f32 ? fp8_quantize_kernel<true, true, THREADS><<<grid, THREADS, 0, s>>>(p, tiles_k)
-                   : fp8_quantize_kernel<true, false, THREADS><<<grid, THREADS, 0, s>>>(p, tiles_k);
-    else f32 ? fp8_quantize_kernel<false, true, THREADS><<<grid, THREADS, 0, s>>>(p, tiles_k)
-             : fp8_quantize_kernel<false, false, THREADS><<<grid, THREADS, 0, s>>>(p, tiles_k);
+    // Codes larger than the L2s hold together are stored non-temporally: 117 -> 115 us in
+    // the case above, tiles 107 -> 105.
+    const bool nt = (int64_t)p.rows * p.K * ((p.codes ? 1 : 0) + (p.codes_t ? 1 : 0)) > (int64_t)16 << 20;
+#define TMT_Q(TILES_, F32_)                                                                              \
+    (nt ? fp8_quantize_kernel<TILES_, F32_, true><<<grid, kThreads8, 0, s>>>(p, tiles_k)                 \
+        : fp8_quantize_kernel<TILES_, F32_, false><<<grid, kThreads8, 0, s>>>(p, tiles_k))
+    if (tiles) f32 ? TMT_Q(true, true) : TMT_Q(true, false);
+    else f32 ? TMT_Q(false, true) : TMT_Q(false, false);
+#undef TMT_Q
     return hipGetLastError();
 }
 

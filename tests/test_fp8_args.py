@@ -77,7 +77,7 @@ def _quantize(q):
     (dict(codes=U), "codes"), (dict(ldc=240), "codes"), (dict(ldc=264), "codes"), (dict(scales=0), "scales"), (dict(lds=31), "scales"),
     (dict(codes_t=U), "codes_t"), (dict(ldct=16), "codes_t"), (dict(ldct=40), "codes_t"), (dict(scales_t=0), "scales_t"),
     (dict(ldst=255), "scales_t"), (dict(blocks=1, lds=1), "scales"), (dict(blocks=1, ldst=0), "scales_t"), (dict(scales=V), "scales"),
-    (dict(rows=1 << 30, K=1 << 9, ldx=1 << 9), "2^24"), (dict(rows=1 << 23, lds=1 << 23, ldct=1 << 23), "over"),
+    (dict(rows=1 << 30, K=1 << 9, ldx=1 << 9), "2^23"), (dict(rows=1 << 23, lds=1 << 23, ldct=1 << 23), "over"),
 ])
 def test_quantize_refusals(change, text):
     refused(_quantize(dict(QUANT, **change)), text)
