@@ -22,11 +22,18 @@ __device__ __forceinline__ Fp8Scale fp8_scale(uint32_t amax) {
     return {bad ? __uint_as_float(0x7fc00000u) : m / 448.0f, bad ? 0.0f : 448.0f / m};
 }
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-// A store that is written once and read by a later kernel (NT), or a plain one.
-template <bool NT, class T>
+// How a kernel passes memory: kCached; kStoreOnce, whose stores are non-temporal; or
+// kOnce, whose loads of its large inputs are as well.
+enum { kCached, kStoreOnce, kOnce };
+template <int PASS, class T>
 __device__ __forceinline__ void put(void* p, T v) {
-    if constexpr (NT) __builtin_nontemporal_store(v, static_cast<T*>(p));
+    if constexpr (PASS != kCached) __builtin_nontemporal_store(v, static_cast<T*>(p));
     else *static_cast<T*>(p) = v;
+}
+template <int PASS, class T>
+__device__ __forceinline__ T get(const void* p) {
+    if constexpr (PASS == kOnce) return __builtin_nontemporal_load(static_cast<const T*>(p));
+    else return *static_cast<const T*>(p);
 }
 // Codes of four values, one a byte.
 __device__ __forceinline__ uint32_t fp8_codes(const float* v, float inv) {

@@ -32,7 +32,7 @@ struct Quant {
     static constexpr int WAVES = THREADS / 64;
 };
 
-template <bool TILES, bool F32, bool NT>
+template <bool TILES, bool F32, int PASS>
 __global__ __launch_bounds__(kThreads8) void fp8_quantize_kernel(Fp8QuantParams p, int tiles_k) {
     constexpr int THREADS = kThreads8;
     using Q = Quant<THREADS>;
@@ -55,12 +55,12 @@ __global__ __launch_bounds__(kThreads8) void fp8_quantize_kernel(Fp8QuantParams 
         const int64_t at = (r0 + row) * p.ldx + c0 + 8 * a;
         if (8 * a + 8 <= cols) {
             if constexpr (F32) {
-                const f32x4* x = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.x) + at);
-                const f32x4 lo = x[0], hi = x[1];
+                const float* x = static_cast<const float*>(p.x) + at;
+                const f32x4 lo = get<PASS, f32x4>(x), hi = get<PASS, f32x4>(x + 4);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[i][j] = lo[j], v[i][j + 4] = hi[j];
             } else {
-                unpack8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + at), v[i]);
+                unpack8(__builtin_bit_cast(uint4, get<PASS, u32x4_t>(static_cast<const uint16_t*>(p.x) + at)), v[i]);
             }
         } else {  // a row's last columns, one by one
 #pragma unroll
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kThreads8) void fp8_quantize_kernel(Fp8QuantParams 
                 if (a == 0) row_scale[row] = q.scale;
             }
             if (row < rows && 8 * a < width)
-                put<NT>(p.codes + (r0 + row) * p.ldc + c0 + 8 * a, u32x2_t{fp8_codes(v[i], q.inv), fp8_codes(v[i] + 4, q.inv)});
+                put<PASS>(p.codes + (r0 + row) * p.ldc + c0 + 8 * a, u32x2_t{fp8_codes(v[i], q.inv), fp8_codes(v[i] + 4, q.inv)});
         }
     }
 
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(kThreads8) void fp8_quantize_kernel(Fp8QuantParams 
         for (int i = 0; i < kTile * 8 / THREADS; ++i) {
             const int col = i * (THREADS / 8) + tid / 8, chunk = tid & 7;
             if (col < cols && 16 * chunk < height)
-                put<NT>(p.codes_t + (int64_t)(c0 + col) * p.ldct + r0 + 16 * chunk,
+                put<PASS>(p.codes_t + (int64_t)(c0 + col) * p.ldct + r0 + 16 * chunk,
                         *reinterpret_cast<const u32x4_t*>(ct + col * kTile + ((chunk ^ ((col >> 3) & 7)) * 16)));
         }
     }
@@ -178,8 +178,8 @@ hipError_t launch_fp8_quantize(bool tiles, bool f32, const Fp8QuantParams& p, hi
     // the case above, tiles 107 -> 105.
     const bool nt = (int64_t)p.rows * p.K * ((p.codes ? 1 : 0) + (p.codes_t ? 1 : 0)) > (int64_t)16 << 20;
 #define TMT_Q(TILES_, F32_)                                                                              \
-    (nt ? fp8_quantize_kernel<TILES_, F32_, true><<<grid, kThreads8, 0, s>>>(p, tiles_k)                 \
-        : fp8_quantize_kernel<TILES_, F32_, false><<<grid, kThreads8, 0, s>>>(p, tiles_k))
+    (nt ? fp8_quantize_kernel<TILES_, F32_, kStoreOnce><<<grid, kThreads8, 0, s>>>(p, tiles_k)                 \
+        : fp8_quantize_kernel<TILES_, F32_, kCached><<<grid, kThreads8, 0, s>>>(p, tiles_k))
     if (tiles) f32 ? TMT_Q(true, true) : TMT_Q(true, false);
     else f32 ? TMT_Q(false, true) : TMT_Q(false, false);
 #undef TMT_Q

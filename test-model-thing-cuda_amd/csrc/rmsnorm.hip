@@ -10,18 +10,21 @@
 // Bound by memory. A row belongs to 16 lanes (d <= 128) or 32 (d <= 256), a wave (d <=
 // 1024), or a workgroup of four waves (d <= 4096) or of sixteen, and is held in
 // registers between its statistics and its outputs, so each value is read once and
-// written once; V = 8 or 16 values a lane in pieces of 16 bytes of the stream (8 bf16 or 4 fp32 values:
-// with 8 fp32 values a wave's store would cover every second 16 bytes). A wave's
-// pieces are consecutive, so 16 (32) neighbouring lanes own a block of 128
-// columns and find its maximum by DPP.
+// written once. A lane has V = 8 or 16 values (4 of the narrowest fp32 rows) in pieces
+// of 16 bytes of the stream: 8 bf16 or 4 fp32 values (with 8 fp32 values a wave's store
+// would cover every second 16 bytes). A row's pieces are consecutive, so 16 (32)
+// neighbouring lanes own a block of 128 columns and find its maximum by DPP. us, and
+// TB/s of what has to pass: forward 32768 x 1024 fp32 to stream and codes 61, 6.0; 16384 x
+// 4096 126, 5.8; 777 x 1280 bf16 4.6; one row 3.4; backward 32768 x 1024 fp32 84, 5.6; 16384 x
+// 4096 bf16 113, 4.8; 5003 x 1000 13.0. A copy of 1 GiB reaches 5.0 TB/s.
 //
 // Sums are in fp32 over the values of a lane, then, for the forward's squares, in
 // 64 bits over the lanes (a butterfly) and the waves (in order): rstd moves a whole
 // row, and with it which way its codes round (32768 x 1024, codes against 64 bits in
-// norm: with the butterfly in fp32 2.2 times as far off as with this). The backward's waves keep dgamma of their columns in
-// registers over the rows that they walk; a workgroup's sums are added in wave
-// order into one row of the workspace, and those rows by launch_colsum: no
-// atomics, the same bits every time.
+// norm: with the butterfly in fp32 2.2 times as far off as with this). The backward's
+// lanes keep dgamma of their columns in registers over the rows that they walk; a
+// workgroup's sums are added in the order of its rows into one row of the workspace, and
+// those rows by launch_colsum: no atomics, the same bits every time.
 #include <algorithm>
 
 #include "fp8.hpp"
@@ -33,12 +36,12 @@ namespace {
 
 // N consecutive elements of a row from k0 on (16-byte aligned where a piece is
 // whole); TAIL: d is not a multiple of N, and elements from d on are zeros.
-template <int N, bool TAIL>
+template <int N, bool TAIL, int PASS>
 __device__ __forceinline__ void load_piece(const float* row, int k0, int d, float* v) {
     if (!TAIL || k0 + N <= d) {
 #pragma unroll
         for (int q = 0; q < N; q += 4) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(row + k0 + q);
+            const f32x4 a = get<PASS, f32x4>(row + k0 + q);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[q + i] = a[i];
         }
@@ -47,36 +50,36 @@ __device__ __forceinline__ void load_piece(const float* row, int k0, int d, floa
         for (int i = 0; i < N; ++i) v[i] = k0 + i < d ? row[k0 + i] : 0.0f;
     }
 }
-template <int N, bool TAIL>
+template <int N, bool TAIL, int PASS>
 __device__ __forceinline__ void load_piece(const uint16_t* row, int k0, int d, float* v) {
     if (!TAIL || k0 + N <= d) {
         if constexpr (N == 8) {
-            unpack8(*reinterpret_cast<const uint4*>(row + k0), v);
+            unpack8(__builtin_bit_cast(uint4, get<PASS, u32x4_t>(row + k0)), v);
         } else {
-            const uint2 a = *reinterpret_cast<const uint2*>(row + k0);
-            v[0] = bf_lo(a.x), v[1] = bf_hi(a.x), v[2] = bf_lo(a.y), v[3] = bf_hi(a.y);
+            const u32x2_t a = get<PASS, u32x2_t>(row + k0);
+            v[0] = bf_lo(a[0]), v[1] = bf_hi(a[0]), v[2] = bf_lo(a[1]), v[3] = bf_hi(a[1]);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = k0 + i < d ? bf1(row[k0 + i]) : 0.0f;
     }
 }
-template <int N, bool TAIL, bool NT>
+template <int N, bool TAIL, int PASS>
 __device__ __forceinline__ void store_piece(float* row, int k0, int d, const float* v) {
     if (!TAIL || k0 + N <= d) {
 #pragma unroll
-        for (int q = 0; q < N; q += 4) put<NT>(row + k0 + q, f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]});
+        for (int q = 0; q < N; q += 4) put<PASS>(row + k0 + q, f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]});
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (k0 + i < d) row[k0 + i] = v[i];
     }
 }
-template <int N, bool TAIL, bool NT>
+template <int N, bool TAIL, int PASS>
 __device__ __forceinline__ void store_piece(uint16_t* row, int k0, int d, const float* v) {
     if (!TAIL || k0 + N <= d) {
-        if constexpr (N == 8) put<NT>(row + k0, __builtin_bit_cast(u32x4_t, pack8(v)));
-        else put<NT>(row + k0, u32x2_t{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])});
+        if constexpr (N == 8) put<PASS>(row + k0, __builtin_bit_cast(u32x4_t, pack8(v)));
+        else put<PASS>(row + k0, u32x2_t{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])});
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -111,7 +114,7 @@ __device__ __forceinline__ void load_gamma(const float* gamma, int lane, int d, 
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k0 = c * S::STRIDE + lane * N;
-        if (k0 < d) load_piece<N, TAIL>(gamma, k0, d, g[c]);
+        if (k0 < d) load_piece<N, TAIL, kCached>(gamma, k0, d, g[c]);
         else
 #pragma unroll
             for (int i = 0; i < N; ++i) g[c][i] = 0.0f;
@@ -148,7 +151,7 @@ __device__ __forceinline__ F row_sum(F v, F* red) {
     return v;
 }
 
-template <bool F32, bool TAIL, int LANES, int V, bool NT>
+template <bool F32, bool TAIL, int LANES, int V, int PASS>
 __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_fwd_kernel(RmsParams p) {
     using S = Shape<F32, LANES, V>;
     using E = typename StreamType<F32>::T;
@@ -167,9 +170,9 @@ __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_fwd_kerne
         for (int i = 0; i < N; ++i) v[c][i] = 0.0f;
         if (k0 < d) {
             float x[N];
-            if (p.R) load_piece<N, TAIL>(static_cast<const E*>(p.R) + r * p.ldr, k0, d, v[c]);
+            if (p.R) load_piece<N, TAIL, PASS>(static_cast<const E*>(p.R) + r * p.ldr, k0, d, v[c]);
             if (p.X) {
-                load_piece<N, TAIL>(p.X + r * p.ldx, k0, d, x);
+                load_piece<N, TAIL, kCached>(p.X + r * p.ldx, k0, d, x);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     v[c][i] += x[i];
@@ -188,10 +191,10 @@ __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_fwd_kerne
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k0 = c * S::STRIDE + lane * N;
-        if (k0 < d && p.S) store_piece<N, TAIL, NT>(static_cast<E*>(p.S) + r * p.lds, k0, d, v[c]);
+        if (k0 < d && p.S) store_piece<N, TAIL, PASS>(static_cast<E*>(p.S) + r * p.lds, k0, d, v[c]);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[c][i] = v[c][i] * rstd * g[c][i];
-        if (k0 < d && p.Y) store_piece<N, TAIL, NT>(p.Y + r * p.ldy, k0, d, v[c]);
+        if (k0 < d && p.Y) store_piece<N, TAIL, PASS>(p.Y + r * p.ldy, k0, d, v[c]);
         if (p.codes) {
             uint32_t m = 0;
 #pragma unroll
@@ -205,18 +208,20 @@ __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_fwd_kerne
             if (lane % (kFp8Block / N) == 0 && k0 < d) p.scales[(int64_t)(k0 / kFp8Block) * p.ldsc + r] = q.scale;
             if (k0 < ((d + 15) & ~15)) {  // up to the 16 bytes' end: zeros
                 uint8_t* o = p.codes + r * p.ldc + k0;
-                if constexpr (N == 8) put<NT>(o, u32x2_t{fp8_codes(v[c], q.inv), fp8_codes(v[c] + 4, q.inv)});
-                else put<NT>(o, fp8_codes(v[c], q.inv));
+                if constexpr (N == 8) put<PASS>(o, u32x2_t{fp8_codes(v[c], q.inv), fp8_codes(v[c] + 4, q.inv)});
+                else put<PASS>(o, fp8_codes(v[c], q.inv));
             }
         }
     }
 }
 
-template <bool F32, bool TAIL, int LANES, int V, bool NT>
+template <bool F32, bool TAIL, int LANES, int V, int PASS>
 __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_bwd_kernel(RmsParams p, int rows_per_block) {
     using S = Shape<F32, LANES, V>;
     using E = typename StreamType<F32>::T;
     constexpr int N = S::N, C = S::C;
+    // dr's loads go out with the others, but for the widest rows, whose registers they overrun
+    constexpr bool EARLY = V * LANES < kRmsMaxWidth;
     __shared__ float red[2][S::WAVES];
     const int d = p.d, sub = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const int first = blockIdx.x * rows_per_block, last = min(p.T, first + rows_per_block);
@@ -229,16 +234,16 @@ __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_bwd_kerne
         for (int i = 0; i < N; ++i) dg[c][i] = 0.0f;
     int turn = 0;
     for (int r = first + sub; r < last; r += S::ROWS) {
-        float dy[C][N], xh[C][N], o[C][N];
+        float dy[C][N], xh[C][N], o[C][N] = {};
         float dot = 0.0f;
         const float rstd = p.rstd[r];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int k0 = c * S::STRIDE + lane * N;
             if (k0 < d) {
-                load_piece<N, TAIL>(p.dY + (int64_t)r * p.lddy, k0, d, dy[c]);
-                load_piece<N, TAIL>(static_cast<const E*>(p.S) + (int64_t)r * p.lds, k0, d, xh[c]);
-                if (p.dR) load_piece<N, TAIL>(static_cast<const E*>(p.dR) + (int64_t)r * p.lddr, k0, d, o[c]);
+                load_piece<N, TAIL, kCached>(p.dY + (int64_t)r * p.lddy, k0, d, dy[c]);
+                load_piece<N, TAIL, PASS>(static_cast<const E*>(p.S) + (int64_t)r * p.lds, k0, d, xh[c]);
+                if (EARLY && p.dR) load_piece<N, TAIL, PASS>(static_cast<const E*>(p.dR) + (int64_t)r * p.lddr, k0, d, o[c]);
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) dy[c][i] = xh[c][i] = 0.0f;
@@ -260,12 +265,10 @@ __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_bwd_kerne
         for (int c = 0; c < C; ++c) {
             const int k0 = c * S::STRIDE + lane * N;
             if (k0 < d) {
+                if (!EARLY && p.dR) load_piece<N, TAIL, PASS>(static_cast<const E*>(p.dR) + (int64_t)r * p.lddr, k0, d, o[c]);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float t = rstd * __builtin_fmaf(-xh[c][i], mean, dy[c][i]);
-                    o[c][i] = p.dR ? o[c][i] + t : t;
-                }
-                store_piece<N, TAIL, NT>(static_cast<E*>(p.dS) + (int64_t)r * p.ldds, k0, d, o[c]);
+                for (int i = 0; i < N; ++i) o[c][i] += rstd * __builtin_fmaf(-xh[c][i], mean, dy[c][i]);
+                store_piece<N, TAIL, PASS>(static_cast<E*>(p.dS) + (int64_t)r * p.ldds, k0, d, o[c]);
             }
         }
     }
@@ -314,39 +317,47 @@ int rows_per_block(bool f32, int T, int d, int cus) {
     return (each + rows - 1) / rows * rows;
 }
 // Outputs larger than the L2s hold together are stored non-temporally: 32768 x 1024
-// forward fp32 75 -> 71 us, bf16 51 -> 48, backward fp32 105 -> 102.
-bool streams(int T, int d, int bytes) { return (int64_t)T * d * bytes > (int64_t)16 << 20; }
+// forward fp32 75 -> 68 us, bf16 51 -> 44, backward fp32 112 -> 105. A call that passes
+// more than the memory-side cache holds also loads s, r and dr like that, but not x and
+// dy, which the products before it have just written: backward of that shape fp32 (448
+// MB) 105 -> 84, bf16 (268 MB) 62 -> 48, forward fp32 (369 MB) 68 -> 61; x and dy too: 98,
+// 57, 65; forward bf16 (235 MB, below the bound) 44 -> 53.
+int pass_of(int64_t in, int64_t out) { return in + out > 250'000'000 ? kOnce : out > 16 << 20 ? kStoreOnce : kCached; }
 
-template <bool F32, bool TAIL, int LANES, int V, bool NT>
+template <bool F32, bool TAIL, int LANES, int V, int PASS>
 void launch(bool fwd, const RmsParams& p, int grid, int rpb, hipStream_t s) {
     using S = Shape<F32, LANES, V>;
     if (fwd) {  // in two dimensions, for one's threads are counted in 32 bits
         const int64_t blocks = ((int64_t)p.T + S::ROWS - 1) / S::ROWS, x = std::min<int64_t>(blocks, 1 << 20);
-        rms_fwd_kernel<F32, TAIL, LANES, V, NT><<<dim3(x, (blocks + x - 1) / x), S::THREADS, 0, s>>>(p);
-    } else rms_bwd_kernel<F32, TAIL, LANES, V, NT><<<grid, S::THREADS, 0, s>>>(p, rpb);
+        rms_fwd_kernel<F32, TAIL, LANES, V, PASS><<<dim3(x, (blocks + x - 1) / x), S::THREADS, 0, s>>>(p);
+    } else rms_bwd_kernel<F32, TAIL, LANES, V, PASS><<<grid, S::THREADS, 0, s>>>(p, rpb);
 }
-template <bool F32, bool TAIL, bool NT>
+template <bool F32, bool TAIL, int PASS>
 void launch_width(bool fwd, const RmsParams& p, int grid, int rpb, hipStream_t s) {
     const int d = p.d;
-    if (d <= 128) launch<F32, TAIL, F32 ? 32 : 16, F32 ? 4 : 8, NT>(fwd, p, grid, rpb, s);
-    else if (d <= 256) launch<F32, TAIL, 32, 8, NT>(fwd, p, grid, rpb, s);
-    else if (d <= 512) launch<F32, TAIL, 64, 8, NT>(fwd, p, grid, rpb, s);
-    else if (d <= 1024) launch<F32, TAIL, 64, 16, NT>(fwd, p, grid, rpb, s);
-    else if (d <= 2048) launch<F32, TAIL, 256, 8, NT>(fwd, p, grid, rpb, s);
-    else if (d <= 4096) launch<F32, TAIL, 256, 16, NT>(fwd, p, grid, rpb, s);
-    else if (d <= 8192) launch<F32, TAIL, 1024, 8, NT>(fwd, p, grid, rpb, s);
-    else launch<F32, TAIL, 1024, 16, NT>(fwd, p, grid, rpb, s);
+    if (d <= 128) launch<F32, TAIL, F32 ? 32 : 16, F32 ? 4 : 8, PASS>(fwd, p, grid, rpb, s);
+    else if (d <= 256) launch<F32, TAIL, 32, 8, PASS>(fwd, p, grid, rpb, s);
+    else if (d <= 512) launch<F32, TAIL, 64, 8, PASS>(fwd, p, grid, rpb, s);
+    else if (d <= 1024) launch<F32, TAIL, 64, 16, PASS>(fwd, p, grid, rpb, s);
+    else if (d <= 2048) launch<F32, TAIL, 256, 8, PASS>(fwd, p, grid, rpb, s);
+    else if (d <= 4096) launch<F32, TAIL, 256, 16, PASS>(fwd, p, grid, rpb, s);
+    else if (d <= 8192) launch<F32, TAIL, 1024, 8, PASS>(fwd, p, grid, rpb, s);
+    else launch<F32, TAIL, 1024, 16, PASS>(fwd, p, grid, rpb, s);
 }
-template <bool F32, bool TAIL>
-void launch_stores(bool fwd, const RmsParams& p, int grid, int rpb, hipStream_t s) {
+template <bool F32>
+void launch_pass(bool fwd, const RmsParams& p, int grid, int rpb, hipStream_t s) {
     const int stream = F32 ? 4 : 2;
-    const int bytes = fwd ? (p.S ? stream : 0) + (p.Y ? 2 : 0) + (p.codes ? 1 : 0) : stream;
-    streams(p.T, p.d, bytes) ? launch_width<F32, TAIL, true>(fwd, p, grid, rpb, s) : launch_width<F32, TAIL, false>(fwd, p, grid, rpb, s);
+    const int64_t n = (int64_t)p.T * p.d;
+    const int in = fwd ? (p.X ? 2 : 0) + (p.R ? stream : 0) : 2 + stream + (p.dR ? stream : 0);
+    const int out = fwd ? (p.S ? stream : 0) + (p.Y ? 2 : 0) + (p.codes ? 1 : 0) : stream;
+    const int pass = pass_of(n * in, n * out);
+    if (p.d % (F32 ? 4 : 8) != 0) launch_width<F32, true, kCached>(fwd, p, grid, rpb, s);
+    else if (pass == kOnce) launch_width<F32, false, kOnce>(fwd, p, grid, rpb, s);
+    else if (pass == kStoreOnce) launch_width<F32, false, kStoreOnce>(fwd, p, grid, rpb, s);
+    else launch_width<F32, false, kCached>(fwd, p, grid, rpb, s);
 }
 void launch_rms(bool fwd, const RmsParams& p, int grid, int rpb, hipStream_t s) {
-    const bool tail = p.d % (p.f32 ? 4 : 8) != 0;
-    if (p.f32) tail ? launch_stores<true, true>(fwd, p, grid, rpb, s) : launch_stores<true, false>(fwd, p, grid, rpb, s);
-    else tail ? launch_stores<false, true>(fwd, p, grid, rpb, s) : launch_stores<false, false>(fwd, p, grid, rpb, s);
+    p.f32 ? launch_pass<true>(fwd, p, grid, rpb, s) : launch_pass<false>(fwd, p, grid, rpb, s);
 }
 
 }  // namespace
