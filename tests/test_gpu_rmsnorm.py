@@ -242,3 +242,38 @@ def test_repeats_and_captures(fn):
         torch.cuda.synchronize()
         call(held, a)
         assert all(torch.equal(i, j) for i, j in zip(bits(a), bits(c)))
+
+
+@pytest.mark.parametrize("T,d,stream", [(40000, 1024, F32), (40000, 1024, BF16), (9000, 512, BF16), (20000, 4096, BF16), (5000, 16000, F32)])
+def test_large_calls_as_small_ones(T, d, stream):
+    """A row's results do not depend on how many rows a call has, nor on how it passes memory:
+    the same bits as in calls of 500 rows."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    X = torch.randn(T, d, device="cuda", generator=g).to(BF16)
+    R = torch.randn(T, d, device="cuda", generator=g).to(stream)
+    dY, gamma = torch.randn(T, d, device="cuda", generator=g).to(BF16), torch.randn(d, device="cuda", generator=g)
+
+    def both(a, b):
+        n = b - a
+        S, C = torch.empty(n, d, dtype=stream, device="cuda"), torch.empty(n, d, dtype=torch.uint8, device="cuda")
+        Y, rs = torch.empty(n, d, dtype=BF16, device="cuda"), torch.empty(n, device="cuda")
+        sc = torch.empty(d // 128, n, device="cuda")
+        tmt_moe.rmsnorm_forward(X[a:b], R[a:b], gamma, S=S, Y=Y, codes=C, scales=sc, rstd=rs)
+        dS, dg = torch.empty(n, d, dtype=stream, device="cuda"), torch.empty(d, device="cuda")
+        ws = torch.empty(tmt_moe.rmsnorm_workspace_size(n, d), dtype=torch.uint8, device="cuda")
+        tmt_moe.rmsnorm_backward(dY[a:b], S, gamma, rs, dS, dg, ws, dR=R[a:b])
+        return S, C, Y, rs, sc.t(), dS, dg
+
+    whole = both(0, T)
+    for a in range(0, T, 500):
+        b = min(T, a + 500)
+        for name, big, small in zip(("S", "codes", "Y", "rstd", "scales", "dS"), whole, both(a, b)):
+            assert torch.equal(big[a:b], small), (name, a)
+    # dgamma: no addition is off by more than 2^-24 of the sum of magnitudes, and no value
+    # stands behind more than the rows of its lane (160 here), 16 rows of a workgroup and 1024
+    # workgroups; the product adds 3 roundings
+    dg, most = torch.zeros(d, dtype=torch.float64, device="cuda"), torch.zeros(d, dtype=torch.float64, device="cuda")
+    for a in range(0, T, 500):
+        t = dY[a:a + 500].double() * whole[0][a:a + 500].double() * whole[3][a:a + 500].double()[:, None]
+        dg, most = dg + t.sum(0), most + t.abs().sum(0)
+    assert ((whole[6].double() - dg).abs() <= most * (160 + 16 + 1024 + 3) * 2.0 ** -24).all()
