@@ -512,11 +512,11 @@ enum { TMT_MOE_FP8_ROWS = 0, TMT_MOE_FP8_TILES = 1 };
  * Norm of the residual stream, per row of d values (1 to 16384):
  *   S = X + R, rounded to the stream's type `dtype` (R and S; X is bf16)
  *   rstd = 1 / sqrt(mean(S^2) + eps),  y = (S * rstd) * gamma
- * y is written as bf16 to Y, and in blocks of rows (FP8_ROWS) from its fp32
- * values to codes and scales. Without R, S is X (dtype is then TMT_MOE_BF16);
+ * y is written as bf16 to Y, and in blocks of rows (FP8_ROWS) to codes and scales:
+ * the codes are those of y in 64 bits, the scales off by fp32's roundings. Without R, S is X (dtype is then TMT_MOE_BF16);
  * without X, it is R. S, Y, codes (with scales) and rstd [T] may each be NULL,
  * not all of them. S may be X or R itself (the same address and stride), where it
- * has its type. Squares are summed in fp32: a row's must stay below 2^128.
+ * has its type. Squares are summed in 64 bits.
  */
 int tmt_moe_rmsnorm_forward(void* stream, int32_t T, int32_t d, int32_t dtype, const uint16_t* X, int64_t ldx,
                             const void* R, int64_t ldr, const float* gamma, float eps, void* S, int64_t lds, uint16_t* Y,

@@ -35,11 +35,14 @@ __device__ __forceinline__ T get(const void* p) {
     if constexpr (PASS == kOnce) return __builtin_nontemporal_load(static_cast<const T*>(p));
     else return *static_cast<const T*>(p);
 }
+__device__ __forceinline__ float fp8_scaled(float v, float inv) {
+    return inv == 0.0f ? 0.0f : v * inv;  // inv is 0 for a block that is NaN
+}
 // Codes of four values, one a byte.
 __device__ __forceinline__ uint32_t fp8_codes(const float* v, float inv) {
     float q[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = inv == 0.0f ? 0.0f : v[i] * inv;  // inv is 0 for a block that is NaN
+    for (int i = 0; i < 4; ++i) q[i] = fp8_scaled(v[i], inv);
     return to_e4m3(q);
 }
 

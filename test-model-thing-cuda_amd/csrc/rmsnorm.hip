@@ -3,7 +3,7 @@
 //
 //   forward   s = x + r, rounded to the stream's type; rstd = 1 / sqrt(mean(s^2) + eps);
 //             y = (s * rstd) * gamma, to bf16 and to e4m3 codes with a scale for
-//             every 128 columns (the codes from y in fp32, not from bf16)
+//             every 128 columns (the codes not from y in bf16 but as from 64 bits)
 //   backward  g = dy gamma, xh = s rstd, c = mean(g xh);
 //             ds = dr + rstd (g - xh c); dgamma = sum over rows of dy xh
 //
@@ -15,13 +15,12 @@
 // would cover every second 16 bytes). A row's pieces are consecutive, so 16 (32)
 // neighbouring lanes own a block of 128 columns and find its maximum by DPP. us, and
 // TB/s of what has to pass: forward 32768 x 1024 fp32 to stream and codes 61, 6.0; 16384 x
-// 4096 126, 5.8; 777 x 1280 bf16 4.6; one row 3.4; backward 32768 x 1024 fp32 84, 5.6; 16384 x
+// 4096 125, 5.9; 777 x 1280 bf16 to bf16 and codes 4.8; one row 3.5; backward 32768 x 1024 fp32 84, 5.6; 16384 x
 // 4096 bf16 113, 4.8; 5003 x 1000 13.0. A copy of 1 GiB reaches 5.0 TB/s.
 //
-// Sums are in fp32 over the values of a lane, then, for the forward's squares, in
-// 64 bits over the lanes (a butterfly) and the waves (in order): rstd moves a whole
-// row, and with it which way its codes round (32768 x 1024, codes against 64 bits in
-// norm: with the butterfly in fp32 2.2 times as far off as with this). The backward's
+// The forward's squares are added in 64 bits, a lane's values, the lanes (a butterfly)
+// and the waves (in order): rstd moves a whole row, and with it which way its codes
+// round. The backward's
 // lanes keep dgamma of their columns in registers over the rows that they walk; a
 // workgroup's sums are added in the order of its rows into one row of the workspace, and
 // those rows by launch_colsum: no atomics, the same bits every time.
@@ -122,10 +121,13 @@ __device__ __forceinline__ void load_gamma(const float* gamma, int lane, int d, 
 }
 
 template <int OFF>
-__device__ __forceinline__ double add_xor_lane(double v) {
+__device__ __forceinline__ double xor_lane_f64(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint64_t o = ((uint64_t)xor_lane_u32<OFF>((uint32_t)(b >> 32)) << 32) | xor_lane_u32<OFF>((uint32_t)b);
-    return v + __builtin_bit_cast(double, o);
+    return __builtin_bit_cast(double, ((uint64_t)xor_lane_u32<OFF>((uint32_t)(b >> 32)) << 32) | xor_lane_u32<OFF>((uint32_t)b));
+}
+template <int OFF>
+__device__ __forceinline__ double add_xor_lane(double v) {
+    return v + xor_lane_f64<OFF>(v);
 }
 template <int OFF>
 __device__ __forceinline__ float add_xor_lane(float v) {
@@ -151,6 +153,40 @@ __device__ __forceinline__ F row_sum(F v, F* red) {
     return v;
 }
 
+// Cut off after 20 bits of the mantissa, the last of which is set if anything was lost:
+// rounded to e4m3 that is the value's own rounding, where fp32's nearest may be the middle
+// between two codes.
+__device__ __forceinline__ float odd_float(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t hi = (uint32_t)(b >> 32) | min((uint32_t)b, 1u);
+    return (float)__builtin_bit_cast(double, (uint64_t)hi << 32);
+}
+// A code goes one way or the other by the last bits where its value lies near the middle
+// between two. In fp32 rstd, the two products, the same three in the block's maximum, its
+// quotient and the last product leave it at most 4 units of the last place off, 8 where
+// those of the maximum's binade are twice as large; where a value of a wave lies that near
+// (one piece of a hundred), its codes are found in 64 bits. Codes of 2^25 values that are
+// not those of 64 bits: 25, now none; in 64 bits throughout, 32768 x 1024 bf16 takes 54 us.
+constexpr uint32_t kNear = 8;
+template <int N>
+__device__ void exact_scaled(const float* v, const float* g, double rstd, float inv, float* q) {
+    double y[N], m = 0x1p-100;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        y[i] = (double)v[i] * rstd * (double)g[i];
+        m = fmax(m, fabs(y[i]));
+    }
+    m = fmax(m, xor_lane_f64<1>(m));
+    m = fmax(m, xor_lane_f64<2>(m));
+    m = fmax(m, xor_lane_f64<4>(m));
+    m = fmax(m, xor_lane_f64<8>(m));
+    if constexpr (N == 4) m = fmax(m, xor_lane_f64<16>(m));
+    const double inv64 = 448.0 / m;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (inv != 0.0f) q[i] = odd_float(y[i] * inv64);
+}
+
 template <bool F32, bool TAIL, int LANES, int V, int PASS>
 __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_fwd_kernel(RmsParams p) {
     using S = Shape<F32, LANES, V>;
@@ -162,7 +198,7 @@ __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_fwd_kerne
     if (r >= p.T) return;  // whole rows
     float v[C][N], g[C][N];
     load_gamma<S, TAIL>(p.gamma, lane, d, g);
-    float sq = 0.0f;
+    double sq = 0.0;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k0 = c * S::STRIDE + lane * N;
@@ -184,32 +220,41 @@ __global__ __launch_bounds__((Shape<F32, LANES, V>::THREADS)) void rms_fwd_kerne
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int i = 0; i < N; ++i) sq = __builtin_fmaf(v[c][i], v[c][i], sq);
-    const double sum = row_sum<LANES>((double)sq, red);
-    const float rstd = (float)(1.0 / sqrt(sum / d + p.eps));
+        for (int i = 0; i < N; ++i) sq = __builtin_fma((double)v[c][i], (double)v[c][i], sq);
+    const double rstd64 = 1.0 / sqrt(row_sum<LANES>(sq, red) / d + p.eps);
+    const float rstd = (float)rstd64;
     if (p.rstd && lane == 0) p.rstd[r] = rstd;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int k0 = c * S::STRIDE + lane * N;
         if (k0 < d && p.S) store_piece<N, TAIL, PASS>(static_cast<E*>(p.S) + r * p.lds, k0, d, v[c]);
+        float y[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[c][i] = v[c][i] * rstd * g[c][i];
-        if (k0 < d && p.Y) store_piece<N, TAIL, PASS>(p.Y + r * p.ldy, k0, d, v[c]);
+        for (int i = 0; i < N; ++i) y[i] = v[c][i] * rstd * g[c][i];
+        if (k0 < d && p.Y) store_piece<N, TAIL, PASS>(p.Y + r * p.ldy, k0, d, y);
         if (p.codes) {
             uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) m = max(m, k0 < d ? abs_bits(v[c][i]) : 0u);
+            for (int i = 0; i < N; ++i) m = max(m, k0 < d ? abs_bits(y[i]) : 0u);
             m = max(m, xor_lane_u32<1>(m));
             m = max(m, xor_lane_u32<2>(m));
             m = max(m, xor_lane_u32<4>(m));
             m = max(m, xor_lane_u32<8>(m));
             if constexpr (N == 4) m = max(m, xor_lane_u32<16>(m));
-            const Fp8Scale q = fp8_scale(m);
-            if (lane % (kFp8Block / N) == 0 && k0 < d) p.scales[(int64_t)(k0 / kFp8Block) * p.ldsc + r] = q.scale;
+            const Fp8Scale f = fp8_scale(m);
+            if (lane % (kFp8Block / N) == 0 && k0 < d) p.scales[(int64_t)(k0 / kFp8Block) * p.ldsc + r] = f.scale;
+            float q[N];
+            uint32_t near = ~0u;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                q[i] = fp8_scaled(y[i], f.inv);
+                near = min(near, (__float_as_uint(q[i]) - (0x80000u - kNear)) & 0xfffffu);
+            }
+            if (__any(near <= 2 * kNear)) exact_scaled<N>(v[c], g[c], rstd64, f.inv, q);
             if (k0 < ((d + 15) & ~15)) {  // up to the 16 bytes' end: zeros
                 uint8_t* o = p.codes + r * p.ldc + k0;
-                if constexpr (N == 8) put<PASS>(o, u32x2_t{fp8_codes(v[c], q.inv), fp8_codes(v[c] + 4, q.inv)});
-                else put<PASS>(o, fp8_codes(v[c], q.inv));
+                if constexpr (N == 8) put<PASS>(o, u32x2_t{to_e4m3(q), to_e4m3(q + 4)});
+                else put<PASS>(o, to_e4m3(q));
             }
         }
     }

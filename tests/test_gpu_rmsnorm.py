@@ -277,3 +277,27 @@ def test_large_calls_as_small_ones(T, d, stream):
         t = dY[a:a + 500].double() * whole[0][a:a + 500].double() * whole[3][a:a + 500].double()[:, None]
         dg, most = dg + t.sum(0), most + t.abs().sum(0)
     assert ((whole[6].double() - dg).abs() <= most * (160 + 16 + 1024 + 3) * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("d", [1024, 1280, 100])
+@pytest.mark.parametrize("stream", [BF16, F32])
+def test_codes_of_64_bits(d, stream):
+    """No code above e4m3's subnormals goes another way than that of the norm in 64 bits."""
+    T = (1 << 24) // d
+    g = torch.Generator(device="cuda").manual_seed(d)
+    ld = ref.up(d, 8)
+    X = torch.randn(T, ld, device="cuda", generator=g).to(BF16)[:, :d]
+    R = (3 * torch.randn(T, ld, device="cuda", generator=g)).to(stream)[:, :d]
+    gamma = 1 + 0.3 * torch.randn(d, device="cuda", generator=g)
+    C = torch.empty(T, ref.up(d, 16), dtype=torch.uint8, device="cuda")[:, :d]
+    scales, S = torch.empty(ref.blocks_of(d), T, device="cuda"), torch.empty(T, ld, dtype=stream, device="cuda")[:, :d]
+    tmt_moe.rmsnorm_forward(X, R, gamma, S=S, codes=C, scales=scales)
+    s = S.double()
+    y = s * (s.square().mean(1, keepdim=True) + float(torch.tensor(1e-5))) ** -0.5 * gamma.double()
+    for c in range(0, d, 128):
+        q = y[:, c:c + 128]
+        q = q * 448 / q.abs().amax(1, keepdim=True)
+        step = torch.exp2(torch.floor(torch.log2(q.abs().clamp(min=2.0 ** -6))) - 3)  # no |q| is a power of 2 but by chance
+        want = torch.round(q / step) * step
+        got = C[:, c:c + 128].contiguous().view(ref.FP8).double()
+        assert torch.equal(got[q.abs() >= 2.0 ** -6], want[q.abs() >= 2.0 ** -6])
