@@ -323,20 +323,24 @@ __global__ __launch_bounds__(256, 2) void fp8_wide_kernel(Fp8Params p, LinearPla
 // fp32 results, few units, and bf16 results on 64 x 64 tiles: TILE x TILE outputs of 4
 // waves, a wave a quarter of them; a ring of 4, filled ahead, whose steps' operands
 // are read one step ahead too. A step of 64 x 64 is bound by its instructions, of
-// which one 32 x 32 sum a wave has the fewest (T 777, N 1024, K 4096 15.1 us; with
-// 16 x 16 sums, four in flight, 17.4 on 4 waves and 16.3 on 8). The stream does not
+// which one 32 x 32 sum a wave has the fewest (T 777, N 1024, K 4096 in one group 15.1 us;
+// with 16 x 16 sums, four in flight, 17.4 on 4 waves and 16.3 on 8). The stream does not
 // stop between units; the epilogue stages through the slot whose step is in registers
 // already.
-template <int TILE, bool TILES, bool F32, bool SPLIT, bool BETA>
-__global__ __launch_bounds__(256, (TILE == 128 ? 1 : 2)) void fp8_quarter_kernel(Fp8Params p, LinearPlan pl) {
+// GROUPS 2, where there is a CU for every unit: two such groups of waves, each with its
+// ring and half of the reduction; the first adds the second's sums to its own.
+template <int TILE, bool TILES, bool F32, bool SPLIT, bool BETA, int GROUPS>
+__global__ __launch_bounds__(256 * GROUPS, (TILE == 128 ? 1 : 2)) void fp8_quarter_kernel(Fp8Params p, LinearPlan pl) {
     constexpr int WT = TILE / 2, MI = WT / 32, RING = 4;
     using S = Slot<TILE, 4>;
     static_assert(4 * Stage<F32, MI>::BYTES <= S::BYTES, "the epilogue stages in a slot");
-    __shared__ uint4 lds_raw[RING * S::BYTES / 16];
-    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw);
-    const uint32_t lds0 = lds_u32(lds);
+    static_assert(GROUPS == 1 || (!SPLIT && MI == 1 && 4 * 4096 <= S::BYTES), "a group's sums pass through a slot");
+    __shared__ uint4 lds_raw[GROUPS * RING * S::BYTES / 16];
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    uint8_t* lds = reinterpret_cast<uint8_t*>(lds_raw) + group * RING * S::BYTES;
+    const uint32_t lds0 = lds_u32(lds);
     const int wrow = (wave >> 1) * WT, wcol = (wave & 1) * WT, row = lane & 31, h = lane >> 5;
     Unit u;
     int vb = blockIdx.x;
@@ -344,7 +348,7 @@ __global__ __launch_bounds__(256, (TILE == 128 ? 1 : 2)) void fp8_quarter_kernel
     Loader<TILE, 4, TILES, SPLIT, false> ld;
     ld.init(p, wave, lane, 0);
     ld.at.vl = vb;
-    ld.at.set(p, u);
+    ld.at.set(p, GROUPS == 1 ? u : half_of(u, group));
     int sl = 0, slot = 0;  // of the next loads, of the step in registers
     auto load_step = [&]() {
 #pragma unroll
@@ -412,6 +416,7 @@ __global__ __launch_bounds__(256, (TILE == 128 ? 1 : 2)) void fp8_quarter_kernel
     read_step(f[0], 0);
     for (;;) {
         int left = (u.kend - u.kbeg + kFp8Block - 1) / kFp8Block;
+        if constexpr (GROUPS == 2) left = (left + 1) / 2;  // the second's last step may be one of zeros
         for (; left >= 2; left -= 2) {
             step(f[0], f[1]);
             step(f[1], f[0]);
@@ -421,7 +426,23 @@ __global__ __launch_bounds__(256, (TILE == 128 ? 1 : 2)) void fp8_quarter_kernel
             f[0] = f[1];
         }
         lds_barrier();  // the slot of the step in registers is read: the epilogue stages there
+        if constexpr (GROUPS == 2) {
+            f32x4* sums = reinterpret_cast<f32x4*>(reinterpret_cast<uint8_t*>(lds_raw) + (RING + slot) * S::BYTES + wave * 4096) + lane;
+            if (group == 1) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sums[64 * q] = f32x4{acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]};
+            }
+            lds_barrier();
+            if (group == 1) break;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 o = sums[64 * q];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[0][0][4 * q + e] += o[e];
+            }
+        }
         finish_unit<TILE, F32, MI, SPLIT, BETA, false>(acc, lds + slot * S::BYTES + wave * Stage<F32, MI>::BYTES, p, u, p.M, p.N, wrow, wcol);
+        if constexpr (GROUPS == 2) break;  // a unit a workgroup
         vb += gridDim.x;
         if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) break;
         clear(acc);
@@ -780,11 +801,6 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
     wait_vm<0>();  // no load may land in LDS that the next workgroup owns
 }
 
-template <bool TILES, bool F32, int RB, int NB, int NW, int U>
-void launch_rows_as(const Fp8Params& p, hipStream_t s) {
-    const int64_t grid = (int64_t)((p.N + 16 * NB - 1) / (16 * NB)) * ((p.M + 16 * RB - 1) / (16 * RB));
-    fp8_rows_kernel<TILES, F32, RB, NB, NW, U><<<(unsigned)grid, 64 * NW, 0, s>>>(p);
-}
 // y = beta y, where the reduction is empty: 16 bytes a thread, by strides.
 template <bool F32>
 __global__ __launch_bounds__(256) void fp8_scale_kernel(Fp8Params p) {
@@ -840,7 +856,13 @@ void launch_units(const Fp8Params& p, const LinearPlan& pl, int units, int cus, 
             return;
         }
     }
-    if constexpr (F32 || TILE == 64) fp8_quarter_kernel<TILE, TILES, F32, SPLIT, BETA><<<grid, 256, 0, s>>>(p, pl);
+    if constexpr (TILE == 64 && !SPLIT) {
+        if (fp8_paired(TILE, units, p.K, cus)) {
+            fp8_quarter_kernel<TILE, TILES, F32, SPLIT, BETA, 2><<<grid, 512, 0, s>>>(p, pl);
+            return;
+        }
+    }
+    if constexpr (F32 || TILE == 64) fp8_quarter_kernel<TILE, TILES, F32, SPLIT, BETA, 1><<<grid, 256, 0, s>>>(p, pl);
     else fp8_deep_kernel<TILES, SPLIT, BETA><<<grid, 512, 0, s>>>(p, pl);
 }
 template <int TILE, bool TILES, bool F32>

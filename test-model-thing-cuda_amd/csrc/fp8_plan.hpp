@@ -52,6 +52,14 @@ struct Fp8Cursor {
     }
 };
 
+// The first or second half of a unit's reduction, the first the larger.
+TMT_HD Unit half_of(Unit u, int half) {
+    const int mid = u.kbeg + ((u.kend - u.kbeg + kFp8Block - 1) / kFp8Block + 1) / 2 * kFp8Block;
+    if (half == 0) u.kend = mid;
+    else u.kbeg = mid;
+    return u;
+}
+
 // ---- plan ----------------------------------------------------------------------
 // The kernel for few rows, 64 x 64 or 128 x 128 tiles (whole, or the last round's cut
 // along the reduction), or 256 x 256 tiles: the one with the shortest estimate.
@@ -70,6 +78,11 @@ inline int64_t fp8_count(int M, int N, int m, int n) { return (((int64_t)M + m -
 inline int fp8_slots(int tile, bool f32, int cus) { return tile == 256 || (tile == 128 && !f32) ? cus : 2 * cus; }
 // Workgroups of a launch of `units`, a multiple of 8: one for each XCD.
 inline int fp8_grid(int tile, bool f32, int units, int cus) { return std::min((units + 7) & ~7, fp8_slots(tile, f32, cus) & ~7); }
+
+// Workgroups of two groups of waves that halve the reduction: 64 x 64 tiles of which each
+// has a CU for itself. us with / without: M 777, N 1024, K 4096 12.8 / 15.5, K 1024 6.2 /
+// 6.3, K 512 5.2 / 4.8; fp32 2048 x 1024 x 1024 11.4 / 12.7, 777 x 1024 x 1024 8.0 / 7.5.
+inline bool fp8_paired(int tile, int units, int K, int cus) { return tile == 64 && units <= cus && fp8_steps(K) >= 8; }
 
 // Tiles whole or, parts >= 2, the rest of the last round's in parts.
 inline LinearPlan fp8_tiles(bool f32, int M, int N, int K, int tile, int parts, int cus) {
@@ -118,6 +131,7 @@ inline double fp8_launch_time(const Fp8Times& t, int64_t units, int slots, doubl
 inline double fp8_tiles_time(bool f32, const LinearPlan& pl, int K, int cus) {
     const Fp8Times& t = kFp8Times[f32][pl.tile == 128];
     const int slots = fp8_slots(pl.tile, f32, cus);
+    if (pl.tail == 0 && fp8_paired(pl.tile, pl.whole, K, cus)) return t.start + (fp8_steps(K) + 1) / 2 * t.two + 1.0;
     double us = fp8_launch_time(t, pl.whole, slots, fp8_steps(K), cus);
     if (pl.tail > 0) {
         const double mib = (double)pl.tail * pl.parts * pl.tile * pl.tile * 4 / (1 << 20);
@@ -132,7 +146,7 @@ inline double fp8_large_time(int M, int N, int K, int cus) {
 
 // Measured (us, chosen / others): M 128, N 1024, K 4096 8.3 in the kernel for few rows
 // / 10.2 on 64 x 64 tiles in four parts; M 777, N 1024, K 1024 6.3 on 64 x 64 / 8.9
-// few rows, 9.3 on 128 x 128; M 777, N 1024, K 4096 15.3 on 64 x 64 / 17.4 on 128 x 128
+// few rows, 9.3 on 128 x 128; M 777, N 1024, K 4096 12.8 on 64 x 64 / 17.4 on 128 x 128
 // in four parts; M 777, N 4096, K 1024 10.4 on 128 x 128 / 13.2 on 64 x 64; M = N = 4096,
 // K 1024 22.5 on 256 x 256 / 31.4 on 128 x 128. fp32: T 2048, N = K = 1280 17.6 on 64 x
 // 64 / 22.3 on 128 x 128 in four parts; T 32768, N = K = 1024 90.6 on 128 x 128 in

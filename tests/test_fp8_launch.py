@@ -41,18 +41,21 @@ void walk(const Fp8Params& p, const LinearPlan& pl, int cus, bool f32) {
     const uint64_t bs_end = TILES ? address(p.bs + (nb - 1) * p.ldbs + kb) : address(p.bs + (kb - 1) * p.ldbs + p.N);
     std::map<std::pair<int, int>, std::vector<std::pair<int, int>>> seen;
     int64_t count = 0;
+    const int groups = !SPLIT && fp8_paired(TILE, units, p.K, cus) ? 2 : 1;  // of waves, which halve a unit's reduction
+    if (groups == 2 && grid < units) FAIL("%d units on %d workgroups", units, grid);
     for (int block = 0; block < grid; ++block)
-        for (int half = 0; half < nbs; ++half) {
+        for (int half = 0; half < nbs * groups; ++half) {
             Unit u;
             int vb = block;
             if (!unit_at<TILE, SPLIT>(pl, p.K, vb, u)) continue;
+            if (groups == 2) u = half_of(u, half);
             Fp8Cursor<TILE, TILES, SPLIT> at;
-            at.nb = half;
+            at.nb = groups == 2 ? 0 : half;
             at.vl = vb;
             at.set(p, u);
             auto whole_grid = [&]() { return grid; };
             for (bool more = true; more;) {
-                if (half == 0) {
+                if (half == 0 || groups == 2) {
                     seen[{u.m0, u.c0}].push_back({u.kbeg, u.kend});
                     ++count;
                     if (SPLIT && ((int64_t)u.part + 1) * TILE * TILE * 4 > (int64_t)fp8_workspace_bound(p.M, p.N, p.K, cus))
@@ -70,9 +73,9 @@ void walk(const Fp8Params& p, const LinearPlan& pl, int cus, bool f32) {
                     if (at.wa.at + at.wa.bytes > a_end || at.wb.at + at.wb.bytes > b_end) FAIL("codes pass their operand");
                     if (at.wsa.at != address(p.as + (int64_t)(k / 128) * p.ldas + u.m0) || at.wsa.bytes != 4u * rows || at.wsa.at + at.wsa.bytes > as_end) FAIL("scales of a");
                     if (TILES) {
-                        const bool in = u.c0 + 128 * half < p.N;
+                        const bool in = u.c0 + 128 * at.nb < p.N;
                         if (at.wsb.bytes != (in ? 4u : 0u)) FAIL("scale of b: %u bytes", at.wsb.bytes);
-                        if (in && (at.wsb.at != address(p.bs + (int64_t)(u.c0 / 128 + half) * p.ldbs + k / 128) || at.wsb.at + 4 > bs_end)) FAIL("scale of b");
+                        if (in && (at.wsb.at != address(p.bs + (int64_t)(u.c0 / 128 + at.nb) * p.ldbs + k / 128) || at.wsb.at + 4 > bs_end)) FAIL("scale of b");
                     } else if (at.wsb.at != address(p.bs + (int64_t)(k / 128) * p.ldbs + u.c0) || at.wsb.bytes != 4u * cols || at.wsb.at + at.wsb.bytes > bs_end) {
                         FAIL("scales of b");
                     }
@@ -86,7 +89,7 @@ void walk(const Fp8Params& p, const LinearPlan& pl, int cus, bool f32) {
                 at.next(p, pl, whole_grid);
             }
         }
-    if (count != units) FAIL("%lld units, not %d", (long long)count, units);
+    if (count != (int64_t)units * groups) FAIL("%lld units, not %d", (long long)count, units);
     for (auto& s : seen) {
         std::vector<std::pair<int, int>> v = s.second;
         std::sort(v.begin(), v.end());

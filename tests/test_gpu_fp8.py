@@ -183,6 +183,8 @@ KERNELS = [
     (64, 4096, 130, False, BF16, [ROW % (0, 0, 2, 2)]), (63, 12288, 129, True, BF16, [ROW % (1, 0, 4, 4)]),
     (30, 64, 1000, False, F32, [ROW % (0, 1, 1, 1)]), (64, 4096, 200, True, F32, [ROW % (1, 1, 2, 2)]),
     (700, 1032, 2064, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb0E"]), (1000, 2048, 1000, False, BF16, ["fp8_quarter_kernelILi64ELb0ELb0ELb0E"]),
+    (777, 1024, 2050, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb0ELb0ELi2E"]), (777, 1024, 700, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb0ELb0ELi1E"]),
+    (800, 1000, 1120, False, BF16, ["fp8_quarter_kernelILi64ELb0ELb0ELb0ELb0ELi2E"]), (1024, 1000, 1500, False, F32, ["fp8_quarter_kernelILi64ELb0ELb1ELb0ELb0ELi2E"]),
     (777, 256, 4096, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb1E", "linear_fixup_kernelILi64ELb0E"]),
     (1500, 2048, 400, True, BF16, ["fp8_deep_kernelILb1ELb0E"]), (1100, 4000, 700, False, BF16, ["fp8_deep_kernelILb0ELb0E"]),
     (500, 1000, 20000, True, BF16, ["fp8_deep_kernelILb1ELb1E", "linear_fixup_kernelILi128ELb0E"]),
