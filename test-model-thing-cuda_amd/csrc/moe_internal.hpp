@@ -9,7 +9,9 @@
 //   norm.hip      LayerNorm forward / backward in front of the block
 //   adamw.hip     multi-tensor AdamW with global-norm clipping
 // The host orchestration lives in moe_api.cpp. The linear layer on microscaled
-// numbers (mx_quant.hip, linear.hip, linear_api.cpp) is declared in linear.hpp.
+// numbers (mx_quant.hip, linear.hip, linear_api.cpp) is declared in linear.hpp, the
+// one in 8 bits with its norm (rmsnorm.hip, fp8_quant.hip, fp8_gemm.hip,
+// fp8_api.cpp) in fp8.hpp.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

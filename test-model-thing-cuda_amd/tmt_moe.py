@@ -434,7 +434,7 @@ def _rows(what: str, t, dtype, dev: int, rows: int, cols: int, unit: int) -> tup
     if t.dtype is dtype and t.shape == (rows, cols) and t.get_device() == dev:
         ld, one = t.stride()
         if one == 1 or cols <= 1:
-            return t.data_ptr(), cols if rows == 1 and cols % unit == 0 else ld
+            return t.data_ptr(), -(-cols // unit) * unit if rows == 1 else ld
     return _matrix(what, t, dtype, dev, rows, cols)  # says what is wrong
 
 
