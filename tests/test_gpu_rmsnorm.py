@@ -208,6 +208,24 @@ def test_no_rows():
     assert (dgamma == 0).all()
 
 
+@pytest.mark.parametrize("d", [1, 100, 1001])
+def test_one_dense_row(d):
+    """One row of any length needs no room behind it, but for the codes."""
+    x, r, gamma = _inputs(1, d, F32, d)
+    s, rstd, y = ref.norm(x, r, gamma, 1e-5, F32)
+    S, Y, dS = torch.empty(1, d, device="cuda"), torch.empty(1, d, dtype=BF16, device="cuda"), torch.empty(1, d, device="cuda")
+    C, sc = torch.empty(1, ref.up(d, 16), dtype=torch.uint8, device="cuda"), torch.empty(ref.blocks_of(d), 1, device="cuda")
+    rs, dg = torch.empty(1, device="cuda"), torch.empty(d, device="cuda")
+    ws = torch.empty(tmt_moe.rmsnorm_workspace_size(1, d), dtype=torch.uint8, device="cuda")
+    tmt_moe.rmsnorm_forward(x.cuda(), r.cuda(), gamma.cuda(), S=S, Y=Y, codes=C[:, :d], scales=sc, rstd=rs)
+    assert torch.equal(S.cpu(), s) and (C[:, d:] == 0).all()
+    assert ((Y.cpu().double() - y).abs() <= y.abs() * (2.0 ** -8 + 2 * ROW)).all()
+    _check_codes(C[:, :d].cpu(), sc.cpu(), y, ROW + 2.0 ** -23)
+    tmt_moe.rmsnorm_backward(Y, S, gamma.cuda(), rs, dS, dg, ws)
+    want = Y.cpu().double()[0] * S.cpu().double()[0] * rs.cpu().double()
+    assert ((dg.cpu().double() - want).abs() <= want.abs() * 2.0 ** -22).all()  # two products, a sum of one term
+
+
 @pytest.mark.parametrize("fn", ["forward", "backward"])
 def test_repeats_and_captures(fn):
     """The same bits on another stream and from a graph's replays with new inputs."""
