@@ -55,75 +55,104 @@ __device__ __forceinline__ f32x4 mma16(i32x8 b, i32x8 a) {
     }
 }
 
+// Operand rows of 16, from LDS rows of 128 bytes whose chunks of 16 are
+// XOR-swizzled by row / 2: lane l holds chunks g and g + 4 of row l % 16, g = l / 16.
+__device__ __forceinline__ i32x8 read_codes16(const uint8_t* t, int r, int g) {
+    const int sw = (r >> 1) & 7;
+    return join(*reinterpret_cast<const uint4*>(t + r * 128 + ((g ^ sw) * 16)),
+                *reinterpret_cast<const uint4*>(t + r * 128 + (((g + 4) ^ sw) * 16)));
+}
+
 // ---- few rows ----------------------------------------------------------------------
-// A workgroup takes 16 NB columns and 16 RB rows of y; its NW waves deal out the
-// reduction in blocks of 128. Lane l loads chunks l / 16 and l / 16 + 4 (16 codes
-// each) of row l % 16 of a block straight into registers, of both operands: 64
-// bytes of 16 rows a load. The waves' sums meet in LDS and are added in wave order.
-// Bound by a launch and a trip to memory, then by the loads themselves: M 1, N 4096, K
-// 1024 3.0 us (1.4 TB/s), M 64, N 1024, K 4096 6.2.
-template <bool TILES, bool F32, int RB, int NB, int NW>
-__global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8Params p) {
-    constexpr int OUT = 256 * RB * NB;
-    __shared__ float red[NW * OUT];
+// A workgroup takes 16 NB columns and 16 RB rows of y; its 8 waves deal out the
+// reduction in blocks of 128. A wave loads its blocks into LDS of its own, 8 rows of
+// 128 bytes a load, DEPTH blocks ahead (1 where it has no more: ONE, whose LDS leaves
+// room for more workgroups on a CU), and no wave waits for another until their sums
+// meet in LDS and are added in wave order. Bound by a launch and a trip to memory: M 1,
+// N 4096, K 1024 2.9 us, M 64, N 1024, K 4096 4.4 (6.2 with loads straight into
+// registers, where neighbouring lanes hold different rows and four of them take four
+// cache lines).
+template <int RB, int NB, bool ONE>
+struct RowSlot {
+    static constexpr int SA = (RB + NB) * 2048, SB = SA + 256, BYTES = SB + 256;
+    static constexpr int ND = 2 * (RB + NB) + 2;  // loads of a block
+    static constexpr int DEPTH = ONE ? 1 : RB * NB == 1 ? 4 : RB * NB == 2 ? 3 : RB * NB == 4 ? 2 : 1;
+    static constexpr int WAVE = DEPTH * BYTES;    // bytes of a wave
+    static_assert(8 * WAVE <= 160 * 1024 && 1024 * RB * NB <= WAVE && DEPTH * ND < 64, "LDS; a wave's sums; what a wait counts");
+};
+template <bool TILES, bool F32, int RB, int NB, bool ONE>
+__global__ __launch_bounds__(512) void fp8_rows_kernel(Fp8Params p) {
+    using S = RowSlot<RB, NB, ONE>;
+    constexpr int OUT = 256 * RB * NB, NW = 8, DEPTH = S::DEPTH;
+    __shared__ uint4 lds_raw[NW * S::WAVE / 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = lane & 15, g = lane >> 4;
+    uint8_t* own = reinterpret_cast<uint8_t*>(lds_raw) + wave * S::WAVE;
+    const uint32_t lds0 = lds_u32(own);
     const int nb = (p.N + 16 * NB - 1) / (16 * NB);  // blocks of columns, which run fastest
     const int n0 = (int)(blockIdx.x % nb) * 16 * NB, m0 = (int)(blockIdx.x / nb) * 16 * RB;
-    const int blocks = (p.K + kFp8Block - 1) / kFp8Block;
-    // windows: rows past the last one, and chunks past a row's end, read zeros
+    const int rows = min(p.M - m0, 16 * RB), cols = min(p.N - n0, 16 * NB);
+    const int blocks = (p.K + kFp8Block - 1) / kFp8Block, steps = (blocks - wave + NW - 1) / NW;
+    // windows: rows past the last one, and chunks past a row's end, are zeros
     constexpr uint32_t FAR = 0x80000000u;
     const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u;
-    const __amdgpu_buffer_rsrc_t wa = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(p.a) + (int64_t)m0 * p.lda, 0, (int)((uint32_t)(min(p.M - m0, 16 * RB) - 1) * (uint32_t)p.lda + k16), 0x00020000);
-    const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(p.b) + (int64_t)n0 * p.ldb, 0, (int)((uint32_t)(min(p.N - n0, 16 * NB) - 1) * (uint32_t)p.ldb + k16), 0x00020000);
-    const float *psa[RB], *psb[NB];  // past the last row: its scale again, for no output
+    const Window wa = {address(p.a + (int64_t)m0 * p.lda), (uint32_t)(rows - 1) * (uint32_t)p.lda + k16};
+    const Window wb = {address(p.b + (int64_t)n0 * p.ldb), (uint32_t)(cols - 1) * (uint32_t)p.ldb + k16};
+    const int chunk = (lane & 7) ^ (lane >> 4);  // of 16 codes, swizzled as read_codes16 reads them; rows 8 .. 15: ^ 4
+    const uint32_t a_row = (uint32_t)(lane >> 3) * (uint32_t)p.lda, b_row = (uint32_t)(lane >> 3) * (uint32_t)p.ldb;
+    auto load = [&](int n) {
+        const int kb = wave + n * NW, k = kb * kFp8Block;
+        const uint32_t slot = lds0 + (uint32_t)(n % DEPTH) * S::BYTES;
+        uint32_t at[2];
 #pragma unroll
-    for (int r = 0; r < RB; ++r) psa[r] = p.as + min(m0 + 16 * r + row, p.M - 1);
+        for (int o = 0; o < 2; ++o) at[o] = k + 16 * (chunk ^ (4 * o)) < p.K ? (uint32_t)(k + 16 * (chunk ^ (4 * o))) : FAR;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        // rows: the columns 4 g .. + 3 of 16, which are in or out together (N is a multiple of 8)
-        if constexpr (TILES) psb[i] = p.bs + (int64_t)(min(n0 + 16 * i, p.N - 1) / kFp8Block) * p.ldbs;
-        else psb[i] = p.bs + min(n0 + 16 * i + 4 * g, p.N - 4);
-    }
+        for (int i = 0; i < 2 * NB; ++i) dma16(wb, at[i & 1] + b_row + (uint32_t)(8 * i) * (uint32_t)p.ldb, slot + 2048 * RB + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < 2 * RB; ++i) dma16(wa, at[i & 1] + a_row + (uint32_t)(8 * i) * (uint32_t)p.lda, slot + 1024 * i);
+        dma4({address(p.as + (int64_t)kb * p.ldas + m0), 4u * (uint32_t)rows}, 4u * lane, slot + S::SA);
+        if constexpr (TILES) dma4({address(p.bs + (int64_t)(n0 / kFp8Block) * p.ldbs + kb), 4u}, 4u * lane, slot + S::SB);
+        else dma4({address(p.bs + (int64_t)kb * p.ldbs + n0), 4u * (uint32_t)cols}, 4u * lane, slot + S::SB);
+    };
     f32x4 acc[RB][NB];
 #pragma unroll
     for (int r = 0; r < RB; ++r)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[r][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int kb = wave; kb < blocks; kb += NW) {
+        for (int i = 0; i < NB; ++i) acc[r][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < DEPTH; ++n)
+        if (n < steps) load(n);
+    for (int n = 0; n < steps; ++n) {
+        const int behind = min(DEPTH - 1, steps - 1 - n);  // blocks that are still to come
+        if (DEPTH > 3 && behind == 3) wait_vm<(DEPTH > 3 ? 3 : 0) * S::ND>();
+        else if (DEPTH > 2 && behind == 2) wait_vm<(DEPTH > 2 ? 2 : 0) * S::ND>();
+        else if (DEPTH > 1 && behind == 1) wait_vm<(DEPTH > 1 ? 1 : 0) * S::ND>();
+        else wait_vm<0>();
+        const uint8_t* t = own + (n % DEPTH) * S::BYTES;
+        const float* psa = reinterpret_cast<const float*>(t + S::SA);
+        const float* psb = reinterpret_cast<const float*>(t + S::SB);
         i32x8 a[RB], b[NB];
-        float sa[RB], st[NB];
+        float sa[RB];
         f32x4 sb[NB];
-        const int k = kb * kFp8Block + 16 * g;
-        const uint32_t lo = k < p.K ? (uint32_t)k : FAR, hi = k + 64 < p.K ? (uint32_t)(k + 64) : FAR;
-        auto chunks = [&](__amdgpu_buffer_rsrc_t w, uint32_t at) {
-            return join(__builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, (int)(at + lo), 0, 0)),
-                        __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, (int)(at + hi), 0, 0)));
-        };
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            b[i] = chunks(wb, (uint32_t)(16 * i + row) * (uint32_t)p.ldb);
-            if constexpr (TILES) {
-                st[i] = psb[i][kb];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sb[i][e] = psb[i][(int64_t)kb * p.ldbs + e];
-            }
+            b[i] = read_codes16(t + 2048 * (RB + i), row, g);
+            if constexpr (!TILES) sb[i] = *reinterpret_cast<const f32x4*>(psb + 16 * i + 4 * g);
         }
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
-            a[r] = chunks(wa, (uint32_t)(16 * r + row) * (uint32_t)p.lda);
-            sa[r] = psa[r][(int64_t)kb * p.ldas];
+            a[r] = read_codes16(t + 2048 * r, row, g);
+            sa[r] = psa[16 * r + row];
+            if constexpr (TILES) sa[r] *= psb[0];
         }
-        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is read
+        if (n + DEPTH < steps) load(n + DEPTH);
 #pragma unroll
         for (int r = 0; r < RB; ++r)
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 const f32x4 d = mma16<F32>(b[i], a[r]);
-                if constexpr (TILES) acc[r][i] += d * (st[i] * sa[r]);
+                if constexpr (TILES) acc[r][i] += d * sa[r];
                 else acc[r][i] += d * (sb[i] * sa[r]);
             }
     }
@@ -132,16 +161,17 @@ __global__ __launch_bounds__(64 * NW) void fp8_rows_kernel(Fp8Params p) {
     for (int r = 0; r < RB; ++r)
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-            *reinterpret_cast<f32x4*>(red + wave * OUT + (16 * r + row) * (16 * NB) + 16 * i + 4 * g) = acc[r][i];
+            *reinterpret_cast<f32x4*>(own + 4 * ((16 * r + row) * (16 * NB) + 16 * i + 4 * g)) = acc[r][i];
     __syncthreads();
+    const float* red = reinterpret_cast<const float*>(lds_raw);
     for (int o = threadIdx.x * 2; o < OUT; o += 128 * NW) {
         const int m = m0 + o / (16 * NB), n = n0 + o % (16 * NB);
         if (m >= p.M || n >= p.N) continue;
         float v[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            v[0] += red[w * OUT + o];
-            v[1] += red[w * OUT + o + 1];
+            v[0] += red[w * (S::WAVE / 4) + o];
+            v[1] += red[w * (S::WAVE / 4) + o + 1];
         }
         if constexpr (F32) {
             float2* y = reinterpret_cast<float2*>(static_cast<float*>(p.y) + (int64_t)m * p.ldy + n);
@@ -458,14 +488,6 @@ __global__ __launch_bounds__(256 * GROUPS, (TILE == 128 ? 1 : 2)) void fp8_quart
 // ---- sums of 16 x 16 ---------------------------------------------------------------
 // acc[i][j][e] = C[m][c] with m = 16 i + lane % 16 and c = 16 j + 4 (lane / 16) + e
 // in a wave's outputs.
-
-// Operand rows of 16, from LDS rows of 128 bytes whose chunks of 16 are
-// XOR-swizzled by row / 2: lane l holds chunks g and g + 4 of row l % 16, g = l / 16.
-__device__ __forceinline__ i32x8 read_codes16(const uint8_t* t, int r, int g) {
-    const int sw = (r >> 1) & 7;
-    return join(*reinterpret_cast<const uint4*>(t + r * 128 + ((g ^ sw) * 16)),
-                *reinterpret_cast<const uint4*>(t + r * 128 + (((g + 4) ^ sw) * 16)));
-}
 
 // Outputs to memory: 16 rows at a time go through the wave's own LDS (NJ * 512
 // bytes), so that a row's 16 NJ columns leave as one run of 16-byte stores; no
@@ -834,14 +856,14 @@ __global__ __launch_bounds__(256) void fp8_scale_kernel(Fp8Params p) {
 // Blocks of outputs are the largest of which there are enough for 3/4 of the CUs,
 // and 16 x 16 otherwise: a larger block reads its operands less often, but a CU
 // without one is idle. us with 16 x 16 / 16 x 32 (columns) / 32 x 32 / 64 x 64:
-// M 1, N 4096, K 1024 3.0 / 3.7 / 4.0 / 7.6; M 64, N 1024, K 4096 6.1 / 8.0 / 9.8 /
-// 19.0; M 128, N 1024, K 4096 10.0 / 7.8 / 10.1 / 19.2; M 128, N 4096, K 1024 9.8 / 8.1
-// / 6.6 / 8.8; M 256, N 4096, K 1024 17.5 / 13.6 / 10.7 / 9.4. Eight waves, one block of
-// 128 in flight each: with two or four the times are the same.
+// M 1, N 4096, K 1024 2.9 / 3.3 / 3.9 / 7.3; M 64, N 1024, K 4096 4.4 / 5.1 / 5.8 /
+// 11.5; M 128, N 1024, K 4096 7.1 / 5.5 / 5.8 / 11.5; M 128, N 4096, K 1024 6.6 / 7.2
+// / 5.7 / 7.8; M 256, N 4096, K 1024 11.3 / 11.1 / 9.3 / 8.5.
 template <bool TILES, bool F32, int RB, int NB>
 void launch_rows_as(const Fp8Params& p, hipStream_t s) {
     const int64_t grid = (int64_t)((p.N + 16 * NB - 1) / (16 * NB)) * ((p.M + 16 * RB - 1) / (16 * RB));
-    fp8_rows_kernel<TILES, F32, RB, NB, 8><<<(unsigned)grid, 512, 0, s>>>(p);
+    if (RB == 4 || p.K <= 8 * kFp8Block) fp8_rows_kernel<TILES, F32, RB, NB, true><<<(unsigned)grid, 512, 0, s>>>(p);
+    else fp8_rows_kernel<TILES, F32, RB, NB, RB == 4><<<(unsigned)grid, 512, 0, s>>>(p);
 }
 template <bool TILES, bool F32>
 void launch_rows(const Fp8Params& p, int cus, hipStream_t s) {

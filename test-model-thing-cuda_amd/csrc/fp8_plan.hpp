@@ -103,17 +103,20 @@ inline LinearPlan fp8_tiles(bool f32, int M, int N, int K, int tile, int parts, 
 }
 
 // Outputs of a workgroup of the kernel for few rows: 64 x 64, 32 x 32, 16 x 32 (24)
-// or 16 x 16.
+// or 16 x 16, and not twice as many rows as there are.
 inline int fp8_rows_block(int M, int N, int cus) {
     const int64_t enough = 3 * (int64_t)cus / 4;
-    return fp8_count(M, N, 64, 64) >= enough ? 64 : fp8_count(M, N, 32, 32) >= enough ? 32 : fp8_count(M, N, 16, 32) >= enough ? 24 : 16;
+    return M > 32 && fp8_count(M, N, 64, 64) >= enough ? 64 : M > 16 && fp8_count(M, N, 32, 32) >= enough ? 32 : fp8_count(M, N, 16, 32) >= enough ? 24 : 16;
 }
-// us, measured on one MI355X over M 1 .. 2048, N and K 256 .. 4096: a CU takes 33 ns
-// for a KiB of operand rows, and blocks of 64 x 64 run one to a CU and take 2 us more.
-inline double fp8_rows_time(int M, int N, int K, int cus) {
+// us, measured on one MI355X over M 1 .. 2304, N and K 256 .. 16000: a block's own time,
+// that of a KiB of its operand rows (fp32: widened), and 1 us more where a CU runs a
+// second one after the first: with more than one block of 128 a wave, and 64 x 64,
+// they fill a CU's LDS.
+inline double fp8_rows_time(bool f32, int M, int N, int K, int cus) {
     const int b = fp8_rows_block(M, N, cus), m = b == 24 ? 16 : b, n = b == 24 ? 32 : b;
-    const double kib = (m + n) * (double)K / 1024, groups = (double)fp8_count(M, N, m, n) / cus;
-    return 2.5 + (b == 64 ? std::ceil(groups) * (0.033 * kib + 2.0) : std::max(1.0, groups) * 0.033 * kib);
+    const double own = b == 64 ? 3.2 : b == 32 ? 0.8 : 0.1, kib = !f32 ? 0.0145 : b == 64 ? 0.023 : b == 32 ? 0.019 : 0.016;
+    const double groups = (double)fp8_count(M, N, m, n) / cus, us = own + kib * (m + n) * (double)K / 1024;
+    return b == 64 || fp8_steps(K) > 8 ? 1.6 + std::ceil(groups) * (us + 1.0) : 2.6 + std::max(1.0, groups) * us;
 }
 // us of tiles: start of a launch, a step with one workgroup per CU and with two.
 struct Fp8Times {
@@ -144,8 +147,8 @@ inline double fp8_large_time(int M, int N, int K, int cus) {
     return 6.0 + std::ceil(tiles / cus) * (fp8_steps(K) * (1.25 + 0.35 * fill) + 3.0);
 }
 
-// Measured (us, chosen / others): M 128, N 1024, K 4096 8.3 in the kernel for few rows
-// / 10.2 on 64 x 64 tiles in four parts; M 777, N 1024, K 1024 6.3 on 64 x 64 / 8.9
+// Measured (us, chosen / others): M 256, N 1024, K 4096 7.1 in the kernel for few rows
+// / 10.3 on 64 x 64 tiles in four parts; M 777, N 1024, K 1024 6.2 on 64 x 64 / 8.0
 // few rows, 9.3 on 128 x 128; M 777, N 1024, K 4096 12.8 on 64 x 64 / 17.4 on 128 x 128
 // in four parts; M 777, N 4096, K 1024 10.4 on 128 x 128 / 13.2 on 64 x 64; M = N = 4096,
 // K 1024 22.5 on 256 x 256 / 31.4 on 128 x 128. fp32: T 2048, N = K = 1280 17.6 on 64 x
@@ -156,7 +159,7 @@ inline Fp8Plan fp8_plan(bool tiles, bool f32, int M, int N, int K, int cus) {
     Fp8Plan best;
     if (M <= kFp8FewRows) return best;
     // a launch holds 2^32 threads
-    double us = fp8_count(M, N, 16, 16) < (1 << 22) ? fp8_rows_time(M, N, K, cus) : 1e30;
+    double us = fp8_count(M, N, 16, 16) < (1 << 22) ? fp8_rows_time(f32, M, N, K, cus) : 1e30;
     if (tiles && !f32) {
         const double t = fp8_large_time(M, N, K, cus);
         if (t < us) us = t, best = {FP8_LARGE_KERNEL, fp8_tiles(f32, M, N, K, 256, 1, cus)};

@@ -185,7 +185,9 @@ KERNELS = [
     (700, 1032, 2064, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb0E"]), (1000, 2048, 1000, False, BF16, ["fp8_quarter_kernelILi64ELb0ELb0ELb0E"]),
     (777, 1024, 2050, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb0ELb0ELi2E"]), (777, 1024, 700, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb0ELb0ELi1E"]),
     (800, 1000, 1120, False, BF16, ["fp8_quarter_kernelILi64ELb0ELb0ELb0ELb0ELi2E"]), (1024, 1000, 1500, False, F32, ["fp8_quarter_kernelILi64ELb0ELb1ELb0ELb0ELi2E"]),
-    (777, 256, 4096, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb1E", "linear_fixup_kernelILi64ELb0E"]),
+    (777, 256, 4096, True, BF16, [ROW % (1, 0, 2, 2) + "Lb0E"]), (64, 1024, 4096, True, BF16, [ROW % (1, 0, 1, 1) + "Lb0E"]),
+    (100, 1024, 2050, False, F32, [ROW % (0, 1, 1, 2) + "Lb0E"]), (1000, 1000, 16000, False, F32, [ROW % (0, 1, 4, 4) + "Lb1E"]),
+    (900, 264, 9000, True, BF16, ["fp8_quarter_kernelILi64ELb1ELb0ELb1E", "linear_fixup_kernelILi64ELb0E"]),
     (1500, 2048, 400, True, BF16, ["fp8_deep_kernelILb1ELb0E"]), (1100, 4000, 700, False, BF16, ["fp8_deep_kernelILb0ELb0E"]),
     (500, 1000, 20000, True, BF16, ["fp8_deep_kernelILb1ELb1E", "linear_fixup_kernelILi128ELb0E"]),
     (2304, 1896, 6451, False, BF16, ["fp8_deep_kernelILb0ELb0E", "fp8_deep_kernelILb0ELb1E", "linear_fixup_kernelILi128ELb0E"]),
@@ -196,7 +198,7 @@ KERNELS = [
     (300, 264, 9000, True, F32, ["fp8_quarter_kernelILi64ELb1ELb1ELb1E", "linear_fixup_kernelILi64ELb1E"]),
     (2304, 1896, 6451, False, F32, ["fp8_quarter_kernelILi64ELb0ELb1ELb0E", "fp8_quarter_kernelILi64ELb0ELb1ELb1E", "linear_fixup_kernelILi64ELb1E"]),
     (2048, 2048, 1000, False, F32, ["fp8_quarter_kernelILi128ELb0ELb1ELb0E"]),
-    (1000, 1000, 16000, False, F32, ["fp8_quarter_kernelILi128ELb0ELb1ELb1E", "linear_fixup_kernelILi128ELb1E"]),
+    (600, 520, 16000, False, F32, ["fp8_quarter_kernelILi128ELb0ELb1ELb1E", "linear_fixup_kernelILi128ELb1E"]),
     (1100, 1304, 9000, True, F32, ["fp8_wide_kernelILb1ELb1E", "linear_fixup_kernelILi128ELb1E"]),
     (4096, 4200, 1100, False, F32, ["fp8_wide_kernelILb0ELb0E"]),
 ]
