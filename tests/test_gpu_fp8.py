@@ -346,3 +346,31 @@ def test_repeats_and_captures(M, tiles, dtype):
         torch.cuda.synchronize()
         tmt_moe.fp8_matmul(*a, *b, y[0], blocks=blocks, workspace=ws)
         assert torch.equal(y[0], y[2])
+
+
+@pytest.mark.parametrize("M", [40, 300])
+def test_the_widest_strides(M):
+    """Code rows 2^22 bytes apart give the bits of dense ones; what lies between is NaN."""
+    N, K, ld = 72, 1500, 1 << 22
+    g = torch.Generator(device="cuda").manual_seed(M)
+
+    def operand(rows, blocks):
+        x = torch.randn(rows, K, device="cuda", generator=g).to(BF16)
+        X = torch.empty(rows, ref.up(K, 8), dtype=BF16, device="cuda")[:, :K].copy_(x)
+        dense = torch.empty(rows, ref.up(K, 16), dtype=torch.uint8, device="cuda")
+        shape = (ref.blocks_of(rows), ref.blocks_of(K)) if blocks == TILES else (ref.blocks_of(K), rows)
+        scales = torch.empty(shape, device="cuda")
+        tmt_moe.fp8_quantize(X, dense[:, :K], scales, blocks=blocks)
+        wide = torch.full(((rows - 1) * ld + ref.up(K, 16),), 0x7f, dtype=torch.uint8, device="cuda")
+        wide = wide.as_strided((rows, ref.up(K, 16)), (ld, 1)).copy_(dense)
+        return dense[:, :K], wide[:, :K], scales
+
+    a, wide_a, sa = operand(M, ROWS)
+    for blocks in (TILES, ROWS):
+        b, wide_b, sb = operand(N, blocks)
+        for dtype in (BF16, F32):
+            y, z = (torch.empty(M, N, dtype=dtype, device="cuda") for _ in range(2))
+            ws = torch.empty(max(tmt_moe.fp8_workspace_size(M, N, K, blocks), 1), dtype=torch.uint8, device="cuda")
+            tmt_moe.fp8_matmul(a, sa, b, sb, y, blocks=blocks, workspace=ws)
+            tmt_moe.fp8_matmul(wide_a, sa, wide_b, sb, z, blocks=blocks, workspace=ws)
+            assert torch.isfinite(y).all() and torch.equal(y, z)
