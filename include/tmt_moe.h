@@ -546,6 +546,15 @@ int tmt_moe_fp8_quantize(void* stream, int32_t blocks, int32_t dtype, const void
                          int64_t ldct, float* scales_t, int64_t ldst);
 
 /*
+ * The codes of a matrix [rows][K] in the order of its transpose, for a product whose operand
+ * lies in columns: codes [rows][ldc] of any alignment, ldc from K to 2^22, to rows of
+ * codes_t [K][ldct], with zeros up to a multiple of 16. Scales stay as they are. Fewer than 2^23
+ * tiles of 128 x 128.
+ */
+int tmt_moe_fp8_transpose(void* stream, const uint8_t* codes, int64_t ldc, int32_t rows, int32_t K, uint8_t* codes_t,
+                          int64_t ldct);
+
+/*
  * Y [M][ldy] = beta * Y + A B^T: A [M][K] in rows, B [N][K] in rows or tiles
  * (`b_blocks`), Y bf16 or fp32 (`dtype`). A block's products are summed in fp32,
  * multiplied by its two scales and added in fp32; Y is rounded once. For bf16 the

@@ -61,6 +61,9 @@ struct Fp8QuantParams {
 // Arguments as the C ABI has checked them, rows and K > 0.
 hipError_t launch_fp8_quantize(bool tiles, bool f32, const Fp8QuantParams& p, hipStream_t s);
 
+// codes [rows][ldc], of any alignment, to codes_t [K][ldct], zeros up to a multiple of 16.
+hipError_t launch_fp8_transpose(const uint8_t* codes, int64_t ldc, int rows, int K, uint8_t* codes_t, int64_t ldct, hipStream_t s);
+
 // ---- products --------------------------------------------------------------------
 // y[m][n] = beta y + sum over blocks b of a_scale[b][m] b_scale(b, n) sum_{k in b} a[m][k] b[n][k]
 struct Fp8Params {

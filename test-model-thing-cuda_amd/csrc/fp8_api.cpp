@@ -157,6 +157,21 @@ int tmt_moe_fp8_quantize(void* stream, int32_t blocks, int32_t dtype, const void
     return TMT_MOE_OK;
 }
 
+int tmt_moe_fp8_transpose(void* stream, const uint8_t* codes, int64_t ldc, int32_t rows, int32_t K, uint8_t* codes_t,
+                          int64_t ldct) {
+    if (rows < 0 || K < 0) return fail(TMT_MOE_EINVAL, "rows=%d and K=%d must not be negative", rows, K);
+    if (rows == 0 || K == 0) return TMT_MOE_OK;
+    if (blocks_of(rows) * blocks_of(K) >= kMaxGrid)
+        return fail(TMT_MOE_EINVAL, "rows=%d of K=%d are 2^23 tiles of 128 x 128 or more", rows, K);
+    if (!codes) return fail(TMT_MOE_EINVAL, "codes must be non-NULL");
+    if (ldc < K || ldc > kMaxStride)
+        return fail(TMT_MOE_EINVAL, "the row stride %lld of codes must be at least %d and at most %lld", (long long)ldc, K, (long long)kMaxStride);
+    int rc = check_rows("codes_t", codes_t, ldct, rows, 16);
+    if (rc) return rc;
+    HIP_TRY(launch_fp8_transpose(codes, ldc, rows, K, codes_t, ldct, (hipStream_t)stream));
+    return TMT_MOE_OK;
+}
+
 int tmt_moe_fp8_workspace_size(int32_t b_blocks, int32_t M, int32_t N, int32_t K, size_t* bytes) {
     int rc = check_blocks(b_blocks);
     if (rc || (rc = check_product_shape(M, N, K))) return rc;

@@ -64,6 +64,7 @@ EXPORTED = (
     "tmt_moe_rmsnorm_workspace_size",
     "tmt_moe_rmsnorm_backward",
     "tmt_moe_fp8_quantize",
+    "tmt_moe_fp8_transpose",
     "tmt_moe_fp8_workspace_size",
     "tmt_moe_fp8_matmul",
     "tmt_moe_set_profiling",
@@ -148,6 +149,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.tmt_moe_rmsnorm_workspace_size.argtypes = [i32, i32, ctypes.POINTER(size)]
     lib.tmt_moe_rmsnorm_backward.argtypes = [vp, i32, i32, i32, vp, i64, vp, i64, vp, vp, vp, i64, vp, i64, vp, vp, size]
     lib.tmt_moe_fp8_quantize.argtypes = [vp, i32, i32, vp, i64, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64]
+    lib.tmt_moe_fp8_transpose.argtypes = [vp, vp, i64, i32, i32, vp, i64]
     lib.tmt_moe_fp8_workspace_size.argtypes = [i32, i32, i32, i32, ctypes.POINTER(size)]
     lib.tmt_moe_fp8_matmul.argtypes = [vp, i32, i32, i32, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, f32, vp,
                                        size]
@@ -567,6 +569,47 @@ def fp8_quantize(X, codes=None, scales=None, codes_t=None, scales_t=None, blocks
         _check(rc)
 
 
+def fp8_transpose(codes, codes_t, stream=None) -> None:
+    """Codes [rows, K] (uint8 or float8_e4m3fn, rows of any stride) to codes_t
+    [K, rows], whose rows end at a multiple of 16 bytes, zeros behind the last code."""
+    rows, K = codes.shape
+    if (rows | K) >> 31:
+        _past_int32(rows, K)
+    dev, raw = _here(stream)
+    if codes.dtype is not codes_t.dtype:
+        raise ValueError(f"codes are {codes.dtype} and codes_t {codes_t.dtype}")
+    c, ldc = _matrix("codes", codes, codes.dtype, dev, rows, K)
+    ct, ldct = _fp8_codes("codes_t", codes_t, dev, K, rows)
+    rc = load_library().tmt_moe_fp8_transpose(raw, c, ldc, rows, K, ct, ldct)
+    if rc:
+        _check(rc)
+
+
+def _fp8_in_columns(t) -> bool:
+    """Whether a matrix of codes lies in columns: of a single row any that cannot be read as one
+    of rows, because its codes are apart or there is no room up to a multiple of 16 bytes."""
+    rows, K = t.shape
+    if K > 1 and t.stride(-1) != 1:
+        return True
+    if rows == 1:
+        return t.untyped_storage().nbytes() - t.storage_offset() < (K + 15) // 16 * 16
+    return K == 1 and t.stride(0) == 1
+
+
+def _fp8_rows_of(t, dev: int, rows: int, K: int, stream):
+    """Codes [rows, K] whose columns are contiguous, as a transposed view has them, laid out in
+    rows that belong to the call's stream; any others as they are, to be checked as rows."""
+    import torch
+    if t.shape != (rows, K) or not _fp8_in_columns(t) or (t.stride(0) != 1 and rows != 1):
+        return t
+    if t.get_device() != dev or t.dtype not in (torch.uint8, torch.float8_e4m3fn):
+        return t
+    with torch.cuda.stream(stream):  # None: the current one
+        out = torch.empty((rows, (K + 15) // 16 * 16), dtype=t.dtype, device=t.device)[:, :K]
+    fp8_transpose(t.t(), out, stream)
+    return out
+
+
 def fp8_workspace_size(M: int, N: int, K: int, blocks: int = FP8_TILES) -> int:
     """Bytes of device workspace that fp8_matmul needs for up to M rows."""
     if any(n >> 31 not in (0, -1) for n in (M, N, K, blocks)):
@@ -580,19 +623,24 @@ def fp8_matmul(A, A_scales, B, B_scales, Y, beta: float = 0.0, blocks: int = FP8
                stream=None) -> None:
     """Y <- beta*Y + A B^T. A [M, K] e4m3 codes in rows (scales [K/128, M or
     more]), B [N, K] in `blocks` (FP8_TILES: scales [N/128, K/128 or more],
-    FP8_ROWS: [K/128, N or more]), Y [M, N] bf16 or fp32."""
+    FP8_ROWS: [K/128, N or more]), Y [M, N] bf16 or fp32. Codes are read in rows: A or
+    B in columns (a transposed view) is laid out in rows first, in memory that
+    torch's allocator gives; a program that multiplies it again keeps its rows
+    (fp8_transpose, or codes_t of fp8_quantize)."""
     (M, K), N = A.shape, B.shape[0]
     if (M | N | K) >> 31:
         _past_int32(M, N, K)
     dev, raw = _here(stream)
     dtype, piece = _stream_dtype(Y)
     kb, tiles = _blocks_of(K), blocks == FP8_TILES
-    a, lda = _fp8_codes("A", A, dev, M, K)
     sa, ldas = _fp8_scales("A_scales", A_scales, dev, kb, M)
-    b, ldb = _fp8_codes("B", B, dev, N, K)
     sb, ldbs = _fp8_scales("B_scales", B_scales, dev, _blocks_of(N) if tiles else kb, kb if tiles else N)
     y, ldy = _rows("Y", Y, Y.dtype, dev, M, N, piece)
     ws, size = _ws(workspace, dev)
+    if K % 16 or A.stride(-1) != 1 or B.stride(-1) != 1:
+        A, B = _fp8_rows_of(A, dev, M, K, stream), _fp8_rows_of(B, dev, N, K, stream)
+    a, lda = _fp8_codes("A", A, dev, M, K)
+    b, ldb = _fp8_codes("B", B, dev, N, K)
     rc = load_library().tmt_moe_fp8_matmul(raw, blocks, dtype, M, N, K, a, lda, sa, ldas, b, ldb, sb, ldbs, y, ldy, beta,
                                            ws, size)
     if rc:
