@@ -754,8 +754,6 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
     };
     f32x4 acc[MI][NJ], d[DEPTH + 1];
     float last = 0.0f;  // the scale of the sums still in flight from the step before
-#pragma unroll
-    for (int q = 0; q <= DEPTH; ++q) d[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     // sums q of this step (q < 0: the step before) are scaled and added
     auto add = [&](int q) {
         f32x4& t = acc[(q + NQ) % NQ / NJ][(q + NQ) % NQ % NJ];
@@ -788,7 +786,9 @@ __global__ __launch_bounds__(512, 2) void fp8_large_kernel(Fp8Params p, LinearPl
                 acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 asm volatile("" : "+v"(acc[i][j]));  // no first step of its own
             }
-        last = 0.0f;
+        last = 0.0f;  // and no sums in flight: times zero, a NaN of the unit before would stay one
+#pragma unroll
+        for (int q = 0; q <= DEPTH; ++q) d[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < p.K; k += kFp8Block) {
             s[MI - 2] = next[0];
             s[MI - 1] = next[1];
