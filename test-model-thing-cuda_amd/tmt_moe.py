@@ -596,7 +596,7 @@ def _fp8_in_columns(t) -> bool:
     return K == 1 and t.stride(0) == 1
 
 
-def _fp8_rows_of(t, dev: int, rows: int, K: int, stream):
+def _fp8_rows_of(t, dev: int, rows: int, K: int, raw: int, stream):
     """Codes [rows, K] whose columns are contiguous, as a transposed view has them, laid out in
     rows that belong to the call's stream; any others as they are, to be checked as rows."""
     import torch
@@ -604,10 +604,16 @@ def _fp8_rows_of(t, dev: int, rows: int, K: int, stream):
         return t
     if t.get_device() != dev or t.dtype not in (torch.uint8, torch.float8_e4m3fn):
         return t
-    with torch.cuda.stream(stream):  # None: the current one
-        out = torch.empty((rows, (K + 15) // 16 * 16), dtype=t.dtype, device=t.device)[:, :K]
-    fp8_transpose(t.t(), out, stream)
-    return out
+    shape = (rows, (K + 15) // 16 * 16)
+    if stream is None:
+        out = torch.empty(shape, dtype=t.dtype, device=t.device)
+    else:
+        with torch.cuda.stream(stream):
+            out = torch.empty(shape, dtype=t.dtype, device=t.device)
+    rc = load_library().tmt_moe_fp8_transpose(raw, t.data_ptr(), t.stride(1) if K > 1 else rows, K, rows, out.data_ptr(), shape[1])
+    if rc:
+        _check(rc)
+    return out[:, :K]
 
 
 def fp8_workspace_size(M: int, N: int, K: int, blocks: int = FP8_TILES) -> int:
@@ -638,7 +644,7 @@ def fp8_matmul(A, A_scales, B, B_scales, Y, beta: float = 0.0, blocks: int = FP8
     y, ldy = _rows("Y", Y, Y.dtype, dev, M, N, piece)
     ws, size = _ws(workspace, dev)
     if K % 16 or A.stride(-1) != 1 or B.stride(-1) != 1:
-        A, B = _fp8_rows_of(A, dev, M, K, stream), _fp8_rows_of(B, dev, N, K, stream)
+        A, B = _fp8_rows_of(A, dev, M, K, raw, stream), _fp8_rows_of(B, dev, N, K, raw, stream)
     a, lda = _fp8_codes("A", A, dev, M, K)
     b, ldb = _fp8_codes("B", B, dev, N, K)
     rc = load_library().tmt_moe_fp8_matmul(raw, blocks, dtype, M, N, K, a, lda, sa, ldas, b, ldb, sb, ldbs, y, ldy, beta,
