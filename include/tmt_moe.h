@@ -513,9 +513,10 @@ enum { TMT_MOE_FP8_ROWS = 0, TMT_MOE_FP8_TILES = 1 };
  *   S = X + R, rounded to the stream's type `dtype` (R and S; X is bf16)
  *   rstd = 1 / sqrt(mean(S^2) + eps),  y = (S * rstd) * gamma
  * y is written as bf16 to Y, and in blocks of rows (FP8_ROWS) to codes and scales:
- * the codes are those of y in 64 bits, the scales off by fp32's roundings. Without R, S is X (dtype is then TMT_MOE_BF16);
- * without X, it is R. S, Y, codes (with scales) and rstd [T] may each be NULL,
- * not all of them. S may be X or R itself (the same address and stride), where it
+ * the codes are those of y in 64 bits, e4m3's subnormals among them (but where S * rstd
+ * is below fp32's normal range), the scales off by fp32's roundings. Without R, S is X
+ * (dtype is then TMT_MOE_BF16); without X, it is R. S, Y, codes (with scales) and
+ * rstd [T] may each be NULL, not all of them. S may be X or R itself (the same address and stride), where it
  * has its type. Squares are summed in 64 bits.
  */
 int tmt_moe_rmsnorm_forward(void* stream, int32_t T, int32_t d, int32_t dtype, const uint16_t* X, int64_t ldx,
