@@ -166,10 +166,10 @@ __device__ __forceinline__ float odd_float(double v) {
 // quotient and the last product leave it at most 4 units of the last place off, 8 where
 // those of the maximum's binade are twice as large; where a value of a wave lies that near
 // (one piece of a hundred), its codes are found in 64 bits. Codes of 2^25 values that are
-// not those of 64 bits: 25, now none; in 64 bits throughout, 32768 x 1024 bf16 takes 54 us.
-// e4m3's subnormals lie 2^-9 apart, as the codes of [2^-6, 2^-5) do: moved there, they have
-// their middles at the same bit. Their values' error is less than half of that binade's 8
-// units, the sum's rounding half of one.
+// not those of 64 bits: 25, now none; in 64 bits throughout, 32768 x 1024 bf16 takes 54 us,
+// so 48. e4m3's subnormals lie 2^-9 apart, as the codes of [2^-6, 2^-5) do: moved there, they
+// have their middles at the same bit. Their values are at most 4 of that binade's units off,
+// the sum half of one more.
 constexpr uint32_t kNear = 8;
 __device__ __forceinline__ float middle_bits(float q) {
     const float a = fabsf(q);
