@@ -370,10 +370,13 @@ int rows_per_block(bool f32, int T, int d, int cus) {
 }
 // Outputs larger than the L2s hold together are stored non-temporally: 32768 x 1024
 // forward fp32 75 -> 68 us, bf16 51 -> 44, backward fp32 112 -> 105. A call that passes
-// more than the memory-side cache holds also loads s, r and dr like that, but not x and
-// dy, which the products before it have just written: backward of that shape fp32 (448
-// MB) 105 -> 84, bf16 (268 MB) 62 -> 48, forward fp32 (369 MB) 68 -> 61; x and dy too: 98,
-// 57, 65; forward bf16 (235 MB, below the bound) 44 -> 53.
+// over 250 MB, about what the memory-side cache (256 MiB) holds, also loads s, r and dr like
+// that, but not x and dy, which the products before it have just written: backward of
+// that shape fp32 105 -> 84, bf16 62 -> 48, forward fp32 68 -> 61; x and dy too: 98, 57, 65.
+// What decides is whether the inputs are still there, as they may be below the bound: widths
+// 256 to 8192 after other calls, 260 MB forward 3 to 9% faster and backward 9 to 20%, 200 MB
+// 0 to 4 and 9 to 20, 150 MB forward 3 to 15% slower; on the same buffers again, 150 to 300
+// MB, all 3 to 22% slower.
 int pass_of(int64_t in, int64_t out) { return in + out > 250'000'000 ? kOnce : out > 16 << 20 ? kStoreOnce : kCached; }
 
 template <bool F32, bool TAIL, int LANES, int V, int PASS>
