@@ -72,14 +72,6 @@ __device__ __forceinline__ i32x8 read_codes16(const uint8_t* t, int r, int g) {
 // N 4096, K 1024 2.9 us, M 64, N 1024, K 4096 4.4 (6.2 with loads straight into
 // registers, where neighbouring lanes hold different rows and four of them take four
 // cache lines).
-template <int RB, int NB, bool ONE>
-struct RowSlot {
-    static constexpr int SA = (RB + NB) * 2048, SB = SA + 256, BYTES = SB + 256;
-    static constexpr int ND = 2 * (RB + NB) + 2;  // loads of a block
-    static constexpr int DEPTH = ONE ? 1 : RB * NB == 1 ? 4 : RB * NB == 2 ? 3 : RB * NB == 4 ? 2 : 1;
-    static constexpr int WAVE = DEPTH * BYTES;    // bytes of a wave
-    static_assert(8 * WAVE <= 160 * 1024 && 1024 * RB * NB <= WAVE && DEPTH * ND < 64, "LDS; a wave's sums; what a wait counts");
-};
 template <bool TILES, bool F32, int RB, int NB, bool ONE>
 __global__ __launch_bounds__(512) void fp8_rows_kernel(Fp8Params p) {
     using S = RowSlot<RB, NB, ONE>;
@@ -89,30 +81,23 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(Fp8Params p) {
     const int row = lane & 15, g = lane >> 4;
     uint8_t* own = reinterpret_cast<uint8_t*>(lds_raw) + wave * S::WAVE;
     const uint32_t lds0 = lds_u32(own);
-    const int nb = (p.N + 16 * NB - 1) / (16 * NB);  // blocks of columns, which run fastest
-    const int n0 = (int)(blockIdx.x % nb) * 16 * NB, m0 = (int)(blockIdx.x / nb) * 16 * RB;
-    const int rows = min(p.M - m0, 16 * RB), cols = min(p.N - n0, 16 * NB);
+    RowBlock<TILES, RB, NB> at;
+    at.set(p, blockIdx.x);
     const int blocks = (p.K + kFp8Block - 1) / kFp8Block, steps = (blocks - wave + NW - 1) / NW;
-    // windows: rows past the last one, and chunks past a row's end, are zeros
-    constexpr uint32_t FAR = 0x80000000u;
-    const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u;
-    const Window wa = {address(p.a + (int64_t)m0 * p.lda), (uint32_t)(rows - 1) * (uint32_t)p.lda + k16};
-    const Window wb = {address(p.b + (int64_t)n0 * p.ldb), (uint32_t)(cols - 1) * (uint32_t)p.ldb + k16};
-    const int chunk = (lane & 7) ^ (lane >> 4);  // of 16 codes, swizzled as read_codes16 reads them; rows 8 .. 15: ^ 4
+    const int chunk = row_chunk(lane);
     const uint32_t a_row = (uint32_t)(lane >> 3) * (uint32_t)p.lda, b_row = (uint32_t)(lane >> 3) * (uint32_t)p.ldb;
     auto load = [&](int n) {
         const int kb = wave + n * NW, k = kb * kFp8Block;
         const uint32_t slot = lds0 + (uint32_t)(n % DEPTH) * S::BYTES;
-        uint32_t at[2];
+        uint32_t from[2];
 #pragma unroll
-        for (int o = 0; o < 2; ++o) at[o] = k + 16 * (chunk ^ (4 * o)) < p.K ? (uint32_t)(k + 16 * (chunk ^ (4 * o))) : FAR;
+        for (int o = 0; o < 2; ++o) from[o] = row_chunk_at(p.K, k, chunk ^ (4 * o));
 #pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) dma16(wb, at[i & 1] + b_row + (uint32_t)(8 * i) * (uint32_t)p.ldb, slot + 2048 * RB + 1024 * i);
+        for (int i = 0; i < 2 * NB; ++i) dma16(at.wb, from[i & 1] + b_row + (uint32_t)(8 * i) * (uint32_t)p.ldb, slot + 2048 * RB + 1024 * i);
 #pragma unroll
-        for (int i = 0; i < 2 * RB; ++i) dma16(wa, at[i & 1] + a_row + (uint32_t)(8 * i) * (uint32_t)p.lda, slot + 1024 * i);
-        dma4({address(p.as + (int64_t)kb * p.ldas + m0), 4u * (uint32_t)rows}, 4u * lane, slot + S::SA);
-        if constexpr (TILES) dma4({address(p.bs + (int64_t)(n0 / kFp8Block) * p.ldbs + kb), 4u}, 4u * lane, slot + S::SB);
-        else dma4({address(p.bs + (int64_t)kb * p.ldbs + n0), 4u * (uint32_t)cols}, 4u * lane, slot + S::SB);
+        for (int i = 0; i < 2 * RB; ++i) dma16(at.wa, from[i & 1] + a_row + (uint32_t)(8 * i) * (uint32_t)p.lda, slot + 1024 * i);
+        dma4(at.a_scales(p, kb), 4u * lane, slot + S::SA);
+        dma4(at.b_scales(p, kb), 4u * lane, slot + S::SB);
     };
     f32x4 acc[RB][NB];
 #pragma unroll
@@ -165,7 +150,7 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(Fp8Params p) {
     __syncthreads();
     const float* red = reinterpret_cast<const float*>(lds_raw);
     for (int o = threadIdx.x * 2; o < OUT; o += 128 * NW) {
-        const int m = m0 + o / (16 * NB), n = n0 + o % (16 * NB);
+        const int m = at.m0 + o / (16 * NB), n = at.n0 + o % (16 * NB);
         if (m >= p.M || n >= p.N) continue;
         float v[2] = {0.0f, 0.0f};
 #pragma unroll

@@ -60,6 +60,42 @@ TMT_HD Unit half_of(Unit u, int half) {
     return u;
 }
 
+// ---- few rows ------------------------------------------------------------------
+// A wave's slot in LDS: 16 RB rows of a's codes and 16 NB of b's, 128 bytes each, and the
+// scales of both; DEPTH of them.
+template <int RB, int NB, bool ONE>
+struct RowSlot {
+    static constexpr int SA = (RB + NB) * 2048, SB = SA + 256, BYTES = SB + 256;
+    static constexpr int ND = 2 * (RB + NB) + 2;  // loads of a block
+    static constexpr int DEPTH = ONE ? 1 : RB * NB == 1 ? 4 : RB * NB == 2 ? 3 : RB * NB == 4 ? 2 : 1;
+    static constexpr int WAVE = DEPTH * BYTES;    // bytes of a wave
+    static_assert(8 * WAVE <= 160 * 1024 && 1024 * RB * NB <= WAVE && DEPTH * ND < 64, "LDS; a wave's sums; what a wait counts");
+};
+// A workgroup's outputs and the windows of its loads: rows past the last one, and chunks
+// past a row's end, are zeros.
+template <bool TILES, int RB, int NB>
+struct RowBlock {
+    int m0, n0, rows, cols;
+    Window wa, wb;
+    TMT_HD void set(const Fp8Params& p, unsigned block) {
+        const int nb = (p.N + 16 * NB - 1) / (16 * NB);  // blocks of columns, which run fastest
+        n0 = (int)(block % nb) * 16 * NB, m0 = (int)(block / nb) * 16 * RB;
+        rows = min(p.M - m0, 16 * RB), cols = min(p.N - n0, 16 * NB);
+        const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u;
+        wa = {address(p.a + (int64_t)m0 * p.lda), (uint32_t)(rows - 1) * (uint32_t)p.lda + k16};
+        wb = {address(p.b + (int64_t)n0 * p.ldb), (uint32_t)(cols - 1) * (uint32_t)p.ldb + k16};
+    }
+    TMT_HD Window a_scales(const Fp8Params& p, int kb) const { return {address(p.as + (int64_t)kb * p.ldas + m0), 4u * (uint32_t)rows}; }
+    TMT_HD Window b_scales(const Fp8Params& p, int kb) const {
+        if constexpr (TILES) return {address(p.bs + (int64_t)(n0 / kFp8Block) * p.ldbs + kb), 4u};
+        else return {address(p.bs + (int64_t)kb * p.ldbs + n0), 4u * (uint32_t)cols};
+    }
+};
+// A load takes 8 rows of 128 codes, a lane 16 codes: chunk (of rows 8 .. 15: ^ 4) of the
+// lane's row lane / 8, swizzled as they are read, and where it begins in a row from k on.
+TMT_HD int row_chunk(int lane) { return (lane & 7) ^ (lane >> 4); }
+TMT_HD uint32_t row_chunk_at(int K, int k, int chunk) { return k + 16 * chunk < K ? (uint32_t)(k + 16 * chunk) : 0x80000000u; }
+
 // ---- plan ----------------------------------------------------------------------
 // The kernel for few rows, 64 x 64 or 128 x 128 tiles (whole, or the last round's cut
 // along the reduction), or 256 x 256 tiles: the one with the shortest estimate.
@@ -68,7 +104,11 @@ struct Fp8Plan {
     Fp8Kernel kernel = FP8_ROWS_KERNEL;
     LinearPlan tiles;
 };
-constexpr int kFp8FewRows = 64;  // up to these the kernel for few rows, which needs no workspace
+// Up to these the kernel for few rows, which needs no workspace, so that a decode step has none.
+// A long reduction to few outputs would be faster in parts. us, M 64 / 72, whose rest goes
+// over 64 x 64 or 128 x 128 tiles: K 32768, N 64 fp32 16.3 / 11.9, bf16 13.6 / 11.2; N 256 16.7 / 14.5,
+// 14.1 / 13.1; K 16384, N 1024 bf16 10.1 / 13.7.
+constexpr int kFp8FewRows = 64;
 constexpr int kFp8MinSteps = 4;  // blocks of 128 that a part of a split reduction has at least
 
 inline int fp8_steps(int K) { return (int)(((int64_t)K + kFp8Block - 1) / kFp8Block); }
