@@ -26,18 +26,20 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
 }
 
 // One wave-wide 16-byte-per-lane load from global memory into LDS at
-// lds_base + 16 * lane (lds_base wave-uniform); M0 is declared clobbered.
+// lds_base + 16 * lane (lds_base wave-uniform); M0 is declared clobbered. Between M0's
+// write and the load that reads it one wait state has to pass, which the compiler does not
+// add inside such a block.
 // These loads count on the vector-memory counter like any other, but the
 // compiler does not see them: a compiler-placed wait for a later load waits
 // for them too (the counter completes in order).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16_lds(const void* g, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base) : "m0", "memory");
 }
 // The same with 4 bytes per lane (to lds_base + 4 * lane).
 __device__ __forceinline__ void dma4_lds(const void* g, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_base) : "m0", "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_base) : "m0", "memory");
 }
 #pragma clang diagnostic pop
 // LDS address of a pointer into shared memory.

@@ -162,8 +162,9 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // M0 is written here and declared clobbered (clang warns that it is reserved).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+// (a wait state between M0's write and the load)
 __device__ __forceinline__ void dma16(const void* g, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base) : "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base) : "m0");
 }
 #pragma clang diagnostic pop
 template <int N>

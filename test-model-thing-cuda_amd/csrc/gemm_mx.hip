@@ -77,13 +77,15 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 #pragma clang diagnostic ignored "-Winline-asm"
 // One wave-wide 16-byte-per-lane load from global memory (wave-uniform base
 // plus a 32-bit per-lane byte offset) into LDS at lds_base + 16 * lane
-// (lds_base wave-uniform); M0 is declared clobbered.
+// (lds_base wave-uniform); M0 is declared clobbered. M0's write needs one wait state ahead of
+// the load, and a base that a vector instruction has written (one that comes back from a
+// register's lane, where the scalar registers do not suffice) five, the move among them.
 __device__ __forceinline__ void dma16(const void* sbase, uint32_t voff, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "m0");
 }
 // The same with 4 bytes per lane, to LDS at lds_base + 4 * lane.
 __device__ __forceinline__ void dma4(const void* sbase, uint32_t voff, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "m0");
 }
 #pragma clang diagnostic pop
 template <int N>

@@ -47,9 +47,9 @@ __device__ __align__(16) const uint32_t zero_piece[4] = {0, 0, 0, 0};
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // 16 bytes per lane from the lane's 64-bit address into LDS at lds_base + 16 * lane
-// (lds_base wave-uniform); M0 is written.
+// (lds_base wave-uniform); M0 is written, one wait state ahead of the load.
 __device__ __forceinline__ void dma16v(const void* g, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base) : "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base) : "m0");
 }
 #pragma clang diagnostic pop
 

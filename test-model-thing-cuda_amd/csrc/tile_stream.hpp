@@ -22,12 +22,12 @@ __device__ __forceinline__ i32x4 descriptor(const Window& w) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // 16 (4) bytes per lane from a window into LDS at lds_base + 16 (4) * lane
-// (lds_base wave-uniform); M0 is written.
+// (lds_base wave-uniform); M0 is written, one wait state ahead of the load.
 __device__ __forceinline__ void dma16(const Window& w, uint32_t voff, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(descriptor(w)), "s"(lds_base) : "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(descriptor(w)), "s"(lds_base) : "m0");
 }
 __device__ __forceinline__ void dma4(const Window& w, uint32_t voff, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(descriptor(w)), "s"(lds_base) : "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(descriptor(w)), "s"(lds_base) : "m0");
 }
 #pragma clang diagnostic pop
 template <int N>
