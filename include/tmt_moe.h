@@ -560,9 +560,12 @@ int tmt_moe_fp8_transpose(void* stream, const uint8_t* codes, int64_t ldc, int32
  * (`b_blocks`), Y bf16 or fp32 (`dtype`). A block's products are summed in fp32,
  * multiplied by its two scales and added in fp32; Y is rounded once. For bf16 the
  * sums are those of the 8-bit matrix instruction, which keeps 13 bits below the
- * largest of eight neighbouring products (1.5e-5 off in norm). N a multiple of 8, at most 2^22 as K is; M*N at most 2^40. With beta == 0 Y is not read;
- * M == 0 or N == 0 is no work and K == 0 gives beta * Y. Where the product of two
- * scales is past fp32's range, the outputs may be infinite or NaN.
+ * largest of eight neighbouring products (1.5e-5 off in norm; where products cancel, it
+ * is the largest that the error goes by). N a multiple of 8, at most 2^22 as K is; M*N at
+ * most 2^40. With beta == 0 Y is not read; M == 0 or N == 0 is no work and K == 0 gives
+ * beta * Y. A NaN code makes the outputs of its row of A or B NaN. Where the product of
+ * two scales is past fp32's range, the outputs may be infinite or NaN; below its normal
+ * range they lose bits.
  */
 int tmt_moe_fp8_workspace_size(int32_t b_blocks, int32_t M, int32_t N, int32_t K, size_t* bytes);
 int tmt_moe_fp8_matmul(void* stream, int32_t b_blocks, int32_t dtype, int32_t M, int32_t N, int32_t K, const uint8_t* A,

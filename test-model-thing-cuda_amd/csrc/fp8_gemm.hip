@@ -266,7 +266,7 @@ struct Loader {
 // before the previous unit's epilogue, which stages through the other slot. Bound by
 // the issue port: a matrix instruction takes 20 clocks of it and 32 of the matrix
 // cores, and each of the 8 vector instructions that widen and scale for it 4. T 32768,
-// 4096 x 1024 285 us, 0.96 PFLOP/s, with 9 of them for the split sums; a plain bf16
+// 4096 x 1024 290 to 300 us, 0.93 PFLOP/s, with 9 of them for the split sums; a plain bf16
 // product would take 198.
 template <bool TILES, bool SPLIT, bool BETA>
 __global__ __launch_bounds__(256, 2) void fp8_wide_kernel(Fp8Params p, LinearPlan pl) {
@@ -680,9 +680,9 @@ __global__ __launch_bounds__(512, 2) void fp8_deep_kernel(Fp8Params p, LinearPla
 // the vector unit scales and adds: 128 a wave.
 // 16 x 16 sums, whose instruction takes a whole block of 128: four of them are in
 // flight, and the vector unit adds the one issued three before while the next run,
-// so that neither waits for the other. T 32768, N 4096, K 1024 138 to 143 us, 1.95
+// so that neither waits for the other. T 32768, N 4096, K 1024 138 to 148 us, 1.9
 // PFLOP/s (32 x 32 sums, two instructions a block, with one in flight: 162); T = N = K =
-// 8192 451, 2.44, at the power limit.
+// 8192 442 to 459, 2.45, at the power limit.
 // Ring of 2. A wave holds a step's b and streams its a. Behind the last but one
 // read the whole slot is in registers: the barrier stands there; the last sums cover
 // the next slot's first reads, and the freed slot's loads begin. The stream does not

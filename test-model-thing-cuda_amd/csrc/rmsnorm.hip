@@ -15,7 +15,7 @@
 // would cover every second 16 bytes). A row's pieces are consecutive, so 16 (32)
 // neighbouring lanes own a block of 128 columns and find its maximum by DPP. us, and
 // TB/s of what has to pass: forward 32768 x 1024 fp32 to stream and codes 61, 6.0; 16384 x
-// 4096 125, 5.9; 777 x 1280 bf16 to bf16 and codes 4.8; one row 3.5; backward 32768 x 1024 fp32 84, 5.6; 16384 x
+// 4096 125, 5.9; 777 x 1280 bf16 to bf16 and codes 5.0; one row 3.5; backward 32768 x 1024 fp32 84, 5.6; 16384 x
 // 4096 bf16 113, 4.8; 5003 x 1000 13.0. A copy of 1 GiB reaches 5.0 TB/s.
 //
 // The forward's squares are added in 64 bits, a lane's values, the lanes (a butterfly)
